@@ -20,9 +20,9 @@ from torch.autograd import forward_ad
 _CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libneox_fused.so")
 CALLS_PATH = os.path.join(_CSRC, "neox_torch.so")
-ABI_VERSION = 4
+ABI_VERSION = 5
 
-NEOX_F16, NEOX_BF16, NEOX_F32 = 0, 1, 2
+NEOX_F16, NEOX_BF16, NEOX_F32, NEOX_I8, NEOX_F8 = 0, 1, 2, 3, 4
 _DTYPE_CODE = {torch.float16: NEOX_F16, torch.bfloat16: NEOX_BF16, torch.float32: NEOX_F32}
 
 _c_i64p = ctypes.POINTER(ctypes.c_int64)
@@ -93,6 +93,23 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _c_i64p, _c_i64p, _c_i64p,
          _c_i64p, _i64, _i32, _i32, _i32, _vp],
+    ),
+    "neox_window_attention_fwd": (
+        ctypes.c_int, [_vp] * 6 + [_i32] * 6 + [_c_i64p] * 4 + [_f32, _i32, _i32, _i32, _vp]
+    ),
+    "neox_window_attention_bwd": (
+        ctypes.c_int, [_vp] * 11 + [_i32] * 6 + [_c_i64p] * 8 + [_f32, _i32, _i32, _i32, _vp]
+    ),
+    "neox_paged_attention_workspace": (ctypes.c_int, [_c_i64p] + [_i32] * 9),
+    "neox_paged_attention": (
+        ctypes.c_int,
+        [_vp, _vp, _i64] + [_vp] * 8 + [_i32] * 7 + [_i64, _i32, _i32, _i64] + [_c_i64p] * 6 + [_f32, _i32, _i32, _i32, _i32, _vp],
+    ),
+    "neox_cache_write": (
+        ctypes.c_int, [_vp] * 7 + [_i32, _i64, _i32, _i32, _i64, _i32] + [_c_i64p] * 6 + [_i32, _i32, _vp]
+    ),
+    "neox_cache_read": (
+        ctypes.c_int, [_vp] * 7 + [_i32, _i64, _i32, _i32, _i64, _i32] + [_c_i64p] * 6 + [_i32, _i32, _vp]
     ),
 }
 
@@ -276,3 +293,31 @@ def strides3(t):
             _strides3_cache.clear()
         arr = _strides3_cache[key] = (ctypes.c_int64 * 3)(*key)
     return arr
+
+
+def row_strides(t):
+    """Element strides of all axes of ``t`` but the dense last one, as a C int64 array; an axis of one element, which
+    no kernel steps along, counts as 0.  One array per distinct tuple, as in :func:`strides3`."""
+    key = tuple(0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    arr = _strides3_cache.get(key)
+    if arr is None or len(arr) != len(key):
+        if len(_strides3_cache) > 4096:
+            _strides3_cache.clear()
+        arr = _strides3_cache[key] = (ctypes.c_int64 * len(key))(*key)
+    return arr
+
+
+def whole_pieces(t):
+    """Whether the attention kernels can read the 16-bit tensor ``t`` as it lies: rows of its last axis dense, apart
+    from one another, and on 16-byte boundaries."""
+    if t.stride(-1) != 1 or t.data_ptr() % 16:
+        return False
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        if n > 1 and (s % 8 or s < 0):
+            return False
+    return t.shape[-2] == 1 or t.stride(-2) >= t.shape[-1]
+
+
+def in_pieces(t):
+    """``t``, or a dense copy of it where the attention kernels cannot read it as it lies."""
+    return t if whole_pieces(t) else t.clone(memory_format=torch.contiguous_format)

@@ -20,21 +20,6 @@ int fail(int status, const char* fmt, ...) {
     return status;
 }
 
-static inline bool aligned(const void* p, uintptr_t n) {
-    return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
-}
-
-static int check_launch(hipError_t e, const char* what) {
-    if (e == hipSuccess) return NEOX_OK;
-    return fail(NEOX_ERR_LAUNCH, "%s: kernel launch failed: %s", what, hipGetErrorString(e));
-}
-
-static int check_dtype(int dtype, const char* what) {
-    if (dtype == NEOX_F16 || dtype == NEOX_BF16) return NEOX_OK;
-    return fail(NEOX_ERR_BAD_DTYPE, "%s: Only fp16 and bf16 are supported (dtype code %d)", what,
-                dtype);
-}
-
 // rows of a [.., sq, sk] score tensor must be countable in 31 bits
 static int check_rows(int64_t rows, int sq, int sk, const char* what) {
     if (sq < 1 || sk < 1) return fail(NEOX_ERR_BAD_SHAPE, "%s: sq=%d sk=%d must be >= 1", what, sq, sk);

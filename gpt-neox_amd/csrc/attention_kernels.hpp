@@ -1,0 +1,1103 @@
+// Attention without stored scores: the device code shared by the forward kernel (training, evaluation,
+// prompts over a paged cache) and the two backward kernels.
+//
+// One (sample, key head) at a time.  Its queries are "rows": row = token * group + head in the group, so
+// that the heads that share keys share the tiles of those keys too.  All products run on the matrix cores as
+// 32x32x16 tiles with the row (or, for the key gradients, the key) in the column of the result: lane l then
+// holds the results of column l % 32, sixteen of the 32 along the other axis, and the maximum and sum of a
+// softmax row stay within a lane and its partner l ^ 32.
+//   forward:   S^T = K Q^T;  O^T  += V^T P^T
+//   queries:   S^T = K Q^T;  dP^T = V dO^T;  dQ^T += K^T dS^T
+//   keys:      S   = Q K^T;  dP   = dO V^T;  dV^T += dO^T P;  dK^T += Q^T dS
+// The result of the first product of each chain is the second operand of the last without a move: result
+// register 8 t + e of a lane is what k-slot e of step t takes, if the other operand numbers its k-slots by
+// element key_of(t, half, e) -- two transposing LDS reads of four consecutive elements each.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "wave.hpp"
+
+namespace neox {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr int kTileKeys = 64;   // keys of one step of the forward and the query-gradient kernel
+constexpr int kTileRows = 128;  // rows of a workgroup there: 32 for each of its four waves
+constexpr int kStepRows = 32;   // rows of one step of the key-gradient kernel
+constexpr int kGradKeys = 128;  // keys of a workgroup there: 32 for each of its four waves
+
+// where keys and values come from
+enum KvSource { kStrided = 0, kPaged16 = 1, kPagedI8 = 2, kPagedF8 = 3 };
+
+struct AttnArgs {
+    const char *q, *k, *v;       // 16-bit elements (k, v: 8-bit codes for the last two sources)
+    char* o;
+    float* lse;                  // log2 of every row's sum of exponentials, +inf for an empty row; [b, kv, rows]
+    const float *k_scale, *v_scale;
+    // element strides.  q, o: token, sample (strided only), head.  k, v: token, sample, head; for pages the token
+    // stride within a page, the page stride and the head stride
+    int64_t q_st[3], o_st[3], k_st[3], v_st[3];
+    int64_t ks_st[3], vs_st[3];  // the scales': token within a page, page, head
+    const int32_t* lengths;      // keys of every sample (null, strided only: all of them)
+    const int32_t* starts;       // paged: first token of every sequence in q, and the end
+    const int32_t* table;        // paged: [b, table_stride] page numbers
+    int64_t table_stride;
+    int table_keys;              // keys that a row of the table can name
+    int64_t pages;
+    int tokens;                  // paged: rows of q
+    float scale_log2;            // |scale| * log2(e)
+    uint32_t flip;               // 0x80008000: the queries change sign on their way in (a negative scale)
+    int d, kv, group;
+    int sq, sk;                  // strided: queries and keys of a sample; paged: the most new tokens of a sequence
+    int b;
+    int window;                  // < 0: none
+    int sinks;
+    int row_tiles;               // of the longest sample
+    int splits;                  // parts of the key axis; with more than one, o and lse are partial results:
+    float* part_o;               //   [split][row slot][d] and
+    float* part_lse;             //   [split][row slot], row slot = (token * kv + key head) * group + head in the group
+    int64_t part_rows;           //   row slots of one split
+    FastDiv by_group, by_page, by_row_tiles, by_kv;
+    // backward
+    const char *dout;            // [token, sample, head] like q
+    const char* out;
+    int64_t do_st[3];
+    char *dq, *dk, *dv;
+    int64_t dq_st[3], dk_st[3], dv_st[3];
+    float* delta;                // sum over d of dO * O of every row, [b, kv, rows]
+    float scale;
+    int key_tiles;
+    FastDiv by_key_tiles;
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<BF16> {
+    static __device__ __forceinline__ f32x16 op(const u32x4& a, const u32x4& b, const f32x16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 op16(const u32x4& a, const u32x4& b, const f32x4& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<F16> {
+    static __device__ __forceinline__ f32x16 op(const u32x4& a, const u32x4& b, const f32x16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 op16(const u32x4& a, const u32x4& b, const f32x4& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+// One head dim class: DP is the padded head dim.  A tile row in LDS has kRow bytes (a power of two), cut into
+// 16-byte pieces whose order is permuted by the row number, so that both kinds of read spread over all banks:
+// 16 rows at one piece (row operand), and 4 rows at 4 neighbouring pieces (transposing reads).
+template <int DP>
+struct Tile {
+    static constexpr int kRow = DP <= 64 ? 128 : DP <= 128 ? 256 : 512;
+    static constexpr int kPieces = DP / 8;  // of a row that hold data
+    static __device__ __forceinline__ uint32_t turn(uint32_t row) {
+        if constexpr (kRow == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+        return (row & 3) << 2 | ((row >> 2) & 3);
+    }
+    static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t piece) {
+        return row * kRow + ((piece ^ turn(row)) << 4);
+    }
+};
+
+// Operand of 32 tile rows (row0 ..) and the 16 dims of step s, row-major: lane l has row l % 32, dims 8 (l / 32) ..
+template <int DP>
+__device__ __forceinline__ u32x4 row_operand(const char* tile, int row0, int s) {
+    const uint32_t lane = threadIdx.x & 63;
+    return *reinterpret_cast<const u32x4*>(tile + Tile<DP>::at(row0 + (lane & 31), 2 * s + (lane >> 5)));
+}
+
+// Operand of the 32 dims from 32 * db and the 16 tile rows from row0, transposed: lane l has dim l % 32 and, in
+// slot e, row row0 + 8 (e / 4) + 4 (l / 32) + e % 4.
+template <int DP>
+__device__ __forceinline__ u32x4 turned_operand(char* tile, int row0, int db) {
+    const uint32_t lane = threadIdx.x & 63, i = lane & 15;
+    const uint32_t row = row0 + 4 * (lane >> 5) + (i >> 2);
+    const uint32_t piece = 4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
+    const uint32_t half = (i & 1) * 8;
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + Tile<DP>::at(row, piece) + half));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + Tile<DP>::at(row + 8, piece) + half));
+    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+    return u32x4{a.x, a.y, b.x, b.y};
+}
+
+// The values of lane l and of lane l ^ 32, combined.  (The results go through integers of their own: a bit cast of
+// a vector's element takes the first element, whichever is asked for.)
+struct HalfPair {
+    float a, b;
+};
+__device__ __forceinline__ HalfPair both_halves(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
+__device__ __forceinline__ float both_halves_max(float x) {
+    const HalfPair p = both_halves(x);
+    return fmaxf(p.a, p.b);
+}
+__device__ __forceinline__ float both_halves_sum(float x) {
+    const HalfPair p = both_halves(x);
+    return p.a + p.b;
+}
+
+// the element of a 32-long result axis that register r of a lane in this half holds
+__device__ __forceinline__ int element_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// 8 elements at p, or zeros
+__device__ __forceinline__ u32x4 load8(const char* p, bool there) {
+    u32x4 z = {0, 0, 0, 0};
+    return there ? *reinterpret_cast<const u32x4*>(p) : z;
+}
+
+// Writes the 32 columns' results of one wave (lane: column, registers: 32 dims per block) times f as rows of 16-bit
+// elements.  The halves exchange registers, so that every lane stores 16 bytes.
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(char* row, const f32x16 (&acc)[DP / 32], float f, int d, bool there) {
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int r = 8 * p;
+            const uint32_t a0 = Elem<T>::pack(acc[b][r] * f, acc[b][r + 1] * f), a1 = Elem<T>::pack(acc[b][r + 2] * f, acc[b][r + 3] * f);
+            const uint32_t b0 = Elem<T>::pack(acc[b][r + 4] * f, acc[b][r + 5] * f), b1 = Elem<T>::pack(acc[b][r + 6] * f, acc[b][r + 7] * f);
+            const auto x = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+            const int dim = 32 * b + 16 * p + 8 * half;
+            if (there && dim < d) *reinterpret_cast<u32x4*>(row + dim * 2) = u32x4{x[0], y[0], x[1], y[1]};
+        }
+    }
+}
+
+// eight 8-bit codes as numbers
+template <int SRC>
+__device__ __forceinline__ void decode8(const u32x2& w, float (&f)[8]) {
+    if constexpr (SRC == kPagedI8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int word = (int)(i ? w.y : w.x);
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false);
+            const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
+            f[4 * i] = lo[0];
+            f[4 * i + 1] = lo[1];
+            f[4 * i + 2] = hi[0];
+            f[4 * i + 3] = hi[1];
+        }
+    }
+}
+// ... and as 16-bit values, exactly: no code has more than 7 bits of significand
+template <typename T, int SRC>
+__device__ __forceinline__ u32x4 widen8(const u32x2& w) {
+    float f[8];
+    decode8<SRC>(w, f);
+    return pack8<T>(f);
+}
+
+// The tiles of keys that rows with positions first .. last look at: some at the front for the sinks, then those of
+// the window.
+struct KeyTiles {
+    int front, from, count;
+    __device__ __forceinline__ int tile(int i) const { return i < front ? i : from + (i - front); }
+};
+template <int TILE>
+__device__ __forceinline__ KeyTiles key_tiles(int first, int last, int keys, int window, int sinks) {
+    const int end = min(last + 1, keys);
+    if (end <= 0) return {0, 0, 0};
+    int lo = window < 0 ? 0 : max(0, first - window);
+    lo = min(lo, end);
+    const int from = lo / TILE, to = (end + TILE - 1) / TILE;
+    const int front = min((min(sinks, end) + TILE - 1) / TILE, from);
+    return {front, from, front + max(0, to - from)};
+}
+
+// One sequence of a paged call.  What the device's tables say is kept inside what the tensors hold.
+__device__ __forceinline__ void paged_sample(const AttnArgs& a, int b, int& token0, int& tokens, int& keys) {
+    token0 = max(0, min(a.starts[b], a.tokens));
+    tokens = max(0, min(a.starts[b + 1], a.tokens) - token0);
+    tokens = min(tokens, a.sq);
+    keys = max(0, min(a.lengths[b], a.table_keys));
+}
+
+// ---- staging -----------------------------------------------------------------------------------------
+// One tile of ROWS rows (of keys, say) on its way from memory to LDS through registers: 256 threads, a piece
+// of 8 elements at a time.  Rows behind the last key and dims behind d come as zeros: what lies there may be anything.
+template <typename T, int DP, int SRC, int ROWS>
+struct Stage {
+    static constexpr int kRowsAtOnce = 256 / Tile<DP>::kPieces;  // DP = 96: 21, the last threads idle
+    static constexpr int kSteps = (ROWS + kRowsAtOnce - 1) / kRowsAtOnce;
+    static constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
+    u32x4 w[kCodes ? 1 : kSteps];
+    u32x2 c[kCodes ? kSteps : 1];
+
+    static __device__ __forceinline__ int row(int step) { return (int)(threadIdx.x / Tile<DP>::kPieces) + step * kRowsAtOnce; }
+    static __device__ __forceinline__ int piece() { return (int)(threadIdx.x % Tile<DP>::kPieces); }
+    static __device__ __forceinline__ bool works(int step) {
+        return (int)threadIdx.x < kRowsAtOnce * Tile<DP>::kPieces && row(step) < ROWS;
+    }
+
+    __device__ __forceinline__ void load(int step, const char* at, bool there) {
+        if constexpr (kCodes) {
+            c[step] = u32x2{0, 0};
+            if (there) c[step] = *reinterpret_cast<const u32x2*>(at);
+        } else {
+            w[step] = load8(at, there);
+        }
+    }
+    __device__ __forceinline__ void put(char* tile) const {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (!works(s)) continue;
+            u32x4 x;
+            if constexpr (kCodes) x = widen8<T, SRC>(c[s]);
+            else x = w[s];
+            *reinterpret_cast<u32x4*>(tile + Tile<DP>::at(row(s), piece())) = x;
+        }
+    }
+};
+
+// ---- forward --------------------------------------------------------------------------------------------
+template <typename T, int DP, int SRC, bool SPLIT>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
+    constexpr bool kPages = SRC != kStrided;
+    constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
+    constexpr int kBytes = kCodes ? 1 : 2;
+    constexpr int kTile = kTileKeys * Tile<DP>::kRow;
+    constexpr int kBuffers = DP <= 128 ? 2 : 1;  // (DP = 256: two tiles of 32 KiB each, one buffer)
+    __shared__ __attribute__((aligned(16))) char lds[kBuffers * 2 * kTile + (kCodes ? 2 * 2 * kTileKeys * 4 : 0)];
+
+    // block -> (sample, key head), row tile, part: neighbours in time on one XCD (blocks go to the 8 XCDs in
+    // turn) are the row tiles of one key head, whose keys they share
+    uint32_t block = blockIdx.x;
+    const uint32_t split = SPLIT ? blockIdx.y : 0;
+    const uint32_t heads = a.b * a.kv;
+    uint32_t bh, mt;
+    if (heads % 8 == 0) {
+        const uint32_t xcd = block & 7, k = block >> 3;
+        const uint32_t part = a.by_row_tiles.div(k);
+        bh = part * 8 + xcd;
+        mt = k - part * a.row_tiles;
+    } else {
+        bh = a.by_row_tiles.div(block);
+        mt = block - bh * a.row_tiles;
+    }
+    mt = a.row_tiles - 1 - mt;  // the later rows, which see most keys, first
+    const int b = a.by_kv.div(bh), g = bh - b * a.kv;
+
+    int token0 = 0, tokens = a.sq, keys = a.sk, position0 = a.sk - a.sq;
+    if constexpr (kPages) {
+        paged_sample(a, b, token0, tokens, keys);
+        position0 = keys - tokens;
+    } else if (a.lengths) {
+        keys = max(0, min(a.lengths[b], a.sk));
+    }
+    const int rows = tokens * a.group, row0 = mt * kTileRows;
+    if (row0 >= rows) return;
+
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+    const int row = row0 + wave * 32 + (lane & 31);
+    const bool there = row < rows;
+    const int token = a.by_group.div(min(row, rows - 1)), head = g * a.group + (min(row, rows - 1) - token * a.group);
+    const int position = position0 + token;
+    // positions of the workgroup's and of the wave's rows
+    const int wg_first = position0 + (int)a.by_group.div(row0), wg_last = position0 + (int)a.by_group.div(min(row0 + kTileRows, rows) - 1);
+    const int wave_row0 = min(row0 + wave * 32, rows - 1);
+    const int wv_first = __builtin_amdgcn_readfirstlane(position0 + (int)a.by_group.div(wave_row0));
+    const int wv_last = __builtin_amdgcn_readfirstlane(position0 + (int)a.by_group.div(min(row0 + wave * 32 + 32, rows) - 1));
+    const bool wave_works = row0 + wave * 32 < rows;
+
+    KeyTiles tiles = key_tiles<kTileKeys>(wg_first, wg_last, keys, a.window, a.sinks);
+    int first_tile = 0, end_tile = tiles.count;
+    if constexpr (SPLIT) {
+        const int each = (tiles.count + a.splits - 1) / a.splits;
+        first_tile = min((int)split * each, tiles.count);
+        end_tile = min(first_tile + each, tiles.count);
+    }
+
+    // queries, the second operand of the scores
+    u32x4 q[DP / 16];
+    {
+        const char* p = a.q + ((int64_t)(token0 + token) * a.q_st[0] + (kPages ? 0 : (int64_t)b * a.q_st[1]) + (int64_t)head * a.q_st[2]) * 2;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int dim = 16 * s + 8 * half;
+            q[s] = load8(p + dim * 2, there && dim < a.d);
+            q[s] ^= a.flip;
+        }
+    }
+
+    typedef Stage<T, DP, SRC, kTileKeys> St;
+    St ks, vs;
+    const int piece = St::piece();
+    const bool dims_there = piece * 8 < a.d;
+    int page_of[kPages ? St::kSteps : 1];   // the pages of the next tile's rows, looked up one step ahead
+    int page_at = 0;                        // (the scales' row of this thread: its page)
+    const int32_t* table = kPages ? a.table + (int64_t)b * a.table_stride : nullptr;
+    auto look_up = [&](int tile) {
+        if constexpr (kPages) {
+#pragma unroll
+            for (int s = 0; s < St::kSteps; ++s) {
+                const int key = tile * kTileKeys + St::row(s);
+                page_of[s] = key < keys ? table[a.by_page.div(key)] : -1;
+            }
+            if constexpr (kCodes) {
+                const int key = tile * kTileKeys + lane;
+                page_at = (wave < 2 && key < keys) ? table[a.by_page.div(key)] : -1;
+            }
+        }
+    };
+    float scale_of_key = 0.f;  // waves 0 and 1: the scales of the tile's keys and of its values
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int s = 0; s < St::kSteps; ++s) {
+            const int key = tile * kTileKeys + St::row(s);
+            const char *kp, *vp;
+            bool ok = St::works(s) && key < keys && dims_there;
+            if constexpr (kPages) {
+                const int64_t page = page_of[s], in = a.by_page.mod(key);
+                ok = ok && (uint64_t)page < (uint64_t)a.pages;
+                kp = a.k + (page * a.k_st[1] + in * a.k_st[0] + (int64_t)g * a.k_st[2] + piece * 8) * kBytes;
+                vp = a.v + (page * a.v_st[1] + in * a.v_st[0] + (int64_t)g * a.v_st[2] + piece * 8) * kBytes;
+            } else {
+                kp = a.k + ((int64_t)key * a.k_st[0] + (int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2] + piece * 8) * 2;
+                vp = a.v + ((int64_t)key * a.v_st[0] + (int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2] + piece * 8) * 2;
+            }
+            ks.load(s, kp, ok);
+            vs.load(s, vp, ok);
+        }
+        if constexpr (kCodes) {
+            scale_of_key = 0.f;
+            if (wave < 2 && (uint64_t)(int64_t)page_at < (uint64_t)a.pages) {
+                const int64_t in = a.by_page.mod(tile * kTileKeys + lane);
+                const float* p = wave ? a.v_scale : a.k_scale;
+                const int64_t* st = wave ? a.vs_st : a.ks_st;
+                scale_of_key = p[page_at * st[1] + in * st[0] + (int64_t)g * st[2]];
+            }
+        }
+    };
+    float* const scales = reinterpret_cast<float*>(lds + kBuffers * 2 * kTile);  // [buffer][keys, values][64]
+    auto put = [&](int buffer) {
+        ks.put(lds + buffer * 2 * kTile);
+        vs.put(lds + buffer * 2 * kTile + kTile);
+        if constexpr (kCodes) {
+            if (wave < 2) scales[(buffer * 2 + wave) * kTileKeys + lane] = scale_of_key;
+        }
+    };
+
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    float m = kNegInf, l = 0.f;
+
+    if (first_tile < end_tile) {
+        look_up(tiles.tile(first_tile));
+        fetch(tiles.tile(first_tile));
+        if (first_tile + 1 < end_tile) look_up(tiles.tile(first_tile + 1));
+        put(0);
+    }
+    __syncthreads();
+
+    for (int it = first_tile; it < end_tile; ++it) {
+        const int buffer = kBuffers == 2 ? (it - first_tile) & 1 : 0;
+        char* const kt = lds + buffer * 2 * kTile;
+        char* const vt = kt + kTile;
+        const int key0 = tiles.tile(it) * kTileKeys;
+        if (it + 1 < end_tile) {
+            fetch(tiles.tile(it + 1));
+            if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
+        }
+        // what of the tile this wave's rows see: nothing, all, or some of it
+        const int key_end = key0 + kTileKeys;
+        const bool none = !wave_works || key0 > wv_last || key0 >= keys ||
+                          (a.window >= 0 && key_end - 1 < wv_first - a.window && key0 >= a.sinks);
+        const bool all = key_end - 1 <= wv_first && key_end <= keys &&
+                         (a.window < 0 || key0 >= wv_last - a.window || key_end <= a.sinks);
+        if (!none) {
+            f32x16 s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+                for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<T>::op(row_operand<DP>(kt, 32 * kb, st), q[st], s[kb]);
+            }
+            if constexpr (kCodes) {
+                const float* f = scales + buffer * 2 * kTileKeys;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kb][r + i] *= c[i];
+                    }
+            }
+            if (!all) {
+                const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = key0 + 32 * kb + element_of(r, half);
+                        const bool sees = key <= hi && (key >= lo || key < a.sinks);
+                        s[kb][r] = sees ? s[kb][r] : kNegInf;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[0][r]);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[1][r]);
+            top = both_halves_max(top) * a.scale_log2;
+            // The running maximum follows only where a row has outgrown it by 2^8: until then its exponentials stay
+            // below 256 and the accumulators need no rescaling.
+            if (__any(top > m + 8.f)) {
+                const float higher = fmaxf(m, top);
+                const float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
+                m = higher;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+            }
+            const float base = m == kNegInf ? 0.f : m;
+            float sum = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], a.scale_log2, -base));
+                    sum += s[kb][r];
+                }
+            l += sum;
+            if constexpr (kCodes) {
+                const float* f = scales + (buffer * 2 + 1) * kTileKeys;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kb][r + i] = all || s[kb][r + i] != 0.f ? s[kb][r + i] * c[i] : 0.f;
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                u32x4 p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[t >> 1][8 * (t & 1) + 2 * e], s[t >> 1][8 * (t & 1) + 2 * e + 1]);
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(turned_operand<DP>(vt, 16 * t, i), p, acc[i]);
+            }
+        }
+        if (it + 1 < end_tile) {
+            if constexpr (kBuffers == 1) __syncthreads();
+            put(kBuffers == 2 ? buffer ^ 1 : 0);
+        }
+        __syncthreads();
+    }
+
+    const float total = both_halves_sum(l);
+    const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);  // (a NaN stays one)
+    if constexpr (SPLIT) {
+        const int64_t slot = (int64_t)split * a.part_rows + ((int64_t)(token0 + token) * a.kv + g) * a.group + (head - g * a.group);
+        float* p = a.part_o + slot * a.d;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int dim = 32 * i + element_of(r, half);
+                const f32x4 x = {acc[i][r] * inverse, acc[i][r + 1] * inverse, acc[i][r + 2] * inverse, acc[i][r + 3] * inverse};
+                if (there && dim < a.d) *reinterpret_cast<f32x4*>(p + dim) = x;
+            }
+        if (there && half == 0) a.part_lse[slot] = total == 0.f ? kNegInf : m + __builtin_amdgcn_logf(total);
+    } else {
+        char* p = a.o + ((int64_t)(token0 + token) * a.o_st[0] + (kPages ? 0 : (int64_t)b * a.o_st[1]) + (int64_t)head * a.o_st[2]) * 2;
+        store_rows<T, DP>(p, acc, inverse, a.d, there);
+        if (!kPages && a.lse && there && half == 0)
+            a.lse[(int64_t)bh * rows + row] = total == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(total);
+    }
+}
+
+// ---- single tokens ----------------------------------------------------------------------------------------
+// At most 16 rows per key head: the bytes of the keys and values bound it, so every wave streams keys of its own,
+// 32 at a time, with no barrier before the end.  16x16x32 tiles; the keys go from memory into the first operand as
+// they are (lane: key l % 16; 16-bit: 8 dims from 32 s + 8 (l / 16); codes: 16 dims from 64 s + 16 (l / 16)), the
+// values through LDS of the wave's own for the transposing reads.
+template <typename T, int DP, int SRC, bool SPLIT>
+__global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void attn_token_kernel(AttnArgs a) {
+    constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
+    constexpr int kBytes = kCodes ? 1 : 2;
+    constexpr int kKeys = 32;
+    constexpr int kLoads = kCodes ? (DP + 63) / 64 : DP / 32;  // 16-byte loads of one key per lane
+    constexpr int kPerRow = DP * kBytes / 16;                   // lanes that load one row of values
+    constexpr int kRowsAtOnce = 64 / kPerRow;
+    constexpr int kValueLoads = (kKeys + kRowsAtOnce - 1) / kRowsAtOnce;
+    constexpr int kWaveBytes = kKeys * Tile<DP>::kRow;
+    __shared__ __attribute__((aligned(16))) char lds[4 * kWaveBytes];
+    __shared__ __attribute__((aligned(16))) float scales[4][2][kKeys];
+    __shared__ float wave_m[4][16], wave_l[4][16];
+
+    const uint32_t bh = blockIdx.x;
+    const int split = SPLIT ? (int)blockIdx.y : 0;
+    const int b = a.by_kv.div(bh), g = bh - b * a.kv;
+    int token0, tokens, keys;
+    paged_sample(a, b, token0, tokens, keys);
+    const int rows = min(tokens * a.group, 16);
+    if (rows == 0) return;
+    const int position0 = keys - tokens;
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4, col = lane & 15;
+    const bool there = col < rows;
+    const int row = min(col, rows - 1);
+    const int token = a.by_group.div(row), head = g * a.group + row - token * a.group;
+    const int position = position0 + token;
+
+    const KeyTiles tiles = key_tiles<kKeys>(position0, position0 + tokens - 1, keys, a.window, a.sinks);
+    int first = 0, end = tiles.count;
+    if constexpr (SPLIT) {
+        const int each = ((tiles.count + a.splits - 1) / a.splits + 3) / 4 * 4;
+        first = min(split * each, tiles.count);
+        end = min(first + each, tiles.count);
+    }
+
+    // dim of the first element of step s's (first half of the) operand
+    auto dim_of = [&](int s) { return kCodes ? 64 * s + 16 * quad : 32 * s + 8 * quad; };
+    u32x4 q[kCodes ? 2 * kLoads : kLoads];
+    {
+        const char* p = a.q + ((int64_t)(token0 + token) * a.q_st[0] + (int64_t)head * a.q_st[2]) * 2;
+#pragma unroll
+        for (int s = 0; s < kLoads; ++s) {
+#pragma unroll
+            for (int t = 0; t < (kCodes ? 2 : 1); ++t) {
+                const int dim = dim_of(s) + 8 * t;
+                u32x4 x = load8(p + dim * 2, there && dim < a.d);
+                x ^= a.flip;
+                q[kCodes ? 2 * s + t : s] = x;
+            }
+        }
+    }
+
+    char* const vt = lds + wave * kWaveBytes;
+    const int32_t* const table = a.table + (int64_t)b * a.table_stride;
+    u32x4 kw[2][kLoads], vw[kValueLoads];
+    float k_scale = 0.f, v_scale = 0.f;
+    auto look_up = [&](int i) {  // lane l: the page of key l % 32 of the wave's block i
+        const int key = tiles.tile(i) * kKeys + (lane & 31);
+        return i < end && key < keys ? table[a.by_page.div(key)] : -1;
+    };
+    auto fetch = [&](int i, int page) {
+        const int key = tiles.tile(i) * kKeys + (lane & 31);
+        const bool ok = (uint64_t)(int64_t)page < (uint64_t)a.pages;
+        const int in = a.by_page.mod(key);
+        const int64_t k_at = ok ? (int64_t)page * a.k_st[1] + in * a.k_st[0] + (int64_t)g * a.k_st[2] : -1;
+        const int64_t v_at = ok ? (int64_t)page * a.v_st[1] + in * a.v_st[0] + (int64_t)g * a.v_st[2] : -1;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const int64_t at = __shfl(k_at, 16 * kb + col);
+#pragma unroll
+            for (int s = 0; s < kLoads; ++s)
+                kw[kb][s] = load8(a.k + (at + dim_of(s)) * kBytes, at >= 0 && dim_of(s) < a.d);
+        }
+#pragma unroll
+        for (int s = 0; s < kValueLoads; ++s) {
+            const int r = s * kRowsAtOnce + lane / kPerRow, dim = lane % kPerRow * (16 / kBytes);
+            const int64_t at = __shfl(v_at, r & 31);
+            vw[s] = load8(a.v + (at + dim) * kBytes, at >= 0 && r < kKeys && lane < kRowsAtOnce * kPerRow && dim < a.d);
+        }
+        if constexpr (kCodes) {
+            k_scale = v_scale = 0.f;
+            if (ok) {
+                k_scale = a.k_scale[page * a.ks_st[1] + in * a.ks_st[0] + (int64_t)g * a.ks_st[2]];
+                v_scale = a.v_scale[page * a.vs_st[1] + in * a.vs_st[0] + (int64_t)g * a.vs_st[2]];
+            }
+        }
+    };
+
+    f32x4 acc[DP / 16];
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = kNegInf, l = 0.f;
+
+    int page = look_up(first + wave);
+    if (first + wave < end) fetch(first + wave, page);
+    page = look_up(first + wave + 4);
+    for (int i = first + wave; i < end; i += 4) {
+        const int key0 = tiles.tile(i) * kKeys;
+        f32x4 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < kLoads; ++st) {
+                if constexpr (kCodes) {
+                    s[kb] = Mma<T>::op16(widen8<T, SRC>(u32x2{kw[kb][st].x, kw[kb][st].y}), q[2 * st], s[kb]);
+                    s[kb] = Mma<T>::op16(widen8<T, SRC>(u32x2{kw[kb][st].z, kw[kb][st].w}), q[2 * st + 1], s[kb]);
+                } else {
+                    s[kb] = Mma<T>::op16(kw[kb][st], q[st], s[kb]);
+                }
+            }
+        }
+#pragma unroll
+        for (int st = 0; st < kValueLoads; ++st) {
+            const int r = st * kRowsAtOnce + lane / kPerRow, part = lane % kPerRow;
+            if (r < kKeys && lane < kRowsAtOnce * kPerRow) {
+                if constexpr (kCodes) {
+                    *reinterpret_cast<u32x4*>(vt + Tile<DP>::at(r, 2 * part)) = widen8<T, SRC>(u32x2{vw[st].x, vw[st].y});
+                    *reinterpret_cast<u32x4*>(vt + Tile<DP>::at(r, 2 * part + 1)) = widen8<T, SRC>(u32x2{vw[st].z, vw[st].w});
+                } else {
+                    *reinterpret_cast<u32x4*>(vt + Tile<DP>::at(r, part)) = vw[st];
+                }
+            }
+        }
+        if constexpr (kCodes) {
+            scales[wave][0][lane & 31] = k_scale;
+            scales[wave][1][lane & 31] = v_scale;
+        }
+        if (i + 4 < end) {
+            fetch(i + 4, page);
+            page = look_up(i + 8);
+        }
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (kCodes) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[kb] *= *reinterpret_cast<const f32x4*>(&scales[wave][0][16 * kb + 4 * quad]);
+        }
+        const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
+        float top = kNegInf;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = key0 + 16 * kb + 4 * quad + r;
+                const bool sees = key <= hi && (key >= lo || key < a.sinks);
+                s[kb][r] = sees ? s[kb][r] * a.scale_log2 : kNegInf;
+                top = fmaxf(top, s[kb][r]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = both_halves_max(top);
+        if (__any(top > m + 8.f)) {
+            const float higher = fmaxf(m, top);
+            const float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
+            m = higher;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < DP / 16; ++j) acc[j] *= f;
+        }
+        const float base = m == kNegInf ? 0.f : m;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[kb][r] = __builtin_amdgcn_exp2f(s[kb][r] - base);
+                l += s[kb][r];
+            }
+        if constexpr (kCodes) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const f32x4 c = *reinterpret_cast<const f32x4*>(&scales[wave][1][16 * kb + 4 * quad]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[kb][r] = s[kb][r] != 0.f ? s[kb][r] * c[r] : 0.f;
+            }
+        }
+        const u32x4 p = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
+                         Elem<T>::pack(s[1][0], s[1][1]), Elem<T>::pack(s[1][2], s[1][3])};
+        typedef __attribute__((address_space(3))) s16x4 lds4;
+        const uint32_t j = lane & 15, r = 4 * quad + (j >> 2), sub = (j >> 1) & 1, bytes = (j & 1) * 8;
+#pragma unroll
+        for (int db = 0; db < DP / 16; ++db) {
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vt + Tile<DP>::at(r, 2 * db + sub) + bytes));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vt + Tile<DP>::at(r + 16, 2 * db + sub) + bytes));
+            const u32x2 u = __builtin_bit_cast(u32x2, x), v = __builtin_bit_cast(u32x2, y);
+            acc[db] = Mma<T>::op16(u32x4{u.x, u.y, v.x, v.y}, p, acc[db]);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // the four waves' results: rows of DP values in each wave's own LDS, joined by the whole workgroup
+    l += __shfl_xor(l, 16);
+    l = both_halves_sum(l);
+    float* const mine = reinterpret_cast<float*>(vt);
+#pragma unroll
+    for (int db = 0; db < DP / 16; ++db) *reinterpret_cast<f32x4*>(mine + col * DP + 16 * db + 4 * quad) = acc[db];
+    if (quad == 0) {
+        wave_m[wave][col] = m;
+        wave_l[wave][col] = l;
+    }
+    __syncthreads();
+    for (int at = threadIdx.x * 8; at < rows * DP; at += 256 * 8) {
+        const int r = at / DP, dim = at % DP;
+        if (dim >= a.d) continue;
+        float high = wave_m[0][r];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) high = fmaxf(high, wave_m[w][r]);
+        const float base = high == kNegInf ? 0.f : high;
+        float total = 0.f, x[8] = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(wave_m[w][r] - base);
+            total += wave_l[w][r] * f;
+            const float* from = reinterpret_cast<const float*>(lds + w * kWaveBytes) + r * DP + dim;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] += from[e] * f;
+        }
+        const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= inverse;
+        const int t = a.by_group.div(r), h = g * a.group + r - t * a.group;
+        if constexpr (SPLIT) {
+            const int64_t slot = (int64_t)split * a.part_rows + (int64_t)(token0 + t) * a.kv * a.group + h;
+            float* p = a.part_o + slot * a.d + dim;
+            *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+            if (dim == 0) a.part_lse[slot] = total == 0.f ? kNegInf : high + __builtin_amdgcn_logf(total);
+        } else {
+            *reinterpret_cast<u32x4*>(a.o + ((int64_t)(token0 + t) * a.o_st[0] + (int64_t)h * a.o_st[2] + dim) * 2) = pack8<T>(x);
+        }
+    }
+}
+
+// Joins the parts of a split key axis: a wave per row, lane l the dims 4 l .. of it.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    const int64_t slot = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (slot >= a.part_rows) return;
+    const int lane = threadIdx.x & 63;
+    float high = kNegInf;
+    for (int s = lane; s < a.splits; s += 64) high = fmaxf(high, a.part_lse[s * a.part_rows + slot]);
+    for (int x = 1; x < 64; x *= 2) high = fmaxf(high, __shfl_xor(high, x));
+    const float base = high == kNegInf ? 0.f : high;
+    const int dim = lane * 4;
+    float total = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t at = s * a.part_rows + slot;
+        const float f = __builtin_amdgcn_exp2f(a.part_lse[at] - base);
+        total += f;
+        if (dim < a.d) sum += *reinterpret_cast<const f32x4*>(a.part_o + at * a.d + dim) * f;
+    }
+    const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+    if (dim < a.d) {
+        const int64_t token = slot / (a.kv * a.group), head = slot - token * (a.kv * a.group);
+        const u32x2 w = {Elem<T>::pack(sum[0] * inverse, sum[1] * inverse), Elem<T>::pack(sum[2] * inverse, sum[3] * inverse)};
+        *reinterpret_cast<u32x2*>(a.o + (token * a.o_st[0] + head * a.o_st[2] + dim) * 2) = w;
+    }
+}
+
+// ---- backward: the queries' gradient, and the rows' sums of dO * O -----------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
+    constexpr int kTile = kTileKeys * Tile<DP>::kRow;
+    constexpr int kBuffers = DP <= 128 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) char lds[kBuffers * 2 * kTile];
+
+    const uint32_t block = blockIdx.x, heads = a.b * a.kv;
+    uint32_t bh, mt;
+    if (heads % 8 == 0) {
+        const uint32_t xcd = block & 7, k = block >> 3, part = a.by_row_tiles.div(k);
+        bh = part * 8 + xcd;
+        mt = k - part * a.row_tiles;
+    } else {
+        bh = a.by_row_tiles.div(block);
+        mt = block - bh * a.row_tiles;
+    }
+    mt = a.row_tiles - 1 - mt;
+    const int b = a.by_kv.div(bh), g = bh - b * a.kv;
+    const int keys = a.lengths ? max(0, min(a.lengths[b], a.sk)) : a.sk, position0 = a.sk - a.sq;
+    const int rows = a.sq * a.group, row0 = mt * kTileRows;
+
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+    const int row = row0 + wave * 32 + (lane & 31);
+    const bool there = row < rows;
+    const int token = a.by_group.div(min(row, rows - 1)), head = g * a.group + (min(row, rows - 1) - token * a.group);
+    const int position = position0 + token;
+    const int wg_first = position0 + (int)a.by_group.div(row0), wg_last = position0 + (int)a.by_group.div(min(row0 + kTileRows, rows) - 1);
+    const int wv_first = __builtin_amdgcn_readfirstlane(position0 + (int)a.by_group.div(min(row0 + wave * 32, rows - 1)));
+    const int wv_last = __builtin_amdgcn_readfirstlane(position0 + (int)a.by_group.div(min(row0 + wave * 32 + 32, rows) - 1));
+    const bool wave_works = row0 + wave * 32 < rows;
+    const KeyTiles tiles = key_tiles<kTileKeys>(wg_first, wg_last, keys, a.window, a.sinks);
+
+    u32x4 q[DP / 16], dout[DP / 16];
+    float delta = 0.f, lse = __builtin_inff();
+    {
+        const char* qp = a.q + ((int64_t)token * a.q_st[0] + (int64_t)b * a.q_st[1] + (int64_t)head * a.q_st[2]) * 2;
+        const char* dp = a.dout + ((int64_t)token * a.do_st[0] + (int64_t)b * a.do_st[1] + (int64_t)head * a.do_st[2]) * 2;
+        const char* op = a.out + ((int64_t)token * a.o_st[0] + (int64_t)b * a.o_st[1] + (int64_t)head * a.o_st[2]) * 2;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int dim = 16 * s + 8 * half;
+            const bool ok = there && dim < a.d;
+            q[s] = load8(qp + dim * 2, ok);
+            dout[s] = load8(dp + dim * 2, ok);
+            float x[8], y[8];
+            unpack8<T>(dout[s], x);
+            unpack8<T>(load8(op + dim * 2, ok), y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+        }
+        delta = both_halves_sum(delta);
+        if (there) {
+            lse = a.lse[(int64_t)bh * rows + row];
+            if (half == 0) a.delta[(int64_t)bh * rows + row] = delta;
+        }
+    }
+
+    typedef Stage<T, DP, kStrided, kTileKeys> St;
+    St ks, vs;
+    const int piece = St::piece();
+    const bool dims_there = piece * 8 < a.d;
+    const char* const kbase = a.k + ((int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2] + piece * 8) * 2;
+    const char* const vbase = a.v + ((int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2] + piece * 8) * 2;
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int s = 0; s < St::kSteps; ++s) {
+            const int key = tile * kTileKeys + St::row(s);
+            const bool ok = St::works(s) && key < keys && dims_there;
+            ks.load(s, kbase + (int64_t)key * a.k_st[0] * 2, ok);
+            vs.load(s, vbase + (int64_t)key * a.v_st[0] * 2, ok);
+        }
+    };
+    auto put = [&](int buffer) {
+        ks.put(lds + buffer * 2 * kTile);
+        vs.put(lds + buffer * 2 * kTile + kTile);
+    };
+
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    const float scale_log2 = a.scale * kLog2e;
+
+    if (tiles.count) {
+        fetch(tiles.tile(0));
+        put(0);
+    }
+    __syncthreads();
+    for (int it = 0; it < tiles.count; ++it) {
+        const int buffer = kBuffers == 2 ? it & 1 : 0;
+        char* const kt = lds + buffer * 2 * kTile;
+        char* const vt = kt + kTile;
+        const int key0 = tiles.tile(it) * kTileKeys;
+        if (it + 1 < tiles.count) fetch(tiles.tile(it + 1));
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const int k0 = key0 + 32 * kb, k1 = k0 + 32;
+            const bool none = !wave_works || k0 > wv_last || k0 >= keys ||
+                              (a.window >= 0 && k1 - 1 < wv_first - a.window && k0 >= a.sinks);
+            const bool all = k1 - 1 <= wv_first && k1 <= keys &&
+                             (a.window < 0 || k0 >= wv_last - a.window || k1 <= a.sinks);
+            if (none) continue;
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(row_operand<DP>(kt, 32 * kb, st), q[st], s);
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(row_operand<DP>(vt, 32 * kb, st), dout[st], dp);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -lse)) * (dp[r] - delta);
+            if (!all) {
+                const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = k0 + element_of(r, half);
+                    s[r] = key <= hi && (key >= lo || key < a.sinks) ? s[r] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                u32x4 p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(turned_operand<DP>(kt, 32 * kb + 16 * t, i), p, acc[i]);
+            }
+        }
+        if (it + 1 < tiles.count) {
+            if constexpr (kBuffers == 1) __syncthreads();
+            put(kBuffers == 2 ? buffer ^ 1 : 0);
+        }
+        __syncthreads();
+    }
+    char* p = a.dq + ((int64_t)token * a.dq_st[0] + (int64_t)b * a.dq_st[1] + (int64_t)head * a.dq_st[2]) * 2;
+    store_rows<T, DP>(p, acc, a.scale, a.d, there);
+}
+
+// ---- backward: the gradients of keys and values -------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
+    constexpr int kTile = kStepRows * Tile<DP>::kRow;
+    __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTile];
+    __shared__ __attribute__((aligned(16))) float row_lse[2][kStepRows], row_delta[2][kStepRows];
+    __shared__ __attribute__((aligned(16))) int row_at[2][kStepRows];
+
+    const uint32_t block = blockIdx.x, heads = a.b * a.kv;
+    uint32_t bh, kt;
+    if (heads % 8 == 0) {
+        const uint32_t xcd = block & 7, k = block >> 3, part = a.by_key_tiles.div(k);
+        bh = part * 8 + xcd;
+        kt = k - part * a.key_tiles;
+    } else {
+        bh = a.by_key_tiles.div(block);
+        kt = block - bh * a.key_tiles;
+    }
+    const int b = a.by_kv.div(bh), g = bh - b * a.kv;
+    const int keys = a.lengths ? max(0, min(a.lengths[b], a.sk)) : a.sk, position0 = a.sk - a.sq;
+    const int rows = a.sq * a.group, key0 = kt * kGradKeys;
+
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+    const int key = key0 + wave * 32 + (lane & 31);
+    const int wv_first = __builtin_amdgcn_readfirstlane(key0 + wave * 32), wv_last = wv_first + 31;
+
+    // the rows that see some key of the tile: those at its first position and behind, to the end of the window
+    int row_begin = 0, row_end = 0;
+    if (key0 < keys) {
+        const int last = min(key0 + kGradKeys, keys) - 1;
+        const int t0 = max(0, key0 - position0);
+        const int t1 = (a.window < 0 || key0 < a.sinks) ? a.sq : min((int64_t)a.sq, (int64_t)last + a.window - position0 + 1);
+        row_begin = min(t0, a.sq) * a.group;
+        row_end = max(t1, 0) * a.group;
+    }
+
+    u32x4 kreg[DP / 16], vreg[DP / 16];
+    {
+        const char* kp = a.k + ((int64_t)key * a.k_st[0] + (int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2]) * 2;
+        const char* vp = a.v + ((int64_t)key * a.v_st[0] + (int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2]) * 2;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int dim = 16 * s + 8 * half;
+            kreg[s] = load8(kp + dim * 2, key < keys && dim < a.d);
+            vreg[s] = load8(vp + dim * 2, key < keys && dim < a.d);
+        }
+    }
+
+    typedef Stage<T, DP, kStrided, kStepRows> St;
+    St qs, ds;
+    const int piece = St::piece();
+    const bool dims_there = piece * 8 < a.d;
+    const char* const qbase = a.q + ((int64_t)b * a.q_st[1] + (int64_t)g * a.group * a.q_st[2] + piece * 8) * 2;
+    const char* const dbase = a.dout + ((int64_t)b * a.do_st[1] + (int64_t)g * a.group * a.do_st[2] + piece * 8) * 2;
+    float lse = 0.f, delta = 0.f;
+    auto fetch = [&](int row0) {
+#pragma unroll
+        for (int s = 0; s < St::kSteps; ++s) {
+            const int row = row0 + St::row(s);
+            const bool ok = St::works(s) && row < row_end && dims_there;
+            const int token = a.by_group.div(row), h = row - token * a.group;
+            qs.load(s, qbase + ((int64_t)token * a.q_st[0] + (int64_t)h * a.q_st[2]) * 2, ok);
+            ds.load(s, dbase + ((int64_t)token * a.do_st[0] + (int64_t)h * a.do_st[2]) * 2, ok);
+        }
+        if (threadIdx.x < kStepRows) {
+            const int row = row0 + (int)threadIdx.x;
+            lse = row < row_end ? a.lse[(int64_t)bh * rows + row] : __builtin_inff();
+            delta = row < row_end ? a.delta[(int64_t)bh * rows + row] : 0.f;
+        }
+    };
+    auto put = [&](int buffer, int row0) {
+        qs.put(lds + buffer * 2 * kTile);
+        ds.put(lds + buffer * 2 * kTile + kTile);
+        if (threadIdx.x < kStepRows) {
+            row_lse[buffer][threadIdx.x] = lse;
+            row_delta[buffer][threadIdx.x] = delta;
+            row_at[buffer][threadIdx.x] = position0 + (int)a.by_group.div(row0 + threadIdx.x);
+        }
+    };
+
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
+    const float scale_log2 = a.scale * kLog2e;
+
+    if (row_begin < row_end) {
+        fetch(row_begin);
+        put(0, row_begin);
+    }
+    __syncthreads();
+    int buffer = 0;
+    for (int row0 = row_begin; row0 < row_end; row0 += kStepRows, buffer ^= 1) {
+        char* const qt = lds + buffer * 2 * kTile;
+        char* const dt = qt + kTile;
+        if (row0 + kStepRows < row_end) fetch(row0 + kStepRows);
+        const int at_first = position0 + (int)a.by_group.div(row0);
+        const int at_last = position0 + (int)a.by_group.div(min(row0 + kStepRows, row_end) - 1);
+        const bool none = at_last < wv_first || wv_first >= keys ||
+                          (a.window >= 0 && wv_last < at_first - a.window && wv_first >= a.sinks);
+        const bool all = at_first >= wv_last && wv_last < keys &&
+                         (a.window < 0 || wv_first >= at_last - a.window || wv_last < a.sinks);
+        if (!none) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(row_operand<DP>(qt, 0, st), kreg[st], s);
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_lse[buffer][8 * (r >> 2) + 4 * half]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[r + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + i], scale_log2, -c[i]));
+            }
+            if (!all) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int at = row_at[buffer][element_of(r, half)];
+                    const bool sees = key < keys && at >= key && (a.window < 0 || key >= at - a.window || key < a.sinks);
+                    s[r] = sees ? s[r] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(row_operand<DP>(dt, 0, st), vreg[st], dp);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                u32x4 p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(turned_operand<DP>(dt, 16 * t, i), p, dv[i]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_delta[buffer][8 * (r >> 2) + 4 * half]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[r + i] *= dp[r + i] - c[i];
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                u32x4 p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) dk[i] = Mma<T>::op(turned_operand<DP>(qt, 16 * t, i), p, dk[i]);
+            }
+        }
+        if (row0 + kStepRows < row_end) put(buffer ^ 1, row0 + kStepRows);
+        __syncthreads();
+    }
+    const bool there = key < a.sk;
+    store_rows<T, DP>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2]) * 2, dk, a.scale, a.d, there);
+    store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, 1.f, a.d, there);
+}
+
+}  // namespace neox

@@ -7,11 +7,27 @@
 #include "../../include/neox_fused.h"
 #include "rope_kernels.hpp"
 #include "softmax_kernels.hpp"
+#include "cache_kernels.hpp"
 
 namespace neox {
 
 // Records a message for neox_fused_last_error() on this thread and returns `status`.
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+inline bool aligned(const void* p, uintptr_t n) {
+    return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
+}
+
+inline int check_launch(hipError_t e, const char* what) {
+    if (e == hipSuccess) return NEOX_OK;
+    return fail(NEOX_ERR_LAUNCH, "%s: kernel launch failed: %s", what, hipGetErrorString(e));
+}
+
+inline int check_dtype(int dtype, const char* what) {
+    if (dtype == NEOX_F16 || dtype == NEOX_BF16) return NEOX_OK;
+    return fail(NEOX_ERR_BAD_DTYPE, "%s: Only fp16 and bf16 are supported (dtype code %d)", what,
+                dtype);
+}
 
 // Launchers: pick the kernel shape for the row length and launch on `stream`.
 // `vec_ok` says that every row starts on a 16-byte boundary (sk % 8 == 0, pointers 16-byte
@@ -51,6 +67,26 @@ hipError_t launch_mask_classify(int32_t* record, int32_t* row_end, const uint8_t
 constexpr int kRopeAngles = -1;
 hipError_t launch_rope(const RopeArgs& a, int s, int n_outer, int w, int dtype, int cs_dtype,
                        bool backward, hipStream_t stream);
+
+// Attention: one translation unit per padded head dim (64, 96, 128, 256).
+template <int DP>
+hipError_t launch_attn_fwd(const AttnArgs& a, int source, int dtype, hipStream_t stream);
+template <int DP>
+hipError_t launch_attn_token(const AttnArgs& a, int source, int dtype, hipStream_t stream);
+template <int DP>
+hipError_t launch_attn_bwd(const AttnArgs& a, int dtype, hipStream_t stream);
+#define NEOX_ATTN_DIMS(X) X(64) X(96) X(128) X(256)
+#define NEOX_DECLARE_ATTN(DP)                                                          \
+    template <>                                                                        \
+    hipError_t launch_attn_fwd<DP>(const AttnArgs&, int, int, hipStream_t);            \
+    template <>                                                                        \
+    hipError_t launch_attn_token<DP>(const AttnArgs&, int, int, hipStream_t);          \
+    template <>                                                                        \
+    hipError_t launch_attn_bwd<DP>(const AttnArgs&, int, hipStream_t);
+NEOX_ATTN_DIMS(NEOX_DECLARE_ATTN)
+#undef NEOX_DECLARE_ATTN
+hipError_t launch_attn_join(const AttnArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_cache(const CacheArgs& a, int source, int dtype, bool write, hipStream_t stream);
 
 // Longest row the register-resident kernels take (16 waves x 4 chunks x 512 columns).
 constexpr int kMaxRegisterRow = 16 * 4 * kChunk;

@@ -29,18 +29,22 @@ extern "C" {
 /*
  * ABI versions.  A version is bumped when an entry point is added or its parameter list changes; the
  * Python binding refuses a library of another version.
+ *   5  + neox_window_attention_fwd/_bwd, neox_paged_attention, neox_paged_attention_workspace,
+ *      neox_cache_write, neox_cache_read
  *   4  + neox_mask_scan, neox_masked_softmax_ends_fwd, neox_masked_softmax_ends_bwd
  *   3  + neox_masked_softmax_alibi_fwd, neox_sliding_window_softmax_fwd/_bwd, neox_mask_classify;
  *      neox_*_softmax_bias_fwd and neox_masked_softmax_dropout_fwd take ALiBi slopes too
  *   2  + the dropout, bias and ALiBi entry points, neox_rope_apply_freqs
  *   1  the four softmax entry points, neox_rope_apply, neox_get_batch_per_block
  */
-#define NEOX_FUSED_ABI_VERSION 4
+#define NEOX_FUSED_ABI_VERSION 5
 
 typedef enum neox_dtype {
     NEOX_F16 = 0,  /* IEEE binary16 */
     NEOX_BF16 = 1, /* bfloat16 */
-    NEOX_F32 = 2   /* only valid for the rotary cos/sin tables */
+    NEOX_F32 = 2,  /* only valid for the rotary cos/sin tables */
+    NEOX_I8 = 3,   /* only valid for a paged cache: int8 codes */
+    NEOX_F8 = 4    /* only valid for a paged cache: 8-bit floats, e4m3 without infinities */
 } neox_dtype;
 
 typedef enum neox_status {
@@ -339,6 +343,80 @@ int neox_rope_apply_freqs(void* out_q, void* out_k, const void* q, const void* k
                           const int64_t out_q_strides[3], const int64_t out_k_strides[3],
                           int64_t freqs_stride, int32_t pos_offset, int32_t dtype, int32_t backward,
                           void* stream);
+
+/*
+ * Attention without stored scores, over a window of keys and the first few (sinks).
+ *   out = softmax_j(scale * q . k_j) v over the keys j that the query sees
+ * Query i stands at position p = i + sk - sq and sees key j if j <= p, j < key_lengths[sample], and
+ * j >= p - window (the rule of neox_sliding_window_softmax_fwd) or j < sinks.  window < 0: no window.
+ * A query that sees no key gets zeros, and passes no gradient on.  q, out: [sq, b, h, d], k, v:
+ * [sk, b, h_kv, d], addressed by the element strides {token, sample, head}, the last axis dense; query head x
+ * uses key head x / (h / h_kv).  d: a multiple of 8, at most 256; every stride a multiple of 8 elements
+ * and every pointer 16-byte aligned.  key_lengths: int32 [b] in device memory, or NULL for sk keys
+ * everywhere; keys and values behind a length, or behind the window of every query of a tile, are not
+ * looked at.  (A value that is infinite or NaN reaches the queries of its own tile -- 64 keys, 128
+ * query rows -- also where the mask hides it.)  lse, fp32 [b * h * sq]: what the backward pass
+ * needs, in an order of its own (NULL: not wanted).  fp32 arithmetic on the matrix cores' 16-bit
+ * products; the probabilities are rounded to the 16-bit type before they meet the values.
+ * Backward: dk and dv are summed over the query heads of their key head in a fixed order; delta, fp32
+ * [b * h * sq], is scratch.  The gradients may not alias anything else.
+ * Takes the place of the flash-attention path
+ *   megatron/model/transformer.py:573-690
+ */
+int neox_window_attention_fwd(void* out, float* lse, const void* q, const void* k, const void* v, const int32_t* key_lengths,
+                              int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d,
+                              const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                              const int64_t out_strides[3], float scale, int32_t window, int32_t sinks, int32_t dtype,
+                              void* stream);
+int neox_window_attention_bwd(void* dq, void* dk, void* dv, float* delta, const void* dout, const void* out,
+                              const float* lse, const void* q, const void* k, const void* v, const int32_t* key_lengths,
+                              int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d,
+                              const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
+                              const int64_t dout_strides[3], const int64_t out_strides[3], const int64_t q_strides[3],
+                              const int64_t k_strides[3], const int64_t v_strides[3], float scale, int32_t window,
+                              int32_t sinks, int32_t dtype, void* stream);
+
+/*
+ * A paged cache of keys and values: pages of page_size tokens, [pages, page_size, h_kv, d] by the element
+ * strides {page, token, head}, the last axis dense, holding 16-bit values (cache_dtype == dtype) or 8-bit codes
+ * (NEOX_I8, NEOX_F8; d a multiple of 16, strides of 16) with an fp32 scale for each token and head in
+ * k_scales, v_scales (NULL for 16 bits): value = code * scale, scale = largest |value| / 127 (448), code =
+ * the value / scale rounded to nearest even.  A row that holds an infinity or a NaN reads back as NaN.
+ * slots: int32 or int64 [tokens] in device memory, slot = page * page_size + token in the page.
+ * write: k, v [tokens, h_kv, d] by strides {token, head} into their slots; a slot outside the cache is
+ * skipped, and no slot may be named twice.  read: the reverse; a slot outside the cache reads as zeros.
+ */
+int neox_cache_write(void* k_cache, void* v_cache, float* k_scales, float* v_scales, const void* k, const void* v,
+                     const void* slots, int32_t slots_64, int64_t tokens, int32_t h_kv, int32_t d, int64_t pages,
+                     int32_t page_size, const int64_t k_cache_strides[3], const int64_t v_cache_strides[3],
+                     const int64_t k_scale_strides[3], const int64_t v_scale_strides[3], const int64_t k_strides[2],
+                     const int64_t v_strides[2], int32_t dtype, int32_t cache_dtype, void* stream);
+int neox_cache_read(void* k, void* v, const void* k_cache, const void* v_cache, const float* k_scales,
+                    const float* v_scales, const void* slots, int32_t slots_64, int64_t tokens, int32_t h_kv, int32_t d,
+                    int64_t pages, int32_t page_size, const int64_t k_strides[2], const int64_t v_strides[2],
+                    const int64_t k_cache_strides[3], const int64_t v_cache_strides[3], const int64_t k_scale_strides[3],
+                    const int64_t v_scale_strides[3], int32_t dtype, int32_t cache_dtype, void* stream);
+
+/*
+ * Attention of the newest tokens of every sequence over its pages of such a cache, in which they are already.
+ * q, out: [tokens, h, d] by strides {token, head}, the sequences one behind the other: sequence s has the
+ * tokens query_starts[s] .. query_starts[s + 1] (int32 [b + 1]) and, those included, context_lengths[s]
+ * keys (int32 [b]), key j in page page_table[s * table_stride + j / page_size].  The last token stands at
+ * the last key; window and sinks as in neox_window_attention_fwd.  All three tables are in device memory
+ * and looked at by the kernels only: max_query and max_context, on the host, must be at least the longest of
+ * them (what goes beyond is not computed), and a page outside [0, pages) counts as zeros.  workspace: as many
+ * bytes as neox_paged_attention_workspace says for the same sizes (0: NULL will do).
+ */
+int neox_paged_attention_workspace(int64_t* bytes, int32_t b, int32_t tokens, int32_t max_query, int32_t max_context,
+                                   int32_t h, int32_t h_kv, int32_t d, int32_t window, int32_t sinks);
+int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, const void* q, const void* k_cache,
+                         const void* v_cache, const float* k_scales, const float* v_scales, const int32_t* page_table,
+                         const int32_t* query_starts, const int32_t* context_lengths, int32_t b, int32_t tokens,
+                         int32_t max_query, int32_t max_context, int32_t h, int32_t h_kv, int32_t d, int64_t pages,
+                         int32_t page_size, int32_t table_columns, int64_t table_stride, const int64_t out_strides[2],
+                         const int64_t q_strides[2], const int64_t k_cache_strides[3], const int64_t v_cache_strides[3],
+                         const int64_t k_scale_strides[3], const int64_t v_scale_strides[3], float scale, int32_t window,
+                         int32_t sinks, int32_t dtype, int32_t cache_dtype, void* stream);
 
 #ifdef __cplusplus
 }
