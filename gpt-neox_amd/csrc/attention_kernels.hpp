@@ -32,6 +32,12 @@ constexpr int kTileRows = 128;  // rows of a workgroup there: 32 for each of its
 constexpr int kStepRows = 32;   // rows of one step of the key-gradient kernel
 constexpr int kGradKeys = 128;  // keys of a workgroup there: 32 for each of its four waves
 
+// p + i * bytes + j * more, one instruction for each product (strides are below 2^31 elements, which the entry
+// points see to)
+__device__ __forceinline__ const char* step_to(const char* p, uint32_t i, uint32_t bytes) {
+    return reinterpret_cast<const char*>((uint64_t)i * bytes + reinterpret_cast<uint64_t>(p));
+}
+
 // where keys and values come from
 enum KvSource { kStrided = 0, kPaged16 = 1, kPagedI8 = 2, kPagedF8 = 3 };
 
@@ -113,26 +119,36 @@ struct Tile {
     }
 };
 
-// Operand of 32 tile rows (row0 ..) and the 16 dims of step s, row-major: lane l has row l % 32, dims 8 (l / 32) ..
+// Where in LDS the lanes of a wave find the operands of a tile at byte `at` of LDS.  Of the permuted address only
+// an exclusive or with a constant changes from operand to operand, so two registers serve a whole tile; they are hidden
+// from the compiler, which would otherwise keep an address for every operand in a register of its own.
 template <int DP>
-__device__ __forceinline__ u32x4 row_operand(const char* tile, int row0, int s) {
-    const uint32_t lane = threadIdx.x & 63;
-    return *reinterpret_cast<const u32x4*>(tile + Tile<DP>::at(row0 + (lane & 31), 2 * s + (lane >> 5)));
-}
-
-// Operand of the 32 dims from 32 * db and the 16 tile rows from row0, transposed: lane l has dim l % 32 and, in
-// slot e, row row0 + 8 (e / 4) + 4 (l / 32) + e % 4.
-template <int DP>
-__device__ __forceinline__ u32x4 turned_operand(char* tile, int row0, int db) {
-    const uint32_t lane = threadIdx.x & 63, i = lane & 15;
-    const uint32_t row = row0 + 4 * (lane >> 5) + (i >> 2);
-    const uint32_t piece = 4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
-    const uint32_t half = (i & 1) * 8;
-    typedef __attribute__((address_space(3))) s16x4 lds4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + Tile<DP>::at(row, piece) + half));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + Tile<DP>::at(row + 8, piece) + half));
-    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
-    return u32x4{a.x, a.y, b.x, b.y};
+struct Operands {
+    uint32_t straight, turned;
+    __device__ __forceinline__ explicit Operands(uint32_t at) {
+        const uint32_t lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+        straight = at + (row * Tile<DP>::kRow | (Tile<DP>::turn(row) ^ half) << 4);
+        const uint32_t i = lane & 15, trow = 4 * half + (i >> 2);
+        turned = at + (trow * Tile<DP>::kRow | (Tile<DP>::turn(trow) ^ (2 * ((lane >> 4) & 1) + ((i >> 1) & 1))) << 4 | (i & 1) * 8);
+        asm("" : "+v"(straight), "+v"(turned));
+    }
+    // 32 tile rows from row0 and the 16 dims of step s, row-major: lane l has row l % 32, dims 8 (l / 32) ..
+    __device__ __forceinline__ u32x4 rows(int row0, int s) const {
+        typedef const __attribute__((address_space(3))) u32x4* from;
+        return *(from)(uintptr_t)((straight ^ (s << 5)) + row0 * Tile<DP>::kRow);
+    }
+    // 32 dims from 32 * db and 16 tile rows from row0, transposed: lane l has dim l % 32 and, in slot e, row
+    // row0 + 8 (e / 4) + 4 (l / 32) + e % 4.
+    __device__ __forceinline__ u32x4 columns(int row0, int db) const {
+        typedef __attribute__((address_space(3))) s16x4* from;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((from)(uintptr_t)((turned ^ (db << 6)) + row0 * Tile<DP>::kRow));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((from)(uintptr_t)((turned ^ (db << 6) ^ 32) + (row0 + 8) * Tile<DP>::kRow));
+        const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+        return u32x4{a.x, a.y, b.x, b.y};
+    }
+};
+__device__ __forceinline__ uint32_t lds_byte(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
 
 // The values of lane l and of lane l ^ 32, combined.  (The results go through integers of their own: a bit cast of
@@ -272,6 +288,31 @@ struct Stage {
         }
     }
 };
+
+// The same without registers in between: every lane names the 16 bytes that go to its place of the tile (256
+// threads, a wave 1 KiB at a time).  A lane without data copies nothing: its place keeps what it has, which is zeros
+// (clear()) or a row of an earlier tile.  The copies are in flight until landed().
+template <int DP, int ROWS>
+struct Flight {
+    static constexpr int kSteps = ROWS * Tile<DP>::kRow / 4096;
+    static_assert(kSteps * 4096 == ROWS * Tile<DP>::kRow, "whole steps");
+    static constexpr int kPlaces = Tile<DP>::kRow / 16;
+    static __device__ __forceinline__ uint32_t place(int step) { return step * 256 + threadIdx.x; }
+    static __device__ __forceinline__ int row(int step) { return (int)(place(step) / kPlaces); }
+    static __device__ __forceinline__ int piece(int step) { return (int)((place(step) % kPlaces) ^ Tile<DP>::turn(row(step))); }
+    static __device__ __forceinline__ void load(int step, const char* from, char* tile) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                         (__attribute__((address_space(3))) void*)(tile + step * 4096 + wave * 1024), 16, 0, 0);
+    }
+};
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int BYTES>
+__device__ __forceinline__ void clear(char* lds) {
+    static_assert(BYTES % 4096 == 0, "whole steps");
+#pragma unroll
+    for (int i = 0; i < BYTES / 4096; ++i) *reinterpret_cast<u32x4*>(lds + i * 4096 + threadIdx.x * 16) = u32x4{0, 0, 0, 0};
+}
 
 // ---- forward --------------------------------------------------------------------------------------------
 template <typename T, int DP, int SRC, bool SPLIT>
@@ -418,8 +459,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
 
     for (int it = first_tile; it < end_tile; ++it) {
         const int buffer = kBuffers == 2 ? (it - first_tile) & 1 : 0;
-        char* const kt = lds + buffer * 2 * kTile;
-        char* const vt = kt + kTile;
+        const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
         const int key0 = tiles.tile(it) * kTileKeys;
         if (it + 1 < end_tile) {
             fetch(tiles.tile(it + 1));
@@ -438,7 +478,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
-                for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<T>::op(row_operand<DP>(kt, 32 * kb, st), q[st], s[kb]);
+                for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s[kb]);
             }
             if constexpr (kCodes) {
                 const float* f = scales + buffer * 2 * kTileKeys;
@@ -507,7 +547,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[t >> 1][8 * (t & 1) + 2 * e], s[t >> 1][8 * (t & 1) + 2 * e + 1]);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(turned_operand<DP>(vt, 16 * t, i), p, acc[i]);
+                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(vt_ops.columns(16 * t, i), p, acc[i]);
             }
         }
         if (it + 1 < end_tile) {
@@ -896,8 +936,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
     __syncthreads();
     for (int it = 0; it < tiles.count; ++it) {
         const int buffer = kBuffers == 2 ? it & 1 : 0;
-        char* const kt = lds + buffer * 2 * kTile;
-        char* const vt = kt + kTile;
+        const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
         const int key0 = tiles.tile(it) * kTileKeys;
         if (it + 1 < tiles.count) fetch(tiles.tile(it + 1));
 #pragma unroll
@@ -910,13 +949,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
             if (none) continue;
             f32x16 s, dp;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+            for (int r = 0; r < 16; ++r) {
+                s[r] = 0.f;
+                dp[r] = -delta;
+            }
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(row_operand<DP>(kt, 32 * kb, st), q[st], s);
+            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s);
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(row_operand<DP>(vt, 32 * kb, st), dout[st], dp);
+            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(vt_ops.rows(32 * kb, st), dout[st], dp);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -lse)) * (dp[r] - delta);
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -lse)) * dp[r];
             if (!all) {
                 const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
 #pragma unroll
@@ -931,7 +973,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(turned_operand<DP>(kt, 32 * kb + 16 * t, i), p, acc[i]);
+                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(kt_ops.columns(32 * kb + 16 * t, i), p, acc[i]);
             }
         }
         if (it + 1 < tiles.count) {
@@ -949,8 +991,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
     constexpr int kTile = kStepRows * Tile<DP>::kRow;
     __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTile];
-    __shared__ __attribute__((aligned(16))) float row_lse[2][kStepRows], row_delta[2][kStepRows];
-    __shared__ __attribute__((aligned(16))) int row_at[2][kStepRows];
+    __shared__ __attribute__((aligned(16))) float row_sums[2][2][kStepRows];  // lse and delta of the tile's rows
 
     const uint32_t block = blockIdx.x, heads = a.b * a.kv;
     uint32_t bh, kt;
@@ -966,7 +1007,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
     const int keys = a.lengths ? max(0, min(a.lengths[b], a.sk)) : a.sk, position0 = a.sk - a.sq;
     const int rows = a.sq * a.group, key0 = kt * kGradKeys;
 
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
     const int key = key0 + wave * 32 + (lane & 31);
     const int wv_first = __builtin_amdgcn_readfirstlane(key0 + wave * 32), wv_last = wv_first + 31;
 
@@ -992,35 +1033,30 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         }
     }
 
-    typedef Stage<T, DP, kStrided, kStepRows> St;
-    St qs, ds;
-    const int piece = St::piece();
-    const bool dims_there = piece * 8 < a.d;
-    const char* const qbase = a.q + ((int64_t)b * a.q_st[1] + (int64_t)g * a.group * a.q_st[2] + piece * 8) * 2;
-    const char* const dbase = a.dout + ((int64_t)b * a.do_st[1] + (int64_t)g * a.group * a.do_st[2] + piece * 8) * 2;
-    float lse = 0.f, delta = 0.f;
-    auto fetch = [&](int row0) {
+    typedef Flight<DP, kStepRows> Fl;
+    const char* const qbase = a.q + ((int64_t)b * a.q_st[1] + (int64_t)g * a.group * a.q_st[2]) * 2;
+    const char* const dbase = a.dout + ((int64_t)b * a.do_st[1] + (int64_t)g * a.group * a.do_st[2]) * 2;
+    // half a wave each fetches the rows' lse and delta; rows behind the end see nothing
+    const float* const sums = half ? a.delta : a.lse;
+    auto fetch = [&](int row0, int buffer) {
 #pragma unroll
-        for (int s = 0; s < St::kSteps; ++s) {
-            const int row = row0 + St::row(s);
-            const bool ok = St::works(s) && row < row_end && dims_there;
-            const int token = a.by_group.div(row), h = row - token * a.group;
-            qs.load(s, qbase + ((int64_t)token * a.q_st[0] + (int64_t)h * a.q_st[2]) * 2, ok);
-            ds.load(s, dbase + ((int64_t)token * a.do_st[0] + (int64_t)h * a.do_st[2]) * 2, ok);
+        for (int s = 0; s < Fl::kSteps; ++s) {
+            const int row = row0 + Fl::row(s), piece = Fl::piece(s);
+            if (row < row_end && piece * 8 < a.d) {
+                const uint32_t token = a.by_group.div(row), h = row - token * a.group;
+                Fl::load(s, step_to(step_to(qbase + piece * 16, token, (uint32_t)a.q_st[0] * 2), h, (uint32_t)a.q_st[2] * 2),
+                         lds + buffer * 2 * kTile);
+                Fl::load(s, step_to(step_to(dbase + piece * 16, token, (uint32_t)a.do_st[0] * 2), h, (uint32_t)a.do_st[2] * 2),
+                         lds + buffer * 2 * kTile + kTile);
+            }
         }
-        if (threadIdx.x < kStepRows) {
-            const int row = row0 + (int)threadIdx.x;
-            lse = row < row_end ? a.lse[(int64_t)bh * rows + row] : __builtin_inff();
-            delta = row < row_end ? a.delta[(int64_t)bh * rows + row] : 0.f;
-        }
-    };
-    auto put = [&](int buffer, int row0) {
-        qs.put(lds + buffer * 2 * kTile);
-        ds.put(lds + buffer * 2 * kTile + kTile);
-        if (threadIdx.x < kStepRows) {
-            row_lse[buffer][threadIdx.x] = lse;
-            row_delta[buffer][threadIdx.x] = delta;
-            row_at[buffer][threadIdx.x] = position0 + (int)a.by_group.div(row0 + threadIdx.x);
+        if (wave == 0) {
+            const int row = row0 + (lane & 31);
+            if (row < row_end)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(sums + (int64_t)bh * rows + row),
+                                                 (__attribute__((address_space(3))) void*)row_sums[buffer], 4, 0, 0);
+            else
+                row_sums[buffer][half][lane & 31] = half ? 0.f : __builtin_inff();
         }
     };
 
@@ -1031,16 +1067,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
     const float scale_log2 = a.scale * kLog2e;
 
-    if (row_begin < row_end) {
-        fetch(row_begin);
-        put(0, row_begin);
-    }
+    clear<4 * kTile>(lds);
+    __syncthreads();
+    if (row_begin < row_end) fetch(row_begin, 0);
+    landed();
     __syncthreads();
     int buffer = 0;
     for (int row0 = row_begin; row0 < row_end; row0 += kStepRows, buffer ^= 1) {
-        char* const qt = lds + buffer * 2 * kTile;
-        char* const dt = qt + kTile;
-        if (row0 + kStepRows < row_end) fetch(row0 + kStepRows);
+        const Operands<DP> qt_ops(lds_byte(lds) + buffer * 2 * kTile), dt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
+        if (row0 + kStepRows < row_end) fetch(row0 + kStepRows, buffer ^ 1);
         const int at_first = position0 + (int)a.by_group.div(row0);
         const int at_last = position0 + (int)a.by_group.div(min(row0 + kStepRows, row_end) - 1);
         const bool none = at_last < wv_first || wv_first >= keys ||
@@ -1050,49 +1085,51 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         if (!none) {
             f32x16 s, dp;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(row_operand<DP>(qt, 0, st), kreg[st], s);
+            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(qt_ops.rows(0, st), kreg[st], s);
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_lse[buffer][8 * (r >> 2) + 4 * half]);
+                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_sums[buffer][0][8 * (r >> 2) + 4 * half]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[r + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + i], scale_log2, -c[i]));
             }
             if (!all) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int at = row_at[buffer][element_of(r, half)];
+                    const int at = position0 + (int)a.by_group.div(row0 + element_of(r, half));
                     const bool sees = key < keys && at >= key && (a.window < 0 || key >= at - a.window || key < a.sinks);
                     s[r] = sees ? s[r] : 0.f;
                 }
             }
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(row_operand<DP>(dt, 0, st), vreg[st], dp);
+            for (int r = 0; r < 16; r += 4) {  // dP - delta: the sum starts at -delta
+                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_sums[buffer][1][8 * (r >> 2) + 4 * half]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dp[r + i] = -c[i];
+            }
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(dt_ops.rows(0, st), vreg[st], dp);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 u32x4 p;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(turned_operand<DP>(dt, 16 * t, i), p, dv[i]);
+                for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(dt_ops.columns(16 * t, i), p, dv[i]);
             }
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_delta[buffer][8 * (r >> 2) + 4 * half]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[r + i] *= dp[r + i] - c[i];
-            }
+            for (int r = 0; r < 16; ++r) s[r] *= dp[r];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 u32x4 p;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) dk[i] = Mma<T>::op(turned_operand<DP>(qt, 16 * t, i), p, dk[i]);
+                for (int i = 0; i < DP / 32; ++i) dk[i] = Mma<T>::op(qt_ops.columns(16 * t, i), p, dk[i]);
             }
         }
-        if (row0 + kStepRows < row_end) put(buffer ^ 1, row0 + kStepRows);
+        landed();
         __syncthreads();
     }
     const bool there = key < a.sk;
