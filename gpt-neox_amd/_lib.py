@@ -97,8 +97,9 @@ SIGNATURES = {
     "neox_window_attention_fwd": (
         ctypes.c_int, [_vp] * 6 + [_i32] * 6 + [_c_i64p] * 4 + [_f32, _i32, _i32, _i32, _vp]
     ),
+    "neox_window_attention_bwd_workspace": (ctypes.c_int, [_c_i64p] + [_i32] * 8),
     "neox_window_attention_bwd": (
-        ctypes.c_int, [_vp] * 11 + [_i32] * 6 + [_c_i64p] * 8 + [_f32, _i32, _i32, _i32, _vp]
+        ctypes.c_int, [_vp] * 4 + [_i64] + [_vp] * 7 + [_i32] * 6 + [_c_i64p] * 8 + [_f32, _i32, _i32, _i32, _vp]
     ),
     "neox_paged_attention_workspace": (ctypes.c_int, [_c_i64p] + [_i32] * 9),
     "neox_paged_attention": (
@@ -313,7 +314,7 @@ def whole_pieces(t):
     if t.stride(-1) != 1 or t.data_ptr() % 16:
         return False
     for n, s in zip(t.shape[:-1], t.stride()[:-1]):
-        if n > 1 and (s % 8 or s < 0):
+        if n > 1 and (s % 8 or not 0 <= s < 2**31):
             return False
     return t.shape[-2] == 1 or t.stride(-2) >= t.shape[-1]
 

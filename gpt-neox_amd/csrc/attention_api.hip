@@ -50,6 +50,8 @@ static int check_strides(const int64_t* st, int n, int heads, int d, int unit, c
     if (!st) return fail(NEOX_ERR_NULL_POINTER, "%s: %s strides are null", what, name);
     for (int i = 0; i < n; ++i) {
         if (st[i] < 0) return fail(NEOX_ERR_BAD_STRIDE, "%s: %s stride[%d]=%lld is negative", what, name, i, (long long)st[i]);
+        if (st[i] >= (int64_t)1 << 31)
+            return fail(NEOX_ERR_BAD_STRIDE, "%s: %s stride[%d]=%lld is not below 2^31", what, name, i, (long long)st[i]);
         if (unit && st[i] % unit != 0)
             return fail(NEOX_ERR_BAD_STRIDE, "%s: %s stride[%d]=%lld is not a multiple of %d elements", what, name, i, (long long)st[i], unit);
     }
@@ -119,7 +121,7 @@ static int check_window_sizes(int b, int sq, int sk, int h, int h_kv, int d, con
         return fail(NEOX_ERR_BAD_SHAPE, "%s: b=%d sq=%d sk=%d must be at least 1 (and sq, sk below 2^30)", what, b, sq, sk);
     NEOX_TRY(check_heads(h, h_kv, d, what));
     const int64_t rows = (int64_t)sq * (h / h_kv), tiles = (rows + kTileRows - 1) / kTileRows, units = (int64_t)b * h_kv;
-    if (rows >= kMost || units * tiles >= kMost || units * (((int64_t)sk + 127) / 128) >= kMost)
+    if (rows >= kMost || units * tiles >= kMost || units * (((int64_t)sk + 127) / 128) * 128 >= kMost || sk > 65535 * 128)
         return fail(NEOX_ERR_BAD_SHAPE, "%s: b=%d sq=%d sk=%d h=%d is too large for one call", what, b, sq, sk, h);
     return NEOX_OK;
 }
@@ -133,12 +135,42 @@ static void set_window_sizes(AttnArgs& a, int b, int sq, int sk, int h, int h_kv
     a.d = d;
     a.splits = 1;
     a.row_tiles = (sq * a.group + kTileRows - 1) / kTileRows;
-    a.key_tiles = (sk + kGradKeys - 1) / kGradKeys;
     a.by_group = FastDiv::by((uint32_t)a.group);
     a.by_kv = FastDiv::by((uint32_t)h_kv);
     a.by_row_tiles = FastDiv::by((uint32_t)a.row_tiles);
-    a.by_key_tiles = FastDiv::by((uint32_t)a.key_tiles);
     a.by_page = FastDiv::by(1);
+}
+
+// how the key gradients' work is cut into pieces, and the scratch it needs: fp32 sums of pieces, then delta
+struct GradPlan {
+    int key_tiles, near_parts, sink_tiles, far_parts;
+    int64_t parts_bytes, bytes;
+};
+
+// Pieces of a tile's near rows: so many that two workgroups run on every CU, 256 rows or more for each.  Rows behind the
+// window of a tile that holds sinks come in pieces of 512 rows.
+static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int window, int sinks) {
+    GradPlan p{};
+    const int64_t group = h / h_kv, units = (int64_t)b * h_kv;
+    p.key_tiles = (sk + kGradKeys - 1) / kGradKeys;
+    const int64_t near = window < 0 ? sq : (int64_t)window + kGradKeys < sq ? (int64_t)window + kGradKeys : sq;
+    int64_t parts = (512 + units * p.key_tiles - 1) / (units * p.key_tiles);
+    if (parts > near * group / 256) parts = near * group / 256;
+    p.near_parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
+    const int64_t last = (sinks < sk ? sinks : sk);
+    // the last position whose window reaches the first tile is kGradKeys - 1 + window
+    const int64_t behind = window < 0 || last < 1 ? 0 : (int64_t)sk - kGradKeys - window;
+    if (behind > 0) {
+        p.sink_tiles = (int)((last + kGradKeys - 1) / kGradKeys);
+        const int64_t rows = (behind < sq ? behind : sq) * group;
+        const int64_t far = (rows + 511) / 512;
+        p.far_parts = far > 64 ? 64 : (int)far;
+    }
+    const bool cut = p.near_parts > 1 || p.far_parts > 0;
+    const int64_t pieces = (int64_t)p.key_tiles * p.near_parts + (int64_t)p.sink_tiles * p.far_parts;
+    p.parts_bytes = cut ? units * pieces * 2 * kGradKeys * d * (int64_t)sizeof(float) : 0;
+    p.bytes = p.parts_bytes + (int64_t)b * h * sq * (int64_t)sizeof(float);
+    return p;
 }
 
 // how a call over pages is cut: single tokens or row tiles, and how many parts of the key axis
@@ -301,7 +333,17 @@ int neox_window_attention_fwd(void* out, float* lse, const void* q, const void* 
     return check_launch(run_fwd(a, kStrided, dtype, (hipStream_t)stream), what);
 }
 
-int neox_window_attention_bwd(void* dq, void* dk, void* dv, float* delta, const void* dout, const void* out, const float* lse, const void* q,
+int neox_window_attention_bwd_workspace(int64_t* bytes, int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d, int32_t window,
+                                        int32_t sinks) {
+    static const char* what = "neox_window_attention_bwd_workspace";
+    if (!bytes) return fail(NEOX_ERR_NULL_POINTER, "%s: bytes is null", what);
+    NEOX_TRY(check_window_sizes(b, sq, sk, h, h_kv, d, what));
+    NEOX_TRY(check_scale_window(1.f, sinks, what));
+    *bytes = plan_grad(b, sq, sk, h, h_kv, d, window, sinks).bytes;
+    return NEOX_OK;
+}
+
+int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, const void* dout, const void* out, const float* lse, const void* q,
                               const void* k, const void* v, const int32_t* key_lengths, int32_t b, int32_t sq, int32_t sk, int32_t h,
                               int32_t h_kv, int32_t d, const int64_t dq_strides[3], const int64_t dk_strides[3],
                               const int64_t dv_strides[3], const int64_t dout_strides[3], const int64_t out_strides[3],
@@ -320,14 +362,27 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, float* delta, const 
                            {k, k_strides, true, "k"},           {v, v_strides, true, "v"}};
     for (const Given& g : given) NEOX_TRY(check_pointer(g.p, 16, what, g.name));
     NEOX_TRY(check_pointer(lse, 4, what, "lse"));
-    NEOX_TRY(check_pointer(delta, 4, what, "delta"));
+    NEOX_TRY(check_pointer(workspace, 16, what, "workspace"));
     if (!aligned(key_lengths, 4)) return fail(NEOX_ERR_MISALIGNED, "%s: misaligned pointer", what);
     NEOX_TRY(check_window_sizes(b, sq, sk, h, h_kv, d, what));
     for (const Given& g : given) NEOX_TRY(check_strides(g.st, 3, g.grouped ? h_kv : h, d, 8, what, g.name));
     NEOX_TRY(check_scale_window(scale, sinks, what));
+    const GradPlan plan = plan_grad(b, sq, sk, h, h_kv, d, window, sinks);
+    if (workspace_bytes < plan.bytes)
+        return fail(NEOX_ERR_BAD_SHAPE, "%s: workspace of %lld bytes, needs %lld", what, (long long)workspace_bytes, (long long)plan.bytes);
     AttnArgs a{};
     set_window_sizes(a, b, sq, sk, h, h_kv, d);
     set_scale_window(a, scale, window, sinks);
+    a.key_tiles = plan.key_tiles;
+    a.near_parts = plan.near_parts;
+    a.sink_tiles = plan.sink_tiles;
+    a.far_parts = plan.far_parts;
+    a.units = plan.key_tiles * plan.near_parts + plan.sink_tiles * plan.far_parts;
+    a.by_units = FastDiv::by((uint32_t)a.units);
+    a.by_near_parts = FastDiv::by((uint32_t)a.near_parts);
+    a.by_far_parts = FastDiv::by((uint32_t)(a.far_parts > 0 ? a.far_parts : 1));
+    a.part_o = static_cast<float*>(workspace);
+    a.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.parts_bytes);
     a.q = static_cast<const char*>(q);
     a.k = static_cast<const char*>(k);
     a.v = static_cast<const char*>(v);
@@ -337,7 +392,6 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, float* delta, const 
     a.dk = static_cast<char*>(dk);
     a.dv = static_cast<char*>(dv);
     a.lse = const_cast<float*>(lse);
-    a.delta = delta;
     a.lengths = key_lengths;
     copy_strides(a.q_st, q_strides);
     copy_strides(a.k_st, k_strides);

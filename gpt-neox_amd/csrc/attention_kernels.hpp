@@ -79,7 +79,11 @@ struct AttnArgs {
     float* delta;                // sum over d of dO * O of every row, [b, kv, rows]
     float scale;
     int key_tiles;
-    FastDiv by_key_tiles;
+    // The key-gradient kernel's work: every key tile's near rows (those whose window reaches it) in near_parts
+    // pieces; for the first sink_tiles tiles, the rows behind in far_parts pieces.  A tile in more than one piece
+    // leaves fp32 sums in part_o, [b, kv][piece][dk, dv][kGradKeys][d], far pieces for the keys below `sinks` only.
+    int near_parts, far_parts, sink_tiles, units;
+    FastDiv by_units, by_near_parts, by_far_parts;
 };
 
 template <typename T>
@@ -149,6 +153,11 @@ struct Operands {
 };
 __device__ __forceinline__ uint32_t lds_byte(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+// four floats at a byte of LDS (where a copy into another part of the same array may be in flight, which the compiler
+// would wait for if it knew the array)
+__device__ __forceinline__ f32x4 lds_floats(uint32_t at) {
+    return *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)at;
 }
 
 // The values of lane l and of lane l ^ 32, combined.  (The results go through integers of their own: a bit cast of
@@ -289,30 +298,30 @@ struct Stage {
     }
 };
 
-// The same without registers in between: every lane names the 16 bytes that go to its place of the tile (256
-// threads, a wave 1 KiB at a time).  A lane without data copies nothing: its place keeps what it has, which is zeros
-// (clear()) or a row of an earlier tile.  The copies are in flight until landed().
+// The same for 16-bit rows without registers in between: every lane names the 16 bytes that go to its place of the
+// tile (256 threads, a wave 1 KiB at a time), or writes zeros there.  The copies are in flight until landed().
 template <int DP, int ROWS>
 struct Flight {
     static constexpr int kSteps = ROWS * Tile<DP>::kRow / 4096;
     static_assert(kSteps * 4096 == ROWS * Tile<DP>::kRow, "whole steps");
     static constexpr int kPlaces = Tile<DP>::kRow / 16;
-    static __device__ __forceinline__ uint32_t place(int step) { return step * 256 + threadIdx.x; }
-    static __device__ __forceinline__ int row(int step) { return (int)(place(step) / kPlaces); }
-    static __device__ __forceinline__ int piece(int step) { return (int)((place(step) % kPlaces) ^ Tile<DP>::turn(row(step))); }
+    uint32_t thread = threadIdx.x;
+    // The compiler forgets where the thread's number came from: what follows from it is computed again for every tile
+    // and not kept in registers, which the accumulators need.
+    __device__ __forceinline__ void again() { asm("" : "+v"(thread)); }
+    __device__ __forceinline__ uint32_t place(int step) const { return step * 256 + thread; }
+    __device__ __forceinline__ int row(int step) const { return (int)(place(step) / kPlaces); }
+    __device__ __forceinline__ int piece(int step) const { return (int)((place(step) % kPlaces) ^ Tile<DP>::turn(row(step))); }
     static __device__ __forceinline__ void load(int step, const char* from, char* tile) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                          (__attribute__((address_space(3))) void*)(tile + step * 4096 + wave * 1024), 16, 0, 0);
     }
+    __device__ __forceinline__ void zero(int step, char* tile) const {
+        *reinterpret_cast<u32x4*>(tile + place(step) * 16) = u32x4{0, 0, 0, 0};
+    }
 };
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-template <int BYTES>
-__device__ __forceinline__ void clear(char* lds) {
-    static_assert(BYTES % 4096 == 0, "whole steps");
-#pragma unroll
-    for (int i = 0; i < BYTES / 4096; ++i) *reinterpret_cast<u32x4*>(lds + i * 4096 + threadIdx.x * 16) = u32x4{0, 0, 0, 0};
-}
 
 // ---- forward --------------------------------------------------------------------------------------------
 template <typename T, int DP, int SRC, bool SPLIT>
@@ -321,7 +330,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
     constexpr int kBytes = kCodes ? 1 : 2;
     constexpr int kTile = kTileKeys * Tile<DP>::kRow;
-    constexpr int kBuffers = DP <= 128 ? 2 : 1;  // (DP = 256: two tiles of 32 KiB each, one buffer)
+    constexpr int kBuffers = 2;
     __shared__ __attribute__((aligned(16))) char lds[kBuffers * 2 * kTile + (kCodes ? 2 * 2 * kTileKeys * 4 : 0)];
 
     // block -> (sample, key head), row tile, part: neighbours in time on one XCD (blocks go to the 8 XCDs in
@@ -384,18 +393,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
         }
     }
 
-    typedef Stage<T, DP, SRC, kTileKeys> St;
+    // One tile of keys and values into one of the buffers: 16-bit rows are copied there as they are; codes come through
+    // registers and are widened on the way, which put() does when the tile's turn is near.
+    typedef Stage<T, DP, kCodes ? SRC : kPagedI8, kTileKeys> St;
+    typedef Flight<DP, kTileKeys> Fl;
+    Fl fl;
+    constexpr int kSteps = kCodes ? St::kSteps : Fl::kSteps;
     St ks, vs;
-    const int piece = St::piece();
-    const bool dims_there = piece * 8 < a.d;
-    int page_of[kPages ? St::kSteps : 1];   // the pages of the next tile's rows, looked up one step ahead
-    int page_at = 0;                        // (the scales' row of this thread: its page)
+    auto row_of = [&](int s) { return kCodes ? St::row(s) : fl.row(s); };
+    int page_of[kPages ? kSteps : 1];   // the pages of the next tile's rows, looked up one step ahead
+    int page_at = -1;                   // the same for the scale that this thread fetches
     const int32_t* table = kPages ? a.table + (int64_t)b * a.table_stride : nullptr;
     auto look_up = [&](int tile) {
         if constexpr (kPages) {
 #pragma unroll
-            for (int s = 0; s < St::kSteps; ++s) {
-                const int key = tile * kTileKeys + St::row(s);
+            for (int s = 0; s < kSteps; ++s) {
+                const int key = tile * kTileKeys + row_of(s);
                 page_of[s] = key < keys ? table[a.by_page.div(key)] : -1;
             }
             if constexpr (kCodes) {
@@ -404,41 +417,54 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
             }
         }
     };
+    const char* const kbase = a.k + ((kPages ? 0 : (int64_t)b * a.k_st[1]) + (int64_t)g * a.k_st[2]) * kBytes;
+    const char* const vbase = a.v + ((kPages ? 0 : (int64_t)b * a.v_st[1]) + (int64_t)g * a.v_st[2]) * kBytes;
     float scale_of_key = 0.f;  // waves 0 and 1: the scales of the tile's keys and of its values
-    auto fetch = [&](int tile) {
+    auto fetch = [&](int tile, int buffer) {
+        char* const kt = lds + buffer * 2 * kTile;
+        fl.again();
 #pragma unroll
-        for (int s = 0; s < St::kSteps; ++s) {
-            const int key = tile * kTileKeys + St::row(s);
-            const char *kp, *vp;
-            bool ok = St::works(s) && key < keys && dims_there;
+        for (int s = 0; s < kSteps; ++s) {
+            const int key = tile * kTileKeys + row_of(s), piece = kCodes ? St::piece() : fl.piece(s);
+            bool ok = key < keys && piece * 8 < a.d;
+            const char *kp = kbase + piece * 8 * kBytes, *vp = vbase + piece * 8 * kBytes;
             if constexpr (kPages) {
-                const int64_t page = page_of[s], in = a.by_page.mod(key);
-                ok = ok && (uint64_t)page < (uint64_t)a.pages;
-                kp = a.k + (page * a.k_st[1] + in * a.k_st[0] + (int64_t)g * a.k_st[2] + piece * 8) * kBytes;
-                vp = a.v + (page * a.v_st[1] + in * a.v_st[0] + (int64_t)g * a.v_st[2] + piece * 8) * kBytes;
+                const uint32_t page = page_of[s], in = a.by_page.mod(key);
+                ok = ok && page < (uint32_t)a.pages;
+                kp = step_to(step_to(kp, page, (uint32_t)a.k_st[1] * kBytes), in, (uint32_t)a.k_st[0] * kBytes);
+                vp = step_to(step_to(vp, page, (uint32_t)a.v_st[1] * kBytes), in, (uint32_t)a.v_st[0] * kBytes);
             } else {
-                kp = a.k + ((int64_t)key * a.k_st[0] + (int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2] + piece * 8) * 2;
-                vp = a.v + ((int64_t)key * a.v_st[0] + (int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2] + piece * 8) * 2;
+                kp = step_to(kp, key, (uint32_t)a.k_st[0] * 2);
+                vp = step_to(vp, key, (uint32_t)a.v_st[0] * 2);
             }
-            ks.load(s, kp, ok);
-            vs.load(s, vp, ok);
+            if constexpr (kCodes) {
+                ks.load(s, kp, ok && St::works(s));
+                vs.load(s, vp, ok && St::works(s));
+            } else if (ok) {
+                Fl::load(s, kp, kt);
+                Fl::load(s, vp, kt + kTile);
+            } else {
+                fl.zero(s, kt);
+                fl.zero(s, kt + kTile);
+            }
         }
         if constexpr (kCodes) {
             scale_of_key = 0.f;
-            if (wave < 2 && (uint64_t)(int64_t)page_at < (uint64_t)a.pages) {
+            if (wave < 2 && (uint32_t)page_at < (uint32_t)a.pages) {
                 const int64_t in = a.by_page.mod(tile * kTileKeys + lane);
-                const float* p = wave ? a.v_scale : a.k_scale;
-                const int64_t* st = wave ? a.vs_st : a.ks_st;
-                scale_of_key = p[page_at * st[1] + in * st[0] + (int64_t)g * st[2]];
+                if (wave) scale_of_key = a.v_scale[page_at * a.vs_st[1] + in * a.vs_st[0] + (int64_t)g * a.vs_st[2]];
+                else scale_of_key = a.k_scale[page_at * a.ks_st[1] + in * a.ks_st[0] + (int64_t)g * a.ks_st[2]];
             }
         }
     };
     float* const scales = reinterpret_cast<float*>(lds + kBuffers * 2 * kTile);  // [buffer][keys, values][64]
     auto put = [&](int buffer) {
-        ks.put(lds + buffer * 2 * kTile);
-        vs.put(lds + buffer * 2 * kTile + kTile);
         if constexpr (kCodes) {
+            ks.put(lds + buffer * 2 * kTile);
+            vs.put(lds + buffer * 2 * kTile + kTile);
             if (wave < 2) scales[(buffer * 2 + wave) * kTileKeys + lane] = scale_of_key;
+        } else {
+            landed();
         }
     };
 
@@ -451,7 +477,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
 
     if (first_tile < end_tile) {
         look_up(tiles.tile(first_tile));
-        fetch(tiles.tile(first_tile));
+        fetch(tiles.tile(first_tile), 0);
         if (first_tile + 1 < end_tile) look_up(tiles.tile(first_tile + 1));
         put(0);
     }
@@ -461,8 +487,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
         const int buffer = kBuffers == 2 ? (it - first_tile) & 1 : 0;
         const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
         const int key0 = tiles.tile(it) * kTileKeys;
-        if (it + 1 < end_tile) {
-            fetch(tiles.tile(it + 1));
+        const int next = kBuffers == 2 ? buffer ^ 1 : 0;
+        if (kBuffers == 2 && it + 1 < end_tile) {
+            fetch(tiles.tile(it + 1), next);
             if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
         }
         // what of the tile this wave's rows see: nothing, all, or some of it
@@ -551,8 +578,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
             }
         }
         if (it + 1 < end_tile) {
-            if constexpr (kBuffers == 1) __syncthreads();
-            put(kBuffers == 2 ? buffer ^ 1 : 0);
+            if constexpr (kBuffers == 1) {
+                __syncthreads();
+                fetch(tiles.tile(it + 1), next);
+                if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
+            }
+            put(next);
         }
         __syncthreads();
     }
@@ -848,8 +879,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
     constexpr int kTile = kTileKeys * Tile<DP>::kRow;
-    constexpr int kBuffers = DP <= 128 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) char lds[kBuffers * 2 * kTile];
+    __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTile];
 
     const uint32_t block = blockIdx.x, heads = a.b * a.kv;
     uint32_t bh, mt;
@@ -902,24 +932,24 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
         }
     }
 
-    typedef Stage<T, DP, kStrided, kTileKeys> St;
-    St ks, vs;
-    const int piece = St::piece();
-    const bool dims_there = piece * 8 < a.d;
-    const char* const kbase = a.k + ((int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2] + piece * 8) * 2;
-    const char* const vbase = a.v + ((int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2] + piece * 8) * 2;
-    auto fetch = [&](int tile) {
+    typedef Flight<DP, kTileKeys> Fl;
+    Fl fl;
+    const char* const kbase = a.k + ((int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2]) * 2;
+    const char* const vbase = a.v + ((int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2]) * 2;
+    auto fetch = [&](int tile, int buffer) {
+        char* const kt = lds + buffer * 2 * kTile;
+        fl.again();
 #pragma unroll
-        for (int s = 0; s < St::kSteps; ++s) {
-            const int key = tile * kTileKeys + St::row(s);
-            const bool ok = St::works(s) && key < keys && dims_there;
-            ks.load(s, kbase + (int64_t)key * a.k_st[0] * 2, ok);
-            vs.load(s, vbase + (int64_t)key * a.v_st[0] * 2, ok);
+        for (int s = 0; s < Fl::kSteps; ++s) {
+            const int key = tile * kTileKeys + fl.row(s), piece = fl.piece(s);
+            if (key < keys && piece * 8 < a.d) {
+                Fl::load(s, step_to(kbase + piece * 16, key, (uint32_t)a.k_st[0] * 2), kt);
+                Fl::load(s, step_to(vbase + piece * 16, key, (uint32_t)a.v_st[0] * 2), kt + kTile);
+            } else {
+                fl.zero(s, kt);
+                fl.zero(s, kt + kTile);
+            }
         }
-    };
-    auto put = [&](int buffer) {
-        ks.put(lds + buffer * 2 * kTile);
-        vs.put(lds + buffer * 2 * kTile + kTile);
     };
 
     f32x16 acc[DP / 32];
@@ -929,16 +959,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     const float scale_log2 = a.scale * kLog2e;
 
-    if (tiles.count) {
-        fetch(tiles.tile(0));
-        put(0);
-    }
+    if (tiles.count) fetch(tiles.tile(0), 0);
+    landed();
     __syncthreads();
     for (int it = 0; it < tiles.count; ++it) {
-        const int buffer = kBuffers == 2 ? it & 1 : 0;
+        const int buffer = it & 1;
         const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
         const int key0 = tiles.tile(it) * kTileKeys;
-        if (it + 1 < tiles.count) fetch(tiles.tile(it + 1));
+        if (it + 1 < tiles.count) fetch(tiles.tile(it + 1), buffer ^ 1);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const int k0 = key0 + 32 * kb, k1 = k0 + 32;
@@ -976,14 +1004,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
                 for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(kt_ops.columns(32 * kb + 16 * t, i), p, acc[i]);
             }
         }
-        if (it + 1 < tiles.count) {
-            if constexpr (kBuffers == 1) __syncthreads();
-            put(kBuffers == 2 ? buffer ^ 1 : 0);
-        }
+        landed();
         __syncthreads();
     }
     char* p = a.dq + ((int64_t)token * a.dq_st[0] + (int64_t)b * a.dq_st[1] + (int64_t)head * a.dq_st[2]) * 2;
     store_rows<T, DP>(p, acc, a.scale, a.d, there);
+}
+
+// the first piece of a key tile in the partial sums
+__device__ __forceinline__ int64_t grad_piece(const AttnArgs& a, uint32_t bh, int tile) {
+    const int64_t each = (int64_t)a.key_tiles * a.near_parts + a.sink_tiles * a.far_parts;
+    return bh * each + (int64_t)tile * a.near_parts + min(tile, a.sink_tiles) * a.far_parts;
 }
 
 // ---- backward: the gradients of keys and values -------------------------------------------------------------
@@ -994,15 +1025,20 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
     __shared__ __attribute__((aligned(16))) float row_sums[2][2][kStepRows];  // lse and delta of the tile's rows
 
     const uint32_t block = blockIdx.x, heads = a.b * a.kv;
-    uint32_t bh, kt;
+    uint32_t bh, unit;
     if (heads % 8 == 0) {
-        const uint32_t xcd = block & 7, k = block >> 3, part = a.by_key_tiles.div(k);
+        const uint32_t xcd = block & 7, k = block >> 3, part = a.by_units.div(k);
         bh = part * 8 + xcd;
-        kt = k - part * a.key_tiles;
+        unit = k - part * a.units;
     } else {
-        bh = a.by_key_tiles.div(block);
-        kt = block - bh * a.key_tiles;
+        bh = a.by_units.div(block);
+        unit = block - bh * a.units;
     }
+    const int far_units = a.sink_tiles * a.far_parts;  // short, and first
+    const bool far = (int)unit < far_units;
+    const int kt = far ? a.by_far_parts.div(unit) : a.by_near_parts.div(unit - far_units);
+    const int part = far ? unit - kt * a.far_parts : unit - far_units - kt * a.near_parts;
+    const int far_of_tile = kt < a.sink_tiles ? a.far_parts : 0;
     const int b = a.by_kv.div(bh), g = bh - b * a.kv;
     const int keys = a.lengths ? max(0, min(a.lengths[b], a.sk)) : a.sk, position0 = a.sk - a.sq;
     const int rows = a.sq * a.group, key0 = kt * kGradKeys;
@@ -1011,14 +1047,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
     const int key = key0 + wave * 32 + (lane & 31);
     const int wv_first = __builtin_amdgcn_readfirstlane(key0 + wave * 32), wv_last = wv_first + 31;
 
-    // the rows that see some key of the tile: those at its first position and behind, to the end of the window
+    // The rows that see some key of the tile: those from its first position to the end of its last one's window, and
+    // where it holds sinks all behind.
     int row_begin = 0, row_end = 0;
     if (key0 < keys) {
         const int last = min(key0 + kGradKeys, keys) - 1;
-        const int t0 = max(0, key0 - position0);
-        const int t1 = (a.window < 0 || key0 < a.sinks) ? a.sq : min((int64_t)a.sq, (int64_t)last + a.window - position0 + 1);
-        row_begin = min(t0, a.sq) * a.group;
-        row_end = max(t1, 0) * a.group;
+        const int t0 = min(max(0, key0 - position0), a.sq);
+        int t1 = a.window < 0 ? a.sq : max(0, (int)min((int64_t)a.sq, (int64_t)last + a.window - position0 + 1));
+        if (key0 < a.sinks && !far_of_tile) t1 = a.sq;
+        const int begin = (far ? max(t0, t1) : t0) * a.group, end = (far ? a.sq : t1) * a.group;
+        const int parts = far ? a.far_parts : a.near_parts;
+        const int each = max(0, (end - begin + kStepRows - 1) / kStepRows + parts - 1) / parts * kStepRows;
+        row_begin = min(begin + part * each, end);
+        row_end = min(row_begin + each, end);
     }
 
     u32x4 kreg[DP / 16], vreg[DP / 16];
@@ -1034,29 +1075,34 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
     }
 
     typedef Flight<DP, kStepRows> Fl;
+    Fl fl;
     const char* const qbase = a.q + ((int64_t)b * a.q_st[1] + (int64_t)g * a.group * a.q_st[2]) * 2;
     const char* const dbase = a.dout + ((int64_t)b * a.do_st[1] + (int64_t)g * a.group * a.do_st[2]) * 2;
     // half a wave each fetches the rows' lse and delta; rows behind the end see nothing
-    const float* const sums = half ? a.delta : a.lse;
     auto fetch = [&](int row0, int buffer) {
+        fl.again();
 #pragma unroll
         for (int s = 0; s < Fl::kSteps; ++s) {
-            const int row = row0 + Fl::row(s), piece = Fl::piece(s);
+            const int row = row0 + fl.row(s), piece = fl.piece(s);
             if (row < row_end && piece * 8 < a.d) {
                 const uint32_t token = a.by_group.div(row), h = row - token * a.group;
                 Fl::load(s, step_to(step_to(qbase + piece * 16, token, (uint32_t)a.q_st[0] * 2), h, (uint32_t)a.q_st[2] * 2),
                          lds + buffer * 2 * kTile);
                 Fl::load(s, step_to(step_to(dbase + piece * 16, token, (uint32_t)a.do_st[0] * 2), h, (uint32_t)a.do_st[2] * 2),
                          lds + buffer * 2 * kTile + kTile);
+            } else {
+                fl.zero(s, lds + buffer * 2 * kTile);
+                fl.zero(s, lds + buffer * 2 * kTile + kTile);
             }
         }
         if (wave == 0) {
-            const int row = row0 + (lane & 31);
+            const int row = row0 + (int)(fl.thread & 31);
+            const float* const sums = (fl.thread & 32 ? a.delta : a.lse) + (int64_t)bh * rows;
             if (row < row_end)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(sums + (int64_t)bh * rows + row),
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(sums + row),
                                                  (__attribute__((address_space(3))) void*)row_sums[buffer], 4, 0, 0);
             else
-                row_sums[buffer][half][lane & 31] = half ? 0.f : __builtin_inff();
+                row_sums[buffer][0][fl.thread] = fl.thread & 32 ? 0.f : __builtin_inff();
         }
     };
 
@@ -1067,14 +1113,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
     const float scale_log2 = a.scale * kLog2e;
 
-    clear<4 * kTile>(lds);
-    __syncthreads();
     if (row_begin < row_end) fetch(row_begin, 0);
     landed();
     __syncthreads();
     int buffer = 0;
     for (int row0 = row_begin; row0 < row_end; row0 += kStepRows, buffer ^= 1) {
         const Operands<DP> qt_ops(lds_byte(lds) + buffer * 2 * kTile), dt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
+        uint32_t sums_at = lds_byte(row_sums) + buffer * 8 * kStepRows + 16 * half;
+        asm("" : "+v"(sums_at));
         if (row0 + kStepRows < row_end) fetch(row0 + kStepRows, buffer ^ 1);
         const int at_first = position0 + (int)a.by_group.div(row0);
         const int at_last = position0 + (int)a.by_group.div(min(row0 + kStepRows, row_end) - 1);
@@ -1090,7 +1136,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
             for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(qt_ops.rows(0, st), kreg[st], s);
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_sums[buffer][0][8 * (r >> 2) + 4 * half]);
+                const f32x4 c = lds_floats(sums_at + 32 * (r >> 2));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[r + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + i], scale_log2, -c[i]));
             }
@@ -1104,7 +1150,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
             }
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {  // dP - delta: the sum starts at -delta
-                const f32x4 c = *reinterpret_cast<const f32x4*>(&row_sums[buffer][1][8 * (r >> 2) + 4 * half]);
+                const f32x4 c = lds_floats(sums_at + 4 * kStepRows + 32 * (r >> 2));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dp[r + i] = -c[i];
             }
@@ -1132,9 +1178,50 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         landed();
         __syncthreads();
     }
-    const bool there = key < a.sk;
-    store_rows<T, DP>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2]) * 2, dk, a.scale, a.d, there);
-    store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, 1.f, a.d, there);
+    if (a.near_parts + far_of_tile == 1) {
+        const bool there = key < a.sk;
+        store_rows<T, DP>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2]) * 2, dk, a.scale, a.d, there);
+        store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, 1.f, a.d, there);
+        return;
+    }
+    float* const to = a.part_o + (grad_piece(a, bh, kt) + (far ? a.near_parts + part : part)) * 2 * kGradKeys * a.d + (key - key0) * a.d;
+    if (!far || key < a.sinks) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int dim = 32 * i + element_of(r, half);
+                if (dim < a.d) {
+                    *reinterpret_cast<f32x4*>(to + dim) = f32x4{dk[i][r], dk[i][r + 1], dk[i][r + 2], dk[i][r + 3]};
+                    *reinterpret_cast<f32x4*>(to + kGradKeys * a.d + dim) = f32x4{dv[i][r], dv[i][r + 1], dv[i][r + 2], dv[i][r + 3]};
+                }
+            }
+    }
+}
+
+// Sums the pieces of the key tiles that were done in several, in order: a thread per four dims of a key.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnArgs a) {
+    const int quads = a.d / 4, tile = blockIdx.y;
+    const uint32_t bh = blockIdx.x / (kGradKeys / 32), slice = blockIdx.x % (kGradKeys / 32);
+    const int b = a.by_kv.div(bh), g = bh - b * a.kv;
+    for (int at = threadIdx.x; at < 32 * quads; at += 256) {
+        const int row = slice * 32 + at / quads, dim = at % quads * 4, key = tile * kGradKeys + row;
+        if (key >= a.sk) return;
+        const float* from = a.part_o + grad_piece(a, bh, tile) * 2 * kGradKeys * a.d + row * a.d + dim;
+        const int pieces = a.near_parts + (key < a.sinks && tile < a.sink_tiles ? a.far_parts : 0);
+        f32x4 dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
+        for (int p = 0; p < pieces; ++p) {
+            dk += *reinterpret_cast<const f32x4*>(from);
+            dv += *reinterpret_cast<const f32x4*>(from + kGradKeys * a.d);
+            from += 2 * kGradKeys * a.d;
+        }
+        dk *= a.scale;
+        *reinterpret_cast<u32x2*>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2] + dim) * 2) =
+            u32x2{Elem<T>::pack(dk[0], dk[1]), Elem<T>::pack(dk[2], dk[3])};
+        *reinterpret_cast<u32x2*>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2] + dim) * 2) =
+            u32x2{Elem<T>::pack(dv[0], dv[1]), Elem<T>::pack(dv[2], dv[3])};
+    }
 }
 
 }  // namespace neox

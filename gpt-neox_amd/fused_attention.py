@@ -6,6 +6,7 @@ backward pass recomputes them.  Two things come on top: the first ``sinks`` keys
 query heads may share key heads.  The kernels are those of ``csrc/attention_kernels.hpp``, through
 ``neox_window_attention_fwd`` and ``neox_window_attention_bwd``; there is no CPU fallback.
 """
+import ctypes
 import math
 
 import torch
@@ -65,11 +66,14 @@ class WindowAttention(torch.autograd.Function):
         if grad.shape != out.shape or grad.dtype != out.dtype or grad.device != out.device:
             raise RuntimeError("the gradient must have the shape, dtype and device of the attention's output")
         q, k, v, out, grad = (_lib.in_pieces(t) for t in (q, k, v, out, grad))
-        delta = torch.empty_like(lse)
+        need = ctypes.c_int64()
+        _lib.check(_lib.lib().neox_window_attention_bwd_workspace(need, b, sq, sk, h, h_kv, d, *ctx.call[1:]))
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
         strides = [_lib.row_strides(t) for t in (dq, dk, dv, grad, out, q, k, v)]
         with _lib.device_guard(q):
             _lib.check(_lib.lib().neox_window_attention_bwd(
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), grad.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), need.value, grad.data_ptr(), out.data_ptr(),
+                lse.data_ptr(),
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), key_lengths.data_ptr() if key_lengths is not None else None,
                 b, sq, sk, h, h_kv, d, *strides, *ctx.call, _lib.dtype_code(q.dtype), _lib.current_stream(q)))
         return dq, dk, dv, None, None, None, None

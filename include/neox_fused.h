@@ -29,8 +29,8 @@ extern "C" {
 /*
  * ABI versions.  A version is bumped when an entry point is added or its parameter list changes; the
  * Python binding refuses a library of another version.
- *   5  + neox_window_attention_fwd/_bwd, neox_paged_attention, neox_paged_attention_workspace,
- *      neox_cache_write, neox_cache_read
+ *   5  + neox_window_attention_fwd/_bwd, neox_window_attention_bwd_workspace, neox_paged_attention,
+ *      neox_paged_attention_workspace, neox_cache_write, neox_cache_read
  *   4  + neox_mask_scan, neox_masked_softmax_ends_fwd, neox_masked_softmax_ends_bwd
  *   3  + neox_masked_softmax_alibi_fwd, neox_sliding_window_softmax_fwd/_bwd, neox_mask_classify;
  *      neox_*_softmax_bias_fwd and neox_masked_softmax_dropout_fwd take ALiBi slopes too
@@ -352,14 +352,15 @@ int neox_rope_apply_freqs(void* out_q, void* out_k, const void* q, const void* k
  * A query that sees no key gets zeros, and passes no gradient on.  q, out: [sq, b, h, d], k, v:
  * [sk, b, h_kv, d], addressed by the element strides {token, sample, head}, the last axis dense; query head x
  * uses key head x / (h / h_kv).  d: a multiple of 8, at most 256; every stride a multiple of 8 elements
- * and every pointer 16-byte aligned.  key_lengths: int32 [b] in device memory, or NULL for sk keys
+ * below 2^31 and every pointer 16-byte aligned.  key_lengths: int32 [b] in device memory, or NULL for sk keys
  * everywhere; keys and values behind a length, or behind the window of every query of a tile, are not
  * looked at.  (A value that is infinite or NaN reaches the queries of its own tile -- 64 keys, 128
  * query rows -- also where the mask hides it.)  lse, fp32 [b * h * sq]: what the backward pass
  * needs, in an order of its own (NULL: not wanted).  fp32 arithmetic on the matrix cores' 16-bit
  * products; the probabilities are rounded to the 16-bit type before they meet the values.
- * Backward: dk and dv are summed over the query heads of their key head in a fixed order; delta, fp32
- * [b * h * sq], is scratch.  The gradients may not alias anything else.
+ * Backward: dk and dv are summed over the query heads of their key head in a fixed order; workspace holds
+ * as many bytes of scratch as neox_window_attention_bwd_workspace says for the same sizes.  The gradients may
+ * not alias anything else.
  * Takes the place of the flash-attention path
  *   megatron/model/transformer.py:573-690
  */
@@ -368,8 +369,10 @@ int neox_window_attention_fwd(void* out, float* lse, const void* q, const void* 
                               const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
                               const int64_t out_strides[3], float scale, int32_t window, int32_t sinks, int32_t dtype,
                               void* stream);
-int neox_window_attention_bwd(void* dq, void* dk, void* dv, float* delta, const void* dout, const void* out,
-                              const float* lse, const void* q, const void* k, const void* v, const int32_t* key_lengths,
+int neox_window_attention_bwd_workspace(int64_t* bytes, int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d,
+                                        int32_t window, int32_t sinks);
+int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, const void* dout,
+                              const void* out, const float* lse, const void* q, const void* k, const void* v, const int32_t* key_lengths,
                               int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d,
                               const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
                               const int64_t dout_strides[3], const int64_t out_strides[3], const int64_t q_strides[3],
