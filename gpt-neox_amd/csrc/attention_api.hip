@@ -7,7 +7,7 @@ namespace neox {
 
 // ---- launches whose kernels do not depend on the head dim ------------------------------------------------
 hipError_t launch_attn_join(const AttnArgs& a, int dtype, hipStream_t stream) {
-    const uint32_t blocks = (uint32_t)((a.part_rows + 3) / 4);
+    const uint32_t blocks = (uint32_t)a.part_rows;
     if (dtype == NEOX_BF16) attn_join_kernel<BF16><<<blocks, 256, 0, stream>>>(a);
     else attn_join_kernel<F16><<<blocks, 256, 0, stream>>>(a);
     return hipGetLastError();
@@ -180,8 +180,10 @@ struct PagedPlan {
     int64_t bytes;
 };
 
-// Parts: so many that every CU has workgroups enough (four for single tokens, whose kernel only streams, two for row
-// tiles), with at least 256 keys for each part.
+// Parts: so many that every CU has workgroups enough, with at least 256 keys for each part and 128 parts at most.  Row
+// tiles: two to a CU.  Single tokens: eight, twice what fits, because sequences differ in length and the host does not
+// know by how much: 64 sequences of 2048 to 8192 tokens, int8, take 191 us with four (170 before four fitted), 158 with
+// eight, 169 with sixteen; one of 131001 tokens in bf16 takes 125 us with 128 parts and 128 with 256.
 static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, int h, int h_kv, int d, int window, int sinks) {
     PagedPlan p{};
     const int64_t group = h / h_kv, rows = max_query * group;
@@ -192,11 +194,11 @@ static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, i
         const int64_t seen = (int64_t)window + max_query + sinks;
         if (seen < keys) keys = seen;
     }
-    const int64_t units = (int64_t)b * h_kv * p.row_tiles, target = 256 * (p.token ? 4 : 2);
+    const int64_t units = (int64_t)b * h_kv * p.row_tiles, target = 256 * (p.token ? 8 : 2);
     int64_t splits = (target + units - 1) / units;
     const int64_t most = (keys + 255) / 256;
     if (splits > most) splits = most;
-    if (splits > 256) splits = 256;
+    if (splits > 128) splits = 128;
     if (splits < 1) splits = 1;
     p.splits = (int)splits;
     p.bytes = splits > 1 ? splits * tokens * h * (d + 1) * (int64_t)sizeof(float) : 0;
@@ -458,6 +460,7 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
     a.by_group = FastDiv::by((uint32_t)a.group);
     a.by_kv = FastDiv::by((uint32_t)h_kv);
     a.by_row_tiles = FastDiv::by((uint32_t)a.row_tiles);
+    a.by_splits = FastDiv::by((uint32_t)a.splits);
     a.by_page = FastDiv::by((uint32_t)page_size);
     set_scale_window(a, scale, window, sinks);
     a.q = static_cast<const char*>(q);

@@ -69,7 +69,7 @@ struct AttnArgs {
     float* part_o;               //   [split][row slot][d] and
     float* part_lse;             //   [split][row slot], row slot = (token * kv + key head) * group + head in the group
     int64_t part_rows;           //   row slots of one split
-    FastDiv by_group, by_page, by_row_tiles, by_kv;
+    FastDiv by_group, by_page, by_row_tiles, by_kv, by_splits;
     // backward
     const char *dout;            // [token, sample, head] like q
     const char* out;
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
     constexpr int kBytes = kCodes ? 1 : 2;
     constexpr int kTile = kTileKeys * Tile<DP>::kRow;
     constexpr int kBuffers = 2;
-    __shared__ __attribute__((aligned(16))) char lds[kBuffers * 2 * kTile + (kCodes ? 2 * 2 * kTileKeys * 4 : 0)];
+    __shared__ __attribute__((aligned(512))) char lds[kBuffers * 2 * kTile + (kCodes ? 2 * 2 * kTileKeys * 4 : 0)];
 
     // block -> (sample, key head), row tile, part: neighbours in time on one XCD (blocks go to the 8 XCDs in
     // turn) are the row tiles of one key head, whose keys they share
@@ -612,26 +612,25 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
 
 // ---- single tokens ----------------------------------------------------------------------------------------
 // At most 16 rows per key head: the bytes of the keys and values bound it, so every wave streams keys of its own,
-// 32 at a time, with no barrier before the end.  16x16x32 tiles; the keys go from memory into the first operand as
-// they are (lane: key l % 16; 16-bit: 8 dims from 32 s + 8 (l / 16); codes: 16 dims from 64 s + 16 (l / 16)), the
-// values through LDS of the wave's own for the transposing reads.
+// 32 at a time, with no barrier before the end.  16x16x32 tiles.  A lane fetches, of keys l % 16 and 16 + l % 16, the
+// 16-byte pieces that go into its first operands as they are (16-bit: 8 dims from 32 s + 8 (l / 16); codes: 16 dims from
+// 64 s + 16 (l / 16)); the same pieces of the values go through LDS of the wave's own for the transposing reads.
 template <typename T, int DP, int SRC, bool SPLIT>
-__global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void attn_token_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(AttnArgs a) {
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
     constexpr int kBytes = kCodes ? 1 : 2;
     constexpr int kKeys = 32;
-    constexpr int kLoads = kCodes ? (DP + 63) / 64 : DP / 32;  // 16-byte loads of one key per lane
-    constexpr int kPerRow = DP * kBytes / 16;                   // lanes that load one row of values
-    constexpr int kRowsAtOnce = 64 / kPerRow;
-    constexpr int kValueLoads = (kKeys + kRowsAtOnce - 1) / kRowsAtOnce;
+    constexpr int kLoads = kCodes ? (DP + 63) / 64 : DP / 32;  // 16-byte pieces of one key per lane
     constexpr int kWaveBytes = kKeys * Tile<DP>::kRow;
-    __shared__ __attribute__((aligned(16))) char lds[4 * kWaveBytes];
+    __shared__ __attribute__((aligned(512))) char lds[4 * kWaveBytes];
     __shared__ __attribute__((aligned(16))) float scales[4][2][kKeys];
     __shared__ float wave_m[4][16], wave_l[4][16];
 
-    const uint32_t bh = blockIdx.x;
-    const int split = SPLIT ? (int)blockIdx.y : 0;
-    const int b = a.by_kv.div(bh), g = bh - b * a.kv;
+    // The heads of one part of a sequence run on one XCD at about the same time: their rows are neighbours in memory.
+    const uint32_t turn = blockIdx.x >> 3, at = a.by_kv.div(turn), item = at * 8 + (blockIdx.x & 7);
+    const int g = turn - at * a.kv;
+    if (item >= (uint32_t)a.b * a.splits) return;
+    const int b = SPLIT ? a.by_splits.div(item) : item, split = SPLIT ? item - b * a.splits : 0;
     int token0, tokens, keys;
     paged_sample(a, b, token0, tokens, keys);
     const int rows = min(tokens * a.group, 16);
@@ -670,37 +669,45 @@ __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void attn_token_kernel(Attn
     }
 
     char* const vt = lds + wave * kWaveBytes;
+    // Where this lane's pieces of the values go, and where the transposing reads find dims 16 db + l % 16 of keys
+    // 4 (l / 16) ..: as in Operands, an exclusive or with a constant away from one register each.
+    uint32_t put_at, get_at;
+    {
+        put_at = lds_byte(vt) + (col * Tile<DP>::kRow | (Tile<DP>::turn(col) ^ (kCodes ? 2 * quad : quad)) << 4);
+        const uint32_t j = col, r = 4 * quad + (j >> 2);
+        get_at = lds_byte(vt) + (r * Tile<DP>::kRow | (Tile<DP>::turn(r) ^ ((j >> 1) & 1)) << 4 | (j & 1) * 8);
+    }
     const int32_t* const table = a.table + (int64_t)b * a.table_stride;
-    u32x4 kw[2][kLoads], vw[kValueLoads];
+    u32x4 kw[2][kLoads], vw[2][kLoads];
     float k_scale = 0.f, v_scale = 0.f;
-    auto look_up = [&](int i) {  // lane l: the page of key l % 32 of the wave's block i
-        const int key = tiles.tile(i) * kKeys + (lane & 31);
-        return i < end && key < keys ? table[a.by_page.div(key)] : -1;
-    };
-    auto fetch = [&](int i, int page) {
-        const int key = tiles.tile(i) * kKeys + (lane & 31);
-        const bool ok = (uint64_t)(int64_t)page < (uint64_t)a.pages;
-        const int in = a.by_page.mod(key);
-        const int64_t k_at = ok ? (int64_t)page * a.k_st[1] + in * a.k_st[0] + (int64_t)g * a.k_st[2] : -1;
-        const int64_t v_at = ok ? (int64_t)page * a.v_st[1] + in * a.v_st[0] + (int64_t)g * a.v_st[2] : -1;
+    int pages[2];  // of this lane's two keys of the next block
+    auto look_up = [&](int i) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            const int64_t at = __shfl(k_at, 16 * kb + col);
-#pragma unroll
-            for (int s = 0; s < kLoads; ++s)
-                kw[kb][s] = load8(a.k + (at + dim_of(s)) * kBytes, at >= 0 && dim_of(s) < a.d);
+            const int key = tiles.tile(i) * kKeys + 16 * kb + col;
+            pages[kb] = i < end && key < keys ? table[a.by_page.div(key)] : -1;
         }
+    };
+    const char* const kbase = a.k + ((int64_t)g * a.k_st[2] + dim_of(0)) * kBytes;
+    const char* const vbase = a.v + ((int64_t)g * a.v_st[2] + dim_of(0)) * kBytes;
+    auto fetch = [&](int i) {
 #pragma unroll
-        for (int s = 0; s < kValueLoads; ++s) {
-            const int r = s * kRowsAtOnce + lane / kPerRow, dim = lane % kPerRow * (16 / kBytes);
-            const int64_t at = __shfl(v_at, r & 31);
-            vw[s] = load8(a.v + (at + dim) * kBytes, at >= 0 && r < kKeys && lane < kRowsAtOnce * kPerRow && dim < a.d);
-        }
-        if constexpr (kCodes) {
-            k_scale = v_scale = 0.f;
-            if (ok) {
-                k_scale = a.k_scale[page * a.ks_st[1] + in * a.ks_st[0] + (int64_t)g * a.ks_st[2]];
-                v_scale = a.v_scale[page * a.vs_st[1] + in * a.vs_st[0] + (int64_t)g * a.vs_st[2]];
+        for (int kb = 0; kb < 2; ++kb) {
+            const uint32_t page = pages[kb], in = a.by_page.mod(tiles.tile(i) * kKeys + 16 * kb + col);
+            const bool ok = page < (uint32_t)a.pages;
+            const char* const kp = step_to(step_to(kbase, page, (uint32_t)a.k_st[1] * kBytes), in, (uint32_t)a.k_st[0] * kBytes);
+            const char* const vp = step_to(step_to(vbase, page, (uint32_t)a.v_st[1] * kBytes), in, (uint32_t)a.v_st[0] * kBytes);
+#pragma unroll
+            for (int s = 0; s < kLoads; ++s) {
+                kw[kb][s] = load8(kp + s * 64, ok && dim_of(s) < a.d);
+                vw[kb][s] = load8(vp + s * 64, ok && dim_of(s) < a.d);
+            }
+            if constexpr (kCodes) {
+                // (all four lanes of a key fetch its scales; those of the quad that stores them count)
+                if (quad == kb) {
+                    k_scale = ok ? a.k_scale[(int64_t)page * a.ks_st[1] + (int64_t)in * a.ks_st[0] + (int64_t)g * a.ks_st[2]] : 0.f;
+                    v_scale = ok ? a.v_scale[(int64_t)page * a.vs_st[1] + (int64_t)in * a.vs_st[0] + (int64_t)g * a.vs_st[2]] : 0.f;
+                }
             }
         }
     };
@@ -710,11 +717,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void attn_token_kernel(Attn
     for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = kNegInf, l = 0.f;
 
-    int page = look_up(first + wave);
-    if (first + wave < end) fetch(first + wave, page);
-    page = look_up(first + wave + 4);
+    look_up(first + wave);
+    if (first + wave < end) fetch(first + wave);
+    look_up(first + wave + 4);
     for (int i = first + wave; i < end; i += 4) {
         const int key0 = tiles.tile(i) * kKeys;
+        asm("" : "+v"(put_at), "+v"(get_at));
+        typedef __attribute__((address_space(3))) u32x4 lds16;
+        typedef __attribute__((address_space(3))) s16x4 lds4;
         f32x4 s[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -730,24 +740,28 @@ __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void attn_token_kernel(Attn
             }
         }
 #pragma unroll
-        for (int st = 0; st < kValueLoads; ++st) {
-            const int r = st * kRowsAtOnce + lane / kPerRow, part = lane % kPerRow;
-            if (r < kKeys && lane < kRowsAtOnce * kPerRow) {
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int st = 0; st < kLoads; ++st) {
+                const u32x4 w = vw[kb][st];
                 if constexpr (kCodes) {
-                    *reinterpret_cast<u32x4*>(vt + Tile<DP>::at(r, 2 * part)) = widen8<T, SRC>(u32x2{vw[st].x, vw[st].y});
-                    *reinterpret_cast<u32x4*>(vt + Tile<DP>::at(r, 2 * part + 1)) = widen8<T, SRC>(u32x2{vw[st].z, vw[st].w});
+                    if (DP % 64 == 0 || dim_of(st) < DP) {
+                        *(lds16*)(uintptr_t)((put_at ^ (st << 7)) + 16 * kb * Tile<DP>::kRow) = widen8<T, SRC>(u32x2{w.x, w.y});
+                        *(lds16*)(uintptr_t)((put_at ^ (st << 7) ^ 16) + 16 * kb * Tile<DP>::kRow) = widen8<T, SRC>(u32x2{w.z, w.w});
+                    }
                 } else {
-                    *reinterpret_cast<u32x4*>(vt + Tile<DP>::at(r, part)) = vw[st];
+                    *(lds16*)(uintptr_t)((put_at ^ (st << 6)) + 16 * kb * Tile<DP>::kRow) = w;
                 }
             }
-        }
         if constexpr (kCodes) {
-            scales[wave][0][lane & 31] = k_scale;
-            scales[wave][1][lane & 31] = v_scale;
+            if (quad < 2) {
+                scales[wave][0][lane] = k_scale;
+                scales[wave][1][lane] = v_scale;
+            }
         }
         if (i + 4 < end) {
-            fetch(i + 4, page);
-            page = look_up(i + 8);
+            fetch(i + 4);
+            look_up(i + 8);
         }
         __builtin_amdgcn_wave_barrier();
         if constexpr (kCodes) {
@@ -793,12 +807,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void attn_token_kernel(Attn
         }
         const u32x4 p = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
                          Elem<T>::pack(s[1][0], s[1][1]), Elem<T>::pack(s[1][2], s[1][3])};
-        typedef __attribute__((address_space(3))) s16x4 lds4;
-        const uint32_t j = lane & 15, r = 4 * quad + (j >> 2), sub = (j >> 1) & 1, bytes = (j & 1) * 8;
 #pragma unroll
         for (int db = 0; db < DP / 16; ++db) {
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vt + Tile<DP>::at(r, 2 * db + sub) + bytes));
-            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vt + Tile<DP>::at(r + 16, 2 * db + sub) + bytes));
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)(get_at ^ (db << 5)));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(uintptr_t)((get_at ^ (db << 5)) + 16 * Tile<DP>::kRow));
             const u32x2 u = __builtin_bit_cast(u32x2, x), v = __builtin_bit_cast(u32x2, y);
             acc[db] = Mma<T>::op16(u32x4{u.x, u.y, v.x, v.y}, p, acc[db]);
         }
@@ -848,38 +860,54 @@ __global__ __launch_bounds__(256, DP <= 128 ? 4 : 2) void attn_token_kernel(Attn
     }
 }
 
-// Joins the parts of a split key axis: a wave per row, lane l the dims 4 l .. of it.
+// Joins the parts of a split key axis: a workgroup per row, 64 threads for the dims (four each), four groups of them for
+// every fourth part.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    const int64_t slot = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (slot >= a.part_rows) return;
-    const int lane = threadIdx.x & 63;
-    float high = kNegInf;
-    for (int s = lane; s < a.splits; s += 64) high = fmaxf(high, a.part_lse[s * a.part_rows + slot]);
-    for (int x = 1; x < 64; x *= 2) high = fmaxf(high, __shfl_xor(high, x));
+    __shared__ __attribute__((aligned(16))) f32x4 sums[4][64];
+    __shared__ float weights[128];
+    const int64_t slot = blockIdx.x;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, dim = lane * 4;
+    // every wave reduces the parts' logarithms by itself: at most 128 of them
+    float lse[2], high = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int s = i * 64 + lane;
+        lse[i] = s < a.splits ? a.part_lse[s * a.part_rows + slot] : kNegInf;
+        high = fmaxf(high, lse[i]);
+    }
+    high = wave_reduce<OpMax>(high);  // (a NaN is not the largest; it reaches the total)
     const float base = high == kNegInf ? 0.f : high;
-    const int dim = lane * 4;
     float total = 0.f;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t at = s * a.part_rows + slot;
-        const float f = __builtin_amdgcn_exp2f(a.part_lse[at] - base);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float f = __builtin_amdgcn_exp2f(lse[i] - base);
         total += f;
-        if (dim < a.d) sum += *reinterpret_cast<const f32x4*>(a.part_o + at * a.d + dim) * f;
+        if (wave == 0) weights[i * 64 + lane] = f;
     }
-    const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+    total = wave_reduce<OpSum>(total);
+    __syncthreads();
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     if (dim < a.d) {
-        const int64_t token = slot / (a.kv * a.group), head = slot - token * (a.kv * a.group);
-        const u32x2 w = {Elem<T>::pack(sum[0] * inverse, sum[1] * inverse), Elem<T>::pack(sum[2] * inverse, sum[3] * inverse)};
-        *reinterpret_cast<u32x2*>(a.o + (token * a.o_st[0] + head * a.o_st[2] + dim) * 2) = w;
+        const float* from = a.part_o + slot * a.d + dim;
+#pragma unroll 4
+        for (int s = wave; s < a.splits; s += 4) sum += *reinterpret_cast<const f32x4*>(from + s * a.part_rows * a.d) * weights[s];
     }
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave || dim >= a.d) return;
+    sum = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+    const int64_t token = slot / (a.kv * a.group), head = slot - token * (a.kv * a.group);
+    const u32x2 w = {Elem<T>::pack(sum[0] * inverse, sum[1] * inverse), Elem<T>::pack(sum[2] * inverse, sum[3] * inverse)};
+    *reinterpret_cast<u32x2*>(a.o + (token * a.o_st[0] + head * a.o_st[2] + dim) * 2) = w;
 }
 
 // ---- backward: the queries' gradient, and the rows' sums of dO * O -----------------------------------------
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
     constexpr int kTile = kTileKeys * Tile<DP>::kRow;
-    __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTile];
+    __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile];
 
     const uint32_t block = blockIdx.x, heads = a.b * a.kv;
     uint32_t bh, mt;
@@ -1021,7 +1049,7 @@ __device__ __forceinline__ int64_t grad_piece(const AttnArgs& a, uint32_t bh, in
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
     constexpr int kTile = kStepRows * Tile<DP>::kRow;
-    __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTile];
+    __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile];
     __shared__ __attribute__((aligned(16))) float row_sums[2][2][kStepRows];  // lse and delta of the tile's rows
 
     const uint32_t block = blockIdx.x, heads = a.b * a.kv;

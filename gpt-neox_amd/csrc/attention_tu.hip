@@ -20,7 +20,7 @@ static void forward(const AttnArgs& a, int source, hipStream_t stream) {
 template <typename T, bool SPLIT>
 static void token(const AttnArgs& a, int source, hipStream_t stream) {
     constexpr int DP = NEOX_ATTN_DIM;
-    const dim3 grid((uint32_t)a.b * a.kv, SPLIT ? a.splits : 1);
+    const uint32_t grid = ((uint32_t)a.b * a.splits + 7) / 8 * 8 * a.kv;
     switch (source) {
         case kPaged16: attn_token_kernel<T, DP, kPaged16, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedI8: attn_token_kernel<T, DP, kPagedI8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
