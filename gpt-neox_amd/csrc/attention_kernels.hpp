@@ -294,6 +294,7 @@ struct Stage {
             if constexpr (kCodes) x = widen8<T, SRC>(c[s]);
             else x = w[s];
             *reinterpret_cast<u32x4*>(tile + Tile<DP>::at(row(s), piece())) = x;
+            __builtin_amdgcn_sched_barrier(0);  // one step after the other: their values together would not fit the registers
         }
     }
 };
@@ -317,10 +318,19 @@ struct Flight {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                          (__attribute__((address_space(3))) void*)(tile + step * 4096 + wave * 1024), 16, 0, 0);
     }
+    // Whole tiles of rows a fixed stride apart: the addresses are a scalar for the step and a lane's own offset, which
+    // stays the same from step to step (but for the permutation, which repeats every 16 rows) and from tile to tile.
+    static constexpr int kRowsAtOnce = 4096 / Tile<DP>::kRow;
+    __device__ __forceinline__ uint32_t offset(uint32_t row_bytes) const { return row(0) * row_bytes + piece(0) * 16; }
+    static __device__ __forceinline__ void load(int step, const char* first, uint32_t row_bytes, uint32_t offset, uint32_t piece, char* tile) {
+        if constexpr (kRowsAtOnce < 16) offset += ((piece ^ (step & 1) * 2) - piece) * 16;
+        load(step, first + (uint64_t)(step * kRowsAtOnce) * row_bytes + offset, tile);
+    }
     __device__ __forceinline__ void zero(int step, char* tile) const {
         *reinterpret_cast<u32x4*>(tile + place(step) * 16) = u32x4{0, 0, 0, 0};
     }
 };
+constexpr int64_t kSmallStride = 1 << 25;  // elements: a tile's offsets fit 32 bits
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---- forward --------------------------------------------------------------------------------------------
@@ -329,9 +339,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
     constexpr bool kPages = SRC != kStrided;
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
     constexpr int kBytes = kCodes ? 1 : 2;
-    constexpr int kTile = kTileKeys * Tile<DP>::kRow;
+    // Keys of one step.  32 leave registers and LDS for a third workgroup on a CU (measured with 64 and 32, us: 2 x 64
+    // heads of 96 dims, 2048 keys, window 512: 126, 105; 32 heads of 128 dims, 8192 keys, window 4096: 562, 539); with
+    // codes, whose widening takes the registers anyway, 64 save barriers (chunks of 512 over 16384 in fp8: 251, 275).
+    constexpr int kFwdKeys = kCodes ? 64 : 32;
+    constexpr int kTile = kFwdKeys * Tile<DP>::kRow;
     constexpr int kBuffers = 2;
-    __shared__ __attribute__((aligned(512))) char lds[kBuffers * 2 * kTile + (kCodes ? 2 * 2 * kTileKeys * 4 : 0)];
+    __shared__ __attribute__((aligned(512))) char lds[kBuffers * 2 * kTile + (kCodes ? 2 * 2 * kFwdKeys * 4 : 0)];
 
     // block -> (sample, key head), row tile, part: neighbours in time on one XCD (blocks go to the 8 XCDs in
     // turn) are the row tiles of one key head, whose keys they share
@@ -373,7 +387,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
     const int wv_last = __builtin_amdgcn_readfirstlane(position0 + (int)a.by_group.div(min(row0 + wave * 32 + 32, rows) - 1));
     const bool wave_works = row0 + wave * 32 < rows;
 
-    KeyTiles tiles = key_tiles<kTileKeys>(wg_first, wg_last, keys, a.window, a.sinks);
+    KeyTiles tiles = key_tiles<kFwdKeys>(wg_first, wg_last, keys, a.window, a.sinks);
     int first_tile = 0, end_tile = tiles.count;
     if constexpr (SPLIT) {
         const int each = (tiles.count + a.splits - 1) / a.splits;
@@ -395,8 +409,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
 
     // One tile of keys and values into one of the buffers: 16-bit rows are copied there as they are; codes come through
     // registers and are widened on the way, which put() does when the tile's turn is near.
-    typedef Stage<T, DP, kCodes ? SRC : kPagedI8, kTileKeys> St;
-    typedef Flight<DP, kTileKeys> Fl;
+    typedef Stage<T, DP, kCodes ? SRC : kPagedI8, kFwdKeys> St;
+    typedef Flight<DP, kFwdKeys> Fl;
     Fl fl;
     constexpr int kSteps = kCodes ? St::kSteps : Fl::kSteps;
     St ks, vs;
@@ -404,15 +418,32 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
     int page_of[kPages ? kSteps : 1];   // the pages of the next tile's rows, looked up one step ahead
     int page_at = -1;                   // the same for the scale that this thread fetches
     const int32_t* table = kPages ? a.table + (int64_t)b * a.table_stride : nullptr;
+    // Whether whole tiles have their rows a fixed stride apart (for pages: a page holds whole tiles), and this lane's
+    // part in that.  Its places beyond d are zeros from the start and stay so.
+    const bool even = !kCodes && a.k_st[0] < kSmallStride && a.v_st[0] < kSmallStride && (!kPages || a.by_page.d % kFwdKeys == 0) &&
+                      (Fl::kRowsAtOnce >= 16 || a.d == DP);
+    const uint32_t k_row = (uint32_t)a.k_st[0] * 2, v_row = (uint32_t)a.v_st[0] * 2;
+    const uint32_t k_offset = fl.offset(k_row), v_offset = fl.offset(v_row), lane_piece = fl.piece(0);
+    const bool has_dims = (int)lane_piece * 8 < a.d;
+    if (even && !has_dims) {
+#pragma unroll
+        for (int s = 0; s < 2 * kBuffers * Fl::kSteps; ++s) fl.zero(s, lds);
+    }
+    uint32_t tile_page = 0;
     auto look_up = [&](int tile) {
         if constexpr (kPages) {
+            if (even) {
+                const int key = tile * kFwdKeys;
+                tile_page = key < keys ? __builtin_amdgcn_readfirstlane(table[a.by_page.div(key)]) : ~0u;
+                return;
+            }
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const int key = tile * kTileKeys + row_of(s);
+                const int key = tile * kFwdKeys + row_of(s);
                 page_of[s] = key < keys ? table[a.by_page.div(key)] : -1;
             }
             if constexpr (kCodes) {
-                const int key = tile * kTileKeys + lane;
+                const int key = tile * kFwdKeys + lane;
                 page_at = (wave < 2 && key < keys) ? table[a.by_page.div(key)] : -1;
             }
         }
@@ -422,14 +453,36 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
     float scale_of_key = 0.f;  // waves 0 and 1: the scales of the tile's keys and of its values
     auto fetch = [&](int tile, int buffer) {
         char* const kt = lds + buffer * 2 * kTile;
+        if constexpr (!kCodes) {
+            const int key = tile * kFwdKeys;
+            if (even && key + kFwdKeys <= keys && (!kPages || tile_page < (uint32_t)a.pages)) {
+                const char *kp = kbase, *vp = vbase;
+                uint32_t first = key;
+                if constexpr (kPages) {
+                    kp = step_to(kp, tile_page, (uint32_t)a.k_st[1] * 2);
+                    vp = step_to(vp, tile_page, (uint32_t)a.v_st[1] * 2);
+                    first = a.by_page.mod(key);
+                }
+                kp = step_to(kp, first, k_row);
+                vp = step_to(vp, first, v_row);
+                if (has_dims) {
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) {
+                        Fl::load(s, kp, k_row, k_offset, lane_piece, kt);
+                        Fl::load(s, vp, v_row, v_offset, lane_piece, kt + kTile);
+                    }
+                }
+                return;
+            }
+        }
         fl.again();
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int key = tile * kTileKeys + row_of(s), piece = kCodes ? St::piece() : fl.piece(s);
+            const int key = tile * kFwdKeys + row_of(s), piece = kCodes ? St::piece() : fl.piece(s);
             bool ok = key < keys && piece * 8 < a.d;
             const char *kp = kbase + piece * 8 * kBytes, *vp = vbase + piece * 8 * kBytes;
             if constexpr (kPages) {
-                const uint32_t page = page_of[s], in = a.by_page.mod(key);
+                const uint32_t page = even ? tile_page : page_of[s], in = a.by_page.mod(key);
                 ok = ok && page < (uint32_t)a.pages;
                 kp = step_to(step_to(kp, page, (uint32_t)a.k_st[1] * kBytes), in, (uint32_t)a.k_st[0] * kBytes);
                 vp = step_to(step_to(vp, page, (uint32_t)a.v_st[1] * kBytes), in, (uint32_t)a.v_st[0] * kBytes);
@@ -451,7 +504,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
         if constexpr (kCodes) {
             scale_of_key = 0.f;
             if (wave < 2 && (uint32_t)page_at < (uint32_t)a.pages) {
-                const int64_t in = a.by_page.mod(tile * kTileKeys + lane);
+                const int64_t in = a.by_page.mod(tile * kFwdKeys + lane);
                 if (wave) scale_of_key = a.v_scale[page_at * a.vs_st[1] + in * a.vs_st[0] + (int64_t)g * a.vs_st[2]];
                 else scale_of_key = a.k_scale[page_at * a.ks_st[1] + in * a.ks_st[0] + (int64_t)g * a.ks_st[2]];
             }
@@ -462,7 +515,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
         if constexpr (kCodes) {
             ks.put(lds + buffer * 2 * kTile);
             vs.put(lds + buffer * 2 * kTile + kTile);
-            if (wave < 2) scales[(buffer * 2 + wave) * kTileKeys + lane] = scale_of_key;
+            if (wave < 2) scales[(buffer * 2 + wave) * kFwdKeys + lane] = scale_of_key;
         } else {
             landed();
         }
@@ -486,31 +539,31 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
     for (int it = first_tile; it < end_tile; ++it) {
         const int buffer = kBuffers == 2 ? (it - first_tile) & 1 : 0;
         const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
-        const int key0 = tiles.tile(it) * kTileKeys;
+        const int key0 = tiles.tile(it) * kFwdKeys;
         const int next = kBuffers == 2 ? buffer ^ 1 : 0;
         if (kBuffers == 2 && it + 1 < end_tile) {
             fetch(tiles.tile(it + 1), next);
             if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
         }
         // what of the tile this wave's rows see: nothing, all, or some of it
-        const int key_end = key0 + kTileKeys;
+        const int key_end = key0 + kFwdKeys;
         const bool none = !wave_works || key0 > wv_last || key0 >= keys ||
                           (a.window >= 0 && key_end - 1 < wv_first - a.window && key0 >= a.sinks);
         const bool all = key_end - 1 <= wv_first && key_end <= keys &&
                          (a.window < 0 || key0 >= wv_last - a.window || key_end <= a.sinks);
         if (!none) {
-            f32x16 s[2];
+            f32x16 s[kFwdKeys / 32];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
                 for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s[kb]);
             }
             if constexpr (kCodes) {
-                const float* f = scales + buffer * 2 * kTileKeys;
+                const float* f = scales + buffer * 2 * kFwdKeys;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
                     for (int r = 0; r < 16; r += 4) {
                         const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
@@ -521,7 +574,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
             if (!all) {
                 const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int key = key0 + 32 * kb + element_of(r, half);
@@ -533,7 +586,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
 #pragma unroll
             for (int r = 1; r < 16; ++r) top = fmaxf(top, s[0][r]);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[1][r]);
+            for (int r = 0; r < 16 && kFwdKeys > 32; ++r) top = fmaxf(top, s[kFwdKeys / 32 - 1][r]);
             top = both_halves_max(top) * a.scale_log2;
             // The running maximum follows only where a row has outgrown it by 2^8: until then its exponentials stay
             // below 256 and the accumulators need no rescaling.
@@ -550,7 +603,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
             const float base = m == kNegInf ? 0.f : m;
             float sum = 0.f;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], a.scale_log2, -base));
@@ -558,9 +611,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
                 }
             l += sum;
             if constexpr (kCodes) {
-                const float* f = scales + (buffer * 2 + 1) * kTileKeys;
+                const float* f = scales + (buffer * 2 + 1) * kFwdKeys;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
                     for (int r = 0; r < 16; r += 4) {
                         const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
@@ -569,7 +622,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
                     }
             }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < kFwdKeys / 16; ++t) {
                 u32x4 p;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[t >> 1][8 * (t & 1) + 2 * e], s[t >> 1][8 * (t & 1) + 2 * e + 1]);
@@ -964,8 +1017,28 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
     Fl fl;
     const char* const kbase = a.k + ((int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2]) * 2;
     const char* const vbase = a.v + ((int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2]) * 2;
+    const bool even = a.k_st[0] < kSmallStride && a.v_st[0] < kSmallStride && (Fl::kRowsAtOnce >= 16 || a.d == DP);
+    const uint32_t k_row = (uint32_t)a.k_st[0] * 2, v_row = (uint32_t)a.v_st[0] * 2;
+    const uint32_t k_offset = fl.offset(k_row), v_offset = fl.offset(v_row), lane_piece = fl.piece(0);
+    const bool has_dims = (int)lane_piece * 8 < a.d;
+    if (even && !has_dims) {
+#pragma unroll
+        for (int s = 0; s < 4 * Fl::kSteps; ++s) fl.zero(s, lds);
+    }
     auto fetch = [&](int tile, int buffer) {
         char* const kt = lds + buffer * 2 * kTile;
+        if (even && tile * kTileKeys + kTileKeys <= keys) {
+            const char* const kp = step_to(kbase, tile * kTileKeys, k_row);
+            const char* const vp = step_to(vbase, tile * kTileKeys, v_row);
+            if (has_dims) {
+#pragma unroll
+                for (int s = 0; s < Fl::kSteps; ++s) {
+                    Fl::load(s, kp, k_row, k_offset, lane_piece, kt);
+                    Fl::load(s, vp, v_row, v_offset, lane_piece, kt + kTile);
+                }
+            }
+            return;
+        }
         fl.again();
 #pragma unroll
         for (int s = 0; s < Fl::kSteps; ++s) {
@@ -1046,8 +1119,10 @@ __device__ __forceinline__ int64_t grad_piece(const AttnArgs& a, uint32_t bh, in
 }
 
 // ---- backward: the gradients of keys and values -------------------------------------------------------------
-template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
+// Head dims over 128 take two launches, one for each gradient (DK, DV): together their accumulators, keys and values
+// are 384 registers of a lane, and the compiler spilled 330.
+template <typename T, int DP, bool DK, bool DV>
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
     constexpr int kTile = kStepRows * Tile<DP>::kRow;
     __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile];
     __shared__ __attribute__((aligned(16))) float row_sums[2][2][kStepRows];  // lse and delta of the tile's rows
@@ -1090,7 +1165,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         row_end = min(row_begin + each, end);
     }
 
-    u32x4 kreg[DP / 16], vreg[DP / 16];
+    u32x4 kreg[DP / 16], vreg[DK ? DP / 16 : 1];
     {
         const char* kp = a.k + ((int64_t)key * a.k_st[0] + (int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2]) * 2;
         const char* vp = a.v + ((int64_t)key * a.v_st[0] + (int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2]) * 2;
@@ -1098,7 +1173,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         for (int s = 0; s < DP / 16; ++s) {
             const int dim = 16 * s + 8 * half;
             kreg[s] = load8(kp + dim * 2, key < keys && dim < a.d);
-            vreg[s] = load8(vp + dim * 2, key < keys && dim < a.d);
+            if constexpr (DK) vreg[s] = load8(vp + dim * 2, key < keys && dim < a.d);
         }
     }
 
@@ -1107,8 +1182,40 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
     const char* const qbase = a.q + ((int64_t)b * a.q_st[1] + (int64_t)g * a.group * a.q_st[2]) * 2;
     const char* const dbase = a.dout + ((int64_t)b * a.do_st[1] + (int64_t)g * a.group * a.do_st[2]) * 2;
     // half a wave each fetches the rows' lse and delta; rows behind the end see nothing
-    auto fetch = [&](int row0, int buffer) {
+    // Steps begin at a token's first head where the group divides them; a lane then keeps its place in the step, as in
+    // the kernels above.
+    const bool even = kStepRows % a.group == 0 && (Fl::kRowsAtOnce >= 16 || a.d == DP) &&
+                      a.q_st[0] < kSmallStride && a.do_st[0] < kSmallStride && a.q_st[2] < kSmallStride && a.do_st[2] < kSmallStride &&
+                      (Fl::kRowsAtOnce % a.group == 0);
+    if (even && fl.piece(0) * 8 >= a.d) {
+#pragma unroll
+        for (int s = 0; s < 4 * Fl::kSteps; ++s) fl.zero(s, lds);
+    }
+    const uint32_t step_tokens = even ? a.by_group.div(Fl::kRowsAtOnce) : 0;
+    auto fetch_rows = [&](int row0, int buffer) {
         fl.again();
+        if (even && row0 + kStepRows <= row_end) {
+            const uint32_t lane_token = a.by_group.div(fl.row(0)), lane_head = fl.row(0) - lane_token * a.group, lane_piece = fl.piece(0);
+            const uint32_t q_offset = (lane_token * (uint32_t)a.q_st[0] + lane_head * (uint32_t)a.q_st[2] + lane_piece * 8) * 2;
+            const uint32_t d_offset = (lane_token * (uint32_t)a.do_st[0] + lane_head * (uint32_t)a.do_st[2] + lane_piece * 8) * 2;
+            const uint32_t token = a.by_group.div(row0);
+            const char* const qp = step_to(qbase, token, (uint32_t)a.q_st[0] * 2);
+            const char* const dp = step_to(dbase, token, (uint32_t)a.do_st[0] * 2);
+            if ((int)lane_piece * 8 < a.d) {
+#pragma unroll
+                for (int s = 0; s < Fl::kSteps; ++s) {
+                    uint32_t qo = q_offset, dof = d_offset;
+                    if constexpr (Fl::kRowsAtOnce < 16) {
+                        const uint32_t other = ((lane_piece ^ (s & 1) * 2) - lane_piece) * 16;
+                        qo += other;
+                        dof += other;
+                    }
+                    Fl::load(s, step_to(qp, s * step_tokens, (uint32_t)a.q_st[0] * 2) + qo, lds + buffer * 2 * kTile);
+                    Fl::load(s, step_to(dp, s * step_tokens, (uint32_t)a.do_st[0] * 2) + dof, lds + buffer * 2 * kTile + kTile);
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int s = 0; s < Fl::kSteps; ++s) {
             const int row = row0 + fl.row(s), piece = fl.piece(s);
@@ -1123,6 +1230,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
                 fl.zero(s, lds + buffer * 2 * kTile + kTile);
             }
         }
+    };
+    auto fetch = [&](int row0, int buffer) {
+        fetch_rows(row0, buffer);
         if (wave == 0) {
             const int row = row0 + (int)(fl.thread & 31);
             const float* const sums = (fl.thread & 32 ? a.delta : a.lse) + (int64_t)bh * rows;
@@ -1134,7 +1244,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
         }
     };
 
-    f32x16 dk[DP / 32], dv[DP / 32];
+    f32x16 dk[DP / 32], dv[DP / 32];  // (the one that is not wanted never comes to be)
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -1176,31 +1286,37 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
                     s[r] = sees ? s[r] : 0.f;
                 }
             }
+            if constexpr (DK) {
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {  // dP - delta: the sum starts at -delta
-                const f32x4 c = lds_floats(sums_at + 4 * kStepRows + 32 * (r >> 2));
+                for (int r = 0; r < 16; r += 4) {  // dP - delta: the sum starts at -delta
+                    const f32x4 c = lds_floats(sums_at + 4 * kStepRows + 32 * (r >> 2));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dp[r + i] = -c[i];
+                    for (int i = 0; i < 4; ++i) dp[r + i] = -c[i];
+                }
+#pragma unroll
+                for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(dt_ops.rows(0, st), vreg[st], dp);
             }
+            if constexpr (DV) {
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(dt_ops.rows(0, st), vreg[st], dp);
+                for (int t = 0; t < 2; ++t) {
+                    u32x4 p;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                u32x4 p;
+                    for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(dt_ops.columns(16 * t, i), p, dv[i]);
+                    for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(dt_ops.columns(16 * t, i), p, dv[i]);
+                }
             }
+            if constexpr (DK) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= dp[r];
+                for (int r = 0; r < 16; ++r) s[r] *= dp[r];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                u32x4 p;
+                for (int t = 0; t < 2; ++t) {
+                    u32x4 p;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
+                    for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) dk[i] = Mma<T>::op(qt_ops.columns(16 * t, i), p, dk[i]);
+                    for (int i = 0; i < DP / 32; ++i) dk[i] = Mma<T>::op(qt_ops.columns(16 * t, i), p, dk[i]);
+                }
             }
         }
         landed();
@@ -1208,8 +1324,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
     }
     if (a.near_parts + far_of_tile == 1) {
         const bool there = key < a.sk;
-        store_rows<T, DP>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2]) * 2, dk, a.scale, a.d, there);
-        store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, 1.f, a.d, there);
+        if constexpr (DK) store_rows<T, DP>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2]) * 2, dk, a.scale, a.d, there);
+        if constexpr (DV) store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, 1.f, a.d, there);
         return;
     }
     float* const to = a.part_o + (grad_piece(a, bh, kt) + (far ? a.near_parts + part : part)) * 2 * kGradKeys * a.d + (key - key0) * a.d;
@@ -1220,8 +1336,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(Att
             for (int r = 0; r < 16; r += 4) {
                 const int dim = 32 * i + element_of(r, half);
                 if (dim < a.d) {
-                    *reinterpret_cast<f32x4*>(to + dim) = f32x4{dk[i][r], dk[i][r + 1], dk[i][r + 2], dk[i][r + 3]};
-                    *reinterpret_cast<f32x4*>(to + kGradKeys * a.d + dim) = f32x4{dv[i][r], dv[i][r + 1], dv[i][r + 2], dv[i][r + 3]};
+                    if constexpr (DK) *reinterpret_cast<f32x4*>(to + dim) = f32x4{dk[i][r], dk[i][r + 1], dk[i][r + 2], dk[i][r + 3]};
+                    if constexpr (DV) *reinterpret_cast<f32x4*>(to + kGradKeys * a.d + dim) = f32x4{dv[i][r], dv[i][r + 1], dv[i][r + 2], dv[i][r + 3]};
                 }
             }
     }

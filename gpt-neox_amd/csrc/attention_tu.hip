@@ -43,17 +43,22 @@ hipError_t launch_attn_token<NEOX_ATTN_DIM>(const AttnArgs& a, int source, int d
 }
 
 // the queries' kernel first: it leaves the rows' sums of dO * O that the keys' kernel needs
-template <>
-hipError_t launch_attn_bwd<NEOX_ATTN_DIM>(const AttnArgs& a, int dtype, hipStream_t stream) {
+template <typename T>
+static void backward(const AttnArgs& a, hipStream_t stream) {
     constexpr int DP = NEOX_ATTN_DIM;
     const uint32_t q = (uint32_t)a.b * a.kv * a.row_tiles, kv = (uint32_t)a.b * a.kv * a.units;
-    if (dtype == NEOX_BF16) {
-        attn_bwd_q_kernel<BF16, DP><<<q, 256, 0, stream>>>(a);
-        attn_bwd_kv_kernel<BF16, DP><<<kv, 256, 0, stream>>>(a);
+    attn_bwd_q_kernel<T, DP><<<q, 256, 0, stream>>>(a);
+    if constexpr (DP <= 128) {
+        attn_bwd_kv_kernel<T, DP, true, true><<<kv, 256, 0, stream>>>(a);
     } else {
-        attn_bwd_q_kernel<F16, DP><<<q, 256, 0, stream>>>(a);
-        attn_bwd_kv_kernel<F16, DP><<<kv, 256, 0, stream>>>(a);
+        attn_bwd_kv_kernel<T, DP, true, false><<<kv, 256, 0, stream>>>(a);
+        attn_bwd_kv_kernel<T, DP, false, true><<<kv, 256, 0, stream>>>(a);
     }
+}
+
+template <>
+hipError_t launch_attn_bwd<NEOX_ATTN_DIM>(const AttnArgs& a, int dtype, hipStream_t stream) {
+    dtype == NEOX_BF16 ? backward<BF16>(a, stream) : backward<F16>(a, stream);
     if (a.near_parts > 1 || a.far_parts > 0) {
         const dim3 grid((uint32_t)a.b * a.kv * (kGradKeys / 32), a.near_parts > 1 ? a.key_tiles : a.sink_tiles);
         dtype == NEOX_BF16 ? attn_bwd_join_kernel<BF16><<<grid, 256, 0, stream>>>(a) : attn_bwd_join_kernel<F16><<<grid, 256, 0, stream>>>(a);
