@@ -82,7 +82,8 @@ static int check_scale_window(float scale, int sinks, const char* what) {
 
 static void set_scale_window(AttnArgs& a, float scale, int window, int sinks) {
     a.scale = scale;
-    a.scale_log2 = (scale < 0.f ? -scale : scale) * kLog2e;
+    // (never 0: a hidden key's score is minus infinity before it is multiplied)
+    a.scale_log2 = __builtin_fmaxf((scale < 0.f ? -scale : scale) * kLog2e, __FLT_MIN__);
     a.flip = scale < 0.f ? 0x80008000u : 0u;
     a.window = window < 0 || window >= kMost ? -1 : window;
     a.sinks = sinks < kMost ? sinks : kMost;
