@@ -308,6 +308,196 @@ std::optional<Tensor> rope(const Tensor& x, const Tensor& cos, const std::option
     return rope_whole(x, t, transposed, false);
 }
 
+// ---- attention over windows and pages ---------------------------------------------------------------
+// a 16-bit tensor [.., heads, d] that the attention kernels read as it lies (as whole_pieces in _lib.py)
+bool in_pieces(const Tensor& x, int64_t per_piece = 8) {
+    if (x.stride(-1) != 1 || reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 != 0) return false;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i)
+        if (x.size(i) > 1 && (x.stride(i) % per_piece != 0 || x.stride(i) < 0 || x.stride(i) >= (int64_t)1 << 31)) return false;
+    return x.size(-2) == 1 || x.stride(-2) >= x.size(-1);
+}
+// the strides of all axes but the dense last one; an axis of one element counts as 0
+struct RowStrides {
+    int64_t of[3] = {0, 0, 0};
+    RowStrides(const Tensor& x, int64_t axes) {
+        for (int64_t i = 0; i < axes; ++i) of[i] = x.size(i) > 1 ? x.stride(i) : 0;
+    }
+    operator const int64_t*() const { return of; }
+};
+template <typename T>
+T* pointer_or_null(const std::optional<Tensor>& t) {
+    return t ? static_cast<T*>(const_cast<void*>(t->const_data_ptr())) : nullptr;
+}
+
+struct WindowCall {
+    double scale;
+    int64_t window, sinks;
+    const std::optional<Tensor>& lengths;
+};
+
+std::tuple<Tensor, Tensor> window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const WindowCall& c, bool want_lse) {
+    const c10::DeviceGuard guard(q.device());
+    const auto sq = (int32_t)q.size(0), b = (int32_t)q.size(1), h = (int32_t)q.size(2), d = (int32_t)q.size(3);
+    Tensor out = at::empty(q.sizes(), q.options()), lse;
+    if (want_lse) lse = at::empty({(int64_t)b * h * sq}, q.options().dtype(at::kFloat));
+    check(neox_window_attention_fwd(out.mutable_data_ptr(), want_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr,
+                                    q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), pointer_or_null<const int32_t>(c.lengths),
+                                    b, sq, (int32_t)k.size(0), h, (int32_t)k.size(2), d, RowStrides(q, 3), RowStrides(k, 3),
+                                    RowStrides(v, 3), RowStrides(out, 3), (float)c.scale, (int32_t)c.window, (int32_t)c.sinks, code(q),
+                                    stream_of(q)));
+    return {out, lse};
+}
+
+class WindowAttention : public torch::autograd::Function<WindowAttention> {
+public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const WindowCall& c) {
+        auto [out, lse] = window_forward(q, k, v, c, true);
+        ctx->save_for_backward({q, k, v, out, lse, c.lengths ? *c.lengths : Tensor()});
+        ctx->saved_data["scale"] = c.scale;
+        ctx->saved_data["window"] = c.window;
+        ctx->saved_data["sinks"] = c.sinks;
+        return out;
+    }
+    // A saved-tensor hook may have given back other tensors than were left with it: everything the kernels take for
+    // granted is looked at again.
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list v = ctx->get_saved_variables();
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        Tensor g = grads[0];
+        const Tensor lengths = v[5];
+        v.resize(5);
+        for (const Tensor& t : v)
+            if (!on_gpu(t) || t.device() != g.device()) throw std::runtime_error("the saved tensors must be on the device of the gradient");
+        const Tensor &q0 = v[0], &k0 = v[1], &v0 = v[2], &out0 = v[3];
+        const Tensor lse = v[4].contiguous();
+        if (q0.dim() != 4 || k0.dim() != 4 || k0.sizes() != v0.sizes() || out0.sizes() != q0.sizes() || g.sizes() != q0.sizes() ||
+            k0.size(1) != q0.size(1) || k0.size(3) != q0.size(3) || !half_type(q0) || !on_gpu(g) || g.scalar_type() != q0.scalar_type() ||
+            k0.scalar_type() != q0.scalar_type() || v0.scalar_type() != q0.scalar_type() || out0.scalar_type() != q0.scalar_type() ||
+            lse.scalar_type() != at::kFloat || lse.numel() != q0.size(0) * q0.size(1) * q0.size(2))
+            throw std::runtime_error("the gradient and the saved tensors must have the shapes and dtypes of the forward pass");
+        if (lengths.defined() && (!on_gpu(lengths) || lengths.device() != g.device() || lengths.scalar_type() != at::kInt ||
+                                  lengths.numel() != q0.size(1) || !lengths.is_contiguous()))
+            throw std::runtime_error("the saved key lengths have changed");
+        auto readable = [](const Tensor& t) { return in_pieces(t) ? t : t.clone(at::MemoryFormat::Contiguous); };
+        const Tensor q = readable(q0), k = readable(k0), val = readable(v0), out = readable(out0);
+        g = readable(g);
+        const c10::DeviceGuard guard(q.device());
+        const auto sq = (int32_t)q.size(0), b = (int32_t)q.size(1), h = (int32_t)q.size(2), d = (int32_t)q.size(3);
+        const auto sk = (int32_t)k.size(0), h_kv = (int32_t)k.size(2);
+        const auto window = (int32_t)ctx->saved_data["window"].toInt(), sinks = (int32_t)ctx->saved_data["sinks"].toInt();
+        Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
+        int64_t bytes = 0;
+        check(neox_window_attention_bwd_workspace(&bytes, b, sq, sk, h, h_kv, d, window, sinks));
+        const Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+        check(neox_window_attention_bwd(
+            dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), workspace.mutable_data_ptr(), bytes, g.const_data_ptr(),
+            out.const_data_ptr(), static_cast<const float*>(lse.const_data_ptr()), q.const_data_ptr(), k.const_data_ptr(),
+            val.const_data_ptr(), lengths.defined() ? static_cast<const int32_t*>(lengths.const_data_ptr()) : nullptr, b, sq, sk, h, h_kv, d,
+            RowStrides(dq, 3), RowStrides(dk, 3), RowStrides(dv, 3), RowStrides(g, 3), RowStrides(out, 3), RowStrides(q, 3),
+            RowStrides(k, 3), RowStrides(val, 3), (float)ctx->saved_data["scale"].toDouble(), window, sinks, code(q), stream_of(q)));
+        return {dq, dk, dv, Tensor()};
+    }
+};
+
+bool int_list(const Tensor& t, const Tensor& like, int64_t n) {
+    return on_gpu(t) && t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+bool attention_heads(const Tensor& x) { return plain_heads(x) && x.size(3) % 8 == 0 && x.size(3) <= 256 && in_pieces(x); }
+
+// q [sq, b, h, d], k, v [sk, b, h_kv, d]; window < 0: none; lengths int32 [b] -> [sq, b, h, d], or None
+std::optional<Tensor> window_attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, int64_t window, int64_t sinks,
+                                       const std::optional<Tensor>& lengths) {
+    if (!attention_heads(q) || !attention_heads(k) || !attention_heads(v) || k.device() != q.device() || v.device() != q.device() ||
+        k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() || k.sizes() != v.sizes() || k.size(1) != q.size(1) ||
+        k.size(3) != q.size(3) || q.size(2) % k.size(2) != 0 || window > INT32_MAX || window < -1 || !fits_int32(sinks) ||
+        (lengths && !int_list(*lengths, q, q.size(1))))
+        return std::nullopt;
+    const WindowCall c{scale, window, sinks, lengths};
+    if (records(q) || records(k) || records(v)) return WindowAttention::apply(q, k, v, c);
+    return std::get<0>(window_forward(q, k, v, c, false));
+}
+
+// The tensors of a PagedKVCache, which has looked at them; `like` is a 16-bit tensor of the call.
+struct Cache {
+    const Tensor &k, &v;
+    const std::optional<Tensor>&k_scale, &v_scale;
+    int32_t dtype(const Tensor& like) const {
+        switch (k.scalar_type()) {
+            case at::kChar: return NEOX_I8;
+            case at::kFloat8_e4m3fn: return NEOX_F8;
+            default: return code(like);
+        }
+    }
+    bool goes_with(const Tensor& like) const {
+        return half_type(like) && (k_scale ? (k.scalar_type() == at::kChar || k.scalar_type() == at::kFloat8_e4m3fn) : k.scalar_type() == like.scalar_type()) &&
+               k.device() == like.device() && k.dim() == 4 && like.size(-1) == k.size(3);
+    }
+};
+RowStrides scale_strides(const std::optional<Tensor>& t) { return t ? RowStrides(*t, 3) : RowStrides(Tensor(), 0); }
+
+bool slot_list(const Tensor& t, const Tensor& like) {
+    return on_gpu(t) && t.device() == like.device() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.dim() == 1 &&
+           t.numel() > 0 && t.is_contiguous();
+}
+
+// k, v [tokens, heads, d] into slots [tokens]; whether that was done
+bool cache_write(const Tensor& kc, const Tensor& vc, const std::optional<Tensor>& ks, const std::optional<Tensor>& vs, const Tensor& k,
+                 const Tensor& v, const Tensor& slots) {
+    const Cache cache{kc, vc, ks, vs};
+    if (!on_gpu(k) || !on_gpu(v) || k.dim() != 3 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || v.device() != k.device() ||
+        !cache.goes_with(k) || k.size(1) != kc.size(2) || !slot_list(slots, k) || slots.size(0) != k.size(0) || !in_pieces(k) || !in_pieces(v))
+        return false;
+    const c10::DeviceGuard guard(k.device());
+    check(neox_cache_write(kc.mutable_data_ptr(), vc.mutable_data_ptr(), pointer_or_null<float>(ks), pointer_or_null<float>(vs),
+                           k.const_data_ptr(), v.const_data_ptr(), slots.const_data_ptr(), slots.scalar_type() == at::kLong, k.size(0),
+                           (int32_t)k.size(1), (int32_t)k.size(2), kc.size(0), (int32_t)kc.size(1), RowStrides(kc, 3), RowStrides(vc, 3),
+                           scale_strides(ks), scale_strides(vs), RowStrides(k, 2), RowStrides(v, 2), code(k), cache.dtype(k), stream_of(k)));
+    return true;
+}
+
+// the slots' keys and values in fp16 or bf16, or None
+std::optional<std::tuple<Tensor, Tensor>> cache_read(const Tensor& kc, const Tensor& vc, const std::optional<Tensor>& ks,
+                                                     const std::optional<Tensor>& vs, const Tensor& slots, at::ScalarType dtype) {
+    if (!slot_list(slots, kc) || (dtype != at::kHalf && dtype != at::kBFloat16) || (!ks && dtype != kc.scalar_type())) return std::nullopt;
+    const Cache cache{kc, vc, ks, vs};
+    const c10::DeviceGuard guard(kc.device());
+    Tensor k = at::empty({slots.size(0), kc.size(2), kc.size(3)}, kc.options().dtype(dtype)), v = at::empty_like(k);
+    check(neox_cache_read(k.mutable_data_ptr(), v.mutable_data_ptr(), kc.const_data_ptr(), vc.const_data_ptr(), pointer_or_null<const float>(ks),
+                          pointer_or_null<const float>(vs), slots.const_data_ptr(), slots.scalar_type() == at::kLong, slots.size(0),
+                          (int32_t)kc.size(2), (int32_t)kc.size(3), kc.size(0), (int32_t)kc.size(1), RowStrides(k, 2), RowStrides(v, 2),
+                          RowStrides(kc, 3), RowStrides(vc, 3), scale_strides(ks), scale_strides(vs), code(k), cache.dtype(k), stream_of(k)));
+    return std::make_tuple(k, v);
+}
+
+// q [tokens, h, d] over the pages of a cache -> [tokens, h, d], or None; max_context < 0: what the table has room for
+std::optional<Tensor> paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const std::optional<Tensor>& ks,
+                                      const std::optional<Tensor>& vs, const Tensor& table, const Tensor& starts, const Tensor& lengths,
+                                      int64_t max_query, int64_t max_context, double scale, int64_t window, int64_t sinks) {
+    const Cache cache{kc, vc, ks, vs};
+    if (!on_gpu(q) || q.dim() != 3 || q.numel() == 0 || !cache.goes_with(q) || q.size(1) % kc.size(2) != 0 || !fits_int32(q.size(0)) ||
+        !in_pieces(q) || lengths.dim() != 1 || !int_list(lengths, q, lengths.size(0)) || !int_list(starts, q, lengths.size(0) + 1) ||
+        !on_gpu(table) || table.device() != q.device() || table.scalar_type() != at::kInt || table.dim() != 2 ||
+        table.size(0) != lengths.size(0) || table.size(0) < 1 || table.size(1) < 1 || table.stride(1) != 1 || table.stride(0) < 0 ||
+        !fits_int32(table.size(1)) || !fits_int32(max_query) || window > INT32_MAX || window < -1 || !fits_int32(sinks))
+        return std::nullopt;
+    if (max_context < 0) max_context = table.size(1) * kc.size(1);
+    if (!fits_int32(max_context)) return std::nullopt;
+    const c10::DeviceGuard guard(q.device());
+    const auto tokens = (int32_t)q.size(0), h = (int32_t)q.size(1), d = (int32_t)q.size(2), b = (int32_t)lengths.size(0), h_kv = (int32_t)kc.size(2);
+    Tensor out = at::empty(q.sizes(), q.options()), workspace;
+    int64_t bytes = 0;
+    check(neox_paged_attention_workspace(&bytes, b, tokens, (int32_t)max_query, (int32_t)max_context, h, h_kv, d, (int32_t)window, (int32_t)sinks));
+    if (bytes) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+    check(neox_paged_attention(out.mutable_data_ptr(), bytes ? workspace.mutable_data_ptr() : nullptr, bytes, q.const_data_ptr(),
+                               kc.const_data_ptr(), vc.const_data_ptr(), pointer_or_null<const float>(ks), pointer_or_null<const float>(vs),
+                               static_cast<const int32_t*>(table.const_data_ptr()), static_cast<const int32_t*>(starts.const_data_ptr()),
+                               static_cast<const int32_t*>(lengths.const_data_ptr()), b, tokens, (int32_t)max_query, (int32_t)max_context, h,
+                               h_kv, d, kc.size(0), (int32_t)kc.size(1), (int32_t)table.size(1), table.size(0) > 1 ? table.stride(0) : 0,
+                               RowStrides(out, 2), RowStrides(q, 2), RowStrides(kc, 3), RowStrides(vc, 3), scale_strides(ks),
+                               scale_strides(vs), (float)scale, (int32_t)window, (int32_t)sinks, code(q), cache.dtype(q), stream_of(q)));
+    return out;
+}
+
 }  // namespace
 
 // The interpreter is not held while a launch waits for room in its queue.  An exception that a saved-tensor hook
@@ -323,5 +513,10 @@ PYBIND11_MODULE(neox_torch, m) {
     m.def("masked_softmax", wrap_pybind_function_no_gil(masked_softmax), py::arg("x"), py::arg("mask"), py::arg("scale"));
     m.def("rotary", wrap_pybind_function_no_gil(rotary), py::arg("q"), py::arg("k"), py::arg("cos"), py::arg("sin"),
           py::arg("offset"));
+    m.def("window_attention", wrap_pybind_function_no_gil(window_attention), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("scale"),
+          py::arg("window"), py::arg("sinks"), py::arg("lengths"));
+    m.def("cache_write", wrap_pybind_function_no_gil(cache_write));
+    m.def("cache_read", wrap_pybind_function_no_gil(cache_read));
+    m.def("paged_attention", wrap_pybind_function_no_gil(paged_attention));
     m.def("rope", wrap_pybind_function_no_gil(rope), py::arg("x"), py::arg("cos"), py::arg("sin"), py::arg("transposed"));
 }

@@ -95,6 +95,12 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, key_lengths=N
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
             raise RuntimeError(f"expected 4D tensor, got {name} with {t.dim()} dims")
+    w, n = check_window(window, sinks)
+    calls = _lib.calls(q, k, v) if key_lengths is None or type(key_lengths) is torch.Tensor else None
+    if calls is not None:
+        out = calls.window_attention(q, k, v, (1.0 / math.sqrt(max(1, q.shape[3]))) if scale is None else scale, w, n, key_lengths)
+        if out is not None:
+            return out
     if q.dtype not in _HALF:
         raise RuntimeError("Only fp16 and bf16 are supported")
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -116,9 +122,8 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, key_lengths=N
     for t in (k, v, key_lengths):
         if t is not None and t.device != q.device:
             raise RuntimeError("all tensors must be on the same device")
-    window, sinks = check_window(window, sinks)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) or (
             _lib.in_dual_level() and _lib.carries_tangent(q, k, v)):
-        return WindowAttention.apply(q, k, v, scale, window, sinks, key_lengths)
-    return _forward(q, k, v, scale, window, sinks, key_lengths, False)[0]
+        return WindowAttention.apply(q, k, v, scale, w, n, key_lengths)
+    return _forward(q, k, v, scale, w, n, key_lengths, False)[0]

@@ -93,6 +93,9 @@ class PagedKVCache:
     def write(self, k, v, slots):
         """Quantises (or copies) ``k``, ``v`` ``[tokens, heads, dim]`` into ``slots`` ``[tokens]``.  A negative slot, or one
         behind the end, is skipped; no slot may be named twice."""
+        calls = _lib.calls(k, v, slots)
+        if calls is not None and calls.cache_write(self.k, self.v, self.k_scale, self.v_scale, k, v, slots):
+            return
         slots = self._check_slots(slots)
         shape = (slots.shape[0], self.heads, self.dim)
         if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
@@ -113,6 +116,11 @@ class PagedKVCache:
     def read(self, slots, dtype=torch.bfloat16):
         """The keys and values of ``slots`` ``[tokens]``, each ``[tokens, heads, dim]`` in ``dtype`` (fp16 or bf16; of a cache
         in 16 bits: its own); zeros for a slot outside the cache."""
+        calls = _lib.calls(slots)
+        if calls is not None:
+            out = calls.cache_read(self.k, self.v, self.k_scale, self.v_scale, slots, dtype)
+            if out is not None:
+                return out
         slots = self._check_slots(slots)
         code = self._code(dtype)
         k, v = (torch.empty((slots.shape[0], self.heads, self.dim), dtype=dtype, device=self.device) for _ in "kv")
@@ -141,12 +149,22 @@ def paged_attention(q, cache, page_table, query_starts, context_lengths, *, max_
     ``query_starts[s + 1]`` (int32 ``[b + 1]``).  Its keys, those of its new tokens among them, are already in ``cache``:
     ``context_lengths[s]`` of them (int32 ``[b]``), key ``j`` in page ``page_table[s, j // page_size]`` (int32
     ``[b, columns]``).  The last token stands at the last key; ``window`` and ``sinks`` as in ``window_attention``.  A token that
-    sees no key gets zeros; a row of ``q`` that no sequence covers is left unspecified.
+    sees no key gets zeros; a row of ``q`` that no sequence covers is left unspecified.  There is no backward pass.
 
     ``max_query`` and ``max_context`` (default: what ``page_table`` has room for) are known to the host and must not be
     smaller than the longest entries of the tensors, which only the kernels look at: they choose the kernel and the number
     of parts that the keys are split into.  What a table says beyond them is not computed.
     """
+    if torch.is_grad_enabled() and q.requires_grad or _lib.in_dual_level() and _lib.carries_tangent(q):
+        raise RuntimeError("paged_attention computes no gradients: call it under torch.no_grad() or on q.detach()")
+    window, sinks = check_window(window, sinks)
+    calls = _lib.calls(q, page_table, query_starts, context_lengths)
+    if calls is not None:
+        out = calls.paged_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, query_starts, context_lengths, max_query,
+                                    -1 if max_context is None else max_context, 1.0 / math.sqrt(cache.dim) if scale is None else scale,
+                                    window, sinks)
+        if out is not None:
+            return out
     if q.dim() != 3:
         raise RuntimeError(f"expected 3D tensor, got q with {q.dim()} dims")
     code = cache._code(q.dtype)
@@ -167,7 +185,6 @@ def paged_attention(q, cache, page_table, query_starts, context_lengths, *, max_
             raise RuntimeError("all tensors must be on the same device")
     if max_context is None:
         max_context = page_table.shape[1] * cache.page_size
-    window, sinks = check_window(window, sinks)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out = torch.empty((tokens, h, d), dtype=q.dtype, device=q.device)
     if tokens == 0:

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from gpt_neox_amd import _lib
 from gpt_neox_amd.paged_cache import PagedKVCache, paged_attention, slots_of
 from oracle import attention as A
 
@@ -357,6 +358,20 @@ def test_on_another_stream(device):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("codes", [I8, torch.float16])
+def test_without_the_native_calls_the_same_bits(device, codes, monkeypatch):
+    def everything():
+        q, cache, table, starts, lengths = sequences(device, torch.float16, codes, [1, 30], [3000, 900], 8, 2, 128, 64)
+        return (paged_attention(q, cache, table, starts, lengths, max_query=30, window=700, sinks=2),
+                paged_attention(q[:1], cache, table[:1], starts[:2], lengths[:1], max_query=1, max_context=3000),
+                *cache.read(torch.arange(60, device=device), torch.float16))
+
+    want = everything()
+    monkeypatch.setattr(_lib, "calls", lambda *tensors: None)
+    for x, y in zip(want, everything()):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+
+
 def test_no_tokens_at_all(device):
     q, cache, table, starts, lengths = sequences(device, torch.bfloat16, I8, [1], [10], 4, 2, 64, 16)
     assert paged_attention(q[:0], cache, table, starts * 0, lengths, max_query=1).shape == (0, 4, 64)
@@ -390,6 +405,8 @@ def test_refusals(device):
         with pytest.raises(RuntimeError, match=message):
             call()
     q = torch.zeros((2, 4, 64), dtype=torch.bfloat16, device=device)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        paged_attention(q.clone().requires_grad_(), cache, None, None, None, max_query=1)
     table = torch.zeros((2, 3), dtype=torch.int32, device=device)
     starts, lengths = torch.tensor([0, 1, 2], dtype=torch.int32, device=device), torch.tensor([5, 6], dtype=torch.int32, device=device)
     for change, message in (

@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from gpt_neox_amd import _lib
 from gpt_neox_amd.fused_attention import window_attention
 from oracle import attention as A
 
@@ -224,6 +225,28 @@ def test_on_another_stream(device):
         got = run(*args, window=100, sinks=4)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_without_the_native_calls_the_same_bits(device, monkeypatch):
+    args = inputs(300, 300, 2, 4, 2, 96, torch.float16, device)
+    kw = dict(window=100, sinks=4, key_lengths=torch.tensor([300, 77], dtype=torch.int32, device=device))
+    want = run(*args, **kw)
+    monkeypatch.setattr(_lib, "calls", lambda *tensors: None)
+    assert all(torch.equal(x, y) for x, y in zip(want, run(*args, **kw)))
+
+
+def test_saved_tensor_hooks(device):
+    args = inputs(130, 130, 1, 4, 2, 64, torch.bfloat16, device)
+    want = run(*args, window=30, sinks=1)
+    with torch.autograd.graph.save_on_cpu():
+        q, k, v = (t.clone().requires_grad_() for t in args[:3])
+        out = window_attention(q, k, v, window=30, sinks=1)
+    got = torch.autograd.grad(out, (q, k, v), args[3])
+    assert all(torch.equal(x, y) for x, y in zip(want[1:], got))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.float() if t.dtype == torch.bfloat16 else t):
+        out = window_attention(q, k, v, window=30, sinks=1)
+    with pytest.raises(RuntimeError, match="shapes and dtypes"):
+        out.backward(args[3])
 
 
 def test_gradients_are_only_those_asked_for(device):
