@@ -15,11 +15,16 @@ hipError_t launch_attn_join(const AttnArgs& a, int dtype, hipStream_t stream) {
 
 template <typename T, int SRC, bool WRITE>
 static void cache_rows(const CacheArgs& a, hipStream_t stream) {
-    const int lanes = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
+    constexpr int kElems = cache_elems<SRC, WRITE>();
+    const int lanes = a.d <= kElems * 4 ? 4 : a.d <= kElems * 8 ? 8 : a.d <= kElems * 16 ? 16 : 32;
     const uint32_t blocks = (uint32_t)((a.rows * lanes + 255) / 256);
-    if (lanes == 8) cache_kernel<T, SRC, 8, WRITE><<<blocks, 256, 0, stream>>>(a);
-    else if (lanes == 16) cache_kernel<T, SRC, 16, WRITE><<<blocks, 256, 0, stream>>>(a);
-    else cache_kernel<T, SRC, 32, WRITE><<<blocks, 256, 0, stream>>>(a);
+    switch (lanes) {
+        case 4: cache_kernel<T, SRC, 4, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        case 8: cache_kernel<T, SRC, 8, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        case 16: cache_kernel<T, SRC, 16, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        default:
+            if constexpr (kElems == 8) cache_kernel<T, SRC, 32, WRITE><<<blocks, 256, 0, stream>>>(a);
+    }
 }
 template <typename T, bool WRITE>
 static void cache_source(const CacheArgs& a, int source, hipStream_t stream) {
@@ -293,6 +298,8 @@ static int cache_call(const char* what, void* k, void* v, const void* kc, const 
     a.heads = h_kv;
     a.d = d;
     a.page = page_size;
+    a.by_heads = FastDiv::by((uint32_t)h_kv);
+    a.by_page = FastDiv::by((uint32_t)page_size);
     return check_launch(launch_cache(a, source, dtype, write, (hipStream_t)stream), what);
 }
 

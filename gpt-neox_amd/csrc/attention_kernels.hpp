@@ -228,9 +228,26 @@ __device__ __forceinline__ void decode8(const u32x2& w, float (&f)[8]) {
         }
     }
 }
+// two 8-bit floats of a word, the lower or the upper, as 16-bit values
+template <typename T>
+__device__ __forceinline__ uint32_t widen2(uint32_t word, bool upper) {
+    if constexpr (__is_same(T, BF16)) {
+        const auto x = upper ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.f, false);
+        return __builtin_bit_cast(uint32_t, x);
+    } else {
+        const auto x = upper ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.f, false);
+        return __builtin_bit_cast(uint32_t, x);
+    }
+}
 // ... and as 16-bit values, exactly: no code has more than 7 bits of significand
 template <typename T, int SRC>
 __device__ __forceinline__ u32x4 widen8(const u32x2& w) {
+    if constexpr (SRC == kPagedF8) {
+        u32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = widen2<T>(i < 2 ? w.x : w.y, i & 1);
+        return x;
+    }
     float f[8];
     decode8<SRC>(w, f);
     return pack8<T>(f);
