@@ -95,11 +95,11 @@ SIGNATURES = {
          _c_i64p, _i64, _i32, _i32, _i32, _vp],
     ),
     "neox_window_attention_fwd": (
-        ctypes.c_int, [_vp] * 6 + [_i32] * 6 + [_c_i64p] * 4 + [_f32, _i32, _i32, _i32, _vp]
+        ctypes.c_int, [_vp] * 7 + [_i32] * 6 + [_c_i64p] * 4 + [_f32, _i32, _i32, _i32, _vp]
     ),
     "neox_window_attention_bwd_workspace": (ctypes.c_int, [_c_i64p] + [_i32] * 8),
     "neox_window_attention_bwd": (
-        ctypes.c_int, [_vp] * 4 + [_i64] + [_vp] * 7 + [_i32] * 6 + [_c_i64p] * 8 + [_f32, _i32, _i32, _i32, _vp]
+        ctypes.c_int, [_vp] * 4 + [_i64] + [_vp] * 8 + [_i32] * 6 + [_c_i64p] * 8 + [_f32, _i32, _i32, _i32, _vp]
     ),
     "neox_paged_attention_workspace": (ctypes.c_int, [_c_i64p] + [_i32] * 9),
     "neox_paged_attention": (
@@ -294,6 +294,11 @@ def strides3(t):
             _strides3_cache.clear()
         arr = _strides3_cache[key] = (ctypes.c_int64 * 3)(*key)
     return arr
+
+
+def ptr(t):
+    """The address of a tensor's data, or None for None."""
+    return t.data_ptr() if t is not None else None
 
 
 def row_strides(t):

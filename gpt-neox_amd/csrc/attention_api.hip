@@ -310,7 +310,7 @@ using namespace neox;
 #pragma GCC visibility push(default)
 extern "C" {
 
-int neox_window_attention_fwd(void* out, float* lse, const void* q, const void* k, const void* v, const int32_t* key_lengths, int32_t b,
+int neox_window_attention_fwd(void* out, void* out_low, float* lse, const void* q, const void* k, const void* v, const int32_t* key_lengths, int32_t b,
                               int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d, const int64_t q_strides[3],
                               const int64_t k_strides[3], const int64_t v_strides[3], const int64_t out_strides[3], float scale,
                               int32_t window, int32_t sinks, int32_t dtype, void* stream) {
@@ -320,7 +320,7 @@ int neox_window_attention_fwd(void* out, float* lse, const void* q, const void* 
     NEOX_TRY(check_pointer(q, 16, what, "q"));
     NEOX_TRY(check_pointer(k, 16, what, "k"));
     NEOX_TRY(check_pointer(v, 16, what, "v"));
-    if (!aligned(lse, 4) || !aligned(key_lengths, 4)) return fail(NEOX_ERR_MISALIGNED, "%s: misaligned pointer", what);
+    if (!aligned(out_low, 16) || !aligned(lse, 4) || !aligned(key_lengths, 4)) return fail(NEOX_ERR_MISALIGNED, "%s: misaligned pointer", what);
     NEOX_TRY(check_window_sizes(b, sq, sk, h, h_kv, d, what));
     NEOX_TRY(check_strides(q_strides, 3, h, d, 8, what, "q"));
     NEOX_TRY(check_strides(k_strides, 3, h_kv, d, 8, what, "k"));
@@ -334,6 +334,7 @@ int neox_window_attention_fwd(void* out, float* lse, const void* q, const void* 
     a.k = static_cast<const char*>(k);
     a.v = static_cast<const char*>(v);
     a.o = static_cast<char*>(out);
+    a.o_low = static_cast<char*>(out_low);
     a.lse = lse;
     a.lengths = key_lengths;
     copy_strides(a.q_st, q_strides);
@@ -353,7 +354,7 @@ int neox_window_attention_bwd_workspace(int64_t* bytes, int32_t b, int32_t sq, i
     return NEOX_OK;
 }
 
-int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, const void* dout, const void* out, const float* lse, const void* q,
+int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, const void* dout, const void* out, const void* out_low, const float* lse, const void* q,
                               const void* k, const void* v, const int32_t* key_lengths, int32_t b, int32_t sq, int32_t sk, int32_t h,
                               int32_t h_kv, int32_t d, const int64_t dq_strides[3], const int64_t dk_strides[3],
                               const int64_t dv_strides[3], const int64_t dout_strides[3], const int64_t out_strides[3],
@@ -373,7 +374,7 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int
     for (const Given& g : given) NEOX_TRY(check_pointer(g.p, 16, what, g.name));
     NEOX_TRY(check_pointer(lse, 4, what, "lse"));
     NEOX_TRY(check_pointer(workspace, 16, what, "workspace"));
-    if (!aligned(key_lengths, 4)) return fail(NEOX_ERR_MISALIGNED, "%s: misaligned pointer", what);
+    if (!aligned(out_low, 16) || !aligned(key_lengths, 4)) return fail(NEOX_ERR_MISALIGNED, "%s: misaligned pointer", what);
     NEOX_TRY(check_window_sizes(b, sq, sk, h, h_kv, d, what));
     for (const Given& g : given) NEOX_TRY(check_strides(g.st, 3, g.grouped ? h_kv : h, d, 8, what, g.name));
     NEOX_TRY(check_scale_window(scale, sinks, what));
@@ -397,6 +398,7 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int
     a.k = static_cast<const char*>(k);
     a.v = static_cast<const char*>(v);
     a.out = static_cast<const char*>(out);
+    a.o_low = static_cast<char*>(const_cast<void*>(out_low));
     a.dout = static_cast<const char*>(dout);
     a.dq = static_cast<char*>(dq);
     a.dk = static_cast<char*>(dk);

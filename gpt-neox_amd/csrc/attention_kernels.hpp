@@ -44,6 +44,7 @@ enum KvSource { kStrided = 0, kPaged16 = 1, kPagedI8 = 2, kPagedF8 = 3 };
 struct AttnArgs {
     const char *q, *k, *v;       // 16-bit elements (k, v: 8-bit codes for the last two sources)
     char* o;
+    char* o_low;                 // null, or what rounding the output to 16 bits took away, laid out like the output
     float* lse;                  // log2 of every row's sum of exponentials, +inf for an empty row; [b, kv, rows]
     const float *k_scale, *v_scale;
     // element strides.  q, o: token, sample (strided only), head.  k, v: token, sample, head; for pages the token
@@ -85,6 +86,17 @@ struct AttnArgs {
     int near_parts, far_parts, sink_tiles, units;
     FastDiv by_units, by_near_parts, by_far_parts;
 };
+
+// While a wave feeds the matrix cores it goes before the waves that compute exponentials (8192 tokens of 128-dim
+// heads, window 4096, us: forward 510 -> 474, queries' gradient 696 -> 678).  It also keeps the compiler from moving
+// work in or out, which costs the kernels that have no registers to spare: the key gradients (960 -> 1580) and codes
+// (242 -> 250) go without.
+__device__ __forceinline__ void matrix_first(bool on) {
+    if (on) __builtin_amdgcn_s_setprio(1);
+}
+__device__ __forceinline__ void matrix_done(bool on) {
+    if (on) __builtin_amdgcn_s_setprio(0);
+}
 
 template <typename T>
 struct Mma;
@@ -190,21 +202,40 @@ __device__ __forceinline__ u32x4 load8(const char* p, bool there) {
 }
 
 // Writes the 32 columns' results of one wave (lane: column, registers: 32 dims per block) times f as rows of 16-bit
-// elements.  The halves exchange registers, so that every lane stores 16 bytes.
-template <typename T, int DP>
-__device__ __forceinline__ void store_rows(char* row, const f32x16 (&acc)[DP / 32], float f, int d, bool there) {
+// elements, and at `low` (where that is not null) what the rounding took from them.  The halves exchange registers, so
+// that every lane stores 16 bytes.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_with_rest(float x, float y, uint32_t& rest) {
+    const uint32_t w = Elem<T>::pack(x, y);
+    float a, b;
+    Elem<T>::unpack(w, a, b);
+    rest = Elem<T>::pack(x - a, y - b);
+    return w;
+}
+template <typename T, int DP, bool LOW = false>
+__device__ __forceinline__ void store_rows(char* row, const f32x16 (&acc)[DP / 32], float f, int d, bool there, char* low = nullptr) {
     const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            const int r = 8 * p;
-            const uint32_t a0 = Elem<T>::pack(acc[b][r] * f, acc[b][r + 1] * f), a1 = Elem<T>::pack(acc[b][r + 2] * f, acc[b][r + 3] * f);
-            const uint32_t b0 = Elem<T>::pack(acc[b][r + 4] * f, acc[b][r + 5] * f), b1 = Elem<T>::pack(acc[b][r + 6] * f, acc[b][r + 7] * f);
-            const auto x = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+            uint32_t w[4], rest[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = acc[b][8 * p + 2 * i] * f, y = acc[b][8 * p + 2 * i + 1] * f;
+                if constexpr (LOW) w[i] = pack_with_rest<T>(x, y, rest[i]);
+                else w[i] = Elem<T>::pack(x, y);
+            }
             const int dim = 32 * b + 16 * p + 8 * half;
-            if (there && dim < d) *reinterpret_cast<u32x4*>(row + dim * 2) = u32x4{x[0], y[0], x[1], y[1]};
+            const bool ok = there && dim < d;
+            const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+            if (ok) *reinterpret_cast<u32x4*>(row + dim * 2) = u32x4{x[0], y[0], x[1], y[1]};
+            if constexpr (LOW) {
+                const auto u = __builtin_amdgcn_permlane32_swap(rest[0], rest[2], false, false);
+                const auto v = __builtin_amdgcn_permlane32_swap(rest[1], rest[3], false, false);
+                if (ok) *reinterpret_cast<u32x4*>(low + dim * 2) = u32x4{u[0], v[0], u[1], v[1]};
+            }
         }
     }
 }
@@ -574,8 +605,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
             for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+                matrix_first(!kCodes);
 #pragma unroll
                 for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s[kb]);
+                matrix_done(!kCodes);
             }
             if constexpr (kCodes) {
                 const float* f = scales + buffer * 2 * kFwdKeys;
@@ -643,8 +676,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
                 u32x4 p;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[t >> 1][8 * (t & 1) + 2 * e], s[t >> 1][8 * (t & 1) + 2 * e + 1]);
+                matrix_first(!kCodes);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(vt_ops.columns(16 * t, i), p, acc[i]);
+                matrix_done(!kCodes);
             }
         }
         if (it + 1 < end_tile) {
@@ -673,8 +708,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
             }
         if (there && half == 0) a.part_lse[slot] = total == 0.f ? kNegInf : m + __builtin_amdgcn_logf(total);
     } else {
-        char* p = a.o + ((int64_t)(token0 + token) * a.o_st[0] + (kPages ? 0 : (int64_t)b * a.o_st[1]) + (int64_t)head * a.o_st[2]) * 2;
-        store_rows<T, DP>(p, acc, inverse, a.d, there);
+        const int64_t at = ((int64_t)(token0 + token) * a.o_st[0] + (kPages ? 0 : (int64_t)b * a.o_st[1]) + (int64_t)head * a.o_st[2]) * 2;
+        if (!kPages && a.o_low) store_rows<T, DP, true>(a.o + at, acc, inverse, a.d, there, a.o_low + at);
+        else store_rows<T, DP>(a.o + at, acc, inverse, a.d, there);
         if (!kPages && a.lse && there && half == 0)
             a.lse[(int64_t)bh * rows + row] = total == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(total);
     }
@@ -1010,7 +1046,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
     {
         const char* qp = a.q + ((int64_t)token * a.q_st[0] + (int64_t)b * a.q_st[1] + (int64_t)head * a.q_st[2]) * 2;
         const char* dp = a.dout + ((int64_t)token * a.do_st[0] + (int64_t)b * a.do_st[1] + (int64_t)head * a.do_st[2]) * 2;
-        const char* op = a.out + ((int64_t)token * a.o_st[0] + (int64_t)b * a.o_st[1] + (int64_t)head * a.o_st[2]) * 2;
+        const int64_t o_at = ((int64_t)token * a.o_st[0] + (int64_t)b * a.o_st[1] + (int64_t)head * a.o_st[2]) * 2;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
             const int dim = 16 * s + 8 * half;
@@ -1019,9 +1055,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
             dout[s] = load8(dp + dim * 2, ok);
             float x[8], y[8];
             unpack8<T>(dout[s], x);
-            unpack8<T>(load8(op + dim * 2, ok), y);
+            unpack8<T>(load8(a.out + o_at + dim * 2, ok), y);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+            if (a.o_low) {
+                unpack8<T>(load8(a.o_low + o_at + dim * 2, ok), y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+            }
         }
         delta = both_halves_sum(delta);
         if (there) {
@@ -1099,10 +1140,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
                 s[r] = 0.f;
                 dp[r] = -delta;
             }
+            matrix_first(true);
 #pragma unroll
             for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s);
+            matrix_done(true);
+            matrix_first(true);
 #pragma unroll
             for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(vt_ops.rows(32 * kb, st), dout[st], dp);
+            matrix_done(true);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -lse)) * dp[r];
             if (!all) {
@@ -1118,8 +1163,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
                 u32x4 p;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
+                matrix_first(true);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(kt_ops.columns(32 * kb + 16 * t, i), p, acc[i]);
+                matrix_done(true);
             }
         }
         landed();

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void cache_kernel(CacheArgs a) {
         if (!mine) return;
         if constexpr (WRITE) {
             if (!held) return;
-            const u32x4 k = ld128(kp), v = *reinterpret_cast<const u32x4*>(vp);
+            const u32x4 k = *reinterpret_cast<const u32x4*>(kp), v = *reinterpret_cast<const u32x4*>(vp);
             *reinterpret_cast<u32x4*>(kc) = k;
             *reinterpret_cast<u32x4*>(vc) = v;
         } else {

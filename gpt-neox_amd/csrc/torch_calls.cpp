@@ -335,24 +335,28 @@ struct WindowCall {
     const std::optional<Tensor>& lengths;
 };
 
-std::tuple<Tensor, Tensor> window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const WindowCall& c, bool want_lse) {
+// the output, and for a backward pass what its rounding took away and the rows' logarithms
+std::tuple<Tensor, Tensor, Tensor> window_forward(const Tensor& q, const Tensor& k, const Tensor& v, const WindowCall& c, bool for_backward) {
     const c10::DeviceGuard guard(q.device());
     const auto sq = (int32_t)q.size(0), b = (int32_t)q.size(1), h = (int32_t)q.size(2), d = (int32_t)q.size(3);
-    Tensor out = at::empty(q.sizes(), q.options()), lse;
-    if (want_lse) lse = at::empty({(int64_t)b * h * sq}, q.options().dtype(at::kFloat));
-    check(neox_window_attention_fwd(out.mutable_data_ptr(), want_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr,
-                                    q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), pointer_or_null<const int32_t>(c.lengths),
+    Tensor out = at::empty(q.sizes(), q.options()), low, lse;
+    if (for_backward) {
+        low = at::empty(q.sizes(), q.options());
+        lse = at::empty({(int64_t)b * h * sq}, q.options().dtype(at::kFloat));
+    }
+    check(neox_window_attention_fwd(out.mutable_data_ptr(), for_backward ? low.mutable_data_ptr() : nullptr,
+                                    for_backward ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), pointer_or_null<const int32_t>(c.lengths),
                                     b, sq, (int32_t)k.size(0), h, (int32_t)k.size(2), d, RowStrides(q, 3), RowStrides(k, 3),
                                     RowStrides(v, 3), RowStrides(out, 3), (float)c.scale, (int32_t)c.window, (int32_t)c.sinks, code(q),
                                     stream_of(q)));
-    return {out, lse};
+    return {out, low, lse};
 }
 
 class WindowAttention : public torch::autograd::Function<WindowAttention> {
 public:
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const WindowCall& c) {
-        auto [out, lse] = window_forward(q, k, v, c, true);
-        ctx->save_for_backward({q, k, v, out, lse, c.lengths ? *c.lengths : Tensor()});
+        auto [out, low, lse] = window_forward(q, k, v, c, true);
+        ctx->save_for_backward({q, k, v, out, low, lse, c.lengths ? *c.lengths : Tensor()});
         ctx->saved_data["scale"] = c.scale;
         ctx->saved_data["window"] = c.window;
         ctx->saved_data["sinks"] = c.sinks;
@@ -364,13 +368,14 @@ public:
         variable_list v = ctx->get_saved_variables();
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
         Tensor g = grads[0];
-        const Tensor lengths = v[5];
-        v.resize(5);
+        const Tensor lengths = v[6];
+        v.resize(6);
         for (const Tensor& t : v)
             if (!on_gpu(t) || t.device() != g.device()) throw std::runtime_error("the saved tensors must be on the device of the gradient");
-        const Tensor &q0 = v[0], &k0 = v[1], &v0 = v[2], &out0 = v[3];
-        const Tensor lse = v[4].contiguous();
-        if (q0.dim() != 4 || k0.dim() != 4 || k0.sizes() != v0.sizes() || out0.sizes() != q0.sizes() || g.sizes() != q0.sizes() ||
+        const Tensor &q0 = v[0], &k0 = v[1], &v0 = v[2], &out0 = v[3], &low0 = v[4];
+        const Tensor lse = v[5].contiguous();
+        if (q0.dim() != 4 || k0.dim() != 4 || k0.sizes() != v0.sizes() || out0.sizes() != q0.sizes() ||
+            low0.sizes() != q0.sizes() || low0.scalar_type() != q0.scalar_type() || g.sizes() != q0.sizes() ||
             k0.size(1) != q0.size(1) || k0.size(3) != q0.size(3) || !half_type(q0) || !on_gpu(g) || g.scalar_type() != q0.scalar_type() ||
             k0.scalar_type() != q0.scalar_type() || v0.scalar_type() != q0.scalar_type() || out0.scalar_type() != q0.scalar_type() ||
             lse.scalar_type() != at::kFloat || lse.numel() != q0.size(0) * q0.size(1) * q0.size(2))
@@ -379,7 +384,7 @@ public:
                                   lengths.numel() != q0.size(1) || !lengths.is_contiguous()))
             throw std::runtime_error("the saved key lengths have changed");
         auto readable = [](const Tensor& t) { return in_pieces(t) ? t : t.clone(at::MemoryFormat::Contiguous); };
-        const Tensor q = readable(q0), k = readable(k0), val = readable(v0), out = readable(out0);
+        const Tensor q = readable(q0), k = readable(k0), val = readable(v0), out = out0.contiguous(), low = low0.contiguous();
         g = readable(g);
         const c10::DeviceGuard guard(q.device());
         const auto sq = (int32_t)q.size(0), b = (int32_t)q.size(1), h = (int32_t)q.size(2), d = (int32_t)q.size(3);
@@ -391,7 +396,7 @@ public:
         const Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
         check(neox_window_attention_bwd(
             dq.mutable_data_ptr(), dk.mutable_data_ptr(), dv.mutable_data_ptr(), workspace.mutable_data_ptr(), bytes, g.const_data_ptr(),
-            out.const_data_ptr(), static_cast<const float*>(lse.const_data_ptr()), q.const_data_ptr(), k.const_data_ptr(),
+            out.const_data_ptr(), low.const_data_ptr(), static_cast<const float*>(lse.const_data_ptr()), q.const_data_ptr(), k.const_data_ptr(),
             val.const_data_ptr(), lengths.defined() ? static_cast<const int32_t*>(lengths.const_data_ptr()) : nullptr, b, sq, sk, h, h_kv, d,
             RowStrides(dq, 3), RowStrides(dk, 3), RowStrides(dv, 3), RowStrides(g, 3), RowStrides(out, 3), RowStrides(q, 3),
             RowStrides(k, 3), RowStrides(val, 3), (float)ctx->saved_data["scale"].toDouble(), window, sinks, code(q), stream_of(q)));

@@ -28,20 +28,21 @@ def check_window(window, sinks):
     return min(window, 2**31 - 1), min(sinks, 2**31 - 1)
 
 
-def _forward(q, k, v, scale, window, sinks, key_lengths, want_lse):
+def _forward(q, k, v, scale, window, sinks, key_lengths, for_backward):
     (sq, b, h, d), (sk, _, h_kv, _) = q.shape, k.shape
     out = torch.empty((sq, b, h, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty(b * h * sq, dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty(b * h * sq, dtype=torch.float32, device=q.device) if for_backward else None
+    low = torch.empty_like(out) if for_backward else None
     if out.numel() == 0 or sk == 0:
-        return out.zero_(), lse
+        return out.zero_(), low, lse
     q, k, v = _lib.in_pieces(q), _lib.in_pieces(k), _lib.in_pieces(v)
     with _lib.device_guard(q):
         _lib.check(_lib.lib().neox_window_attention_fwd(
-            out.data_ptr(), lse.data_ptr() if want_lse else None, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            key_lengths.data_ptr() if key_lengths is not None else None, b, sq, sk, h, h_kv, d,
+            out.data_ptr(), _lib.ptr(low), _lib.ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _lib.ptr(key_lengths), b, sq, sk, h, h_kv, d,
             _lib.row_strides(q), _lib.row_strides(k), _lib.row_strides(v), _lib.row_strides(out), scale, window, sinks,
             _lib.dtype_code(q.dtype), _lib.current_stream(q)))
-    return out, lse
+    return out, low, lse
 
 
 class WindowAttention(torch.autograd.Function):
@@ -49,15 +50,15 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, scale, window, sinks, key_lengths):
-        out, lse = _forward(q, k, v, scale, window, sinks, key_lengths, True)
-        ctx.save_for_backward(q, k, v, out, lse, key_lengths)
+        out, low, lse = _forward(q, k, v, scale, window, sinks, key_lengths, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, key_lengths)
         ctx.call = (scale, window, sinks)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse, key_lengths = ctx.saved_tensors
+        q, k, v, out, low, lse, key_lengths = ctx.saved_tensors
         (sq, b, h, d), (sk, _, h_kv, _) = q.shape, k.shape
         dq = torch.empty((sq, b, h, d), dtype=q.dtype, device=q.device)
         dk, dv = (torch.empty((sk, b, h_kv, d), dtype=q.dtype, device=q.device) for _ in "kv")
@@ -65,7 +66,8 @@ class WindowAttention(torch.autograd.Function):
             return dq.zero_(), dk.zero_(), dv.zero_(), None, None, None, None
         if grad.shape != out.shape or grad.dtype != out.dtype or grad.device != out.device:
             raise RuntimeError("the gradient must have the shape, dtype and device of the attention's output")
-        q, k, v, out, grad = (_lib.in_pieces(t) for t in (q, k, v, out, grad))
+        q, k, v, grad = (_lib.in_pieces(t) for t in (q, k, v, grad))
+        out, low = out.contiguous(), low.contiguous()  # (a saved-tensor hook may have changed their layout)
         need = ctypes.c_int64()
         _lib.check(_lib.lib().neox_window_attention_bwd_workspace(need, b, sq, sk, h, h_kv, d, *ctx.call[1:]))
         workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
@@ -73,8 +75,8 @@ class WindowAttention(torch.autograd.Function):
         with _lib.device_guard(q):
             _lib.check(_lib.lib().neox_window_attention_bwd(
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), need.value, grad.data_ptr(), out.data_ptr(),
-                lse.data_ptr(),
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), key_lengths.data_ptr() if key_lengths is not None else None,
+                low.data_ptr(), lse.data_ptr(),
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(key_lengths),
                 b, sq, sk, h, h_kv, d, *strides, *ctx.call, _lib.dtype_code(q.dtype), _lib.current_stream(q)))
         return dq, dk, dv, None, None, None, None
 

@@ -19,10 +19,6 @@ _HALF = (torch.float16, torch.bfloat16)
 _CODES = {torch.int8: _lib.NEOX_I8, torch.float8_e4m3fn: _lib.NEOX_F8}
 
 
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
-
-
 class PagedKVCache:
     """Keys and values ``[pages, page_size, heads, dim]`` in fp16, bf16, int8 or float8_e4m3fn, the last two with scales
     ``[pages, page_size, heads]`` in fp32.  Slot ``page * page_size + i`` is token ``i`` of a page.
@@ -80,7 +76,7 @@ class PagedKVCache:
         return _CODES[self.dtype] if self.quantised else _lib.dtype_code(dtype)
 
     def _pointers(self):
-        return _ptr(self.k), _ptr(self.v), _ptr(self.k_scale), _ptr(self.v_scale)
+        return _lib.ptr(self.k), _lib.ptr(self.v), _lib.ptr(self.k_scale), _lib.ptr(self.v_scale)
 
     def _check_slots(self, slots):
         if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
@@ -199,7 +195,7 @@ def paged_attention(q, cache, page_table, query_starts, context_lengths, *, max_
     workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
     with _lib.device_guard(q):
         _lib.check(lib.neox_paged_attention(
-            out.data_ptr(), _ptr(workspace), need.value, q.data_ptr(), *cache._pointers(), page_table.data_ptr(),
+            out.data_ptr(), _lib.ptr(workspace), need.value, q.data_ptr(), *cache._pointers(), page_table.data_ptr(),
             query_starts.data_ptr(), context_lengths.data_ptr(), b, tokens, max_query, max_context, h, cache.heads, d, cache.pages,
             cache.page_size, page_table.shape[1], page_table.stride(0), _lib.row_strides(out), _lib.row_strides(q), *cache._strides,
             scale, window, sinks, _lib.dtype_code(q.dtype), code, _lib.current_stream(q)))

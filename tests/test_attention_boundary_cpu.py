@@ -29,7 +29,7 @@ def refused(status, code, message):
 
 
 def window_fwd(p, **change):
-    a = dict(out=p, lse=p, q=p, k=p, v=p, lengths=None, b=2, sq=8, sk=8, h=4, h_kv=2, d=64, qs=st(512, 256, 64), ks=st(256, 128, 64),
+    a = dict(out=p, low=p, lse=p, q=p, k=p, v=p, lengths=None, b=2, sq=8, sk=8, h=4, h_kv=2, d=64, qs=st(512, 256, 64), ks=st(256, 128, 64),
              vs=st(256, 128, 64), os=st(512, 256, 64), scale=0.1, window=4, sinks=1, dtype=BF16, stream=None)
     a.update(change)
     return _lib.lib().neox_window_attention_fwd(*a.values())
@@ -57,7 +57,7 @@ def test_window_attention_backward(p):
     q3, k3 = st(512, 256, 64), st(256, 128, 64)
 
     def bwd(**change):
-        a = dict(dq=p, dk=p, dv=p, ws=p, size=256, dout=p, out=p, lse=p, q=p, k=p, v=p, lengths=None, b=2, sq=8, sk=8, h=4, h_kv=2, d=64, s0=q3, s1=k3,
+        a = dict(dq=p, dk=p, dv=p, ws=p, size=256, dout=p, out=p, low=p, lse=p, q=p, k=p, v=p, lengths=None, b=2, sq=8, sk=8, h=4, h_kv=2, d=64, s0=q3, s1=k3,
                  s2=k3, s3=q3, s4=q3, s5=q3, s6=k3, s7=k3, scale=0.1, window=4, sinks=1, dtype=F16, stream=None)
         a.update(change)
         return lib.neox_window_attention_bwd(*a.values())
