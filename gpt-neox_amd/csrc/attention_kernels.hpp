@@ -309,6 +309,27 @@ __device__ __forceinline__ void paged_sample(const AttnArgs& a, int b, int& toke
     keys = max(0, min(a.lengths[b], a.table_keys));
 }
 
+// Which of the 16 keys whose scores a lane has (element_of: first + 8 (r / 4) + 4 half + r % 4) its row sees: those
+// from lo to hi and, where sinks reach this far, the first ones.  One subtraction and one comparison each: an offset
+// below zero is a large unsigned number.
+struct Sight {
+    int lo, width, sinks, hi;
+    __device__ __forceinline__ Sight(int position, int keys, int window, int sinks_, int first, int half) {
+        const int base = first + 4 * half;
+        hi = min(position, keys - 1) - base;
+        lo = window < 0 ? -base : position - window - base;
+        width = hi - lo;
+        if (width < 0) {  // nothing: no offset from here is small enough
+            lo = 1 << 30;
+            width = 0;
+        }
+        sinks = sinks_ - base;
+    }
+    static __device__ __forceinline__ constexpr int offset(int r) { return 8 * (r >> 2) + (r & 3); }
+    __device__ __forceinline__ bool window(int r) const { return (uint32_t)(offset(r) - lo) <= (uint32_t)width; }
+    __device__ __forceinline__ bool any(int r) const { return window(r) || (offset(r) < sinks && offset(r) <= hi); }
+};
+
 // ---- staging -----------------------------------------------------------------------------------------
 // One tile of ROWS rows (of keys, say) on its way from memory to LDS through registers: 256 threads, a piece
 // of 8 elements at a time.  Rows behind the last key and dims behind d come as zeros: what lies there may be anything.
@@ -383,7 +404,7 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 
 // ---- forward --------------------------------------------------------------------------------------------
 template <typename T, int DP, int SRC, bool SPLIT>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged16 ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
     constexpr bool kPages = SRC != kStrided;
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
     constexpr int kBytes = kCodes ? 1 : 2;
@@ -441,18 +462,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
         const int each = (tiles.count + a.splits - 1) / a.splits;
         first_tile = min((int)split * each, tiles.count);
         end_tile = min(first_tile + each, tiles.count);
-    }
-
-    // queries, the second operand of the scores
-    u32x4 q[DP / 16];
-    {
-        const char* p = a.q + ((int64_t)(token0 + token) * a.q_st[0] + (kPages ? 0 : (int64_t)b * a.q_st[1]) + (int64_t)head * a.q_st[2]) * 2;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            const int dim = 16 * s + 8 * half;
-            q[s] = load8(p + dim * 2, there && dim < a.d);
-            q[s] ^= a.flip;
-        }
     }
 
     // One tile of keys and values into one of the buffers: 16-bit rows are copied there as they are; codes come through
@@ -576,12 +585,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     float m = kNegInf, l = 0.f;
 
+    // the first tile is on its way before the queries are waited for
     if (first_tile < end_tile) {
         look_up(tiles.tile(first_tile));
         fetch(tiles.tile(first_tile), 0);
         if (first_tile + 1 < end_tile) look_up(tiles.tile(first_tile + 1));
-        put(0);
     }
+
+    // queries, the second operand of the scores
+    u32x4 q[DP / 16];
+    {
+        const char* p = a.q + ((int64_t)(token0 + token) * a.q_st[0] + (kPages ? 0 : (int64_t)b * a.q_st[1]) + (int64_t)head * a.q_st[2]) * 2;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int dim = 16 * s + 8 * half;
+            q[s] = load8(p + dim * 2, there && dim < a.d);
+            q[s] ^= a.flip;
+        }
+    }
+
+    if (first_tile < end_tile) put(0);
     __syncthreads();
 
     for (int it = first_tile; it < end_tile; ++it) {
@@ -622,15 +645,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_fwd_kernel(AttnAr
                     }
             }
             if (!all) {
-                const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
 #pragma unroll
-                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
+                    const Sight sight(position, keys, a.window, a.sinks, key0 + 32 * kb, half);
+                    if (key0 < a.sinks) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int key = key0 + 32 * kb + element_of(r, half);
-                        const bool sees = key <= hi && (key >= lo || key < a.sinks);
-                        s[kb][r] = sees ? s[kb][r] : kNegInf;
+                        for (int r = 0; r < 16; ++r) s[kb][r] = sight.any(r) ? s[kb][r] : kNegInf;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[kb][r] = sight.window(r) ? s[kb][r] : kNegInf;
                     }
+                }
             }
             float top = s[0][0];
 #pragma unroll
@@ -1041,36 +1066,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
     const bool wave_works = row0 + wave * 32 < rows;
     const KeyTiles tiles = key_tiles<kTileKeys>(wg_first, wg_last, keys, a.window, a.sinks);
 
-    u32x4 q[DP / 16], dout[DP / 16];
-    float delta = 0.f, lse = __builtin_inff();
-    {
-        const char* qp = a.q + ((int64_t)token * a.q_st[0] + (int64_t)b * a.q_st[1] + (int64_t)head * a.q_st[2]) * 2;
-        const char* dp = a.dout + ((int64_t)token * a.do_st[0] + (int64_t)b * a.do_st[1] + (int64_t)head * a.do_st[2]) * 2;
-        const int64_t o_at = ((int64_t)token * a.o_st[0] + (int64_t)b * a.o_st[1] + (int64_t)head * a.o_st[2]) * 2;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            const int dim = 16 * s + 8 * half;
-            const bool ok = there && dim < a.d;
-            q[s] = load8(qp + dim * 2, ok);
-            dout[s] = load8(dp + dim * 2, ok);
-            float x[8], y[8];
-            unpack8<T>(dout[s], x);
-            unpack8<T>(load8(a.out + o_at + dim * 2, ok), y);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
-            if (a.o_low) {
-                unpack8<T>(load8(a.o_low + o_at + dim * 2, ok), y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
-            }
-        }
-        delta = both_halves_sum(delta);
-        if (there) {
-            lse = a.lse[(int64_t)bh * rows + row];
-            if (half == 0) a.delta[(int64_t)bh * rows + row] = delta;
-        }
-    }
-
     typedef Flight<DP, kTileKeys> Fl;
     Fl fl;
     const char* const kbase = a.k + ((int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2]) * 2;
@@ -1119,6 +1114,36 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
     const float scale_log2 = a.scale * kLog2e;
 
     if (tiles.count) fetch(tiles.tile(0), 0);
+    u32x4 q[DP / 16], dout[DP / 16];
+    float delta = 0.f, lse = __builtin_inff();
+    {
+        const char* qp = a.q + ((int64_t)token * a.q_st[0] + (int64_t)b * a.q_st[1] + (int64_t)head * a.q_st[2]) * 2;
+        const char* dp = a.dout + ((int64_t)token * a.do_st[0] + (int64_t)b * a.do_st[1] + (int64_t)head * a.do_st[2]) * 2;
+        const int64_t o_at = ((int64_t)token * a.o_st[0] + (int64_t)b * a.o_st[1] + (int64_t)head * a.o_st[2]) * 2;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int dim = 16 * s + 8 * half;
+            const bool ok = there && dim < a.d;
+            q[s] = load8(qp + dim * 2, ok);
+            dout[s] = load8(dp + dim * 2, ok);
+            float x[8], y[8];
+            unpack8<T>(dout[s], x);
+            unpack8<T>(load8(a.out + o_at + dim * 2, ok), y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+            if (a.o_low) {
+                unpack8<T>(load8(a.o_low + o_at + dim * 2, ok), y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+            }
+        }
+        delta = both_halves_sum(delta);
+        if (there) {
+            lse = a.lse[(int64_t)bh * rows + row];
+            if (half == 0) a.delta[(int64_t)bh * rows + row] = delta;
+        }
+    }
+
     landed();
     __syncthreads();
     for (int it = 0; it < tiles.count; ++it) {
@@ -1151,11 +1176,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -lse)) * dp[r];
             if (!all) {
-                const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
+                const Sight sight(position, keys, a.window, a.sinks, k0, half);
+                if (k0 < a.sinks) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = k0 + element_of(r, half);
-                    s[r] = key <= hi && (key >= lo || key < a.sinks) ? s[r] : 0.f;
+                    for (int r = 0; r < 16; ++r) s[r] = sight.any(r) ? s[r] : 0.f;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = sight.window(r) ? s[r] : 0.f;
                 }
             }
 #pragma unroll
@@ -1190,6 +1217,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
     constexpr int kTile = kStepRows * Tile<DP>::kRow;
     __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile];
     __shared__ __attribute__((aligned(16))) float row_sums[2][2][kStepRows];  // lse and delta of the tile's rows
+    __shared__ __attribute__((aligned(16))) int row_at[2][kStepRows];         // and where they stand
 
     const uint32_t block = blockIdx.x, heads = a.b * a.kv;
     uint32_t bh, unit;
@@ -1227,18 +1255,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
         const int each = max(0, (end - begin + kStepRows - 1) / kStepRows + parts - 1) / parts * kStepRows;
         row_begin = min(begin + part * each, end);
         row_end = min(row_begin + each, end);
-    }
-
-    u32x4 kreg[DP / 16], vreg[DK ? DP / 16 : 1];
-    {
-        const char* kp = a.k + ((int64_t)key * a.k_st[0] + (int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2]) * 2;
-        const char* vp = a.v + ((int64_t)key * a.v_st[0] + (int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2]) * 2;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            const int dim = 16 * s + 8 * half;
-            kreg[s] = load8(kp + dim * 2, key < keys && dim < a.d);
-            if constexpr (DK) vreg[s] = load8(vp + dim * 2, key < keys && dim < a.d);
-        }
     }
 
     typedef Flight<DP, kStepRows> Fl;
@@ -1305,6 +1321,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
                                                  (__attribute__((address_space(3))) void*)row_sums[buffer], 4, 0, 0);
             else
                 row_sums[buffer][0][fl.thread] = fl.thread & 32 ? 0.f : __builtin_inff();
+        } else if (wave == 1 && fl.thread < 64 + kStepRows) {
+            row_at[buffer][fl.thread - 64] = position0 + (int)a.by_group.div(row0 + (int)fl.thread - 64);
         }
     };
 
@@ -1316,6 +1334,18 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
     const float scale_log2 = a.scale * kLog2e;
 
     if (row_begin < row_end) fetch(row_begin, 0);
+    u32x4 kreg[DP / 16], vreg[DK ? DP / 16 : 1];
+    {
+        const char* kp = a.k + ((int64_t)key * a.k_st[0] + (int64_t)b * a.k_st[1] + (int64_t)g * a.k_st[2]) * 2;
+        const char* vp = a.v + ((int64_t)key * a.v_st[0] + (int64_t)b * a.v_st[1] + (int64_t)g * a.v_st[2]) * 2;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int dim = 16 * s + 8 * half;
+            kreg[s] = load8(kp + dim * 2, key < keys && dim < a.d);
+            if constexpr (DK) vreg[s] = load8(vp + dim * 2, key < keys && dim < a.d);
+        }
+    }
+
     landed();
     __syncthreads();
     int buffer = 0;
@@ -1343,11 +1373,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
                 for (int i = 0; i < 4; ++i) s[r + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + i], scale_log2, -c[i]));
             }
             if (!all) {
+                // a row sees this lane's key from `reach` positions behind it at most; a key behind the end stands behind
+                // every row
+                const int mine = wv_first + (int)(fl.thread & 31), key_at = mine < keys ? mine : 1 << 30;
+                const uint32_t reach = a.window < 0 || mine < a.sinks ? 0x7fffffffu : (uint32_t)a.window;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int at = position0 + (int)a.by_group.div(row0 + element_of(r, half));
-                    const bool sees = key < keys && at >= key && (a.window < 0 || key >= at - a.window || key < a.sinks);
-                    s[r] = sees ? s[r] : 0.f;
+                for (int r = 0; r < 16; r += 4) {
+                    const int* at = &row_at[buffer][8 * (r >> 2) + 4 * half];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[r + i] = (uint32_t)(at[i] - key_at) <= reach ? s[r + i] : 0.f;
                 }
             }
             if constexpr (DK) {
