@@ -121,14 +121,16 @@ struct Mma<F16> {
 
 // One head dim class: DP is the padded head dim.  A tile row in LDS has kRow bytes (a power of two), cut into
 // 16-byte pieces whose order is permuted by the row number, so that both kinds of read spread over all banks:
-// 16 rows at one piece (row operand), and 4 rows at 4 neighbouring pieces (transposing reads).
+// 16 rows at one piece (row operand), 4 rows at 4 neighbouring pieces (transposing reads of 32 dims) and 8 rows at 2 (of
+// 16 dims).
 template <int DP>
 struct Tile {
     static constexpr int kRow = DP <= 64 ? 128 : DP <= 128 ? 256 : 512;
     static constexpr int kPieces = DP / 8;  // of a row that hold data
     static __device__ __forceinline__ uint32_t turn(uint32_t row) {
-        if constexpr (kRow == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
-        return (row & 3) << 2 | ((row >> 2) & 3);
+        const uint32_t low = ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+        if constexpr (kRow == 128) return ((row >> 1) & 1) << 2 | low;
+        return (row & 3) << 2 | low;
     }
     static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t piece) {
         return row * kRow + ((piece ^ turn(row)) << 4);
@@ -158,7 +160,7 @@ struct Operands {
     __device__ __forceinline__ u32x4 columns(int row0, int db) const {
         typedef __attribute__((address_space(3))) s16x4* from;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((from)(uintptr_t)((turned ^ (db << 6)) + row0 * Tile<DP>::kRow));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((from)(uintptr_t)((turned ^ (db << 6) ^ 32) + (row0 + 8) * Tile<DP>::kRow));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((from)(uintptr_t)((turned ^ (db << 6) ^ 16) + (row0 + 8) * Tile<DP>::kRow));
         const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
         return u32x4{a.x, a.y, b.x, b.y};
     }
@@ -392,7 +394,7 @@ struct Flight {
     static constexpr int kRowsAtOnce = 4096 / Tile<DP>::kRow;
     __device__ __forceinline__ uint32_t offset(uint32_t row_bytes) const { return row(0) * row_bytes + piece(0) * 16; }
     static __device__ __forceinline__ void load(int step, const char* first, uint32_t row_bytes, uint32_t offset, uint32_t piece, char* tile) {
-        if constexpr (kRowsAtOnce < 16) offset += ((piece ^ (step & 1) * 2) - piece) * 16;
+        if constexpr (kRowsAtOnce < 16) offset += ((piece ^ (step & 1)) - piece) * 16;
         load(step, first + (uint64_t)(step * kRowsAtOnce) * row_bytes + offset, tile);
     }
     __device__ __forceinline__ void zero(int step, char* tile) const {
@@ -811,30 +813,64 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
     const int32_t* const table = a.table + (int64_t)b * a.table_stride;
     u32x4 kw[2][kLoads], vw[2][kLoads];
     float k_scale = 0.f, v_scale = 0.f;
-    int pages[2];  // of this lane's two keys of the next block
+    // Where pages hold whole blocks, a block has one page and its addresses are a scalar and a lane's own offset;
+    // otherwise every lane looks up the pages of its two keys.
+    const bool even = a.by_page.d % kKeys == 0 && a.k_st[0] < kSmallStride && a.v_st[0] < kSmallStride && a.ks_st[0] < kSmallStride &&
+                      a.vs_st[0] < kSmallStride;
+    uint32_t block_page = 0;
+    int pages[2];
     auto look_up = [&](int i) {
+        if (even) {
+            const int key = tiles.tile(i) * kKeys;
+            block_page = i < end ? __builtin_amdgcn_readfirstlane(table[a.by_page.div(key)]) : ~0u;
+            return;
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const int key = tiles.tile(i) * kKeys + 16 * kb + col;
             pages[kb] = i < end && key < keys ? table[a.by_page.div(key)] : -1;
         }
     };
-    const char* const kbase = a.k + ((int64_t)g * a.k_st[2] + dim_of(0)) * kBytes;
-    const char* const vbase = a.v + ((int64_t)g * a.v_st[2] + dim_of(0)) * kBytes;
+    const uint32_t k_row = (uint32_t)a.k_st[0] * kBytes, v_row = (uint32_t)a.v_st[0] * kBytes;
+    const char* const kbase = a.k + (int64_t)g * a.k_st[2] * kBytes;
+    const char* const vbase = a.v + (int64_t)g * a.v_st[2] * kBytes;
+    const uint32_t k_offset = col * k_row + dim_of(0) * kBytes, v_offset = col * v_row + dim_of(0) * kBytes;
     auto fetch = [&](int i) {
+        const int key0 = tiles.tile(i) * kKeys;
+        if (even && key0 + kKeys <= keys && block_page < (uint32_t)a.pages) {
+            const uint32_t in = a.by_page.mod(key0);
+            const char* const kp = step_to(step_to(kbase, block_page, (uint32_t)a.k_st[1] * kBytes), in, k_row);
+            const char* const vp = step_to(step_to(vbase, block_page, (uint32_t)a.v_st[1] * kBytes), in, v_row);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int s = 0; s < kLoads; ++s) {
+                    kw[kb][s] = load8(kp + (uint64_t)(16 * kb) * k_row + s * 64 + k_offset, dim_of(s) < a.d);
+                    vw[kb][s] = load8(vp + (uint64_t)(16 * kb) * v_row + s * 64 + v_offset, dim_of(s) < a.d);
+                }
+            if constexpr (kCodes) {
+                if (quad < 2) {
+                    const float* const kf = a.k_scale + ((int64_t)block_page * a.ks_st[1] + (int64_t)in * a.ks_st[0] + (int64_t)g * a.ks_st[2]);
+                    const float* const vf = a.v_scale + ((int64_t)block_page * a.vs_st[1] + (int64_t)in * a.vs_st[0] + (int64_t)g * a.vs_st[2]);
+                    k_scale = kf[(uint32_t)lane * (uint32_t)a.ks_st[0]];
+                    v_scale = vf[(uint32_t)lane * (uint32_t)a.vs_st[0]];
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            const uint32_t page = pages[kb], in = a.by_page.mod(tiles.tile(i) * kKeys + 16 * kb + col);
-            const bool ok = page < (uint32_t)a.pages;
-            const char* const kp = step_to(step_to(kbase, page, (uint32_t)a.k_st[1] * kBytes), in, (uint32_t)a.k_st[0] * kBytes);
-            const char* const vp = step_to(step_to(vbase, page, (uint32_t)a.v_st[1] * kBytes), in, (uint32_t)a.v_st[0] * kBytes);
+            const int key = key0 + 16 * kb + col;
+            const uint32_t page = even ? block_page : pages[kb], in = a.by_page.mod(key);
+            const bool ok = key < keys && page < (uint32_t)a.pages;
+            const char* const kp = step_to(step_to(kbase, page, (uint32_t)a.k_st[1] * kBytes), in, k_row) + dim_of(0) * kBytes;
+            const char* const vp = step_to(step_to(vbase, page, (uint32_t)a.v_st[1] * kBytes), in, v_row) + dim_of(0) * kBytes;
 #pragma unroll
             for (int s = 0; s < kLoads; ++s) {
                 kw[kb][s] = load8(kp + s * 64, ok && dim_of(s) < a.d);
                 vw[kb][s] = load8(vp + s * 64, ok && dim_of(s) < a.d);
             }
             if constexpr (kCodes) {
-                // (all four lanes of a key fetch its scales; those of the quad that stores them count)
                 if (quad == kb) {
                     k_scale = ok ? a.k_scale[(int64_t)page * a.ks_st[1] + (int64_t)in * a.ks_st[0] + (int64_t)g * a.ks_st[2]] : 0.f;
                     v_scale = ok ? a.v_scale[(int64_t)page * a.vs_st[1] + (int64_t)in * a.vs_st[0] + (int64_t)g * a.vs_st[2]] : 0.f;
@@ -899,19 +935,27 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) s[kb] *= *reinterpret_cast<const f32x4*>(&scales[wave][0][16 * kb + 4 * quad]);
         }
-        const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
+        // (the last token sees furthest ahead, the first least; a window's near end moves with both)
+        const bool all = key0 + kKeys - 1 <= position0 && key0 + kKeys <= keys &&
+                         (a.window < 0 || key0 >= position0 + tokens - 1 - a.window || key0 + kKeys <= a.sinks);
+        if (!all) {
+            const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = key0 + 16 * kb + 4 * quad + r;
+                    const bool sees = key <= hi && (key >= lo || key < a.sinks);
+                    s[kb][r] = sees ? s[kb][r] : kNegInf;
+                }
+        }
         float top = kNegInf;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = key0 + 16 * kb + 4 * quad + r;
-                const bool sees = key <= hi && (key >= lo || key < a.sinks);
-                s[kb][r] = sees ? s[kb][r] * a.scale_log2 : kNegInf;
-                top = fmaxf(top, s[kb][r]);
-            }
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[kb][r]);
         top = fmaxf(top, __shfl_xor(top, 16));
-        top = both_halves_max(top);
+        top = both_halves_max(top) * a.scale_log2;
         if (__any(top > m + 8.f)) {
             const float higher = fmaxf(m, top);
             const float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
@@ -925,7 +969,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[kb][r] = __builtin_amdgcn_exp2f(s[kb][r] - base);
+                s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], a.scale_log2, -base));
                 l += s[kb][r];
             }
         if constexpr (kCodes) {
@@ -933,7 +977,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
             for (int kb = 0; kb < 2; ++kb) {
                 const f32x4 c = *reinterpret_cast<const f32x4*>(&scales[wave][1][16 * kb + 4 * quad]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[kb][r] = s[kb][r] != 0.f ? s[kb][r] * c[r] : 0.f;
+                for (int r = 0; r < 4; ++r) s[kb][r] = all || s[kb][r] != 0.f ? s[kb][r] * c[r] : 0.f;
             }
         }
         const u32x4 p = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
@@ -1286,7 +1330,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
                 for (int s = 0; s < Fl::kSteps; ++s) {
                     uint32_t qo = q_offset, dof = d_offset;
                     if constexpr (Fl::kRowsAtOnce < 16) {
-                        const uint32_t other = ((lane_piece ^ (s & 1) * 2) - lane_piece) * 16;
+                        const uint32_t other = ((lane_piece ^ (s & 1)) - lane_piece) * 16;
                         qo += other;
                         dof += other;
                     }
