@@ -32,11 +32,8 @@ constexpr int kTileRows = 128;  // rows of a workgroup there: 32 for each of its
 constexpr int kStepRows = 32;   // rows of one step of the key-gradient kernel
 constexpr int kGradKeys = 128;  // keys of a workgroup there: 32 for each of its four waves
 
-// p + i * bytes + j * more, one instruction for each product (strides are below 2^31 elements, which the entry
-// points see to)
-__device__ __forceinline__ const char* step_to(const char* p, uint32_t i, uint32_t bytes) {
-    return reinterpret_cast<const char*>((uint64_t)i * bytes + reinterpret_cast<uint64_t>(p));
-}
+// p + i * bytes in one instruction (strides are below 2^31 elements, which the entry points see to)
+__device__ __forceinline__ const char* step_to(const char* p, uint32_t i, uint32_t bytes) { return p + (uint64_t)i * bytes; }
 
 // where keys and values come from
 enum KvSource { kStrided = 0, kPaged16 = 1, kPagedI8 = 2, kPagedF8 = 3 };
@@ -362,8 +359,14 @@ struct Stage {
         for (int s = 0; s < kSteps; ++s) {
             if (!works(s)) continue;
             u32x4 x;
-            if constexpr (kCodes) x = widen8<T, SRC>(c[s]);
-            else x = w[s];
+            if constexpr (kCodes) {
+                // (or the compiler takes the words apart where they are loaded, and waits for them there)
+                u32x2 codes = c[s];
+                asm("" : "+v"(codes.x), "+v"(codes.y));
+                x = widen8<T, SRC>(codes);
+            } else {
+                x = w[s];
+            }
             *reinterpret_cast<u32x4*>(tile + Tile<DP>::at(row(s), piece())) = x;
             __builtin_amdgcn_sched_barrier(0);  // one step after the other: their values together would not fit the registers
         }
@@ -687,7 +690,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                     sum += s[kb][r];
                 }
             l += sum;
-            if constexpr (kCodes) {
+            if (kCodes && !all) {  // a hidden value's scale may be anything
+#pragma unroll
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f32x4 c = *reinterpret_cast<const f32x4*>(scales + (buffer * 2 + 1) * kFwdKeys + 32 * kb + 2 * r + 4 * half);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kb][r + i] = s[kb][r + i] != 0.f ? s[kb][r + i] * c[i] : 0.f;
+                    }
+            } else if constexpr (kCodes) {
                 const float* f = scales + (buffer * 2 + 1) * kFwdKeys;
 #pragma unroll
                 for (int kb = 0; kb < kFwdKeys / 32; ++kb)
@@ -695,7 +707,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                     for (int r = 0; r < 16; r += 4) {
                         const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[kb][r + i] = all || s[kb][r + i] != 0.f ? s[kb][r + i] * c[i] : 0.f;
+                        for (int i = 0; i < 4; ++i) s[kb][r + i] *= c[i];
                     }
             }
 #pragma unroll
@@ -977,7 +989,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
             for (int kb = 0; kb < 2; ++kb) {
                 const f32x4 c = *reinterpret_cast<const f32x4*>(&scales[wave][1][16 * kb + 4 * quad]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[kb][r] = all || s[kb][r] != 0.f ? s[kb][r] * c[r] : 0.f;
+                for (int r = 0; r < 4; ++r) s[kb][r] = s[kb][r] != 0.f ? s[kb][r] * c[r] : 0.f;  // a hidden value's scale may be anything
             }
         }
         const u32x4 p = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
