@@ -74,7 +74,7 @@ struct AttnArgs {
     int64_t do_st[3];
     char *dq, *dk, *dv;
     int64_t dq_st[3], dk_st[3], dv_st[3];
-    float* delta;                // sum over d of dO * O of every row, [b, kv, rows]
+    float* delta;                // minus the sum over d of dO * O of every row, [b, kv, rows]
     float scale;
     int key_tiles;
     // The key-gradient kernel's work: every key tile's near rows (those whose window reaches it) in near_parts
@@ -189,6 +189,13 @@ __device__ __forceinline__ float both_halves_max(float x) {
 __device__ __forceinline__ float both_halves_sum(float x) {
     const HalfPair p = both_halves(x);
     return p.a + p.b;
+}
+
+// the largest of three; of numbers from the matrix cores, which the compiler would first make canonical one by one
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
 }
 
 // the element of a 32-long result axis that register r of a lane in this half holds
@@ -662,11 +669,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                     }
                 }
             }
-            float top = s[0][0];
+            float top = kNegInf;
 #pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[0][r]);
+            for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16 && kFwdKeys > 32; ++r) top = fmaxf(top, s[kFwdKeys / 32 - 1][r]);
+                for (int r = 0; r < 16; r += 2) top = max3(top, s[kb][r], s[kb][r + 1]);
             top = both_halves_max(top) * a.scale_log2;
             // The running maximum follows only where a row has outgrown it by 2^8: until then its exponentials stay
             // below 256 and the accumulators need no rescaling.
@@ -1162,13 +1169,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
         }
     };
 
-    f32x16 acc[DP / 32];
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
-    const float scale_log2 = a.scale * kLog2e;
-
     if (tiles.count) fetch(tiles.tile(0), 0);
     u32x4 q[DP / 16], dout[DP / 16];
     float delta = 0.f, lse = __builtin_inff();
@@ -1196,15 +1196,25 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
         delta = both_halves_sum(delta);
         if (there) {
             lse = a.lse[(int64_t)bh * rows + row];
-            if (half == 0) a.delta[(int64_t)bh * rows + row] = delta;
+            if (half == 0) a.delta[(int64_t)bh * rows + row] = -delta;
         }
     }
+
+    f32x16 minus_delta;  // where the sums of dP start: held in registers of its own, so that no tile has to set it up
+#pragma unroll
+    for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    const float scale_log2 = a.scale * kLog2e;
 
     landed();
     __syncthreads();
     for (int it = 0; it < tiles.count; ++it) {
         const int buffer = it & 1;
-        const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
+        const Operands<DP> ops(lds_byte(lds) + buffer * 2 * kTile);  // the keys' tile, and kTileKeys rows behind it the values'
         const int key0 = tiles.tile(it) * kTileKeys;
         if (it + 1 < tiles.count) fetch(tiles.tile(it + 1), buffer ^ 1);
 #pragma unroll
@@ -1215,19 +1225,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
             const bool all = k1 - 1 <= wv_first && k1 <= keys &&
                              (a.window < 0 || k0 >= wv_last - a.window || k1 <= a.sinks);
             if (none) continue;
-            f32x16 s, dp;
+            f32x16 s, dp = minus_delta;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = 0.f;
-                dp[r] = -delta;
-            }
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
             matrix_first(true);
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s);
+            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(ops.rows(32 * kb, st), q[st], s);
             matrix_done(true);
             matrix_first(true);
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(vt_ops.rows(32 * kb, st), dout[st], dp);
+            for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(ops.rows(kTileKeys + 32 * kb, st), dout[st], dp);
             matrix_done(true);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -lse)) * dp[r];
@@ -1248,7 +1255,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
                 for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
                 matrix_first(true);
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(kt_ops.columns(32 * kb + 16 * t, i), p, acc[i]);
+                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(ops.columns(32 * kb + 16 * t, i), p, acc[i]);
                 matrix_done(true);
             }
         }
@@ -1406,7 +1413,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
     __syncthreads();
     int buffer = 0;
     for (int row0 = row_begin; row0 < row_end; row0 += kStepRows, buffer ^= 1) {
-        const Operands<DP> qt_ops(lds_byte(lds) + buffer * 2 * kTile), dt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
+        const Operands<DP> ops(lds_byte(lds) + buffer * 2 * kTile);  // the queries' tile, and kStepRows rows behind it dO's
         uint32_t sums_at = lds_byte(row_sums) + buffer * 8 * kStepRows + 16 * half;
         asm("" : "+v"(sums_at));
         if (row0 + kStepRows < row_end) fetch(row0 + kStepRows, buffer ^ 1);
@@ -1421,7 +1428,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(qt_ops.rows(0, st), kreg[st], s);
+            for (int st = 0; st < DP / 16; ++st) s = Mma<T>::op(ops.rows(0, st), kreg[st], s);
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const f32x4 c = lds_floats(sums_at + 32 * (r >> 2));
@@ -1442,13 +1449,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
             }
             if constexpr (DK) {
 #pragma unroll
-                for (int r = 0; r < 16; r += 4) {  // dP - delta: the sum starts at -delta
+                for (int r = 0; r < 16; r += 4) {  // dP - delta: the sum starts at -delta, which is what memory holds
                     const f32x4 c = lds_floats(sums_at + 4 * kStepRows + 32 * (r >> 2));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) dp[r + i] = -c[i];
+                    for (int i = 0; i < 4; ++i) dp[r + i] = c[i];
                 }
 #pragma unroll
-                for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(dt_ops.rows(0, st), vreg[st], dp);
+                for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(ops.rows(kStepRows, st), vreg[st], dp);
             }
             if constexpr (DV) {
 #pragma unroll
@@ -1457,7 +1464,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(dt_ops.columns(16 * t, i), p, dv[i]);
+                    for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(ops.columns(kStepRows + 16 * t, i), p, dv[i]);
                 }
             }
             if constexpr (DK) {
@@ -1469,7 +1476,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
 #pragma unroll
                     for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) dk[i] = Mma<T>::op(qt_ops.columns(16 * t, i), p, dk[i]);
+                    for (int i = 0; i < DP / 32; ++i) dk[i] = Mma<T>::op(ops.columns(16 * t, i), p, dk[i]);
                 }
             }
         }
