@@ -149,20 +149,25 @@ static void set_window_sizes(AttnArgs& a, int b, int sq, int sk, int h, int h_kv
 
 // how the key gradients' work is cut into pieces, and the scratch it needs: fp32 sums of pieces, then delta
 struct GradPlan {
-    int key_tiles, near_parts, sink_tiles, far_parts;
+    int key_tiles, near_parts, piece_rows, sink_tiles, far_parts;
     int64_t parts_bytes, bytes;
 };
 
-// Pieces of a tile's near rows: so many that two workgroups run on every CU, 256 rows or more for each.  Rows behind the
-// window of a tile that holds sinks come in pieces of 512 rows.
+// Pieces of a tile's near rows, of one size for all tiles: so many that two workgroups run on every CU, or under a bare
+// causal mask, whose first tiles have twice the rows of the average, so that no piece is longer than a CU's share; 256
+// rows or more for each.  Rows behind the window of a tile that holds sinks come in pieces of 512 rows.
 static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int window, int sinks) {
     GradPlan p{};
     const int64_t group = h / h_kv, units = (int64_t)b * h_kv;
     p.key_tiles = (sk + kGradKeys - 1) / kGradKeys;
-    const int64_t near = window < 0 ? sq : (int64_t)window + kGradKeys < sq ? (int64_t)window + kGradKeys : sq;
-    int64_t parts = (512 + units * p.key_tiles - 1) / (units * p.key_tiles);
-    if (parts > near * group / 256) parts = near * group / 256;
+    const bool all = window < 0 || (int64_t)window + kGradKeys >= sq;
+    const int64_t near = all ? sq : (int64_t)window + kGradKeys;
+    const int64_t tiles = units * p.key_tiles, most = near * group / 256;
+    int64_t parts = ((all ? 1024 : 512) + tiles - 1) / tiles;
+    if (parts > most) parts = most;
     p.near_parts = parts < 1 ? 1 : parts > 64 ? 64 : (int)parts;
+    // (a single piece holds whatever a tile has: with sinks that may be more than the near rows)
+    p.piece_rows = p.near_parts == 1 ? kMost : (int)((near * group + p.near_parts * kStepRows - 1) / (p.near_parts * kStepRows) * kStepRows);
     const int64_t last = (sinks < sk ? sinks : sk);
     // the last position whose window reaches the first tile is kGradKeys - 1 + window
     const int64_t behind = window < 0 || last < 1 ? 0 : (int64_t)sk - kGradKeys - window;
@@ -386,6 +391,7 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int
     set_scale_window(a, scale, window, sinks);
     a.key_tiles = plan.key_tiles;
     a.near_parts = plan.near_parts;
+    a.piece_rows = plan.piece_rows;
     a.sink_tiles = plan.sink_tiles;
     a.far_parts = plan.far_parts;
     a.units = plan.key_tiles * plan.near_parts + plan.sink_tiles * plan.far_parts;

@@ -77,10 +77,11 @@ struct AttnArgs {
     float* delta;                // minus the sum over d of dO * O of every row, [b, kv, rows]
     float scale;
     int key_tiles;
-    // The key-gradient kernel's work: every key tile's near rows (those whose window reaches it) in near_parts
-    // pieces; for the first sink_tiles tiles, the rows behind in far_parts pieces.  A tile in more than one piece
+    // The key-gradient kernel's work: every key tile's near rows (those whose window reaches it) in up to near_parts
+    // pieces of piece_rows; for the first sink_tiles tiles, the rows behind in far_parts pieces.  A tile in more than one piece
     // leaves fp32 sums in part_o, [b, kv][piece][dk, dv][kGradKeys][d], far pieces for the keys below `sinks` only.
     int near_parts, far_parts, sink_tiles, units;
+    int piece_rows;              // of a piece of near rows
     FastDiv by_units, by_near_parts, by_far_parts;
 };
 
@@ -1272,6 +1273,22 @@ __device__ __forceinline__ int64_t grad_piece(const AttnArgs& a, uint32_t bh, in
     return bh * each + (int64_t)tile * a.near_parts + min(tile, a.sink_tiles) * a.far_parts;
 }
 
+// The rows that see some key of a tile: those from its first position to the end of its last one's window, and where
+// it holds sinks, whose rows behind are not work of their own, all.
+struct KeyRows {
+    int begin, end;
+    __device__ __forceinline__ int pieces(const AttnArgs& a) const { return (end - begin + a.piece_rows - 1) / a.piece_rows; }
+};
+__device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, int tile, int keys, bool far_apart) {
+    const int key0 = tile * kGradKeys, position0 = a.sk - a.sq;
+    if (key0 >= keys) return {0, 0};
+    const int last = min(key0 + kGradKeys, keys) - 1;
+    const int t0 = min(max(0, key0 - position0), a.sq);
+    int t1 = a.window < 0 ? a.sq : (int)min((int64_t)a.sq, (int64_t)last + a.window - position0 + 1);
+    if (key0 < a.sinks && !far_apart) t1 = a.sq;
+    return {t0 * a.group, max(t0, t1) * a.group};
+}
+
 // ---- backward: the gradients of keys and values -------------------------------------------------------------
 // Head dims over 128 take two launches, one for each gradient (DK, DV): together their accumulators, keys and values
 // are 384 registers of a lane, and the compiler spilled 330.
@@ -1305,19 +1322,17 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
     const int key = key0 + wave * 32 + (lane & 31);
     const int wv_first = __builtin_amdgcn_readfirstlane(key0 + wave * 32), wv_last = wv_first + 31;
 
-    // The rows that see some key of the tile: those from its first position to the end of its last one's window, and
-    // where it holds sinks all behind.
-    int row_begin = 0, row_end = 0;
-    if (key0 < keys) {
-        const int last = min(key0 + kGradKeys, keys) - 1;
-        const int t0 = min(max(0, key0 - position0), a.sq);
-        int t1 = a.window < 0 ? a.sq : max(0, (int)min((int64_t)a.sq, (int64_t)last + a.window - position0 + 1));
-        if (key0 < a.sinks && !far_of_tile) t1 = a.sq;
-        const int begin = (far ? max(t0, t1) : t0) * a.group, end = (far ? a.sq : t1) * a.group;
-        const int parts = far ? a.far_parts : a.near_parts;
-        const int each = max(0, (end - begin + kStepRows - 1) / kStepRows + parts - 1) / parts * kStepRows;
-        row_begin = min(begin + part * each, end);
-        row_end = min(row_begin + each, end);
+    const KeyRows seen = key_rows(a, kt, keys, far_of_tile != 0);
+    int row_begin, row_end;
+    if (far) {
+        const int each = ((a.sq * a.group - seen.end + kStepRows - 1) / kStepRows + a.far_parts - 1) / a.far_parts * kStepRows;
+        row_begin = min(seen.end + part * each, a.sq * a.group);
+        row_end = min(row_begin + each, a.sq * a.group);
+        if (key0 >= keys) row_end = row_begin;
+    } else {
+        if (part >= seen.pieces(a) && a.near_parts + far_of_tile > 1) return;  // the join knows
+        row_begin = min(seen.begin + part * a.piece_rows, seen.end);
+        row_end = min(row_begin + a.piece_rows, seen.end);
     }
 
     typedef Flight<DP, kStepRows> Fl;
@@ -1510,17 +1525,22 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnArgs a) {
     const int quads = a.d / 4, tile = blockIdx.y;
     const uint32_t bh = blockIdx.x / (kGradKeys / 32), slice = blockIdx.x % (kGradKeys / 32);
     const int b = a.by_kv.div(bh), g = bh - b * a.kv;
+    const int keys = a.lengths ? max(0, min(a.lengths[b], a.sk)) : a.sk;
+    const int near = key_rows(a, tile, keys, tile < a.sink_tiles && a.far_parts > 0).pieces(a);  // those that were written
     for (int at = threadIdx.x; at < 32 * quads; at += 256) {
         const int row = slice * 32 + at / quads, dim = at % quads * 4, key = tile * kGradKeys + row;
         if (key >= a.sk) return;
         const float* from = a.part_o + grad_piece(a, bh, tile) * 2 * kGradKeys * a.d + row * a.d + dim;
-        const int pieces = a.near_parts + (key < a.sinks && tile < a.sink_tiles ? a.far_parts : 0);
         f32x4 dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
-        for (int p = 0; p < pieces; ++p) {
-            dk += *reinterpret_cast<const f32x4*>(from);
-            dv += *reinterpret_cast<const f32x4*>(from + kGradKeys * a.d);
-            from += 2 * kGradKeys * a.d;
-        }
+        auto add = [&](int first, int count) {
+            for (int p = first; p < first + count; ++p) {
+                const float* x = from + (int64_t)p * 2 * kGradKeys * a.d;
+                dk += *reinterpret_cast<const f32x4*>(x);
+                dv += *reinterpret_cast<const f32x4*>(x + kGradKeys * a.d);
+            }
+        };
+        add(0, near);
+        if (key < a.sinks && tile < a.sink_tiles) add(a.near_parts, a.far_parts);
         dk *= a.scale;
         *reinterpret_cast<u32x2*>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2] + dim) * 2) =
             u32x2{Elem<T>::pack(dk[0], dk[1]), Elem<T>::pack(dk[2], dk[3])};

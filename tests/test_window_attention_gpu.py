@@ -84,6 +84,13 @@ def test_rows_far_behind_the_window_reach_the_sinks(device, window, sinks, h, h_
     compare(*inputs(2600, 2600, 1, h, h_kv, 128, torch.float16, device), window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("h,h_kv,lengths", [(4, 1, None), (6, 2, [1300, 40]), (3, 1, [0, 1301])])
+def test_key_gradients_in_pieces_under_a_bare_causal_mask(device, h, h_kv, lengths):
+    # few key tiles, whose first ones have many more rows than the last: pieces of one size, fewer of them for later tiles
+    compare(*inputs(1301, 1301, 2, h, h_kv, 64, torch.bfloat16, device), lengths=lengths)
+    compare(*inputs(700, 1301, 2, h, h_kv, 64, torch.bfloat16, device), lengths=lengths, window=1250, sinks=3)
+
+
 @pytest.mark.parametrize("lengths", [[0, 0, 0], [1, 200, 199], [64, 128, 63], [200, 500, -3]])
 @pytest.mark.parametrize("window,sinks", [(50, 0), (50, 4), (None, 0)])
 def test_key_lengths_leave_rows_empty(device, lengths, window, sinks):
