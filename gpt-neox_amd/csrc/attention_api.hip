@@ -155,7 +155,9 @@ struct GradPlan {
 
 // Pieces of a tile's near rows, of one size for all tiles: so many that two workgroups run on every CU, or under a bare
 // causal mask, whose first tiles have twice the rows of the average, so that no piece is longer than a CU's share; 256
-// rows or more for each.  Rows behind the window of a tile that holds sinks come in pieces of 512 rows.
+// rows or more for each.  Rows behind the window of a tile that holds sinks come in pieces of 512 rows, or longer
+// ones where those would be more than two for every workgroup that fits (many sinks are many such tiles, and every piece is
+// scratch).
 static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int window, int sinks) {
     GradPlan p{};
     const int64_t group = h / h_kv, units = (int64_t)b * h_kv;
@@ -174,8 +176,9 @@ static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int win
     if (behind > 0) {
         p.sink_tiles = (int)((last + kGradKeys - 1) / kGradKeys);
         const int64_t rows = (behind < sq ? behind : sq) * group;
-        const int64_t far = (rows + 511) / 512;
-        p.far_parts = far > 64 ? 64 : (int)far;
+        const int64_t far = (rows + 511) / 512, enough = (1024 + units * p.sink_tiles - 1) / (units * p.sink_tiles);
+        p.far_parts = (int)(far < enough ? far : enough);
+        if (p.far_parts > 64) p.far_parts = 64;
     }
     const bool cut = p.near_parts > 1 || p.far_parts > 0;
     const int64_t pieces = (int64_t)p.key_tiles * p.near_parts + (int64_t)p.sink_tiles * p.far_parts;

@@ -27,8 +27,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
-constexpr int kTileKeys = 64;   // keys of one step of the forward and the query-gradient kernel
-constexpr int kTileRows = 128;  // rows of a workgroup there: 32 for each of its four waves
+constexpr int kTileRows = 128;  // rows of a workgroup of the forward and the query-gradient kernel: 32 for each of its four waves
+constexpr int kTileKeys = 64;   // keys of one step of the query-gradient kernel
 constexpr int kStepRows = 32;   // rows of one step of the key-gradient kernel
 constexpr int kGradKeys = 128;  // keys of a workgroup there: 32 for each of its four waves
 
@@ -208,9 +208,7 @@ __device__ __forceinline__ u32x4 load8(const char* p, bool there) {
     return there ? *reinterpret_cast<const u32x4*>(p) : z;
 }
 
-// Writes the 32 columns' results of one wave (lane: column, registers: 32 dims per block) times f as rows of 16-bit
-// elements, and at `low` (where that is not null) what the rounding took from them.  The halves exchange registers, so
-// that every lane stores 16 bytes.
+// two values rounded to 16 bits, and what the rounding took from them, rounded too
 template <typename T>
 __device__ __forceinline__ uint32_t pack_with_rest(float x, float y, uint32_t& rest) {
     const uint32_t w = Elem<T>::pack(x, y);
@@ -219,6 +217,9 @@ __device__ __forceinline__ uint32_t pack_with_rest(float x, float y, uint32_t& r
     rest = Elem<T>::pack(x - a, y - b);
     return w;
 }
+// Writes the 32 columns' results of one wave (lane: column, registers: 32 dims per block) times f as rows of 16-bit
+// elements, and with LOW at `low` what the rounding took from them.  The halves exchange registers, so that every lane
+// stores 16 bytes.
 template <typename T, int DP, bool LOW = false>
 __device__ __forceinline__ void store_rows(char* row, const f32x16 (&acc)[DP / 32], float f, int d, bool there, char* low = nullptr) {
     const int half = (threadIdx.x & 63) >> 5;
@@ -277,7 +278,7 @@ __device__ __forceinline__ uint32_t widen2(uint32_t word, bool upper) {
         return __builtin_bit_cast(uint32_t, x);
     }
 }
-// ... and as 16-bit values, exactly: no code has more than 7 bits of significand
+// eight codes as 16-bit values, exactly: no code has more than 7 bits of significand
 template <typename T, int SRC>
 __device__ __forceinline__ u32x4 widen8(const u32x2& w) {
     if constexpr (SRC == kPagedF8) {
@@ -338,15 +339,13 @@ struct Sight {
 };
 
 // ---- staging -----------------------------------------------------------------------------------------
-// One tile of ROWS rows (of keys, say) on its way from memory to LDS through registers: 256 threads, a piece
-// of 8 elements at a time.  Rows behind the last key and dims behind d come as zeros: what lies there may be anything.
+// One tile of ROWS rows of codes on its way from memory to LDS through registers, where they become 16-bit values: 256
+// threads, 8 codes at a time.  Rows behind the last key and dims behind d come as zeros: what lies there may be anything.
 template <typename T, int DP, int SRC, int ROWS>
 struct Stage {
     static constexpr int kRowsAtOnce = 256 / Tile<DP>::kPieces;  // DP = 96: 21, the last threads idle
     static constexpr int kSteps = (ROWS + kRowsAtOnce - 1) / kRowsAtOnce;
-    static constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
-    u32x4 w[kCodes ? 1 : kSteps];
-    u32x2 c[kCodes ? kSteps : 1];
+    u32x2 codes[kSteps];
 
     static __device__ __forceinline__ int row(int step) { return (int)(threadIdx.x / Tile<DP>::kPieces) + step * kRowsAtOnce; }
     static __device__ __forceinline__ int piece() { return (int)(threadIdx.x % Tile<DP>::kPieces); }
@@ -355,33 +354,22 @@ struct Stage {
     }
 
     __device__ __forceinline__ void load(int step, const char* at, bool there) {
-        if constexpr (kCodes) {
-            c[step] = u32x2{0, 0};
-            if (there) c[step] = *reinterpret_cast<const u32x2*>(at);
-        } else {
-            w[step] = load8(at, there);
-        }
+        codes[step] = u32x2{0, 0};
+        if (there) codes[step] = *reinterpret_cast<const u32x2*>(at);
     }
     __device__ __forceinline__ void put(char* tile) const {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             if (!works(s)) continue;
-            u32x4 x;
-            if constexpr (kCodes) {
-                // (or the compiler takes the words apart where they are loaded, and waits for them there)
-                u32x2 codes = c[s];
-                asm("" : "+v"(codes.x), "+v"(codes.y));
-                x = widen8<T, SRC>(codes);
-            } else {
-                x = w[s];
-            }
-            *reinterpret_cast<u32x4*>(tile + Tile<DP>::at(row(s), piece())) = x;
+            u32x2 c = codes[s];
+            asm("" : "+v"(c.x), "+v"(c.y));  // (or the compiler takes the words apart where they are loaded, and waits for them there)
+            *reinterpret_cast<u32x4*>(tile + Tile<DP>::at(row(s), piece())) = widen8<T, SRC>(c);
             __builtin_amdgcn_sched_barrier(0);  // one step after the other: their values together would not fit the registers
         }
     }
 };
 
-// The same for 16-bit rows without registers in between: every lane names the 16 bytes that go to its place of the
+// 16-bit rows get there without registers in between: every lane names the 16 bytes that go to its place of the
 // tile (256 threads, a wave 1 KiB at a time), or writes zeros there.  The copies are in flight until landed().
 template <int DP, int ROWS>
 struct Flight {
@@ -416,6 +404,17 @@ constexpr int64_t kSmallStride = 1 << 25;  // elements: a tile's offsets fit 32 
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---- forward --------------------------------------------------------------------------------------------
+// O = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m), x = scale log2(e) q.k over the keys that a row sees, in one pass over
+// them with the running maximum m and the running sum in registers; lse = m + log2(sum).  A workgroup has 128 rows of one
+// (sample, key head), 32 in each wave, and steps over the tiles of keys that any of them sees, copied into one half of LDS
+// while the other is worked on.  The probabilities are rounded to the 16-bit type, as the second product takes them; what
+// that costs is half an ulp of each, as where they are stored.
+// Bound by the matrix cores and, about half as long, by the exponentials and the mask around them, which overlap with
+// them only where two waves of a SIMD are at different places.  Measured, us and what its two products reach: 8192 tokens,
+// 32 heads of 128 dims, window 4096 (bf16) 506, 815 TFLOP/s; 2 x 2048 tokens, 64 heads of 96 dims, window 512 (fp16) 98,
+// 463 TFLOP/s, of which a quarter of the columns are padding and the edges of the window are computed and masked.
+// Chunks of 512 tokens of four sequences over 16384 keys, window 4096, 32 heads on 8, fp8: 197, 521 TFLOP/s, the widening
+// of codes being work of its own.
 template <typename T, int DP, int SRC, bool SPLIT>
 __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged16 ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
     constexpr bool kPages = SRC != kStrided;
@@ -426,8 +425,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     // codes, whose widening takes the registers anyway, 64 save barriers (chunks of 512 over 16384 in fp8: 251, 275).
     constexpr int kFwdKeys = kCodes ? 64 : 32;
     constexpr int kTile = kFwdKeys * Tile<DP>::kRow;
-    constexpr int kBuffers = 2;
-    __shared__ __attribute__((aligned(512))) char lds[kBuffers * 2 * kTile + (kCodes ? 2 * 2 * kFwdKeys * 4 : 0)];
+    __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile + (kCodes ? 2 * 2 * kFwdKeys * 4 : 0)];
 
     // block -> (sample, key head), row tile, part: neighbours in time on one XCD (blocks go to the 8 XCDs in
     // turn) are the row tiles of one key head, whose keys they share
@@ -497,7 +495,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     const bool has_dims = (int)lane_piece * 8 < a.d;
     if (even && !has_dims) {
 #pragma unroll
-        for (int s = 0; s < 2 * kBuffers * Fl::kSteps; ++s) fl.zero(s, lds);
+        for (int s = 0; s < 2 * 2 * Fl::kSteps; ++s) fl.zero(s, lds);
     }
     uint32_t tile_page = 0;
     auto look_up = [&](int tile) {
@@ -580,7 +578,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
             }
         }
     };
-    float* const scales = reinterpret_cast<float*>(lds + kBuffers * 2 * kTile);  // [buffer][keys, values][64]
+    float* const scales = reinterpret_cast<float*>(lds + 2 * 2 * kTile);  // [buffer][keys, values][64]
     auto put = [&](int buffer) {
         if constexpr (kCodes) {
             ks.put(lds + buffer * 2 * kTile);
@@ -621,11 +619,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     __syncthreads();
 
     for (int it = first_tile; it < end_tile; ++it) {
-        const int buffer = kBuffers == 2 ? (it - first_tile) & 1 : 0;
+        const int buffer = (it - first_tile) & 1, next = buffer ^ 1;
         const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
         const int key0 = tiles.tile(it) * kFwdKeys;
-        const int next = kBuffers == 2 ? buffer ^ 1 : 0;
-        if (kBuffers == 2 && it + 1 < end_tile) {
+        if (it + 1 < end_tile) {
             fetch(tiles.tile(it + 1), next);
             if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
         }
@@ -729,14 +726,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                 matrix_done(!kCodes);
             }
         }
-        if (it + 1 < end_tile) {
-            if constexpr (kBuffers == 1) {
-                __syncthreads();
-                fetch(tiles.tile(it + 1), next);
-                if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
-            }
-            put(next);
-        }
+        if (it + 1 < end_tile) put(next);
         __syncthreads();
     }
 
@@ -768,6 +758,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 // 32 at a time, with no barrier before the end.  16x16x32 tiles.  A lane fetches, of keys l % 16 and 16 + l % 16, the
 // 16-byte pieces that go into its first operands as they are (16-bit: 8 dims from 32 s + 8 (l / 16); codes: 16 dims from
 // 64 s + 16 (l / 16)); the same pieces of the values go through LDS of the wave's own for the transposing reads.
+// Measured, 32 heads on 8 of 128 dims: one token of each of 64 sequences of 2048 to 8192 keys, int8, 158 us, 4.4 TB/s, in
+// 4096 workgroups of unequal length; one token over 131001 keys in bf16, 114 us, 4.7 TB/s (a copy of large tensors reaches
+// 4.9, and a kernel that does nothing but read such rows 5.3 to 5.7).
 template <typename T, int DP, int SRC, bool SPLIT>
 __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(AttnArgs a) {
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
@@ -1056,7 +1049,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
 }
 
 // Joins the parts of a split key axis: a workgroup per row, 64 threads for the dims (four each), four groups of them for
-// every fourth part.
+// every fourth part.  O = sum_s 2^(lse_s - m) O_s / sum_s 2^(lse_s - m), m the largest lse.  Latency: 3 to 6 us for 16 to
+// 4096 rows, the launch among them.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 sums[4][64];
@@ -1099,6 +1093,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 }
 
 // ---- backward: the queries' gradient, and the rows' sums of dO * O -----------------------------------------
+// P = 2^(x - lse), dS = P (dO.v - delta), delta = sum_d dO O, dQ = scale sum_j dS_j k_j: the scores once more, row by row as
+// in the forward kernel, with no maximum to keep.  Queries and dO stay in registers, delta is left for the keys' kernel.
+// dS is rounded to the 16-bit type for the last product.  That the scores are computed here and again there (7 products for
+// 5) buys gradients that are summed in registers, in a fixed order, without atomics.
+// Bound by the matrix cores as the forward kernel is.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 735 us, 842
+// TFLOP/s for its three products; 8 x 1001 tokens, 16 heads of 64 dims,
+// window 256 (fp16): 50 us.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
     constexpr int kTile = kTileKeys * Tile<DP>::kRow;
@@ -1290,6 +1291,12 @@ __device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, int tile, int key
 }
 
 // ---- backward: the gradients of keys and values -------------------------------------------------------------
+// dV_j = sum_i P_ij dO_i, dK_j = scale sum_i dS_ij q_i.  A workgroup has 128 keys of one (sample, key head), 32 in each wave,
+// whose keys and values stay in registers, and steps over 32 rows at a time of all the heads that share them: the sum over
+// the group is part of the same chain.  P and dS are rounded to the 16-bit type for the products.  One wave's accumulators
+// are 2 x 64 registers at 128 dims, which with the operands leaves two workgroups on a CU.
+// Bound by the matrix cores and the waits of a CU's few waves.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 927
+// us, 891 TFLOP/s for its four products; 4096 tokens, 32 heads on 8, window 1024: 200 us and 19 of the join.
 // Head dims over 128 take two launches, one for each gradient (DK, DV): together their accumulators, keys and values
 // are 384 registers of a lane, and the compiler spilled 330.
 template <typename T, int DP, bool DK, bool DV>
@@ -1519,7 +1526,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
     }
 }
 
-// Sums the pieces of the key tiles that were done in several, in order: a thread per four dims of a key.
+// Sums the pieces of the key tiles that were done in several, in order: a thread per four dims of a key.  Bound by memory, 4
+// to 19 us.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnArgs a) {
     const int quads = a.d / 4, tile = blockIdx.y;

@@ -354,11 +354,13 @@ int neox_rope_apply_freqs(void* out_q, void* out_k, const void* q, const void* k
  * uses key head x / (h / h_kv).  d: a multiple of 8, at most 256; every stride a multiple of 8 elements
  * below 2^31 and every pointer 16-byte aligned.  key_lengths: int32 [b] in device memory, or NULL for sk keys
  * everywhere; keys and values behind a length, or behind the window of every query of a tile, are not
- * looked at.  (A value that is infinite or NaN reaches the queries of its own tile -- 64 keys, 128
- * query rows -- also where the mask hides it.)  lse, fp32 [b * h * sq], and out_low, laid out
+ * looked at.  (Queries and keys are worked on 32 by 32.  Where one of the queries sees one of the keys, another
+ * of those keys or its value, if infinite or NaN, reaches queries that do not see it: its product with zero is
+ * NaN.)  lse, fp32 [b * h * sq], and out_low, laid out
  * as out, are for the backward pass (NULL: not wanted): every row's logarithm, in an order of its own, and what
- * rounding the output to 16 bits took away, without which (out_low NULL there) the gradients lose some precision.  fp32 arithmetic on the matrix cores' 16-bit
- * products; the probabilities are rounded to the 16-bit type before they meet the values.
+ * rounding the output to 16 bits took away, without which (out_low NULL there) the backward pass takes the
+ * rounded output for the sums of dout * out and its gradients lose some precision.  fp32 sums of the matrix cores' 16-bit products; the
+ * probabilities are rounded to the 16-bit type before they meet the values.
  * Backward: dk and dv are summed over the query heads of their key head in a fixed order; workspace holds
  * as many bytes of scratch as neox_window_attention_bwd_workspace says for the same sizes.  The gradients may
  * not alias anything else.
@@ -373,8 +375,8 @@ int neox_window_attention_fwd(void* out, void* out_low, float* lse, const void* 
 int neox_window_attention_bwd_workspace(int64_t* bytes, int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d,
                                         int32_t window, int32_t sinks);
 int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, const void* dout,
-                              const void* out, const void* out_low, const float* lse, const void* q, const void* k, const void* v, const int32_t* key_lengths,
-                              int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d,
+                              const void* out, const void* out_low, const float* lse, const void* q, const void* k,
+                              const void* v, const int32_t* key_lengths, int32_t b, int32_t sq, int32_t sk, int32_t h, int32_t h_kv, int32_t d,
                               const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
                               const int64_t dout_strides[3], const int64_t out_strides[3], const int64_t q_strides[3],
                               const int64_t k_strides[3], const int64_t v_strides[3], float scale, int32_t window,
