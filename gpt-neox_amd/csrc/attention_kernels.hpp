@@ -321,21 +321,21 @@ __device__ __forceinline__ void paged_sample(const AttnArgs& a, int b, int& toke
 // from lo to hi and, where sinks reach this far, the first ones.  One subtraction and one comparison each: an offset
 // below zero is a large unsigned number.
 struct Sight {
-    int lo, width, sinks, hi;
-    __device__ __forceinline__ Sight(int position, int keys, int window, int sinks_, int first, int half) {
+    int lo, width, front;  // front: the last of the sinks that the row sees
+    __device__ __forceinline__ Sight(int position, int keys, int window, int sinks, int first, int half) {
         const int base = first + 4 * half;
-        hi = min(position, keys - 1) - base;
+        const int hi = min(position, keys - 1) - base;
         lo = window < 0 ? -base : position - window - base;
         width = hi - lo;
         if (width < 0) {  // nothing: no offset from here is small enough
             lo = 1 << 30;
             width = 0;
         }
-        sinks = sinks_ - base;
+        front = min(sinks - 1 - base, hi);
     }
     static __device__ __forceinline__ constexpr int offset(int r) { return 8 * (r >> 2) + (r & 3); }
     __device__ __forceinline__ bool window(int r) const { return (uint32_t)(offset(r) - lo) <= (uint32_t)width; }
-    __device__ __forceinline__ bool any(int r) const { return window(r) || (offset(r) < sinks && offset(r) <= hi); }
+    __device__ __forceinline__ bool any(int r) const { return window(r) | (offset(r) <= front); }
 };
 
 // ---- staging -----------------------------------------------------------------------------------------

@@ -84,6 +84,12 @@ def test_rows_far_behind_the_window_reach_the_sinks(device, window, sinks, h, h_
     compare(*inputs(2600, 2600, 1, h, h_kv, 128, torch.float16, device), window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("h,h_kv,sinks", [(32, 32, 1400), (24, 12, 1100), (40, 20, 2000)])
+def test_many_sinks_over_many_heads(device, h, h_kv, sinks):
+    # more key tiles hold sinks than the rows behind their window can be cut for
+    compare(*inputs(2050, 2048, 1, h, h_kv, 16, torch.bfloat16, device), window=64, sinks=sinks)
+
+
 @pytest.mark.parametrize("h,h_kv,lengths", [(4, 1, None), (6, 2, [1300, 40]), (3, 1, [0, 1301])])
 def test_key_gradients_in_pieces_under_a_bare_causal_mask(device, h, h_kv, lengths):
     # few key tiles, whose first ones have many more rows than the last: pieces of one size, fewer of them for later tiles
