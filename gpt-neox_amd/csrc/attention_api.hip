@@ -6,8 +6,15 @@
 namespace neox {
 
 // ---- launches whose kernels do not depend on the head dim ------------------------------------------------
+// A wave for each row where there are many rows in few parts, else a workgroup (bf16, 128 dims, us: 32768 rows in 2 parts
+// 24 with a workgroup, 11 with a wave; 16384 in 4 14, 9; 4096 in 16 8.6, 7.2; 2048 in 4 4.4, 4.5; 512 in 16 4.8, 6.4).
 hipError_t launch_attn_join(const AttnArgs& a, int dtype, hipStream_t stream) {
     const uint32_t blocks = (uint32_t)a.part_rows;
+    if (a.splits <= 16 && a.part_rows >= 4096) {
+        if (dtype == NEOX_BF16) attn_join_rows_kernel<BF16><<<(blocks + 3) / 4, 256, 0, stream>>>(a);
+        else attn_join_rows_kernel<F16><<<(blocks + 3) / 4, 256, 0, stream>>>(a);
+        return hipGetLastError();
+    }
     if (dtype == NEOX_BF16) attn_join_kernel<BF16><<<blocks, 256, 0, stream>>>(a);
     else attn_join_kernel<F16><<<blocks, 256, 0, stream>>>(a);
     return hipGetLastError();

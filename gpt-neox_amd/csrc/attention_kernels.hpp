@@ -1092,6 +1092,36 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     *reinterpret_cast<u32x2*>(a.o + (token * a.o_st[0] + head * a.o_st[2] + dim) * 2) = w;
 }
 
+// The same with a wave for each row, for many rows in at most 64 parts: 32 lanes for the dims up to 128 (then the halves take every other
+// part), 64 above.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
+    const int lane = threadIdx.x & 63, lanes = a.d <= 128 ? 32 : 64, groups = 64 / lanes, part = lane / lanes, dim = lane % lanes * 4;
+    const int64_t slot = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (slot >= a.part_rows) return;
+    const float lse = lane < a.splits ? a.part_lse[lane * a.part_rows + slot] : kNegInf;
+    const float high = wave_reduce<OpMax>(lse);  // (a NaN is not the largest; it reaches the total)
+    const float f = __builtin_amdgcn_exp2f(lse - (high == kNegInf ? 0.f : high));
+    const float total = wave_reduce<OpSum>(f);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    const float* from = a.part_o + slot * a.d + dim;
+#pragma unroll 4
+    for (int s0 = 0; s0 < a.splits; s0 += groups) {
+        const int s = s0 + part;
+        const float weight = __shfl(f, s);  // (0 behind the last part)
+        if (s < a.splits && dim < a.d) sum += *reinterpret_cast<const f32x4*>(from + s * a.part_rows * a.d) * weight;
+    }
+    if (groups == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = both_halves_sum(sum[i]);
+    }
+    if (part || dim >= a.d) return;
+    const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+    const int64_t token = slot / (a.kv * a.group), head = slot - token * (a.kv * a.group);
+    const u32x2 w = {Elem<T>::pack(sum[0] * inverse, sum[1] * inverse), Elem<T>::pack(sum[2] * inverse, sum[3] * inverse)};
+    *reinterpret_cast<u32x2*>(a.o + (token * a.o_st[0] + head * a.o_st[2] + dim) * 2) = w;
+}
+
 // ---- backward: the queries' gradient, and the rows' sums of dO * O -----------------------------------------
 // P = 2^(x - lse), dS = P (dO.v - delta), delta = sum_d dO O, dQ = scale sum_j dS_j k_j: the scores once more, row by row as
 // in the forward kernel, with no maximum to keep.  Queries and dO stay in registers, delta is left for the keys' kernel.

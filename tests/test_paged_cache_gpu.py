@@ -244,6 +244,15 @@ def test_chunks(device, dtype, codes, d):
     check(*sequences(device, dtype, codes or dtype, [70, 33], [500, 129], 8, 1, d, 48), window=100, sinks=3)
 
 
+@pytest.mark.parametrize("d", [8, 40, 128, 136, 256])
+@pytest.mark.parametrize("new,context", [([601, 500], [3001, 700]), ([1025], [1030]), ([300, 0, 301], [5000, 9, 301])])
+def test_many_rows_in_a_few_parts(device, d, new, context):
+    args = sequences(device, torch.bfloat16, torch.bfloat16, new, context, 8, 2, d, 64)
+    got = check(*args)
+    assert torch.equal(got, check(*args))
+    check(*args, window=700, sinks=5)
+
+
 @pytest.mark.parametrize("page", [1, 3, 16, 31, 32, 64, 100, 256])
 @pytest.mark.parametrize("codes", [I8, torch.bfloat16])
 def test_page_sizes(device, page, codes):
