@@ -202,10 +202,12 @@ struct PagedPlan {
 };
 
 // Parts: so many that every CU has workgroups enough, with at least 256 keys for each part and 128 parts at most.  Row
-// tiles: two to a CU.  Single tokens: eight, twice what fits, because sequences differ in length and the host does not
+// tiles: as many as fit a CU, three that read 16 bits (2 x 512 tokens over 4096, 32 heads on 8: 111 us with two, 95 with three;
+// 2 x 1000 over 3000, 32 heads: 118, 91; but 4 x 512 with a window of 4096: 205, 222) and two that widen codes (1 x 512 over 8192: 121
+// with two, 137 with three).  Single tokens: eight, twice what fits, because sequences differ in length and the host does not
 // know by how much: 64 sequences of 2048 to 8192 tokens, int8, take 191 us with four (170 before four fitted), 158 with
 // eight, 169 with sixteen; one of 131001 tokens in bf16 takes 125 us with 128 parts and 128 with 256.
-static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, int h, int h_kv, int d, int window, int sinks) {
+static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, int h, int h_kv, int d, int window, int sinks, bool codes) {
     PagedPlan p{};
     const int64_t group = h / h_kv, rows = max_query * group;
     p.token = rows <= 16;
@@ -215,7 +217,7 @@ static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, i
         const int64_t seen = (int64_t)window + max_query + sinks;
         if (seen < keys) keys = seen;
     }
-    const int64_t units = (int64_t)b * h_kv * p.row_tiles, target = 256 * (p.token ? 8 : 2);
+    const int64_t units = (int64_t)b * h_kv * p.row_tiles, target = 256 * (p.token ? 8 : codes ? 2 : 3);
     int64_t splits = (target + units - 1) / units;
     const int64_t most = (keys + 255) / 256;
     if (splits > most) splits = most;
@@ -438,7 +440,7 @@ int neox_paged_attention_workspace(int64_t* bytes, int32_t b, int32_t tokens, in
     if (!bytes) return fail(NEOX_ERR_NULL_POINTER, "%s: bytes is null", what);
     NEOX_TRY(check_paged_sizes(b, tokens, max_query, max_context, h, h_kv, d, what));
     NEOX_TRY(check_scale_window(1.f, sinks, what));
-    *bytes = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks).bytes;
+    *bytes = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, false).bytes;  // (codes need no more)
     return NEOX_OK;
 }
 
@@ -464,13 +466,13 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
     if (table_columns < 1 || table_stride < 0)
         return fail(NEOX_ERR_BAD_SHAPE, "%s: page_table needs a column and no negative stride (%d, %lld)", what, table_columns, (long long)table_stride);
     NEOX_TRY(check_scale_window(scale, sinks, what));
-    const PagedPlan plan = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks);
+    const int source = cache_source_of(cache_dtype, dtype);
+    const PagedPlan plan = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, source != kPaged16);
     if (plan.bytes > 0) {
         NEOX_TRY(check_pointer(workspace, 16, what, "workspace"));
         if (workspace_bytes < plan.bytes)
             return fail(NEOX_ERR_BAD_SHAPE, "%s: workspace of %lld bytes, needs %lld", what, (long long)workspace_bytes, (long long)plan.bytes);
     }
-    const int source = cache_source_of(cache_dtype, dtype);
     AttnArgs a{};
     a.b = b;
     a.sq = max_query;
