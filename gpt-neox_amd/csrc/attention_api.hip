@@ -164,7 +164,8 @@ struct GradPlan {
 // causal mask, whose first tiles have twice the rows of the average, so that no piece is longer than a CU's share; 256
 // rows or more for each.  Rows behind the window of a tile that holds sinks come in pieces of 512 rows, or longer
 // ones where those would be more than two for every workgroup that fits (many sinks are many such tiles, and every piece is
-// scratch).
+// scratch).  Where they are no more than 128, and would be the only reason to join pieces, the tile takes them along (256
+// tokens, 8 heads of 64 dims, window 100: a call forward and backward 73 us with them apart, 68 without the second launch).
 static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int window, int sinks) {
     GradPlan p{};
     const int64_t group = h / h_kv, units = (int64_t)b * h_kv;
@@ -180,9 +181,9 @@ static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int win
     const int64_t last = (sinks < sk ? sinks : sk);
     // the last position whose window reaches the first tile is kGradKeys - 1 + window
     const int64_t behind = window < 0 || last < 1 ? 0 : (int64_t)sk - kGradKeys - window;
-    if (behind > 0) {
+    const int64_t rows = (behind < sq ? behind : sq) * group;
+    if (behind > 0 && (p.near_parts > 1 || rows > 128)) {
         p.sink_tiles = (int)((last + kGradKeys - 1) / kGradKeys);
-        const int64_t rows = (behind < sq ? behind : sq) * group;
         const int64_t far = (rows + 511) / 512, enough = (1024 + units * p.sink_tiles - 1) / (units * p.sink_tiles);
         p.far_parts = (int)(far < enough ? far : enough);
         if (p.far_parts > 64) p.far_parts = 64;
