@@ -253,6 +253,11 @@ def test_many_rows_in_a_few_parts(device, d, new, context):
     check(*args, window=700, sinks=5)
 
 
+@pytest.mark.parametrize("codes", [I8, F8, torch.float16])
+def test_many_rows_in_a_few_parts_in_half(device, codes):
+    check(*sequences(device, torch.float16, codes, [601, 500], [3001, 700], 8, 2, 96, 64))
+
+
 @pytest.mark.parametrize("page", [1, 3, 16, 31, 32, 64, 100, 256])
 @pytest.mark.parametrize("codes", [I8, torch.bfloat16])
 def test_page_sizes(device, page, codes):
