@@ -192,12 +192,9 @@ __device__ __forceinline__ float both_halves_sum(float x) {
     return p.a + p.b;
 }
 
-// the largest of three; of numbers from the matrix cores, which the compiler would first make canonical one by one
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
+// the largest of three, in one instruction.  (Written for the compiler to see: behind a matrix instruction it puts the
+// wait states that a reader of the result needs only before instructions that it knows, and not before inline assembly.)
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // the element of a 32-long result axis that register r of a lane in this half holds
 __device__ __forceinline__ int element_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
