@@ -289,6 +289,36 @@ __device__ __forceinline__ u32x4 widen8(const u32x2& w) {
     return pack8<T>(f);
 }
 
+// Where a probability is multiplied by its value's scale before it is rounded to fp16, the product can be anything: scales
+// are the values' own size, over the largest code, and the largest of them may belong to keys that are hardly looked at.
+// The accumulators of a row therefore hold their sums times a power of two of the row's own, which brings the largest
+// product so far to 2^10 .. 2^15: what is then below fp16's normal numbers is less than 2^-24 of it.  bf16 has the
+// range of fp32, and goes without.  4 x 512 tokens over 8192 keys, 32 heads on 8, window 4096, us without it and with: int8 64
+// dims 169, 177, 128 dims 223, 230, 256 dims 647, 713; 64 single tokens over 4096: as before, within 1 %.
+struct Lift {
+    static constexpr uint32_t kField = 0x7f800000u;  // the exponent of a float
+    float times = 0x1p60f;                           // the most, for rows whose products are all zero as yet
+    static __device__ __forceinline__ uint32_t bits(float x) { return __builtin_bit_cast(uint32_t, x); }
+    static __device__ __forceinline__ float power(uint32_t field) { return __builtin_bit_cast(float, field); }
+    static __device__ __forceinline__ float inverse(float p) { return power((254u << 23) - bits(p)); }  // of a power of two
+    __device__ __forceinline__ bool short_of(float most) const { return most * times > 0x1p15f; }
+    // The running maximum has moved and the sums are to be multiplied by f <= 1, as the products that are behind them
+    // are: the power may rise by as much.  Returns the sums' factor.
+    __device__ __forceinline__ float follow(float f) {
+        const uint32_t room = (126u << 23) - min(bits(f) & kField, 126u << 23);  // 1 / f, rounded down, without its bias
+        const float before = times;
+        times = power(min(bits(times) + room, bits(0x1p60f)));
+        return f * (times * inverse(before));
+    }
+    // The power for products up to `most`, no larger than the present one.  Returns the sums' factor.
+    __device__ __forceinline__ float lower(float most) {
+        const float before = times;
+        times = power(min(bits(times), (264u << 23) - max(bits(most) & kField, 77u << 23)));
+        return times * inverse(before);
+    }
+    __device__ __forceinline__ float undone() const { return inverse(times); }
+};
+
 // The tiles of keys that rows with positions first .. last look at: some at the front for the sinks, then those of
 // the window.
 struct KeyTiles {
@@ -592,6 +622,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     float m = kNegInf, l = 0.f;
+    constexpr bool kLifted = kCodes && __is_same(T, F16);
+    Lift lift;
 
     // the first tile is on its way before the queries are waited for
     if (first_tile < end_tile) {
@@ -674,9 +706,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
             // below 256 and the accumulators need no rescaling.
             if (__any(top > m + 8.f)) {
                 const float higher = fmaxf(m, top);
-                const float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
+                float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
                 m = higher;
                 l *= f;
+                if constexpr (kLifted) f = lift.follow(f);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -712,6 +745,25 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                         for (int i = 0; i < 4; ++i) s[kb][r + i] *= c[i];
                     }
             }
+            if constexpr (kLifted) {
+                float most = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 2) most = max3(most, __builtin_fabsf(s[kb][r]), __builtin_fabsf(s[kb][r + 1]));
+                most = both_halves_max(most);
+                if (__any(lift.short_of(most))) {
+                    const float f = lift.lower(most);
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+                }
+#pragma unroll
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] *= lift.times;
+            }
 #pragma unroll
             for (int t = 0; t < kFwdKeys / 16; ++t) {
                 u32x4 p;
@@ -728,7 +780,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     }
 
     const float total = both_halves_sum(l);
-    const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);  // (a NaN stays one)
+    float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);  // (a NaN stays one)
+    if constexpr (kLifted) inverse *= lift.undone();
     if constexpr (SPLIT) {
         const int64_t slot = (int64_t)split * a.part_rows + ((int64_t)(token0 + token) * a.kv + g) * a.group + (head - g * a.group);
         float* p = a.part_o + slot * a.d;
@@ -893,6 +946,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = kNegInf, l = 0.f;
+    constexpr bool kLifted = kCodes && __is_same(T, F16);
+    Lift lift;
 
     look_up(first + wave);
     if (first + wave < end) fetch(first + wave);
@@ -968,9 +1023,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
         top = both_halves_max(top) * a.scale_log2;
         if (__any(top > m + 8.f)) {
             const float higher = fmaxf(m, top);
-            const float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
+            float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
             m = higher;
             l *= f;
+            if constexpr (kLifted) f = lift.follow(f);
 #pragma unroll
             for (int j = 0; j < DP / 16; ++j) acc[j] *= f;
         }
@@ -990,6 +1046,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
                 for (int r = 0; r < 4; ++r) s[kb][r] = s[kb][r] != 0.f ? s[kb][r] * c[r] : 0.f;  // a hidden value's scale may be anything
             }
         }
+        if constexpr (kLifted) {
+            float most = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) most = max3(most, __builtin_fabsf(s[kb][r]), __builtin_fabsf(s[kb][r + 1]));
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = both_halves_max(most);
+            if (__any(lift.short_of(most))) {
+                const float f = lift.lower(most);
+#pragma unroll
+                for (int j = 0; j < DP / 16; ++j) acc[j] *= f;
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[kb] *= lift.times;
+        }
         const u32x4 p = {Elem<T>::pack(s[0][0], s[0][1]), Elem<T>::pack(s[0][2], s[0][3]),
                          Elem<T>::pack(s[1][0], s[1][1]), Elem<T>::pack(s[1][2], s[1][3])};
 #pragma unroll
@@ -1007,7 +1079,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
     l = both_halves_sum(l);
     float* const mine = reinterpret_cast<float*>(vt);
 #pragma unroll
-    for (int db = 0; db < DP / 16; ++db) *reinterpret_cast<f32x4*>(mine + col * DP + 16 * db + 4 * quad) = acc[db];
+    for (int db = 0; db < DP / 16; ++db) {
+        if constexpr (kLifted) acc[db] *= lift.undone();
+        *reinterpret_cast<f32x4*>(mine + col * DP + 16 * db + 4 * quad) = acc[db];
+    }
     if (quad == 0) {
         wave_m[wave][col] = m;
         wave_l[wave][col] = l;

@@ -39,6 +39,12 @@ def attend_paged(q, cache, table, context, **kw):
     return paged_attention(q, cache, table, starts, lengths, max_query=q.shape[0], max_context=context, **kw)
 
 
+def held(cache, table, n):
+    """The keys and values ``[n, h_kv, d]`` that a cache of codes holds, in 64 bits."""
+    return [A.gather(table[0], cache.page_size, n, t.float()).double() * A.gather(table[0], cache.page_size, n, s).double()[..., None]
+            for t, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale))]
+
+
 # ---- the running maximum -------------------------------------------------------------------------------------------
 def steps(d, dtype, device):
     """Queries and keys whose scores come from the last 16 dims alone, and rise from tile to tile by 20 to 70 powers of two:
@@ -66,3 +72,90 @@ def test_the_maximum_is_that_of_the_whole_sums(device, dtype, d):
     within(got, want["out"], want["out_bound"])
     cache, table = one_sequence(k[:, 0], v[:, 0], dtype)
     within(attend_paged(q[:, 0], cache, table, k.shape[0], scale=0.69), want["out"][:, 0], want["out_bound"][:, 0])
+
+
+# ---- small and large values ----------------------------------------------------------------------------------------
+def typical_error(q, k, v, sees, scale, dtype):
+    """One head in 64 bits: the output, and the variance that rounding each weighted value and the output to the type may
+    leave in it.  An error of one rounding is even over half a unit in the last place on both sides, so its variance is a third of
+    (unit roundoff * value)^2 at most, or of half the type's smallest step squared; errors of different keys are independent."""
+    out, p = A.one_head(q, k, v, sees, scale)
+    u, tiny = A.ROUND[dtype], A.TINY[dtype]
+    return out, (u * u * (p.square() @ v.square() + out.square()) + tiny * tiny) / 3
+
+
+def typically_within(got, want, variance):
+    # a quarter more than the roundings' own size: room for the 32-bit part, a tenth of it, and for what a mean over
+    # thousands of elements may be off by
+    assert torch.isfinite(got).all()
+    err, most = (got.double() - want).square().mean().sqrt(), variance.mean().sqrt()
+    assert err <= 1.25 * most, (err / most).item()
+
+
+def sink_and_rest(n, h_kv, d, dtype, device, times, above, seed):
+    """Keys and values ``[n, h_kv, d]``: values of the size ``times``; where ``above`` is given the first key's score is that much above
+    the others' (queries carry 4 in their last dim, with a scale of 1), and its value a hundred times smaller."""
+    k, v = normal((n, h_kv, d), dtype, device, seed, 0.02), normal((n, h_kv, d), dtype, device, seed + 1, times)
+    k[..., -1] = 0
+    if above:
+        k[0, :, -1] = above / 4
+        v[0] *= 0.01
+    return k, v
+
+
+@pytest.mark.parametrize("codes", [I8, F8])
+@pytest.mark.parametrize("times,above", [(1.0, 0), (0.1, 0), (0.01, 0), (0.002, 0), (1.0, 6), (0.3, 8), (0.05, 10)])
+@pytest.mark.parametrize("n,new", [(250, 1), (3000, 1), (250, 60), (3000, 60)])
+def test_codes_keep_the_precision_of_half(device, codes, times, above, n, new):
+    h, h_kv, d = 8, 4, 64
+    k, v = sink_and_rest(n, h_kv, d, torch.float16, device, times, above, 5)
+    q = normal((new, h, d), torch.float16, device, 7)
+    q[..., -1] = 4
+    cache, table = one_sequence(k, v, codes)
+    got = attend_paged(q, cache, table, n, scale=1.0)
+    hk, hv = held(cache, table, n)
+    sees = A.visible(new, n, device=device)
+    want, variance = torch.empty(got.shape, dtype=torch.float64, device=device), torch.empty(got.shape, dtype=torch.float64, device=device)
+    for x in range(h):
+        want[:, x], variance[:, x] = typical_error(q[:, x].double(), hk[:, x // 2], hv[:, x // 2], sees, 1.0, q.dtype)
+    typically_within(got, want, variance)
+
+
+@pytest.mark.parametrize("codes", [I8, F8, torch.float16])
+@pytest.mark.parametrize("n,new", [(250, 1), (3000, 1), (250, 60), (3000, 60)])
+def test_values_near_the_largest_of_half(device, codes, n, new):
+    # scores that rise, behind every wave's first keys, by a little less than what the running maximum may lag behind
+    h, d = 4, 64
+    k = normal((n, h, d), torch.float16, device, 8, 0.02)
+    k[..., -1] = torch.where(torch.arange(n, device=device) % 256 < 128, 0.0, 7.2 * 0.6931 / 4)[:, None]
+    v = (normal((n, h, d), torch.float16, device, 9).sign() * 60000).to(torch.float16)
+    q = normal((new, h, d), torch.float16, device, 10)
+    q[..., -1] = 4
+    cache, table = one_sequence(k, v, codes)
+    got = attend_paged(q, cache, table, n, scale=1.0)
+    quantised = codes in (I8, F8)
+    want, bound = A.paged_attention(q, cache.k.float() if quantised else cache.k, cache.v.float() if quantised else cache.v, cache.k_scale,
+                                    cache.v_scale, table, [0, new], [n], scale=1.0, dtype=q.dtype)
+    within(got, want, bound)
+
+
+@pytest.mark.parametrize("codes", [I8, F8])
+@pytest.mark.parametrize("new", [1, 60])
+def test_large_values_that_the_maximum_leaves_behind(device, codes, new):
+    # the first keys' values are 2^13 times the others', and their scores 30 powers of two below: their products come first,
+    # and are nothing in the end
+    n, h, d = 2000, 4, 64
+    k, v = normal((n, h, d), torch.float16, device, 11, 0.02), normal((n, h, d), torch.float16, device, 12)
+    behind = torch.arange(n, device=device) % 256 < 128  # (so in every part of a split axis)
+    k[..., -1] = torch.where(behind, 0.0, 30 * 0.6931 / 4)[:, None]
+    v *= torch.where(behind, 2.0**13, 1.0)[:, None, None]
+    q = normal((new, h, d), torch.float16, device, 13)
+    q[..., -1] = 4
+    cache, table = one_sequence(k, v, codes)
+    got = attend_paged(q, cache, table, n, scale=1.0)
+    hk, hv = held(cache, table, n)
+    sees = A.visible(new, n, device=device)
+    want, variance = torch.empty(got.shape, dtype=torch.float64, device=device), torch.empty(got.shape, dtype=torch.float64, device=device)
+    for x in range(h):
+        want[:, x], variance[:, x] = typical_error(q[:, x].double(), hk[:, x], hv[:, x], sees, 1.0, q.dtype)
+    typically_within(got, want, variance)
