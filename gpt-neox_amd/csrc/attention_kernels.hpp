@@ -319,6 +319,11 @@ struct Lift {
     __device__ __forceinline__ float undone() const { return inverse(times); }
 };
 
+// Probabilities that meet 16-bit values are rounded to the type as they are: up to 2^8, which is what the running maximum
+// may lag behind.  In fp16 they are 2^7 times that, so that one is a subnormal number only 2^-21 below the largest.
+template <typename T, bool CODES>
+constexpr float probability_bits() { return __is_same(T, F16) && !CODES ? 7.f : 0.f; }
+
 // The tiles of keys that rows with positions first .. last look at: some at the front for the sinks, then those of
 // the window.
 struct KeyTiles {
@@ -623,6 +628,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     float m = kNegInf, l = 0.f;
     constexpr bool kLifted = kCodes && __is_same(T, F16);
+    constexpr float kBits = probability_bits<T, kCodes>();
     Lift lift;
 
     // the first tile is on its way before the queries are waited for
@@ -715,7 +721,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[i][r] *= f;
             }
-            const float base = m == kNegInf ? 0.f : m;
+            const float base = (m == kNegInf ? 0.f : m) - kBits;
             float sum = 0.f;
 #pragma unroll
             for (int kb = 0; kb < kFwdKeys / 32; ++kb)
@@ -793,13 +799,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                 const f32x4 x = {acc[i][r] * inverse, acc[i][r + 1] * inverse, acc[i][r + 2] * inverse, acc[i][r + 3] * inverse};
                 if (there && dim < a.d) *reinterpret_cast<f32x4*>(p + dim) = x;
             }
-        if (there && half == 0) a.part_lse[slot] = total == 0.f ? kNegInf : m + __builtin_amdgcn_logf(total);
+        if (there && half == 0) a.part_lse[slot] = total == 0.f ? kNegInf : m - kBits + __builtin_amdgcn_logf(total);
     } else {
         const int64_t at = ((int64_t)(token0 + token) * a.o_st[0] + (kPages ? 0 : (int64_t)b * a.o_st[1]) + (int64_t)head * a.o_st[2]) * 2;
         if (!kPages && a.o_low) store_rows<T, DP, true>(a.o + at, acc, inverse, a.d, there, a.o_low + at);
         else store_rows<T, DP>(a.o + at, acc, inverse, a.d, there);
         if (!kPages && a.lse && there && half == 0)
-            a.lse[(int64_t)bh * rows + row] = total == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(total);
+            a.lse[(int64_t)bh * rows + row] = total == 0.f ? __builtin_inff() : m - kBits + __builtin_amdgcn_logf(total);
     }
 }
 
@@ -947,6 +953,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
     for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = kNegInf, l = 0.f;
     constexpr bool kLifted = kCodes && __is_same(T, F16);
+    constexpr float kBits = probability_bits<T, kCodes>();
     Lift lift;
 
     look_up(first + wave);
@@ -1030,7 +1037,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
 #pragma unroll
             for (int j = 0; j < DP / 16; ++j) acc[j] *= f;
         }
-        const float base = m == kNegInf ? 0.f : m;
+        const float base = (m == kNegInf ? 0.f : m) - kBits;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -1113,7 +1120,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
             float* p = a.part_o + slot * a.d + dim;
             *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
             *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
-            if (dim == 0) a.part_lse[slot] = total == 0.f ? kNegInf : high + __builtin_amdgcn_logf(total);
+            if (dim == 0) a.part_lse[slot] = total == 0.f ? kNegInf : high - kBits + __builtin_amdgcn_logf(total);
         } else {
             *reinterpret_cast<u32x4*>(a.o + ((int64_t)(token0 + t) * a.o_st[0] + (int64_t)h * a.o_st[2] + dim) * 2) = pack8<T>(x);
         }

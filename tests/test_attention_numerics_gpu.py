@@ -159,3 +159,24 @@ def test_large_values_that_the_maximum_leaves_behind(device, codes, new):
     for x in range(h):
         want[:, x], variance[:, x] = typical_error(q[:, x].double(), hk[:, x], hv[:, x], sees, 1.0, q.dtype)
     typically_within(got, want, variance)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("above", [0, 8, 11, 13])
+@pytest.mark.parametrize("n,new", [(250, 1), (3000, 1), (250, 60), (3000, 60)])
+def test_probabilities_far_below_a_sink_without_a_value(device, dtype, above, n, new):
+    h, d = 4, 64
+    k, v = sink_and_rest(n, h, d, dtype, device, 100.0, above, 14)
+    if above:
+        v[0] = 0
+    q = normal((new, h, d), dtype, device, 16)
+    q[..., -1] = 4
+    cache, table = one_sequence(k, v, dtype)
+    got = attend_paged(q, cache, table, n, scale=1.0)
+    sees = A.visible(new, n, device=device)
+    want, variance = torch.empty(got.shape, dtype=torch.float64, device=device), torch.empty(got.shape, dtype=torch.float64, device=device)
+    for x in range(h):
+        want[:, x], variance[:, x] = typical_error(q[:, x].double(), k[:, x].double(), v[:, x].double(), sees, 1.0, dtype)
+    typically_within(got, want, variance)
+    with torch.no_grad():
+        typically_within(window_attention(q[:, None], k[:, None], v[:, None], scale=1.0)[:, 0], want, variance)
