@@ -42,7 +42,7 @@ struct AttnArgs {
     const char *q, *k, *v;       // 16-bit elements (k, v: 8-bit codes for the last two sources)
     char* o;
     char* o_low;                 // null, or what rounding the output to 16 bits took away, laid out like the output
-    float* lse;                  // log2 of every row's sum of exponentials, +inf for an empty row; [b, kv, rows]
+    float* lse;                  // log2 of every row's sum of exponentials, less gradient_bits(), +inf for an empty row; [b, kv, rows]
     const float *k_scale, *v_scale;
     // element strides.  q, o: token, sample (strided only), head.  k, v: token, sample, head; for pages the token
     // stride within a page, the page stride and the head stride
@@ -196,6 +196,17 @@ __device__ __forceinline__ float both_halves_sum(float x) {
 // wait states that a reader of the result needs only before instructions that it knows, and not before inline assembly.)
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
+// the largest magnitude of a lane's results
+__device__ __forceinline__ float largest(const f32x16& x) {
+    float top = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) top = max3(top, __builtin_fabsf(x[r]), __builtin_fabsf(x[r + 1]));
+    return top;
+}
+
+// the largest of a wave's numbers, none below zero, as a scalar
+__device__ __forceinline__ float wave_largest(float x) { return wave_reduce<OpMax>(x); }
+
 // the element of a 32-long result axis that register r of a lane in this half holds
 __device__ __forceinline__ int element_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
@@ -316,13 +327,24 @@ struct Lift {
         times = power(min(bits(times), (264u << 23) - max(bits(most) & kField, 77u << 23)));
         return times * inverse(before);
     }
+    // The same where `most` has been multiplied by the power already.
+    __device__ __forceinline__ float lower_by(float most) {
+        const float f = power(min(127u << 23, (264u << 23) - max(bits(most) & kField, 77u << 23)));
+        times *= f;
+        return f;
+    }
     __device__ __forceinline__ float undone() const { return inverse(times); }
+    __device__ __forceinline__ float log2() const { return (float)((int)(bits(times) >> 23) - 127); }
 };
 
 // Probabilities that meet 16-bit values are rounded to the type as they are: up to 2^8, which is what the running maximum
 // may lag behind.  In fp16 they are 2^7 times that, so that one is a subnormal number only 2^-21 below the largest.
 template <typename T, bool CODES>
 constexpr float probability_bits() { return __is_same(T, F16) && !CODES ? 7.f : 0.f; }
+// The backward pass knows the rows' sums, so that no probability is above one: in fp16 it takes 2^14 times each.  The
+// forward pass leaves the rows' logarithms less by as much.
+template <typename T>
+constexpr float gradient_bits() { return __is_same(T, F16) ? 14.f : 0.f; }
 
 // The tiles of keys that rows with positions first .. last look at: some at the front for the sinks, then those of
 // the window.
@@ -754,9 +776,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
             if constexpr (kLifted) {
                 float most = 0.f;
 #pragma unroll
-                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; r += 2) most = max3(most, __builtin_fabsf(s[kb][r]), __builtin_fabsf(s[kb][r + 1]));
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb) most = fmaxf(most, largest(s[kb]));
                 most = both_halves_max(most);
                 if (__any(lift.short_of(most))) {
                     const float f = lift.lower(most);
@@ -805,7 +825,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
         if (!kPages && a.o_low) store_rows<T, DP, true>(a.o + at, acc, inverse, a.d, there, a.o_low + at);
         else store_rows<T, DP>(a.o + at, acc, inverse, a.d, there);
         if (!kPages && a.lse && there && half == 0)
-            a.lse[(int64_t)bh * rows + row] = total == 0.f ? __builtin_inff() : m - kBits + __builtin_amdgcn_logf(total);
+            a.lse[(int64_t)bh * rows + row] = total == 0.f ? __builtin_inff() : m - kBits + __builtin_amdgcn_logf(total) - gradient_bits<T>();
     }
 }
 
@@ -1204,7 +1224,8 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
 // ---- backward: the queries' gradient, and the rows' sums of dO * O -----------------------------------------
 // P = 2^(x - lse), dS = P (dO.v - delta), delta = sum_d dO O, dQ = scale sum_j dS_j k_j: the scores once more, row by row as
 // in the forward kernel, with no maximum to keep.  Queries and dO stay in registers, delta is left for the keys' kernel.
-// dS is rounded to the 16-bit type for the last product.  That the scores are computed here and again there (7 products for
+// dS is rounded to the 16-bit type for the last product; in fp16, times a power of two that follows the largest of its row
+// (Lift), since it is as small as the incoming gradient over the number of keys.  That the scores are computed here and again there (7 products for
 // 5) buys gradients that are summed in registers, in a fixed order, without atomics.
 // Bound by the matrix cores as the forward kernel is.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 735 us, 842
 // TFLOP/s for its three products; 8 x 1001 tokens, 16 heads of 64 dims,
@@ -1320,6 +1341,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     const float scale_log2 = a.scale * kLog2e;
+    // fp16: dS times a power of two of the row's own, which is part of the exponent
+    constexpr bool kLifted = __is_same(T, F16);
+    Lift lift;
+    auto lifted_lse = [&] { return kLifted ? lse + gradient_bits<T>() - lift.log2() : lse; };
+    float row_lse = lifted_lse();
 
     landed();
     __syncthreads();
@@ -1348,7 +1374,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
             for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(ops.rows(kTileKeys + 32 * kb, st), dout[st], dp);
             matrix_done(true);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -lse)) * dp[r];
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, -row_lse)) * dp[r];
             if (!all) {
                 const Sight sight(position, keys, a.window, a.sinks, k0, half);
                 if (k0 < a.sinks) {
@@ -1357,6 +1383,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = sight.window(r) ? s[r] : 0.f;
+                }
+            }
+            if constexpr (kLifted) {
+                const float most = both_halves_max(largest(s));
+                if (__any(most > 0x1p15f)) {
+                    const float f = lift.lower_by(most);
+                    row_lse = lifted_lse();
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] *= f;
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
                 }
             }
 #pragma unroll
@@ -1374,7 +1413,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
         __syncthreads();
     }
     char* p = a.dq + ((int64_t)token * a.dq_st[0] + (int64_t)b * a.dq_st[1] + (int64_t)head * a.dq_st[2]) * 2;
-    store_rows<T, DP>(p, acc, a.scale, a.d, there);
+    store_rows<T, DP>(p, acc, kLifted ? a.scale * lift.undone() : a.scale, a.d, there);
 }
 
 // the first piece of a key tile in the partial sums
@@ -1402,7 +1441,11 @@ __device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, int tile, int key
 // ---- backward: the gradients of keys and values -------------------------------------------------------------
 // dV_j = sum_i P_ij dO_i, dK_j = scale sum_i dS_ij q_i.  A workgroup has 128 keys of one (sample, key head), 32 in each wave,
 // whose keys and values stay in registers, and steps over 32 rows at a time of all the heads that share them: the sum over
-// the group is part of the same chain.  P and dS are rounded to the 16-bit type for the products.  One wave's accumulators
+// the group is part of the same chain.  P and dS are rounded to the 16-bit type for the products, in fp16 times a power
+// of two: the row's logarithm has it for P, and dS takes one that follows the largest of the wave's 32 keys, a scalar (a
+// power for each key is a register more, and spilled 56 at 128 dims; this spills 8).  4096 tokens, 32 heads, window 1024, forward and
+// backward in fp16, us, both gradients as they were and with the powers: 64 dims 276, 287, 128 dims 458, 480, 256 dims 1416, 1482.
+// P is packed before dP is summed, which frees its registers.  One wave's accumulators
 // are 2 x 64 registers at 128 dims, which with the operands leaves two workgroups on a CU.
 // Bound by the matrix cores and the waits of a CU's few waves.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 927
 // us, 891 TFLOP/s for its four products; 4096 tokens, 32 heads on 8, window 1024: 200 us and 19 of the join.
@@ -1526,6 +1569,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
 #pragma unroll
         for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
     const float scale_log2 = a.scale * kLog2e;
+    // fp16: P is 2^14 times itself (as its logarithms are less), and dS that times a power of two of the wave's own
+    constexpr bool kLifted = __is_same(T, F16);
+    Lift lift;
 
     if (row_begin < row_end) fetch(row_begin, 0);
     u32x4 kreg[DP / 16], vreg[DK ? DP / 16 : 1];
@@ -1588,19 +1634,36 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
 #pragma unroll
                 for (int st = 0; st < DP / 16; ++st) dp = Mma<T>::op(ops.rows(kStepRows, st), vreg[st], dp);
             }
+            u32x4 prob[DV ? 2 : 1];  // P, rounded
             if constexpr (DV) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    u32x4 p;
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(ops.columns(kStepRows + 16 * t, i), p, dv[i]);
-                }
+                    for (int e = 0; e < 4; ++e) prob[t][e] = Elem<T>::pack(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
             }
             if constexpr (DK) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= dp[r];
+                if constexpr (kLifted) {
+                    const float most = largest(s);
+                    if (__any(lift.short_of(most))) {
+                        const float f = lift.lower(wave_largest(most));
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) dk[i][r] *= f;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] *= lift.times;
+                }
+            }
+            if constexpr (DV) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) dv[i] = Mma<T>::op(ops.columns(kStepRows + 16 * t, i), prob[t], dv[i]);
+            }
+            if constexpr (DK) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     u32x4 p;
@@ -1614,10 +1677,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
         landed();
         __syncthreads();
     }
+    const float dk_times = kLifted ? lift.undone() * 0x1p-14f : 1.f, dv_times = kLifted ? 0x1p-14f : 1.f;
+    static_assert(!kLifted || gradient_bits<T>() == 14.f, "2^-14");
     if (a.near_parts + far_of_tile == 1) {
         const bool there = key < a.sk;
-        if constexpr (DK) store_rows<T, DP>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2]) * 2, dk, a.scale, a.d, there);
-        if constexpr (DV) store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, 1.f, a.d, there);
+        if constexpr (DK) store_rows<T, DP>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2]) * 2, dk, a.scale * dk_times, a.d, there);
+        if constexpr (DV) store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, dv_times, a.d, there);
         return;
     }
     float* const to = a.part_o + (grad_piece(a, bh, kt) + (far ? a.near_parts + part : part)) * 2 * kGradKeys * a.d + (key - key0) * a.d;
@@ -1628,8 +1693,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
             for (int r = 0; r < 16; r += 4) {
                 const int dim = 32 * i + element_of(r, half);
                 if (dim < a.d) {
-                    if constexpr (DK) *reinterpret_cast<f32x4*>(to + dim) = f32x4{dk[i][r], dk[i][r + 1], dk[i][r + 2], dk[i][r + 3]};
-                    if constexpr (DV) *reinterpret_cast<f32x4*>(to + kGradKeys * a.d + dim) = f32x4{dv[i][r], dv[i][r + 1], dv[i][r + 2], dv[i][r + 3]};
+                    if constexpr (DK) *reinterpret_cast<f32x4*>(to + dim) = f32x4{dk[i][r], dk[i][r + 1], dk[i][r + 2], dk[i][r + 3]} * dk_times;
+                    if constexpr (DV) *reinterpret_cast<f32x4*>(to + kGradKeys * a.d + dim) = f32x4{dv[i][r], dv[i][r + 1], dv[i][r + 2], dv[i][r + 3]} * dv_times;
                 }
             }
     }

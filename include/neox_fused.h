@@ -357,7 +357,7 @@ int neox_rope_apply_freqs(void* out_q, void* out_k, const void* q, const void* k
  * looked at.  (Queries and keys are worked on 32 by 32.  Where one of the queries sees one of the keys, another
  * of those keys or its value, if infinite or NaN, reaches queries that do not see it: its product with zero is
  * NaN.)  lse, fp32 [b * h * sq], and out_low, laid out
- * as out, are for the backward pass (NULL: not wanted): every row's logarithm, in an order of its own, and what
+ * as out, are for the backward pass (NULL: not wanted): every row's logarithm, in an order and a form of its own that go with the type, and what
  * rounding the output to 16 bits took away, without which (out_low NULL there) the backward pass takes the
  * rounded output for the sums of dout * out and its gradients lose some precision.  fp32 sums of the matrix cores' 16-bit products; the
  * probabilities are rounded to the 16-bit type before they meet the values.

@@ -180,3 +180,61 @@ def test_probabilities_far_below_a_sink_without_a_value(device, dtype, above, n,
     typically_within(got, want, variance)
     with torch.no_grad():
         typically_within(window_attention(q[:, None], k[:, None], v[:, None], scale=1.0)[:, 0], want, variance)
+
+
+# ---- gradients -----------------------------------------------------------------------------------------------------
+def gradients(q, k, v, g, sees, scale, dtype):
+    """One head ``[n, d]`` in 64 bits: the three gradients, and as in ``typical_error`` the variance that rounding P, dS and
+    the results to the type may leave in each."""
+    q, k, v, g = (t.double() for t in (q, k, v, g))
+    out, p = A.one_head(q, k, v, sees, scale)
+    ds = p * (g @ v.T - (g * out).sum(1, keepdim=True)) * scale
+    u, tiny = A.ROUND[dtype], A.TINY[dtype]
+    want = (ds @ k, ds.T @ q, p.T @ g)
+    terms = (ds.square() @ k.square(), ds.T.square() @ q.square(), p.T.square() @ g.square())
+    return want, [(u * u * (t + w.square()) + tiny * tiny) / 3 for t, w in zip(terms, want)]
+
+
+def check_gradients(q, k, v, g, heads, rows=None, sink=False, **kw):
+    """Heads ``heads`` of a call without shared keys; ``rows``: the tokens whose ``dq`` is looked at, each list by itself.  With
+    ``sink`` the first key's gradients, a few numbers far larger than the others, are held to four deviations each."""
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(window_attention(*leaves, scale=0.125, **kw), leaves, g)
+    sees = A.visible(q.shape[0], k.shape[0], kw.get("window"), kw.get("sinks", 0), device=q.device)
+    for x in heads:
+        want, variance = gradients(q[:, 0, x], k[:, 0, x], v[:, 0, x], g[:, 0, x], sees, 0.125, q.dtype)
+        for some in rows or [slice(None)]:
+            typically_within(got[0][some, 0, x], want[0][some], variance[0][some])
+        for i in (1, 2):
+            typically_within(got[i][sink:, 0, x], want[i][sink:], variance[i][sink:])
+            if sink:
+                within(got[i][0, 0, x], want[i][0], 4 * variance[i][0].sqrt())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("times", [300.0, 1.0, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("n,h,d,kw", [
+    (4096, 2, 64, {}), (4096, 32, 64, {}), (4096, 2, 128, {"window": 2000, "sinks": 4}), (2000, 2, 96, {}), (1500, 2, 256, {}), (300, 3, 64, {"window": 100})])
+def test_gradients_of_small_and_large_sizes(device, dtype, times, n, h, d, kw):
+    q, k, v = (normal((n, 1, h, d), dtype, device, 20 + i) for i in range(3))
+    g = normal((n, 1, h, d), dtype, device, 23, times)
+    check_gradients(q, k, v, g, (0, h - 1), **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_different_sizes_in_one_tile(device, dtype):
+    n = 2000
+    q, k, v = (normal((n, 1, 2, 64), dtype, device, 30 + i) for i in range(3))
+    small = torch.arange(n, device=device) % 3 == 0
+    g = (normal((n, 1, 2, 64), torch.float32, device, 33) * torch.where(small, 1e-3, 10.0)[:, None, None, None]).to(dtype)
+    check_gradients(q, k, v, g, (0, 1), rows=[small, ~small])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("above", [9, 12])
+def test_gradients_of_values_far_below_a_sink(device, dtype, above):
+    # probabilities of about 2^-13 and 2^-17 for all keys but the first
+    k, v = sink_and_rest(2500, 2, 64, dtype, device, 1.0, above, 40)
+    q = normal((2500, 1, 2, 64), dtype, device, 42)
+    q[..., -1] = 32
+    check_gradients(q, k[:, None], v[:, None], normal(q.shape, dtype, device, 43), (0, 1), sink=True)
