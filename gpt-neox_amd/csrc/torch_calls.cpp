@@ -352,6 +352,17 @@ std::tuple<Tensor, Tensor, Tensor> window_forward(const Tensor& q, const Tensor&
     return {out, low, lse};
 }
 
+// Hands on the gradients of a backward pass that is itself recorded (create_graph), as results of the tensors they were
+// computed from: the kernels have no second derivative, and asking for one has to fail and not to leave a term out.
+class OnlyOnce : public torch::autograd::Function<OnlyOnce> {
+public:
+    static variable_list forward(AutogradContext*, const Tensor& dq, const Tensor& dk, const Tensor& dv, const Tensor&, const Tensor&, const Tensor&,
+                                 const Tensor&) {
+        return {dq, dk, dv};
+    }
+    static variable_list backward(AutogradContext*, variable_list) { throw std::runtime_error("window_attention has no second derivative"); }
+};
+
 class WindowAttention : public torch::autograd::Function<WindowAttention> {
 public:
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const WindowCall& c) {
@@ -368,6 +379,7 @@ public:
         variable_list v = ctx->get_saved_variables();
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
         Tensor g = grads[0];
+        const Tensor sources[] = {v[0], v[1], v[2], g};
         const Tensor lengths = v[6];
         v.resize(6);
         for (const Tensor& t : v)
@@ -400,6 +412,10 @@ public:
             val.const_data_ptr(), lengths.defined() ? static_cast<const int32_t*>(lengths.const_data_ptr()) : nullptr, b, sq, sk, h, h_kv, d,
             RowStrides(dq, 3), RowStrides(dk, 3), RowStrides(dv, 3), RowStrides(g, 3), RowStrides(out, 3), RowStrides(q, 3),
             RowStrides(k, 3), RowStrides(val, 3), (float)ctx->saved_data["scale"].toDouble(), window, sinks, code(q), stream_of(q)));
+        if (records(sources[0]) || records(sources[1]) || records(sources[2]) || records(sources[3])) {
+            const variable_list once = OnlyOnce::apply(dq, dk, dv, sources[0], sources[1], sources[2], sources[3]);
+            return {once[0], once[1], once[2], Tensor()};
+        }
         return {dq, dk, dv, Tensor()};
     }
 };

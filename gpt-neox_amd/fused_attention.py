@@ -10,7 +10,6 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -45,6 +44,20 @@ def _forward(q, k, v, scale, window, sinks, key_lengths, for_backward):
     return out, low, lse
 
 
+class _OnlyOnce(torch.autograd.Function):
+    """Hands on the gradients ``dq, dk, dv`` of a backward pass that is itself recorded (``create_graph=True``), as
+    results of the tensors they were computed from: the kernels have no second derivative, and asking for one has to fail
+    and not to leave a term out."""
+
+    @staticmethod
+    def forward(ctx, dq, dk, dv, *sources):
+        return dq, dk, dv
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("window_attention has no second derivative")
+
+
 class WindowAttention(torch.autograd.Function):
     """``apply(q, k, v, scale, window, sinks, key_lengths)``; see :func:`window_attention`, which checks the arguments."""
 
@@ -56,14 +69,22 @@ class WindowAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
+        sources = (*ctx.saved_tensors[:3], grad)
+        with torch.no_grad():
+            grads = WindowAttention._gradients(ctx, grad)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in sources):
+            grads = _OnlyOnce.apply(*grads, *sources)
+        return (*grads, None, None, None, None)
+
+    @staticmethod
+    def _gradients(ctx, grad):
         q, k, v, out, low, lse, key_lengths = ctx.saved_tensors
         (sq, b, h, d), (sk, _, h_kv, _) = q.shape, k.shape
         dq = torch.empty((sq, b, h, d), dtype=q.dtype, device=q.device)
         dk, dv = (torch.empty((sk, b, h_kv, d), dtype=q.dtype, device=q.device) for _ in "kv")
         if out.numel() == 0 or sk == 0:
-            return dq.zero_(), dk.zero_(), dv.zero_(), None, None, None, None
+            return dq.zero_(), dk.zero_(), dv.zero_()
         if grad.shape != out.shape or grad.dtype != out.dtype or grad.device != out.device:
             raise RuntimeError("the gradient must have the shape, dtype and device of the attention's output")
         q, k, v, grad = (_lib.in_pieces(t) for t in (q, k, v, grad))
@@ -78,7 +99,7 @@ class WindowAttention(torch.autograd.Function):
                 low.data_ptr(), lse.data_ptr(),
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(key_lengths),
                 b, sq, sk, h, h_kv, d, *strides, *ctx.call, _lib.dtype_code(q.dtype), _lib.current_stream(q)))
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv
 
 
 def window_attention(q, k, v, *, window=None, sinks=0, scale=None, key_lengths=None):
@@ -92,7 +113,8 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, key_lengths=N
     fp16 or bf16; ``h`` a multiple of ``h_kv``; ``d`` a multiple of 8, at most 256.  Any strides: tensors whose rows
     are dense and start on 16-byte boundaries (views into a fused QKV projection among them) are read as they lie,
     others are copied first.  Sums and the softmax are in fp32.  Gradients flow to ``q``, ``k`` and ``v``; those of shared
-    key heads are summed in a fixed order, so the same inputs give the same bits.
+    key heads are summed in a fixed order, so the same inputs give the same bits.  There is no second derivative: going
+    back through gradients taken with ``create_graph=True`` raises.
     """
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:

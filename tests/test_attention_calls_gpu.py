@@ -1,0 +1,45 @@
+"""How the attention calls behave in a program: derivatives that they do not have, and what they take for granted."""
+import pytest
+import torch
+
+from gpt_neox_amd import _lib
+from gpt_neox_amd.fused_attention import window_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "ctypes"])
+def path(request, monkeypatch):
+    if request.param == "ctypes":
+        monkeypatch.setattr(_lib, "calls", lambda *tensors: None)
+    return request.param
+
+
+def normal(shape, device, seed, dtype=torch.bfloat16):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    return torch.randn(shape, generator=gen, device=device).to(dtype)
+
+
+@pytest.mark.parametrize("of", [0, 1, 2])
+def test_a_second_derivative_is_refused(device, path, of):
+    qkv = [normal((40, 1, 2, 64), device, i) for i in range(3)]
+    qkv[of].requires_grad_()
+    out = window_attention(*qkv, window=9)
+    (grad,) = torch.autograd.grad(out.float().square().sum(), qkv[of], create_graph=True)
+    want = torch.autograd.grad(window_attention(*qkv, window=9).float().square().sum(), qkv[of])[0]
+    assert torch.equal(grad, want) and grad.requires_grad
+    # a penalty on the gradient beside a loss: the loss alone has a gradient, the penalty's may not be left out
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        (out.float().sum() + grad.float().square().sum()).backward()
+
+
+def test_a_second_derivative_with_a_constant_gradient_is_refused(device, path):
+    q, k, v = (normal((40, 1, 2, 64), device, i).requires_grad_() for i in range(3))
+    out = window_attention(q, k, v, window=9)
+    grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out), create_graph=True)
+    for g in grads:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(g.float().square().sum(), (q, k, v), allow_unused=True, retain_graph=True)
+    # and where nothing goes back through them, gradients of a recorded backward pass are those of any other
+    again = torch.autograd.grad(window_attention(q, k, v, window=9), (q, k, v), torch.ones_like(out))
+    assert all(torch.equal(x, y) for x, y in zip(grads, again)) and not any(g.requires_grad for g in again)
