@@ -156,7 +156,7 @@ static void set_window_sizes(AttnArgs& a, int b, int sq, int sk, int h, int h_kv
 
 // how the key gradients' work is cut into pieces, and the scratch it needs: fp32 sums of pieces, then delta
 struct GradPlan {
-    int key_tiles, near_parts, piece_rows, sink_tiles, far_parts;
+    int key_tiles, near_parts, piece_rows, sink_tiles, far_parts, far_keys;
     int64_t parts_bytes, bytes;
 };
 
@@ -187,10 +187,9 @@ static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int win
         const int64_t far = (rows + 511) / 512, enough = (1024 + units * p.sink_tiles - 1) / (units * p.sink_tiles);
         p.far_parts = (int)(far < enough ? far : enough);
         if (p.far_parts > 64) p.far_parts = 64;
+        p.far_keys = last < kGradKeys ? (int)last : kGradKeys;
     }
-    const bool cut = p.near_parts > 1 || p.far_parts > 0;
-    const int64_t pieces = (int64_t)p.key_tiles * p.near_parts + (int64_t)p.sink_tiles * p.far_parts;
-    p.parts_bytes = cut ? units * pieces * 2 * kGradKeys * d * (int64_t)sizeof(float) : 0;
+    p.parts_bytes = units * grad_part_keys(p.key_tiles, p.near_parts, p.sink_tiles, p.far_parts, p.far_keys) * 2 * d * (int64_t)sizeof(float);
     p.bytes = p.parts_bytes + (int64_t)b * h * sq * (int64_t)sizeof(float);
     return p;
 }
@@ -407,6 +406,7 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int
     a.piece_rows = plan.piece_rows;
     a.sink_tiles = plan.sink_tiles;
     a.far_parts = plan.far_parts;
+    a.far_keys = plan.far_keys;
     a.units = plan.key_tiles * plan.near_parts + plan.sink_tiles * plan.far_parts;
     a.by_units = FastDiv::by((uint32_t)a.units);
     a.by_near_parts = FastDiv::by((uint32_t)a.near_parts);

@@ -79,8 +79,10 @@ struct AttnArgs {
     int key_tiles;
     // The key-gradient kernel's work: every key tile's near rows (those whose window reaches it) in up to near_parts
     // pieces of piece_rows; for the first sink_tiles tiles, the rows behind in far_parts pieces.  A tile in more than one piece
-    // leaves fp32 sums in part_o, [b, kv][piece][dk, dv][kGradKeys][d], far pieces for the keys below `sinks` only.
+    // leaves fp32 sums in part_o, [b, kv][such a tile][piece][dk, dv][key][d]; near pieces have kGradKeys keys, far pieces
+    // far_keys, which those below `sinks` are among.
     int near_parts, far_parts, sink_tiles, units;
+    int far_keys;
     int piece_rows;              // of a piece of near rows
     FastDiv by_units, by_near_parts, by_far_parts;
 };
@@ -1416,10 +1418,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(Attn
     store_rows<T, DP>(p, acc, kLifted ? a.scale * lift.undone() : a.scale, a.d, there);
 }
 
-// the first piece of a key tile in the partial sums
-__device__ __forceinline__ int64_t grad_piece(const AttnArgs& a, uint32_t bh, int tile) {
-    const int64_t each = (int64_t)a.key_tiles * a.near_parts + a.sink_tiles * a.far_parts;
-    return bh * each + (int64_t)tile * a.near_parts + min(tile, a.sink_tiles) * a.far_parts;
+// The partial sums of a key head, in keys: those of the tiles that are done in more than one piece.  Where near rows are in
+// one piece, these are the first sink_tiles, and none without far pieces.
+__host__ __device__ __forceinline__ int64_t grad_part_keys(int key_tiles, int near_parts, int sink_tiles, int far_parts, int far_keys) {
+    return (int64_t)(near_parts > 1 ? key_tiles : sink_tiles) * near_parts * kGradKeys + (int64_t)sink_tiles * far_parts * far_keys;
+}
+// the first key of a tile's partial sums: near_parts pieces of kGradKeys, and for a tile with sinks far_parts of far_keys
+__device__ __forceinline__ int64_t grad_part(const AttnArgs& a, uint32_t bh, int tile) {
+    return bh * grad_part_keys(a.key_tiles, a.near_parts, a.sink_tiles, a.far_parts, a.far_keys) + (int64_t)tile * a.near_parts * kGradKeys +
+           (int64_t)min(tile, a.sink_tiles) * a.far_parts * a.far_keys;
 }
 
 // The rows that see some key of a tile: those from its first position to the end of its last one's window, and where
@@ -1685,8 +1692,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
         if constexpr (DV) store_rows<T, DP>(a.dv + ((int64_t)key * a.dv_st[0] + (int64_t)b * a.dv_st[1] + (int64_t)g * a.dv_st[2]) * 2, dv, dv_times, a.d, there);
         return;
     }
-    float* const to = a.part_o + (grad_piece(a, bh, kt) + (far ? a.near_parts + part : part)) * 2 * kGradKeys * a.d + (key - key0) * a.d;
-    if (!far || key < a.sinks) {
+    const int piece_keys = far ? a.far_keys : kGradKeys;
+    float* const to = a.part_o + (grad_part(a, bh, kt) + (far ? a.near_parts * kGradKeys : 0) + part * piece_keys) * 2 * a.d + (key - key0) * a.d;
+    if (!far || (key < a.sinks && key - key0 < a.far_keys)) {
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -1694,7 +1702,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bw
                 const int dim = 32 * i + element_of(r, half);
                 if (dim < a.d) {
                     if constexpr (DK) *reinterpret_cast<f32x4*>(to + dim) = f32x4{dk[i][r], dk[i][r + 1], dk[i][r + 2], dk[i][r + 3]} * dk_times;
-                    if constexpr (DV) *reinterpret_cast<f32x4*>(to + kGradKeys * a.d + dim) = f32x4{dv[i][r], dv[i][r + 1], dv[i][r + 2], dv[i][r + 3]} * dv_times;
+                    if constexpr (DV) *reinterpret_cast<f32x4*>(to + piece_keys * a.d + dim) = f32x4{dv[i][r], dv[i][r + 1], dv[i][r + 2], dv[i][r + 3]} * dv_times;
                 }
             }
     }
@@ -1712,17 +1720,16 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnArgs a) {
     for (int at = threadIdx.x; at < 32 * quads; at += 256) {
         const int row = slice * 32 + at / quads, dim = at % quads * 4, key = tile * kGradKeys + row;
         if (key >= a.sk) return;
-        const float* from = a.part_o + grad_piece(a, bh, tile) * 2 * kGradKeys * a.d + row * a.d + dim;
+        const float* from = a.part_o + grad_part(a, bh, tile) * 2 * a.d + row * a.d + dim;
         f32x4 dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
-        auto add = [&](int first, int count) {
-            for (int p = first; p < first + count; ++p) {
-                const float* x = from + (int64_t)p * 2 * kGradKeys * a.d;
+        auto add = [&](const float* x, int count, int piece_keys) {
+            for (int p = 0; p < count; ++p, x += (int64_t)2 * piece_keys * a.d) {
                 dk += *reinterpret_cast<const f32x4*>(x);
-                dv += *reinterpret_cast<const f32x4*>(x + kGradKeys * a.d);
+                dv += *reinterpret_cast<const f32x4*>(x + piece_keys * a.d);
             }
         };
-        add(0, near);
-        if (key < a.sinks && tile < a.sink_tiles) add(a.near_parts, a.far_parts);
+        add(from, near, kGradKeys);
+        if (tile < a.sink_tiles && key < a.sinks && row < a.far_keys) add(from + (int64_t)a.near_parts * 2 * kGradKeys * a.d, a.far_parts, a.far_keys);
         dk *= a.scale;
         *reinterpret_cast<u32x2*>(a.dk + ((int64_t)key * a.dk_st[0] + (int64_t)b * a.dk_st[1] + (int64_t)g * a.dk_st[2] + dim) * 2) =
             u32x2{Elem<T>::pack(dk[0], dk[1]), Elem<T>::pack(dk[2], dk[3])};
