@@ -24,8 +24,15 @@ class PagedKVCache:
     ``[pages, page_size, heads]`` in fp32.  Slot ``page * page_size + i`` is token ``i`` of a page.
 
     The tensors may be views (of one buffer for all layers, say) as long as every head's values are dense and start on
-    16-byte boundaries.
+    16-byte boundaries.  They are looked at once, here, and stay: other tensors are another cache.
     """
+
+    _FIXED = frozenset(("k", "v", "k_scale", "v_scale", "pages", "page_size", "heads", "dim", "dtype", "device", "quantised", "_strides"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and name in self.__dict__:
+            raise AttributeError(f"{name} of a cache cannot be replaced: make a PagedKVCache of the new tensors")
+        super().__setattr__(name, value)
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
