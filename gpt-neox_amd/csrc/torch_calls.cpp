@@ -490,10 +490,10 @@ std::optional<std::tuple<Tensor, Tensor>> cache_read(const Tensor& kc, const Ten
     return std::make_tuple(k, v);
 }
 
-// q [tokens, h, d] over the pages of a cache -> [tokens, h, d], or None; max_context < 0: what the table has room for
+// q [tokens, h, d] over the pages of a cache -> [tokens, h, d], or None; max_context None: what the table has room for
 std::optional<Tensor> paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const std::optional<Tensor>& ks,
                                       const std::optional<Tensor>& vs, const Tensor& table, const Tensor& starts, const Tensor& lengths,
-                                      int64_t max_query, int64_t max_context, double scale, int64_t window, int64_t sinks) {
+                                      int64_t max_query, std::optional<int64_t> longest, double scale, int64_t window, int64_t sinks) {
     const Cache cache{kc, vc, ks, vs};
     if (!on_gpu(q) || q.dim() != 3 || q.numel() == 0 || !cache.goes_with(q) || q.size(1) % kc.size(2) != 0 || !fits_int32(q.size(0)) ||
         !in_pieces(q) || lengths.dim() != 1 || !int_list(lengths, q, lengths.size(0)) || !int_list(starts, q, lengths.size(0) + 1) ||
@@ -501,7 +501,7 @@ std::optional<Tensor> paged_attention(const Tensor& q, const Tensor& kc, const T
         table.size(0) != lengths.size(0) || table.size(0) < 1 || table.size(1) < 1 || table.stride(1) != 1 || table.stride(0) < 0 ||
         !fits_int32(table.size(1)) || !fits_int32(max_query) || window > INT32_MAX || window < -1 || !fits_int32(sinks))
         return std::nullopt;
-    if (max_context < 0) max_context = table.size(1) * kc.size(1);
+    const int64_t max_context = longest.value_or(table.size(1) * kc.size(1));
     if (!fits_int32(max_context)) return std::nullopt;
     const c10::DeviceGuard guard(q.device());
     const auto tokens = (int32_t)q.size(0), h = (int32_t)q.size(1), d = (int32_t)q.size(2), b = (int32_t)lengths.size(0), h_kv = (int32_t)kc.size(2);

@@ -9,6 +9,7 @@ here looks at the page table, the lengths or the slots on the host, so a step ca
 """
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -164,7 +165,7 @@ def paged_attention(q, cache, page_table, query_starts, context_lengths, *, max_
     calls = _lib.calls(q, page_table, query_starts, context_lengths)
     if calls is not None:
         out = calls.paged_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, query_starts, context_lengths, max_query,
-                                    -1 if max_context is None else max_context, 1.0 / math.sqrt(cache.dim) if scale is None else scale,
+                                    max_context, 1.0 / math.sqrt(cache.dim) if scale is None else scale,
                                     window, sinks)
         if out is not None:
             return out
@@ -188,6 +189,9 @@ def paged_attention(q, cache, page_table, query_starts, context_lengths, *, max_
             raise RuntimeError("all tensors must be on the same device")
     if max_context is None:
         max_context = page_table.shape[1] * cache.page_size
+    for name, n in (("max_query", max_query), ("max_context", max_context)):
+        if not 1 <= operator.index(n) < 2**30:  # (a C integer would take what is left of a larger one in 32 bits)
+            raise RuntimeError(f"{name}={n} must be at least 1 and below 2^30")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out = torch.empty((tokens, h, d), dtype=q.dtype, device=q.device)
     if tokens == 0:

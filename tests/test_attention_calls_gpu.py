@@ -4,6 +4,7 @@ import torch
 
 from gpt_neox_amd import _lib
 from gpt_neox_amd.fused_attention import window_attention
+from gpt_neox_amd.paged_cache import PagedKVCache, paged_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +44,14 @@ def test_a_second_derivative_with_a_constant_gradient_is_refused(device, path):
     # and where nothing goes back through them, gradients of a recorded backward pass are those of any other
     again = torch.autograd.grad(window_attention(q, k, v, window=9), (q, k, v), torch.ones_like(out))
     assert all(torch.equal(x, y) for x, y in zip(grads, again)) and not any(g.requires_grad for g in again)
+
+
+@pytest.mark.parametrize("bounds", [{"max_query": 2**32 + 1}, {"max_query": -1}, {"max_query": 1, "max_context": -5}, {"max_query": 1, "max_context": 2**32 + 7},
+                                    {"max_query": 1, "max_context": 0}, {"max_query": 2**62}, {"max_query": 1, "max_context": 2**30}])
+def test_bounds_that_no_length_can_have_are_refused(device, path, bounds):
+    # (in 32 bits 2^32 + 1 would be 1: all tokens behind the first would have been left out)
+    cache = PagedKVCache.allocate(4, 16, 2, 64, torch.int8, device)
+    table = torch.arange(4, device=device).view(1, 4).int()
+    starts, lengths = (torch.tensor(x, dtype=torch.int32, device=device) for x in ([0, 3], [40]))
+    with pytest.raises(RuntimeError, match="max_query|max_context"):
+        paged_attention(normal((3, 4, 64), device, 5), cache, table, starts, lengths, **bounds)
