@@ -164,8 +164,10 @@ struct GradPlan {
 // causal mask, whose first tiles have twice the rows of the average, so that no piece is longer than a CU's share; 256
 // rows or more for each.  Rows behind the window of a tile that holds sinks come in pieces of 512 rows, or longer
 // ones where those would be more than two for every workgroup that fits (many sinks are many such tiles, and every piece is
-// scratch).  Where they are no more than 128, and would be the only reason to join pieces, the tile takes them along (256
-// tokens, 8 heads of 64 dims, window 100: a call forward and backward 73 us with them apart, 68 without the second launch).
+// scratch).  Where they are no more than 128, and would be the only reason to join pieces, the tile takes them along: apart and
+// with their tile, bf16, forward and backward, us: 28 rows (256 tokens, window 100), 8 heads of 64 dims 75, 72, 2 samples of 128
+// dims 74, 70; 64 rows 75, 71; 128 rows 74, 71; 256 rows (512 tokens, 8 heads of 128 dims) 73, 71, but 640 tokens, 32 heads 77, 82;
+// 512 rows (768 tokens, 32 heads of 64 dims) 74, 70.
 static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int window, int sinks) {
     GradPlan p{};
     const int64_t group = h / h_kv, units = (int64_t)b * h_kv;
@@ -201,12 +203,18 @@ struct PagedPlan {
     int64_t bytes;
 };
 
+// Single tokens are calls of at most 16 rows to a key head, which is what that kernel's instructions hold; what has more goes to
+// row tiles of 128, mostly empty at first.  128 dims, us, 8 rows (one token of 32 heads on 4), 16, 24 and 40: 16 sequences of
+// 8192 keys in int8 41, 44, 52, 59, in bf16 55, 62, 50, 56; one of 65536 in int8 24, 25, 32, 37, in bf16 33, 34, 35, 37; a single key
+// head, 16 and 17 rows, one of 65536: int8 18 and 29, bf16 20 and 30.
 // Parts: so many that every CU has workgroups enough, with at least 256 keys for each part and 128 parts at most.  Row
-// tiles: as many as fit a CU, three that read 16 bits (2 x 512 tokens over 4096, 32 heads on 8: 111 us with two, 95 with three;
-// 2 x 1000 over 3000, 32 heads: 118, 91; but 4 x 512 with a window of 4096: 205, 222) and two that widen codes (1 x 512 over 8192: 121
-// with two, 137 with three).  Single tokens: eight, twice what fits, because sequences differ in length and the host does not
-// know by how much: 64 sequences of 2048 to 8192 tokens, int8, take 191 us with four (170 before four fitted), 158 with
-// eight, 169 with sixteen; one of 131001 tokens in bf16 takes 125 us with 128 parts and 128 with 256.
+// tiles: two that widen codes fit a CU, three that read 16 bits.  Measured in bf16 pages with two and with three, us: 1 x 512 tokens
+// over 8192, 32 heads on 8: 113, 102; 2 x 512 over 4096: 111, 100; 1 x 2048 over 8192, 12 heads of 64 dims: 131, 105; 4 x 64 over
+// 8192: 65, 63; but 2 x 1000 over 3000, 32 heads on 32: 137, 162; 4 x 512 with a window of 4096: 186, 214; 1 x 256 over 32768, 16
+// heads of 256 dims: 372, 391: a second part costs calls whose tiles nearly fill the card.  In int8 with two and with three: 115, 130; 117,
+// 132; 161, 127; 68, 78; 147, 173; 205, 232; 328, 355.  Single tokens: eight, twice what fits, because sequences differ in length and
+// the host does not know by how much: 64 sequences of 2048 to 8192 tokens, int8, take 191 us with four (170 before four fitted),
+// 158 with eight, 169 with sixteen; one of 131001 tokens in bf16 takes 125 us with 128 parts and 128 with 256.
 static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, int h, int h_kv, int d, int window, int sinks, bool codes) {
     PagedPlan p{};
     const int64_t group = h / h_kv, rows = max_query * group;

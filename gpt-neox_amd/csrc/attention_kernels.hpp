@@ -465,12 +465,13 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 // (sample, key head), 32 in each wave, and steps over the tiles of keys that any of them sees, copied into one half of LDS
 // while the other is worked on.  The probabilities are rounded to the 16-bit type, as the second product takes them; what
 // that costs is half an ulp of each, as where they are stored.
-// Bound by the matrix cores and, about half as long, by the exponentials and the mask around them, which overlap with
-// them only where two waves of a SIMD are at different places.  Measured, us and what its two products reach: 8192 tokens,
-// 32 heads of 128 dims, window 4096 (bf16) 506, 815 TFLOP/s; 2 x 2048 tokens, 64 heads of 96 dims, window 512 (fp16) 98,
-// 463 TFLOP/s, of which a quarter of the columns are padding and the edges of the window are computed and masked.
-// Chunks of 512 tokens of four sequences over 16384 keys, window 4096, 32 heads on 8, fp8: 197, 521 TFLOP/s, the widening
-// of codes being work of its own.
+// Bound by the matrix cores and by the exponentials and the mask around them, about half as long: a wave does one after
+// the other, and two waves of a SIMD that are at different places overlap little.  Measured (medians of 100 launches in a row), us and
+// what its two products reach: 8192 tokens, 32 heads of 128 dims, window 4096 (bf16) 470, 877 TFLOP/s; 2 x 2048 tokens, 64 heads of 96
+// dims, window 512 (fp16) 99, 457 TFLOP/s, of which a quarter of the columns are padding and the edges of the window are
+// computed and masked.  Chunks of 512 tokens of four sequences over 16384 keys, window 4096, 32 heads on 8, fp8: 200, 513
+// TFLOP/s, the widening of codes being work of its own.
+// Over codes at 256 dims the fp16 kernels spill 6 to 11 registers.
 template <typename T, int DP, int SRC, bool SPLIT>
 __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged16 ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
     constexpr bool kPages = SRC != kStrided;
@@ -837,8 +838,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 // 16-byte pieces that go into its first operands as they are (16-bit: 8 dims from 32 s + 8 (l / 16); codes: 16 dims from
 // 64 s + 16 (l / 16)); the same pieces of the values go through LDS of the wave's own for the transposing reads.
 // Measured, 32 heads on 8 of 128 dims: one token of each of 64 sequences of 2048 to 8192 keys, int8, 158 us, 4.4 TB/s, in
-// 4096 workgroups of unequal length; one token over 131001 keys in bf16, 114 us, 4.7 TB/s (a copy of large tensors reaches
-// 4.9, and a kernel that does nothing but read such rows 5.3 to 5.7).
+// 4096 workgroups of unequal length; one token over 131001 keys in bf16, 112 us, 4.8 TB/s (a copy of large tensors reaches
+// 4.9, and a kernel that does nothing but read such rows 5.3 to 5.7).  At 256 dims over 16-bit pages two blocks of keys and
+// values do not fit beside the sums: 35 registers are spilled inside the loop (one sequence of 65536 keys on 8 key heads 144 us, 3.7 TB/s).
 template <typename T, int DP, int SRC, bool SPLIT>
 __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(AttnArgs a) {
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
@@ -1193,7 +1195,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     *reinterpret_cast<u32x2*>(a.o + (token * a.o_st[0] + head * a.o_st[2] + dim) * 2) = w;
 }
 
-// The same with a wave for each row, for many rows in at most 64 parts: 32 lanes for the dims up to 128 (then the halves take every other
+// The same with a wave for each row, whose lanes hold a part's logarithm each (launched for at most 16 parts): 32 lanes for the dims up to 128 (then the halves take every other
 // part), 64 above.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
@@ -1229,9 +1231,9 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnArgs a) {
 // dS is rounded to the 16-bit type for the last product; in fp16, times a power of two that follows the largest of its row
 // (Lift), since it is as small as the incoming gradient over the number of keys.  That the scores are computed here and again there (7 products for
 // 5) buys gradients that are summed in registers, in a fixed order, without atomics.
-// Bound by the matrix cores as the forward kernel is.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 735 us, 842
-// TFLOP/s for its three products; 8 x 1001 tokens, 16 heads of 64 dims,
-// window 256 (fp16): 50 us.
+// Bound by the matrix cores as the forward kernel is.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 688 us, 900
+// TFLOP/s for its three products; 8 x 1001 tokens, 16 heads of 64 dims, window 256 (fp16): 50 us.  At 256 dims the fp16 kernel spills 19
+// registers.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
     constexpr int kTile = kTileKeys * Tile<DP>::kRow;
@@ -1450,14 +1452,14 @@ __device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, int tile, int key
 // whose keys and values stay in registers, and steps over 32 rows at a time of all the heads that share them: the sum over
 // the group is part of the same chain.  P and dS are rounded to the 16-bit type for the products, in fp16 times a power
 // of two: the row's logarithm has it for P, and dS takes one that follows the largest of the wave's 32 keys, a scalar (a
-// power for each key is a register more, and spilled 56 at 128 dims; this spills 8).  4096 tokens, 32 heads, window 1024, forward and
+// power for each key is a register more, and spilled 56 at 128 dims).  4096 tokens, 32 heads, window 1024, forward and
 // backward in fp16, us, both gradients as they were and with the powers: 64 dims 276, 287, 128 dims 458, 480, 256 dims 1416, 1482.
 // P is packed before dP is summed, which frees its registers.  One wave's accumulators
 // are 2 x 64 registers at 128 dims, which with the operands leaves two workgroups on a CU.
-// Bound by the matrix cores and the waits of a CU's few waves.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 927
-// us, 891 TFLOP/s for its four products; 4096 tokens, 32 heads on 8, window 1024: 200 us and 19 of the join.
+// Bound by the matrix cores and the waits of a CU's few waves.  Measured: 8192 tokens, 32 heads of 128 dims, window 4096: 852
+// us, 969 TFLOP/s for its four products; 4096 tokens, 32 heads on 8, window 1024: 164 us and 18 of the join.
 // Head dims over 128 take two launches, one for each gradient (DK, DV): together their accumulators, keys and values
-// are 384 registers of a lane, and the compiler spilled 330.
+// are 384 registers of a lane, and the compiler spilled 330.  Of the two, the keys' spills 8 in bf16.
 template <typename T, int DP, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
     constexpr int kTile = kStepRows * Tile<DP>::kRow;

@@ -6,7 +6,7 @@
 // q + fma(-q, b, a) * y of q = a * y gives the rounded a / b, so that exact ties between two codes are seen as ties.
 // Bound by memory: a lane moves 8 or 16 elements in 16-byte accesses, a row takes neighbouring lanes, and the keys' and
 // values' rows of a (token, head) go together, so that every lane has two to four loads in flight.  Measured: 65536 tokens of
-// 32 heads of 128 dims from bf16 into int8 307 us and back 300, 5.3 and 5.5 TB/s (a copy of large tensors: 4.9); 2047
+// 32 heads of 128 dims from bf16 into int8 300 us and back 293, 5.4 and 5.6 TB/s (a copy of large tensors: 4.9); 2047
 // tokens of 64 heads of 96 dims from fp16 into fp8 16 and back 13.
 #pragma once
 
