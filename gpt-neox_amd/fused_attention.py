@@ -44,6 +44,20 @@ def _forward(q, k, v, scale, window, sinks, key_lengths, for_backward):
     return out, low, lse
 
 
+def _check_saved(q, k, v, out, low, lse, key_lengths):
+    """A saved-tensor hook may have given back other tensors than were left with it: the kernels take for granted what was
+    looked at in the forward pass."""
+    _lib.require_gpu(q, k, v, out, low, lse, key_lengths)
+    if any(t is not None and t.device != q.device for t in (k, v, out, low, lse, key_lengths)):
+        raise RuntimeError("the saved tensors must be on one device")
+    if (q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[1] != q.shape[1] or k.shape[3] != q.shape[3]
+            or any(t.shape != q.shape for t in (out, low)) or any(t.dtype != q.dtype for t in (k, v, out, low))
+            or q.dtype not in _HALF or lse.dtype != torch.float32 or lse.numel() != out.numel() // max(1, q.shape[3])):
+        raise RuntimeError("the saved tensors must have the shapes and dtypes of the forward pass")
+    if key_lengths is not None and (key_lengths.dtype != torch.int32 or key_lengths.shape != q.shape[1:2] or not key_lengths.is_contiguous()):
+        raise RuntimeError("the saved key lengths have changed")
+
+
 class _OnlyOnce(torch.autograd.Function):
     """Hands on the gradients ``dq, dk, dv`` of a backward pass that is itself recorded (``create_graph=True``), as
     results of the tensors they were computed from: the kernels have no second derivative, and asking for one has to fail
@@ -80,6 +94,7 @@ class WindowAttention(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, grad):
         q, k, v, out, low, lse, key_lengths = ctx.saved_tensors
+        _check_saved(q, k, v, out, low, lse, key_lengths)
         (sq, b, h, d), (sk, _, h_kv, _) = q.shape, k.shape
         dq = torch.empty((sq, b, h, d), dtype=q.dtype, device=q.device)
         dk, dv = (torch.empty((sk, b, h_kv, d), dtype=q.dtype, device=q.device) for _ in "kv")
@@ -88,7 +103,7 @@ class WindowAttention(torch.autograd.Function):
         if grad.shape != out.shape or grad.dtype != out.dtype or grad.device != out.device:
             raise RuntimeError("the gradient must have the shape, dtype and device of the attention's output")
         q, k, v, grad = (_lib.in_pieces(t) for t in (q, k, v, grad))
-        out, low = out.contiguous(), low.contiguous()  # (a saved-tensor hook may have changed their layout)
+        out, low, lse = out.contiguous(), low.contiguous(), lse.contiguous()  # (a saved-tensor hook may have changed their layout)
         need = ctypes.c_int64()
         _lib.check(_lib.lib().neox_window_attention_bwd_workspace(need, b, sq, sk, h, h_kv, d, *ctx.call[1:]))
         workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)

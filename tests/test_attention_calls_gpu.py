@@ -55,3 +55,31 @@ def test_bounds_that_no_length_can_have_are_refused(device, path, bounds):
     starts, lengths = (torch.tensor(x, dtype=torch.int32, device=device) for x in ([0, 3], [40]))
     with pytest.raises(RuntimeError, match="max_query|max_context"):
         paged_attention(normal((3, 4, 64), device, 5), cache, table, starts, lengths, **bounds)
+
+
+@pytest.mark.parametrize("change", [
+    lambda t: t[:-1] if t.dim() == 4 else t, lambda t: t.float() if t.dtype == torch.bfloat16 else t, lambda t: t[:-1] if t.dtype == torch.float32 else t,
+    lambda t: t[..., :32] if t.dim() == 4 and t.shape[2] == 1 else t, lambda t: t[:1] if t.dtype == torch.int32 else t,
+    lambda t: t.long() if t.dtype == torch.int32 else t, lambda t: t.cpu() if t.dtype == torch.float32 else t])
+def test_saved_tensors_that_hooks_have_changed_are_refused(device, path, change):
+    q = normal((40, 2, 2, 64), device, 0).requires_grad_()
+    k, v = (normal((40, 2, 1, 64), device, i) for i in (1, 2))
+    lengths = torch.tensor([40, 30], dtype=torch.int32, device=device)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        out = window_attention(q, k, v, window=9, key_lengths=lengths)
+    with pytest.raises(RuntimeError, match="shapes and dtypes|lengths have changed|device|GPU"):
+        out.backward(torch.ones_like(out))
+
+
+def test_saved_tensors_of_another_layout_are_those_of_before(device, path):
+    q, k, v = (normal((40, 2, 2, 64), device, i).requires_grad_() for i in range(3))
+    want = torch.autograd.grad(window_attention(q, k, v, window=9), (q, k, v), torch.ones_like(q))
+
+    def spread(t):
+        wide = t.new_empty((*t.shape[:-1], 2 * t.shape[-1]))
+        wide[..., ::2] = t
+        return wide[..., ::2]
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        out = window_attention(q, k, v, window=9)
+    assert all(torch.equal(x, y) for x, y in zip(want, torch.autograd.grad(out, (q, k, v), torch.ones_like(q))))
