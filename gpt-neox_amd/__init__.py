@@ -4,8 +4,9 @@
 modules of the same names under ``megatron/model``; ``fused_rope`` mirrors
 ``megatron/model/fused_rope.py``; ``fused_kernels`` mirrors the loader and the three
 extension-module APIs of ``megatron/fused_kernels``.  ``fused_attention`` (attention over a
-window of keys and sinks, without stored scores) and ``paged_cache`` (a key/value cache in 8
-or 16 bits, and attention over it) go beyond them.  All of them call ONE C-ABI
+window of keys and sinks, without stored scores) and ``paged_cache`` (a key/value cache in 4,
+8 or 16 bits, and attention over it) and ``page_pool`` (the pages of such caches, given and taken back on the
+GPU) go beyond them.  All of them call ONE C-ABI
 library, ``csrc/libneox_fused.so`` (declared in ``include/neox_fused.h``), through
 ``_lib``; there is no CPU or eager fallback for the fused calls.
 
@@ -20,6 +21,7 @@ from .fused_softmax import (  # noqa: F401
     ScaledUpperTriangMaskedSoftmax,
     SoftmaxFusionTypes,
 )
+from .page_pool import PagePool, PoolStep  # noqa: F401
 from .paged_cache import PagedKVCache, paged_attention, slots_of  # noqa: F401
 from .positional_embeddings import (  # noqa: F401
     AliBi,
@@ -45,7 +47,9 @@ __all__ = [
     "apply_rotary_pos_emb_qkv_",
     "apply_rotary_pos_emb_torch",
     "rotate_half",
+    "PagePool",
     "PagedKVCache",
+    "PoolStep",
     "WindowAttention",
     "paged_attention",
     "slots_of",

@@ -20,9 +20,9 @@ from torch.autograd import forward_ad
 _CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libneox_fused.so")
 CALLS_PATH = os.path.join(_CSRC, "neox_torch.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
-NEOX_F16, NEOX_BF16, NEOX_F32, NEOX_I8, NEOX_F8 = 0, 1, 2, 3, 4
+NEOX_F16, NEOX_BF16, NEOX_F32, NEOX_I8, NEOX_F8, NEOX_F4 = 0, 1, 2, 3, 4, 5
 _DTYPE_CODE = {torch.float16: NEOX_F16, torch.bfloat16: NEOX_BF16, torch.float32: NEOX_F32}
 
 _c_i64p = ctypes.POINTER(ctypes.c_int64)
@@ -112,6 +112,8 @@ SIGNATURES = {
     "neox_cache_read": (
         ctypes.c_int, [_vp] * 7 + [_i32, _i64, _i32, _i32, _i64, _i32] + [_c_i64p] * 6 + [_i32, _i32, _vp]
     ),
+    "neox_pages_extend": (ctypes.c_int, [_vp] * 10 + [_i32, _i32, _i64, _i32, _i32, _i32, _vp]),
+    "neox_pages_truncate": (ctypes.c_int, [_vp] * 5 + [_i32, _i32, _i64, _i32, _i32, _vp]),
 }
 
 _lock = threading.Lock()

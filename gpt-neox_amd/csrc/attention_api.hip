@@ -39,7 +39,23 @@ static void cache_source(const CacheArgs& a, int source, hipStream_t stream) {
     else if (source == kPagedF8) cache_rows<T, kPagedF8, WRITE>(a, stream);
     else cache_rows<T, kPaged16, WRITE>(a, stream);
 }
+template <typename T, bool WRITE>
+static void cache4_rows(const CacheArgs& a, hipStream_t stream) {
+    const int lanes = a.d <= 32 ? 2 : a.d <= 64 ? 4 : a.d <= 128 ? 8 : 16;
+    const uint32_t blocks = (uint32_t)((a.rows * lanes + 255) / 256);
+    switch (lanes) {
+        case 2: cache4_kernel<T, 2, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        case 4: cache4_kernel<T, 4, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        case 8: cache4_kernel<T, 8, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        default: cache4_kernel<T, 16, WRITE><<<blocks, 256, 0, stream>>>(a);
+    }
+}
 hipError_t launch_cache(const CacheArgs& a, int source, int dtype, bool write, hipStream_t stream) {
+    if (source == kPagedF4) {
+        if (dtype == NEOX_BF16) write ? cache4_rows<BF16, true>(a, stream) : cache4_rows<BF16, false>(a, stream);
+        else write ? cache4_rows<F16, true>(a, stream) : cache4_rows<F16, false>(a, stream);
+        return hipGetLastError();
+    }
     if (dtype == NEOX_BF16) write ? cache_source<BF16, true>(a, source, stream) : cache_source<BF16, false>(a, source, stream);
     else write ? cache_source<F16, true>(a, source, stream) : cache_source<F16, false>(a, source, stream);
     return hipGetLastError();
@@ -251,30 +267,33 @@ static int cache_source_of(int cache_dtype, int dtype) {
     if (cache_dtype == dtype) return kPaged16;
     if (cache_dtype == NEOX_I8) return kPagedI8;
     if (cache_dtype == NEOX_F8) return kPagedF8;
+    if (cache_dtype == NEOX_F4) return kPagedF4;
     return -1;
 }
 
 // The cache's own part of a call: pointers, strides {page, token in the page, head}, sizes.
-static int check_cache(const void* kc, const void* vc, const float* ks, const float* vs, const int64_t* kc_st, const int64_t* vc_st,
+static int check_cache(const void* kc, const void* vc, const void* ks, const void* vs, const int64_t* kc_st, const int64_t* vc_st,
                        const int64_t* ks_st, const int64_t* vs_st, int64_t pages, int page_size, int h_kv, int d, int dtype,
                        int cache_dtype, const char* what) {
     const int source = cache_source_of(cache_dtype, dtype);
     if (source < 0)
-        return fail(NEOX_ERR_BAD_DTYPE, "%s: the cache must hold int8, fp8 (e4m3) or the dtype of the call (code %d)", what, cache_dtype);
-    const bool codes = source != kPaged16;
+        return fail(NEOX_ERR_BAD_DTYPE, "%s: the cache must hold int8, fp8 (e4m3), fp4 (e2m1) or the dtype of the call (code %d)", what, cache_dtype);
+    const bool codes = source != kPaged16, nibbles = source == kPagedF4;
     NEOX_TRY(check_pointer(kc, 16, what, "k_cache"));
     NEOX_TRY(check_pointer(vc, 16, what, "v_cache"));
     if (pages < 1 || pages >= kMost || page_size < 1 || page_size >= kMost)
         return fail(NEOX_ERR_BAD_SHAPE, "%s: pages=%lld page_size=%d must be at least 1 and below 2^30", what, (long long)pages, page_size);
+    if (nibbles && d % 32 != 0) return fail(NEOX_ERR_BAD_SHAPE, "%s: head dim %d of a 4-bit cache must be a multiple of 32", what, d);
     if (codes && d % 16 != 0) return fail(NEOX_ERR_BAD_SHAPE, "%s: head dim %d of an 8-bit cache must be a multiple of 16", what, d);
     const int unit = codes ? 16 : 8;
-    NEOX_TRY(check_strides(kc_st, 3, h_kv, d, unit, what, "k_cache"));
-    NEOX_TRY(check_strides(vc_st, 3, h_kv, d, unit, what, "v_cache"));
+    const int row = nibbles ? d / 2 : d, scales = nibbles ? d / 32 : 1;
+    NEOX_TRY(check_strides(kc_st, 3, h_kv, row, unit, what, "k_cache"));
+    NEOX_TRY(check_strides(vc_st, 3, h_kv, row, unit, what, "v_cache"));
     if (codes) {
-        NEOX_TRY(check_pointer(ks, 4, what, "k_scales"));
-        NEOX_TRY(check_pointer(vs, 4, what, "v_scales"));
-        NEOX_TRY(check_strides(ks_st, 3, h_kv, 1, 0, what, "k_scales"));
-        NEOX_TRY(check_strides(vs_st, 3, h_kv, 1, 0, what, "v_scales"));
+        NEOX_TRY(check_pointer(ks, nibbles ? 1 : 4, what, "k_scales"));
+        NEOX_TRY(check_pointer(vs, nibbles ? 1 : 4, what, "v_scales"));
+        NEOX_TRY(check_strides(ks_st, 3, h_kv, scales, 0, what, "k_scales"));
+        NEOX_TRY(check_strides(vs_st, 3, h_kv, scales, 0, what, "v_scales"));
     }
     return NEOX_OK;
 }
@@ -286,7 +305,7 @@ static void page_strides(int64_t (&to)[3], const int64_t* from) {
     to[2] = from[2];
 }
 
-static int cache_call(const char* what, void* k, void* v, const void* kc, const void* vc, const float* ks, const float* vs, const void* slots,
+static int cache_call(const char* what, void* k, void* v, const void* kc, const void* vc, const void* ks, const void* vs, const void* slots,
                       int slots_64, int64_t tokens, int h_kv, int d, int64_t pages, int page_size, const int64_t* k_st, const int64_t* v_st,
                       const int64_t* kc_st, const int64_t* vc_st, const int64_t* ks_st, const int64_t* vs_st, int dtype, int cache_dtype,
                       bool write, void* stream) {
@@ -313,8 +332,8 @@ static int cache_call(const char* what, void* k, void* v, const void* kc, const 
     page_strides(a.kc_st, kc_st);
     page_strides(a.vc_st, vc_st);
     if (source != kPaged16) {
-        a.ks = const_cast<float*>(ks);
-        a.vs = const_cast<float*>(vs);
+        a.ks = static_cast<float*>(const_cast<void*>(ks));
+        a.vs = static_cast<float*>(const_cast<void*>(vs));
         page_strides(a.ks_st, ks_st);
         page_strides(a.vs_st, vs_st);
     }
@@ -454,7 +473,7 @@ int neox_paged_attention_workspace(int64_t* bytes, int32_t b, int32_t tokens, in
 }
 
 int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, const void* q, const void* k_cache, const void* v_cache,
-                         const float* k_scales, const float* v_scales, const int32_t* page_table, const int32_t* query_starts,
+                         const void* k_scales, const void* v_scales, const int32_t* page_table, const int32_t* query_starts,
                          const int32_t* context_lengths, int32_t b, int32_t tokens, int32_t max_query, int32_t max_context, int32_t h,
                          int32_t h_kv, int32_t d, int64_t pages, int32_t page_size, int32_t table_columns, int64_t table_stride,
                          const int64_t out_strides[2], const int64_t q_strides[2], const int64_t k_cache_strides[3],
@@ -504,8 +523,8 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
     a.k = static_cast<const char*>(k_cache);
     a.v = static_cast<const char*>(v_cache);
     a.o = static_cast<char*>(out);
-    a.k_scale = k_scales;
-    a.v_scale = v_scales;
+    a.k_scale = static_cast<const float*>(k_scales);
+    a.v_scale = static_cast<const float*>(v_scales);
     a.lengths = context_lengths;
     a.starts = query_starts;
     a.table = page_table;
@@ -528,7 +547,7 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
     return a.splits > 1 ? check_launch(launch_attn_join(a, dtype, s), what) : (int)NEOX_OK;
 }
 
-int neox_cache_write(void* k_cache, void* v_cache, float* k_scales, float* v_scales, const void* k, const void* v, const void* slots,
+int neox_cache_write(void* k_cache, void* v_cache, void* k_scales, void* v_scales, const void* k, const void* v, const void* slots,
                      int32_t slots_64, int64_t tokens, int32_t h_kv, int32_t d, int64_t pages, int32_t page_size,
                      const int64_t k_cache_strides[3], const int64_t v_cache_strides[3], const int64_t k_scale_strides[3],
                      const int64_t v_scale_strides[3], const int64_t k_strides[2], const int64_t v_strides[2], int32_t dtype,
@@ -538,7 +557,7 @@ int neox_cache_write(void* k_cache, void* v_cache, float* k_scales, float* v_sca
                       v_scale_strides, dtype, cache_dtype, true, stream);
 }
 
-int neox_cache_read(void* k, void* v, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+int neox_cache_read(void* k, void* v, const void* k_cache, const void* v_cache, const void* k_scales, const void* v_scales,
                     const void* slots, int32_t slots_64, int64_t tokens, int32_t h_kv, int32_t d, int64_t pages, int32_t page_size,
                     const int64_t k_strides[2], const int64_t v_strides[2], const int64_t k_cache_strides[3],
                     const int64_t v_cache_strides[3], const int64_t k_scale_strides[3], const int64_t v_scale_strides[3], int32_t dtype,

@@ -17,6 +17,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "wave.hpp"
 
 namespace neox {
@@ -36,14 +38,14 @@ constexpr int kGradKeys = 128;  // keys of a workgroup there: 32 for each of its
 __device__ __forceinline__ const char* step_to(const char* p, uint32_t i, uint32_t bytes) { return p + (uint64_t)i * bytes; }
 
 // where keys and values come from
-enum KvSource { kStrided = 0, kPaged16 = 1, kPagedI8 = 2, kPagedF8 = 3 };
+enum KvSource { kStrided = 0, kPaged16 = 1, kPagedI8 = 2, kPagedF8 = 3, kPagedF4 = 4 };
 
 struct AttnArgs {
-    const char *q, *k, *v;       // 16-bit elements (k, v: 8-bit codes for the last two sources)
+    const char *q, *k, *v;       // 16-bit elements (k, v: 8-bit codes, or two 4-bit ones to a byte, for the last three sources)
     char* o;
     char* o_low;                 // null, or what rounding the output to 16 bits took away, laid out like the output
     float* lse;                  // log2 of every row's sum of exponentials, less gradient_bits(), +inf for an empty row; [b, kv, rows]
-    const float *k_scale, *v_scale;
+    const float *k_scale, *v_scale;  // (4-bit codes: bytes)
     // element strides.  q, o: token, sample (strided only), head.  k, v: token, sample, head; for pages the token
     // stride within a page, the page stride and the head stride
     int64_t q_st[3], o_st[3], k_st[3], v_st[3];
@@ -302,6 +304,27 @@ __device__ __forceinline__ u32x4 widen8(const u32x2& w) {
     return pack8<T>(f);
 }
 
+// eight 4-bit codes times 2^(e - 127), the scale's bits being e << 23 (255: NaN), as 16-bit values: exactly in bf16, which has
+// its exponents; in fp16 the scale has to bring them into its range
+template <typename T>
+__device__ __forceinline__ u32x4 widen4(uint32_t word, float scale) {
+    if constexpr (__is_same(T, BF16)) {
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3))};
+    } else {
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 3))};
+    }
+}
+// what the byte of a 4-bit scale stands for (0 instead of 2^-127), as the kernels multiply by it
+constexpr uint32_t kScaleNan = 255;
+__device__ __forceinline__ float scale_bits(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+__device__ __forceinline__ float nan_value() { return __builtin_bit_cast(float, 0x7fc00000u); }
+
 // Where a probability is multiplied by its value's scale before it is rounded to fp16, the product can be anything: scales
 // are the values' own size, over the largest code, and the largest of them may belong to keys that are hardly looked at.
 // The accumulators of a row therefore hold their sums times a power of two of the row's own, which brings the largest
@@ -425,6 +448,65 @@ struct Stage {
     }
 };
 
+// The same for 4-bit codes: 32 to a thread, which are one scale's.  In bf16 they take their scale along; a NaN scale of the
+// values (which would reach every row through zero probabilities) is told to the rows instead, as a number of the key's own, 0 or
+// NaN.  In fp16 a key's largest scale stays a factor of its own, as in 8 bits, and the codes are multiplied by what
+// theirs is below it: 23 powers of two below the largest they begin to lose bits.  Neighbouring quads of threads have rows 4, 8
+// and 12 apart, whose turns send their four pieces to sixteen different places.
+template <typename T, int DP, int ROWS>
+struct Stage4 {
+    static constexpr bool kKeyScales = __is_same(T, F16);
+    static constexpr int kLanes = DP <= 64 ? 2 : DP <= 128 ? 4 : 8;  // of a row
+    static constexpr int kRowsAtOnce = 256 / kLanes;
+    static constexpr int kSteps = (ROWS + kRowsAtOnce - 1) / kRowsAtOnce;
+    u32x4 codes[kSteps];
+    uint32_t scale[kSteps];
+
+    static __device__ __forceinline__ int row(int step) {
+        const int i = threadIdx.x / kLanes;
+        return ((i & ~15) | (i & 3) << 2 | ((i >> 2) & 3)) + step * kRowsAtOnce;
+    }
+    static __device__ __forceinline__ int piece() { return (int)(threadIdx.x % kLanes); }
+    static __device__ __forceinline__ bool works(int step) { return row(step) < ROWS && piece() * 32 < DP; }
+
+    __device__ __forceinline__ void load(int step, const char* at, const uint8_t* scale_at, bool there) {
+        codes[step] = u32x4{0, 0, 0, 0};
+        scale[step] = 0;
+        if (there) {
+            codes[step] = *reinterpret_cast<const u32x4*>(at);
+            scale[step] = *scale_at;
+        }
+    }
+    // keys: [ROWS]; whether one of this thread's keys has a NaN that `keys` holds
+    template <bool VALUES>
+    __device__ __forceinline__ bool put(char* tile, float* keys) const {
+        bool bad = false;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            u32x4 c = codes[s];
+            asm("" : "+v"(c.x), "+v"(c.y), "+v"(c.z), "+v"(c.w));
+            uint32_t e = scale[s];
+            if constexpr (kKeyScales) {
+                const uint32_t top = group_largest<kLanes>(e);
+                e = (uint32_t)max((int)(e + 127 - top), 0);
+                if (works(s) && piece() == 0) keys[row(s)] = top == kScaleNan ? nan_value() : scale_bits(top);
+            } else if constexpr (VALUES) {
+                const bool nan = group_largest<kLanes>(e) == kScaleNan;
+                bad |= nan;
+                e = e == kScaleNan ? 0 : e;
+                if (works(s) && piece() == 0) keys[row(s)] = nan ? nan_value() : 0.f;
+            }
+            const float f = scale_bits(e);
+            if (works(s)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(tile + Tile<DP>::at(row(s), 4 * piece() + i)) = widen4<T>(c[i], f);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return bad;
+    }
+};
+
 // 16-bit rows get there without registers in between: every lane names the 16 bytes that go to its place of the
 // tile (256 threads, a wave 1 KiB at a time), or writes zeros there.  The copies are in flight until landed().
 template <int DP, int ROWS>
@@ -475,7 +557,9 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 template <typename T, int DP, int SRC, bool SPLIT>
 __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged16 ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
     constexpr bool kPages = SRC != kStrided;
-    constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8;
+    constexpr bool kF4 = SRC == kPagedF4;
+    constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8 || kF4;
+    constexpr bool kKeyScales = kCodes && !(kF4 && __is_same(T, BF16));  // a factor for each key, apart from its codes
     constexpr int kBytes = kCodes ? 1 : 2;
     // Keys of one step.  32 leave registers and LDS for a third workgroup on a CU (measured with 64 and 32, us: 2 x 64
     // heads of 96 dims, 2048 keys, window 512: 126, 105; 32 heads of 128 dims, 8192 keys, window 4096: 562, 539); with
@@ -483,6 +567,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     constexpr int kFwdKeys = kCodes ? 64 : 32;
     constexpr int kTile = kFwdKeys * Tile<DP>::kRow;
     __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile + (kCodes ? 2 * 2 * kFwdKeys * 4 : 0)];
+    __shared__ __attribute__((aligned(16))) uint32_t nan_keys[kF4 && !kKeyScales ? 2 : 1][4];  // [buffer][wave that staged it]
 
     // block -> (sample, key head), row tile, part: neighbours in time on one XCD (blocks go to the 8 XCDs in
     // turn) are the row tiles of one key head, whose keys they share
@@ -534,7 +619,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 
     // One tile of keys and values into one of the buffers: 16-bit rows are copied there as they are; codes come through
     // registers and are widened on the way, which put() does when the tile's turn is near.
-    typedef Stage<T, DP, kCodes ? SRC : kPagedI8, kFwdKeys> St;
+    typedef std::conditional_t<kF4, Stage4<T, DP, kFwdKeys>, Stage<T, DP, kCodes ? SRC : kPagedI8, kFwdKeys>> St;
     typedef Flight<DP, kFwdKeys> Fl;
     Fl fl;
     constexpr int kSteps = kCodes ? St::kSteps : Fl::kSteps;
@@ -567,7 +652,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                 const int key = tile * kFwdKeys + row_of(s);
                 page_of[s] = key < keys ? table[a.by_page.div(key)] : -1;
             }
-            if constexpr (kCodes) {
+            if constexpr (kCodes && !kF4) {
                 const int key = tile * kFwdKeys + lane;
                 page_at = (wave < 2 && key < keys) ? table[a.by_page.div(key)] : -1;
             }
@@ -603,8 +688,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
         fl.again();
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int key = tile * kFwdKeys + row_of(s), piece = kCodes ? St::piece() : fl.piece(s);
-            bool ok = key < keys && piece * 8 < a.d;
+            const int key = tile * kFwdKeys + row_of(s), piece = kCodes ? St::piece() * (kF4 ? 2 : 1) : fl.piece(s);
+            bool ok = key < keys && piece * (kF4 ? 16 : 8) < a.d;
             const char *kp = kbase + piece * 8 * kBytes, *vp = vbase + piece * 8 * kBytes;
             if constexpr (kPages) {
                 const uint32_t page = even ? tile_page : page_of[s], in = a.by_page.mod(key);
@@ -615,7 +700,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                 kp = step_to(kp, key, (uint32_t)a.k_st[0] * 2);
                 vp = step_to(vp, key, (uint32_t)a.v_st[0] * 2);
             }
-            if constexpr (kCodes) {
+            if constexpr (kF4) {
+                const int64_t page = page_of[s], in = a.by_page.mod(key);
+                const uint8_t* const kf = reinterpret_cast<const uint8_t*>(a.k_scale) + (page * a.ks_st[1] + in * a.ks_st[0] + (int64_t)g * a.ks_st[2] + St::piece());
+                const uint8_t* const vf = reinterpret_cast<const uint8_t*>(a.v_scale) + (page * a.vs_st[1] + in * a.vs_st[0] + (int64_t)g * a.vs_st[2] + St::piece());
+                ks.load(s, kp, kf, ok && St::works(s));
+                vs.load(s, vp, vf, ok && St::works(s));
+            } else if constexpr (kCodes) {
                 ks.load(s, kp, ok && St::works(s));
                 vs.load(s, vp, ok && St::works(s));
             } else if (ok) {
@@ -626,7 +717,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                 fl.zero(s, kt + kTile);
             }
         }
-        if constexpr (kCodes) {
+        if constexpr (kCodes && !kF4) {
             scale_of_key = 0.f;
             if (wave < 2 && (uint32_t)page_at < (uint32_t)a.pages) {
                 const int64_t in = a.by_page.mod(tile * kFwdKeys + lane);
@@ -637,7 +728,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     };
     float* const scales = reinterpret_cast<float*>(lds + 2 * 2 * kTile);  // [buffer][keys, values][64]
     auto put = [&](int buffer) {
-        if constexpr (kCodes) {
+        if constexpr (kF4) {
+            ks.template put<false>(lds + buffer * 2 * kTile, scales + buffer * 2 * kFwdKeys);
+            const bool bad = vs.template put<true>(lds + buffer * 2 * kTile + kTile, scales + (buffer * 2 + 1) * kFwdKeys);
+            if constexpr (!kKeyScales) {
+                const uint32_t any = __any(bad);
+                if (lane == 0) nan_keys[buffer][wave] = any;
+            }
+        } else if constexpr (kCodes) {
             ks.put(lds + buffer * 2 * kTile);
             vs.put(lds + buffer * 2 * kTile + kTile);
             if (wave < 2) scales[(buffer * 2 + wave) * kFwdKeys + lane] = scale_of_key;
@@ -652,7 +750,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     float m = kNegInf, l = 0.f;
-    constexpr bool kLifted = kCodes && __is_same(T, F16);
+    constexpr bool kLifted = kKeyScales && __is_same(T, F16);
     constexpr float kBits = probability_bits<T, kCodes>();
     Lift lift;
 
@@ -703,7 +801,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                 for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s[kb]);
                 matrix_done(!kCodes);
             }
-            if constexpr (kCodes) {
+            if constexpr (kKeyScales) {
                 const float* f = scales + buffer * 2 * kFwdKeys;
 #pragma unroll
                 for (int kb = 0; kb < kFwdKeys / 32; ++kb)
@@ -756,7 +854,20 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
                     sum += s[kb][r];
                 }
             l += sum;
-            if (kCodes && !all) {  // a hidden value's scale may be anything
+            if constexpr (kF4 && !kKeyScales) {
+                const u32x4 any = *reinterpret_cast<const u32x4*>(nan_keys[buffer]);
+                if (__builtin_amdgcn_readfirstlane(any.x | any.y | any.z | any.w)) {
+#pragma unroll
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 16; r += 4) {
+                            const f32x4 c = *reinterpret_cast<const f32x4*>(scales + (buffer * 2 + 1) * kFwdKeys + 32 * kb + 2 * r + 4 * half);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[kb][r + i] = s[kb][r + i] != 0.f ? s[kb][r + i] + c[i] : 0.f;
+                        }
+                }
+            }
+            if (kKeyScales && !all) {  // a hidden value's scale may be anything
 #pragma unroll
                 for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
@@ -765,7 +876,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[kb][r + i] = s[kb][r + i] != 0.f ? s[kb][r + i] * c[i] : 0.f;
                     }
-            } else if constexpr (kCodes) {
+            } else if constexpr (kKeyScales) {
                 const float* f = scales + (buffer * 2 + 1) * kFwdKeys;
 #pragma unroll
                 for (int kb = 0; kb < kFwdKeys / 32; ++kb)

@@ -14,6 +14,7 @@ static void forward(const AttnArgs& a, int source, hipStream_t stream) {
         case kPaged16: attn_fwd_kernel<T, DP, kPaged16, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedI8: attn_fwd_kernel<T, DP, kPagedI8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedF8: attn_fwd_kernel<T, DP, kPagedF8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
+        case kPagedF4: attn_fwd_kernel<T, DP, kPagedF4, SPLIT><<<grid, 256, 0, stream>>>(a); break;
     }
 }
 
@@ -25,6 +26,7 @@ static void token(const AttnArgs& a, int source, hipStream_t stream) {
         case kPaged16: attn_token_kernel<T, DP, kPaged16, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedI8: attn_token_kernel<T, DP, kPagedI8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedF8: attn_token_kernel<T, DP, kPagedF8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
+        case kPagedF4: attn_token4_kernel<T, DP, SPLIT><<<grid, 256, 0, stream>>>(a); break;
     }
 }
 

@@ -20,7 +20,7 @@ namespace neox {
 struct CacheArgs {
     char *k, *v;                      // rows outside the cache, 16-bit
     char *kc, *vc;                    // the cache
-    float *ks, *vs;                   // its scales
+    float *ks, *vs;                   // its scales (4 bits: bytes)
     const void* slots;
     int64_t k_st[2], v_st[2];         // token, head
     int64_t kc_st[3], vc_st[3], ks_st[3], vs_st[3];  // token within a page, page, head
@@ -30,18 +30,6 @@ struct CacheArgs {
     FastDiv by_heads, by_page;
     bool wide;                        // 64-bit slots
 };
-
-// the largest of G neighbouring lanes' values, non-negative integers below 2^31
-template <int G>
-__device__ __forceinline__ uint32_t group_largest(uint32_t x) {
-    int v = (int)x;
-    if constexpr (G >= 2) v = max(v, dpp<kDppQuadSwap1>(v));
-    if constexpr (G >= 4) v = max(v, dpp<kDppQuadSwap2>(v));
-    if constexpr (G >= 8) v = max(v, dpp<kDppRowHalfMirror>(v));
-    if constexpr (G >= 16) v = max(v, dpp<kDppRowMirror>(v));
-    static_assert(G <= 16, "a row's lanes are in one DPP row");
-    return (uint32_t)v;
-}
 
 // One row's share of a lane (16 elements in two words of 8) as codes; *scale gets the row's.
 template <typename T, int SRC, int G>

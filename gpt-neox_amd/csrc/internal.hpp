@@ -8,6 +8,7 @@
 #include "rope_kernels.hpp"
 #include "softmax_kernels.hpp"
 #include "cache_kernels.hpp"
+#include "fp4_kernels.hpp"
 
 namespace neox {
 

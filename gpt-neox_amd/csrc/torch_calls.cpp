@@ -446,12 +446,15 @@ struct Cache {
         switch (k.scalar_type()) {
             case at::kChar: return NEOX_I8;
             case at::kFloat8_e4m3fn: return NEOX_F8;
+            case at::kFloat4_e2m1fn_x2: return NEOX_F4;
             default: return code(like);
         }
     }
+    bool coded() const { return k.scalar_type() == at::kChar || k.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == at::kFloat4_e2m1fn_x2; }
+    int64_t dim() const { return k.size(3) * (k.scalar_type() == at::kFloat4_e2m1fn_x2 ? 2 : 1); }
     bool goes_with(const Tensor& like) const {
-        return half_type(like) && (k_scale ? (k.scalar_type() == at::kChar || k.scalar_type() == at::kFloat8_e4m3fn) : k.scalar_type() == like.scalar_type()) &&
-               k.device() == like.device() && k.dim() == 4 && like.size(-1) == k.size(3);
+        return half_type(like) && (k_scale ? coded() : k.scalar_type() == like.scalar_type()) && k.device() == like.device() && k.dim() == 4 &&
+               like.size(-1) == dim();
     }
 };
 RowStrides scale_strides(const std::optional<Tensor>& t) { return t ? RowStrides(*t, 3) : RowStrides(Tensor(), 0); }
@@ -469,7 +472,7 @@ bool cache_write(const Tensor& kc, const Tensor& vc, const std::optional<Tensor>
         !cache.goes_with(k) || k.size(1) != kc.size(2) || !slot_list(slots, k) || slots.size(0) != k.size(0) || !in_pieces(k) || !in_pieces(v))
         return false;
     const c10::DeviceGuard guard(k.device());
-    check(neox_cache_write(kc.mutable_data_ptr(), vc.mutable_data_ptr(), pointer_or_null<float>(ks), pointer_or_null<float>(vs),
+    check(neox_cache_write(kc.mutable_data_ptr(), vc.mutable_data_ptr(), pointer_or_null<void>(ks), pointer_or_null<void>(vs),
                            k.const_data_ptr(), v.const_data_ptr(), slots.const_data_ptr(), slots.scalar_type() == at::kLong, k.size(0),
                            (int32_t)k.size(1), (int32_t)k.size(2), kc.size(0), (int32_t)kc.size(1), RowStrides(kc, 3), RowStrides(vc, 3),
                            scale_strides(ks), scale_strides(vs), RowStrides(k, 2), RowStrides(v, 2), code(k), cache.dtype(k), stream_of(k)));
@@ -482,10 +485,10 @@ std::optional<std::tuple<Tensor, Tensor>> cache_read(const Tensor& kc, const Ten
     if (!slot_list(slots, kc) || (dtype != at::kHalf && dtype != at::kBFloat16) || (!ks && dtype != kc.scalar_type())) return std::nullopt;
     const Cache cache{kc, vc, ks, vs};
     const c10::DeviceGuard guard(kc.device());
-    Tensor k = at::empty({slots.size(0), kc.size(2), kc.size(3)}, kc.options().dtype(dtype)), v = at::empty_like(k);
-    check(neox_cache_read(k.mutable_data_ptr(), v.mutable_data_ptr(), kc.const_data_ptr(), vc.const_data_ptr(), pointer_or_null<const float>(ks),
-                          pointer_or_null<const float>(vs), slots.const_data_ptr(), slots.scalar_type() == at::kLong, slots.size(0),
-                          (int32_t)kc.size(2), (int32_t)kc.size(3), kc.size(0), (int32_t)kc.size(1), RowStrides(k, 2), RowStrides(v, 2),
+    Tensor k = at::empty({slots.size(0), kc.size(2), cache.dim()}, kc.options().dtype(dtype)), v = at::empty_like(k);
+    check(neox_cache_read(k.mutable_data_ptr(), v.mutable_data_ptr(), kc.const_data_ptr(), vc.const_data_ptr(), pointer_or_null<const void>(ks),
+                          pointer_or_null<const void>(vs), slots.const_data_ptr(), slots.scalar_type() == at::kLong, slots.size(0),
+                          (int32_t)kc.size(2), (int32_t)cache.dim(), kc.size(0), (int32_t)kc.size(1), RowStrides(k, 2), RowStrides(v, 2),
                           RowStrides(kc, 3), RowStrides(vc, 3), scale_strides(ks), scale_strides(vs), code(k), cache.dtype(k), stream_of(k)));
     return std::make_tuple(k, v);
 }
@@ -510,13 +513,44 @@ std::optional<Tensor> paged_attention(const Tensor& q, const Tensor& kc, const T
     check(neox_paged_attention_workspace(&bytes, b, tokens, (int32_t)max_query, (int32_t)max_context, h, h_kv, d, (int32_t)window, (int32_t)sinks));
     if (bytes) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
     check(neox_paged_attention(out.mutable_data_ptr(), bytes ? workspace.mutable_data_ptr() : nullptr, bytes, q.const_data_ptr(),
-                               kc.const_data_ptr(), vc.const_data_ptr(), pointer_or_null<const float>(ks), pointer_or_null<const float>(vs),
+                               kc.const_data_ptr(), vc.const_data_ptr(), pointer_or_null<const void>(ks), pointer_or_null<const void>(vs),
                                static_cast<const int32_t*>(table.const_data_ptr()), static_cast<const int32_t*>(starts.const_data_ptr()),
                                static_cast<const int32_t*>(lengths.const_data_ptr()), b, tokens, (int32_t)max_query, (int32_t)max_context, h,
                                h_kv, d, kc.size(0), (int32_t)kc.size(1), (int32_t)table.size(1), table.size(0) > 1 ? table.stride(0) : 0,
                                RowStrides(out, 2), RowStrides(q, 2), RowStrides(kc, 3), RowStrides(vc, 3), scale_strides(ks),
                                scale_strides(vs), (float)scale, (int32_t)window, (int32_t)sinks, code(q), cache.dtype(q), stream_of(q)));
     return out;
+}
+
+// ---- the pages of caches ---------------------------------------------------------------------------
+// The tensors of a PagePool, which has looked at them, and the numbers of a call, one for each sequence.
+bool pool_list(const Tensor& t, const Tensor& lengths) { return int_list(t, lengths, lengths.size(0)); }
+int64_t row_stride(const Tensor& table) { return table.size(0) > 1 ? table.stride(0) : 0; }
+int32_t* words(const Tensor& t) { return static_cast<int32_t*>(t.mutable_data_ptr()); }
+
+// starts, positions, slots and whether granted, or None
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> pages_extend(const Tensor& table, const Tensor& lengths, const Tensor& free, const Tensor& left,
+                                                                       const Tensor& tokens, int64_t page_size, int64_t max_tokens) {
+    if (!pool_list(tokens, lengths) || max_tokens < 0 || max_tokens >= 1 << 30) return std::nullopt;
+    const c10::DeviceGuard guard(table.device());
+    const int64_t n = lengths.size(0);
+    // (one allocation for what has 32 bits, the workspace behind it)
+    const Tensor all = at::empty({2 * (n + 1) + max_tokens}, lengths.options());
+    Tensor starts = all.narrow(0, 0, n + 1), positions = all.narrow(0, n + 1, max_tokens);
+    Tensor slots = at::empty({max_tokens}, lengths.options().dtype(at::kLong)), granted = at::empty({n}, lengths.options().dtype(at::kBool));
+    check(neox_pages_extend(words(starts), words(positions), static_cast<int64_t*>(slots.mutable_data_ptr()), static_cast<uint8_t*>(granted.mutable_data_ptr()),
+                            words(all) + n + 1 + max_tokens, words(table), words(lengths), words(free), words(left), words(tokens), (int32_t)n,
+                            (int32_t)table.size(1), row_stride(table), (int32_t)free.size(0), (int32_t)page_size, (int32_t)max_tokens, stream_of(table)));
+    return std::make_tuple(starts, positions, slots, granted);
+}
+
+// whether that was done
+bool pages_truncate(const Tensor& table, const Tensor& lengths, const Tensor& free, const Tensor& left, const Tensor& keep, int64_t page_size) {
+    if (!pool_list(keep, lengths)) return false;
+    const c10::DeviceGuard guard(table.device());
+    check(neox_pages_truncate(words(table), words(lengths), words(free), words(left), words(keep), (int32_t)lengths.size(0), (int32_t)table.size(1),
+                              row_stride(table), (int32_t)free.size(0), (int32_t)page_size, stream_of(table)));
+    return true;
 }
 
 }  // namespace
@@ -539,5 +573,7 @@ PYBIND11_MODULE(neox_torch, m) {
     m.def("cache_write", wrap_pybind_function_no_gil(cache_write));
     m.def("cache_read", wrap_pybind_function_no_gil(cache_read));
     m.def("paged_attention", wrap_pybind_function_no_gil(paged_attention));
+    m.def("pages_extend", wrap_pybind_function_no_gil(pages_extend));
+    m.def("pages_truncate", wrap_pybind_function_no_gil(pages_truncate));
     m.def("rope", wrap_pybind_function_no_gil(rope), py::arg("x"), py::arg("cos"), py::arg("sin"), py::arg("transposed"));
 }

@@ -228,6 +228,18 @@ __device__ __forceinline__ float group_reduce(float x) {
     return Op::dec(v);
 }
 
+// the largest of G neighbouring lanes' values, non-negative integers below 2^31
+template <int G>
+__device__ __forceinline__ uint32_t group_largest(uint32_t x) {
+    int v = (int)x;
+    if constexpr (G >= 2) v = max(v, dpp<kDppQuadSwap1>(v));
+    if constexpr (G >= 4) v = max(v, dpp<kDppQuadSwap2>(v));
+    if constexpr (G >= 8) v = max(v, dpp<kDppRowHalfMirror>(v));
+    if constexpr (G >= 16) v = max(v, dpp<kDppRowMirror>(v));
+    static_assert(G <= 16, "a row's lanes are in one DPP row");
+    return (uint32_t)v;
+}
+
 // Reduce across the whole wave; the result is wave-uniform.
 template <typename Op>
 __device__ __forceinline__ float wave_reduce(float v) {

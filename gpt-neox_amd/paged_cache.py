@@ -1,8 +1,9 @@
-"""A paged key/value cache in 16 or 8 bits, and the attention of new tokens over it.
+"""A paged key/value cache in 16, 8 or 4 bits, and the attention of new tokens over it.
 
 :class:`PagedKVCache` holds the keys and values of many sequences in pages of a fixed number of tokens; which pages
-belong to a sequence is the caller's page table.  New keys and values are quantised as they are written
-(:meth:`PagedKVCache.write`) to int8 or 8-bit floats with an fp32 scale for each token and head, or kept in 16 bits;
+belong to a sequence is the caller's page table (or a :class:`~gpt_neox_amd.page_pool.PagePool`'s).  New keys and values
+are quantised as they are written (:meth:`PagedKVCache.write`) to int8 or 8-bit floats with an fp32 scale for each token
+and head, to 4-bit floats with a power of two for every 32 values, or kept in 16 bits;
 :func:`paged_attention` reads them where they lie, for one new token of each sequence (generation) or many (prompts in
 chunks), with or without a window and sinks as in :func:`~gpt_neox_amd.fused_attention.window_attention`.  Nothing
 here looks at the page table, the lengths or the slots on the host, so a step can be recorded into a HIP graph.
@@ -17,12 +18,20 @@ from . import _lib
 from .fused_attention import check_window
 
 _HALF = (torch.float16, torch.bfloat16)
-_CODES = {torch.int8: _lib.NEOX_I8, torch.float8_e4m3fn: _lib.NEOX_F8}
+_CODES = {torch.int8: _lib.NEOX_I8, torch.float8_e4m3fn: _lib.NEOX_F8, torch.float4_e2m1fn_x2: _lib.NEOX_F4}
+_F4_GROUP = 32  # values of a 4-bit cache that share a scale
 
 
 class PagedKVCache:
     """Keys and values ``[pages, page_size, heads, dim]`` in fp16, bf16, int8 or float8_e4m3fn, the last two with scales
-    ``[pages, page_size, heads]`` in fp32.  Slot ``page * page_size + i`` is token ``i`` of a page.
+    ``[pages, page_size, heads]`` in fp32, or in float4_e2m1fn_x2, two values to an element (``dim / 2`` of them, the first value
+    in the low half), with scales ``[pages, page_size, heads, dim / 32]`` in float8_e8m0fnu, one for each 32 neighbouring values.
+    Slot ``page * page_size + i`` is token ``i`` of a page.
+
+    Values in 4 bits are 0, 0.5, 1, 1.5, 2, 3, 4 or 6 times a power of two, with a sign.  ``write`` takes the least power of
+    which seven times is no less than the 32 values' largest magnitude, from 2^-125 up to 2^125 (bf16) or 2^13 (fp16), and rounds to
+    the nearest of these, to the even code at ties; what is above six times the power becomes six times.  A token's
+    head that holds an infinity or a NaN gets NaN scales and reads back as NaN, as in 8 bits.
 
     The tensors may be views (of one buffer for all layers, say) as long as every head's values are dense and start on
     16-byte boundaries.  They are looked at once, here, and stay: other tensors are another cache.
@@ -39,20 +48,28 @@ class PagedKVCache:
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
             raise RuntimeError("k and v must have the same shape [pages, page_size, heads, dim] and dtype")
         if k.dtype not in _HALF and k.dtype not in _CODES:
-            raise RuntimeError(f"a cache holds fp16, bf16, int8 or float8_e4m3fn, not {k.dtype}")
+            raise RuntimeError(f"a cache holds fp16, bf16, int8, float8_e4m3fn or float4_e2m1fn_x2, not {k.dtype}")
         _lib.require_gpu(k, v, k_scale, v_scale)
         self.quantised = k.dtype in _CODES
-        dim, per_piece = k.shape[3], 16 // k.element_size()
-        if dim % per_piece or not 8 <= dim <= 256:
-            raise RuntimeError(f"head dim {dim} must be a multiple of {per_piece} up to 256 for a cache in {k.dtype}")
+        per_piece, packed = 16 // k.element_size(), 2 if k.dtype == torch.float4_e2m1fn_x2 else 1
+        dim = k.shape[3] * packed
+        if k.shape[3] % per_piece or not 8 <= dim <= 256:
+            raise RuntimeError(f"head dim {dim} must be a multiple of {per_piece * packed} up to 256 for a cache in {k.dtype}")
         if k.numel() == 0:
             raise RuntimeError("a cache needs at least one page, one token per page and one head")
         for t in (k, v):
             if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % per_piece for n, s in zip(t.shape[:3], t.stride()) if n > 1):
                 raise RuntimeError("every head's values must be dense and start on a 16-byte boundary")
         if self.quantised != (k_scale is not None) or self.quantised != (v_scale is not None):
-            raise RuntimeError("a cache in 8 bits needs k_scale and v_scale, one in 16 bits takes none")
-        if self.quantised:
+            raise RuntimeError("a cache in 8 or 4 bits needs k_scale and v_scale, one in 16 bits takes none")
+        if packed == 2:
+            shape = (*k.shape[:3], dim // _F4_GROUP)
+            for t in (k_scale, v_scale):
+                if t.shape != shape or t.dtype != torch.float8_e8m0fnu:
+                    raise RuntimeError(f"scales must be float8_e8m0fnu {list(shape)}")
+                if t.stride(3) != 1 and t.shape[3] > 1:
+                    raise RuntimeError("the scales of a token's head must be dense")
+        elif self.quantised:
             for t in (k_scale, v_scale):
                 if t.shape != k.shape[:3] or t.dtype != torch.float32:
                     raise RuntimeError(f"scales must be float32 {list(k.shape[:3])}")
@@ -60,15 +77,20 @@ class PagedKVCache:
             if t is not None and t.device != k.device:
                 raise RuntimeError("all tensors must be on the same device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.pages, self.page_size, self.heads, self.dim = k.shape
+        self.pages, self.page_size, self.heads, self.dim = *k.shape[:3], dim
         self.dtype, self.device = k.dtype, k.device
-        # the scales have no dense axis of their own: [..., None] gives row_strides one to leave out
-        scales = [_lib.row_strides(t[..., None]) if t is not None else None for t in (k_scale, v_scale)]
+        # the scales of 8 bits have no dense axis of their own: [..., None] gives row_strides one to leave out
+        scales = [_lib.row_strides(t[..., None] if t.dim() == 3 else t) if t is not None else None for t in (k_scale, v_scale)]
         self._strides = (_lib.row_strides(k), _lib.row_strides(v), *scales)
 
     @classmethod
     def allocate(cls, pages, page_size, heads, dim, dtype=torch.int8, device="cuda"):
         """A cache of zeros."""
+        if dtype == torch.float4_e2m1fn_x2:
+            if dim % _F4_GROUP:
+                raise RuntimeError(f"head dim {dim} must be a multiple of {_F4_GROUP} up to 256 for a cache in {dtype}")
+            k, v, k_scale, v_scale = (torch.zeros((pages, page_size, heads, dim // n), dtype=torch.uint8, device=device) for n in (2, 2, _F4_GROUP, _F4_GROUP))
+            return cls(k.view(dtype), v.view(dtype), k_scale.view(torch.float8_e8m0fnu), v_scale.view(torch.float8_e8m0fnu))
         k, v = (torch.zeros((pages, page_size, heads, dim), dtype=torch.int8, device=device).view(dtype) if dtype in _CODES
                 else torch.zeros((pages, page_size, heads, dim), dtype=dtype, device=device) for _ in "kv")
         if dtype not in _CODES:

@@ -29,6 +29,7 @@ extern "C" {
 /*
  * ABI versions.  A version is bumped when an entry point is added or its parameter list changes; the
  * Python binding refuses a library of another version.
+ *   6  + neox_pages_extend, neox_pages_truncate; caches in 4 bits (NEOX_F4), whose scales are bytes
  *   5  + neox_window_attention_fwd/_bwd, neox_window_attention_bwd_workspace, neox_paged_attention,
  *      neox_paged_attention_workspace, neox_cache_write, neox_cache_read
  *   4  + neox_mask_scan, neox_masked_softmax_ends_fwd, neox_masked_softmax_ends_bwd
@@ -37,14 +38,15 @@ extern "C" {
  *   2  + the dropout, bias and ALiBi entry points, neox_rope_apply_freqs
  *   1  the four softmax entry points, neox_rope_apply, neox_get_batch_per_block
  */
-#define NEOX_FUSED_ABI_VERSION 5
+#define NEOX_FUSED_ABI_VERSION 6
 
 typedef enum neox_dtype {
     NEOX_F16 = 0,  /* IEEE binary16 */
     NEOX_BF16 = 1, /* bfloat16 */
     NEOX_F32 = 2,  /* only valid for the rotary cos/sin tables */
     NEOX_I8 = 3,   /* only valid for a paged cache: int8 codes */
-    NEOX_F8 = 4    /* only valid for a paged cache: 8-bit floats, e4m3 without infinities */
+    NEOX_F8 = 4,   /* only valid for a paged cache: 8-bit floats, e4m3 without infinities */
+    NEOX_F4 = 5    /* only valid for a paged cache: 4-bit floats, e2m1, two to a byte */
 } neox_dtype;
 
 typedef enum neox_status {
@@ -388,17 +390,23 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int
  * (NEOX_I8, NEOX_F8; d a multiple of 16, strides of 16) with an fp32 scale for each token and head in
  * k_scales, v_scales (NULL for 16 bits): value = code * scale, scale = largest |value| / 127 (448), code =
  * the value / scale rounded to nearest even.  A row that holds an infinity or a NaN reads back as NaN.
+ * Or 4-bit codes (NEOX_F4; d a multiple of 32): strides and the last axis count bytes, d / 2 of them to a row, value 2 i
+ * in the low half of byte i; k_scales, v_scales hold a byte for every 32 values, d / 32 dense ones to a row, their strides
+ * count bytes too, and need no alignment: byte s stands for 2^(s - 127), 255 for NaN.  A code's low three bits stand for 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6, the fourth for the sign.  write takes the least power of two of which seven times is no less than the largest of
+ * the 32 magnitudes, from 2^-125 to 2^125 (bf16; fp16: 2^13), and rounds to the nearest value, to the even code at ties, at
+ * most to six times the power.  Where a scale of a row is NaN, attention takes the whole row for NaN.
  * slots: int32 or int64 [tokens] in device memory, slot = page * page_size + token in the page.
  * write: k, v [tokens, h_kv, d] by strides {token, head} into their slots; a slot outside the cache is
  * skipped, and no slot may be named twice.  read: the reverse; a slot outside the cache reads as zeros.
  */
-int neox_cache_write(void* k_cache, void* v_cache, float* k_scales, float* v_scales, const void* k, const void* v,
+int neox_cache_write(void* k_cache, void* v_cache, void* k_scales, void* v_scales, const void* k, const void* v,
                      const void* slots, int32_t slots_64, int64_t tokens, int32_t h_kv, int32_t d, int64_t pages,
                      int32_t page_size, const int64_t k_cache_strides[3], const int64_t v_cache_strides[3],
                      const int64_t k_scale_strides[3], const int64_t v_scale_strides[3], const int64_t k_strides[2],
                      const int64_t v_strides[2], int32_t dtype, int32_t cache_dtype, void* stream);
-int neox_cache_read(void* k, void* v, const void* k_cache, const void* v_cache, const float* k_scales,
-                    const float* v_scales, const void* slots, int32_t slots_64, int64_t tokens, int32_t h_kv, int32_t d,
+int neox_cache_read(void* k, void* v, const void* k_cache, const void* v_cache, const void* k_scales,
+                    const void* v_scales, const void* slots, int32_t slots_64, int64_t tokens, int32_t h_kv, int32_t d,
                     int64_t pages, int32_t page_size, const int64_t k_strides[2], const int64_t v_strides[2],
                     const int64_t k_cache_strides[3], const int64_t v_cache_strides[3], const int64_t k_scale_strides[3],
                     const int64_t v_scale_strides[3], int32_t dtype, int32_t cache_dtype, void* stream);
@@ -416,13 +424,34 @@ int neox_cache_read(void* k, void* v, const void* k_cache, const void* v_cache, 
 int neox_paged_attention_workspace(int64_t* bytes, int32_t b, int32_t tokens, int32_t max_query, int32_t max_context,
                                    int32_t h, int32_t h_kv, int32_t d, int32_t window, int32_t sinks);
 int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, const void* q, const void* k_cache,
-                         const void* v_cache, const float* k_scales, const float* v_scales, const int32_t* page_table,
+                         const void* v_cache, const void* k_scales, const void* v_scales, const int32_t* page_table,
                          const int32_t* query_starts, const int32_t* context_lengths, int32_t b, int32_t tokens,
                          int32_t max_query, int32_t max_context, int32_t h, int32_t h_kv, int32_t d, int64_t pages,
                          int32_t page_size, int32_t table_columns, int64_t table_stride, const int64_t out_strides[2],
                          const int64_t q_strides[2], const int64_t k_cache_strides[3], const int64_t v_cache_strides[3],
                          const int64_t k_scale_strides[3], const int64_t v_scale_strides[3], float scale, int32_t window,
                          int32_t sinks, int32_t dtype, int32_t cache_dtype, void* stream);
+
+/*
+ * The pages of such caches, kept in device memory: page_table [sequences, columns] by rows of table_stride, the
+ * pages of every sequence in order and -1 behind them; lengths [sequences], the tokens each has; free_pages [pages], of which
+ * the first left[0] belong to nobody.  All int32; the calls change them in place.
+ * extend: new_tokens[s] more tokens for every sequence (below 0: none).  With ends the running sum of new_tokens and
+ * need_s = ceil((lengths[s] + new) / page_size) - ceil(lengths[s] / page_size), sequence s is granted if its row and max_tokens
+ * suffice and need_s is 0 or no more than left[0] together with those before it; else it stays as it is and needs
+ * nothing (but where only pages are missing, its need counts for those behind it).  New page i of the call is
+ * free_pages[left[0] - 1 - i].  Out: query_starts [sequences + 1], the ends from 0 on, at most max_tokens; positions [max_tokens];
+ * slots [max_tokens], page * page_size + token in the page, -1 where not granted; both 0 and -1 behind the last token; granted
+ * [sequences], 0 or 1.  workspace: sequences + 1 words.
+ * truncate: lengths[s] = min(lengths[s], max(keep[s], 0)); the pages behind go back to the end of the list, the last sequence's
+ * last page first, so that it undoes an extend.
+ */
+int neox_pages_extend(int32_t* query_starts, int32_t* positions, int64_t* slots, uint8_t* granted, int32_t* workspace,
+                      int32_t* page_table, int32_t* lengths, int32_t* free_pages, int32_t* left, const int32_t* new_tokens,
+                      int32_t sequences, int32_t columns, int64_t table_stride, int32_t pages, int32_t page_size,
+                      int32_t max_tokens, void* stream);
+int neox_pages_truncate(int32_t* page_table, int32_t* lengths, int32_t* free_pages, int32_t* left, const int32_t* keep,
+                        int32_t sequences, int32_t columns, int64_t table_stride, int32_t pages, int32_t page_size, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,439 @@
+"""The paged cache in 4 bits (values bit by bit) and attention over it against the 64-bit oracle."""
+import math
+
+import pytest
+import torch
+
+from gpt_neox_amd import _lib
+from gpt_neox_amd.paged_cache import PagedKVCache, paged_attention, slots_of
+from oracle import attention as A
+from oracle import pages as P
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+F4, E8 = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+
+
+def gen(device, seed):
+    return torch.Generator(device=device).manual_seed(seed)
+
+
+def normal(shape, dtype, device, seed, times=1.0):
+    return (torch.randn(shape, generator=gen(device, seed), device=device) * times).to(dtype)
+
+
+def flat(t):
+    """[pages, page_size, ...] -> bytes [slots, ...]"""
+    return t.view(torch.uint8).reshape(-1, *t.shape[2:])
+
+
+def same(a, b):
+    """equal numbers (zeros of either sign), NaN where NaN"""
+    return torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0))
+
+
+# ---- the cache ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,heads,d,page", [(1, 1, 32, 1), (5, 3, 64, 4), (37, 2, 96, 16), (100, 5, 128, 48), (300, 8, 128, 64), (33, 2, 256, 7), (29, 3, 160, 16),
+                                                 (41, 1, 192, 8), (7, 2, 224, 8)])
+def test_values_and_scales_bit_by_bit(device, dtype, tokens, heads, d, page):
+    pages = tokens // page + 3
+    cache = PagedKVCache.allocate(pages, page, heads, d, F4, device)
+    assert cache.dim == d and cache.k.shape == (pages, page, heads, d // 2) and cache.k_scale.shape == (pages, page, heads, d // 32)
+    k, v = normal((tokens, heads, d), dtype, device, 1, 3.0), normal((tokens, heads, d), dtype, device, 2)
+    slots = torch.randperm(pages * page, generator=gen(device, 3), device=device)[:tokens]
+    cache.write(k, v, slots)
+    for x, held, scales in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        want, scale = P.encode(x)
+        assert torch.equal(flat(scales)[slots], scale)
+        assert same(P.decode(flat(held)[slots], flat(scales)[slots]), want)
+    others = torch.ones(pages * page, dtype=torch.bool, device=device)
+    others[slots] = False
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        assert (flat(t)[others] == 0).all()
+    for out in DTYPES:  # and back, rounded once
+        rk, rv = cache.read(slots, out)
+        for x, got in ((k, rk), (v, rv)):
+            assert got.shape == x.shape and same(got, P.encode(x)[0].to(out))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ties_and_extremes(device, dtype):
+    top, tiny = torch.finfo(dtype).max, torch.finfo(dtype).tiny
+    least = 2.0**-133 if dtype == torch.bfloat16 else 2.0**-24
+    rows = [
+        torch.arange(32) * 0.25 - 1.0,                                   # ties among them, the largest 6.75: saturates
+        torch.arange(32) * -0.125 + 0.125,
+        torch.cat((torch.tensor([7.0]), torch.arange(31) * 0.25)),       # the largest that stays
+        torch.cat((torch.tensor([7.0625]), torch.arange(31) * 0.25)),    # and the first that does not
+        torch.zeros(32), torch.full((32,), top), torch.full((32,), -tiny), torch.arange(32) * least,
+        torch.tensor([top, tiny] * 16), torch.tensor([top, -top / 2] * 16), torch.full((32,), least), torch.arange(32) * least * 64,
+        -torch.arange(32) * 1e-3,
+    ]
+    x = torch.stack(rows).to(dtype).to(device)
+    x = torch.cat((x, x.flip(0)), -1)[:, None, :].contiguous()  # two scales to a row
+    cache = PagedKVCache.allocate(2, 8, 1, 64, F4, device)
+    slots = torch.arange(x.shape[0], device=device)
+    cache.write(x, -x, slots)
+    want, scale = P.encode(x)
+    assert torch.equal(flat(cache.k_scale)[slots], scale) and torch.equal(flat(cache.v_scale)[slots], scale)
+    assert same(P.decode(flat(cache.k)[slots], scale), want) and same(P.decode(flat(cache.v)[slots], scale), -want)
+    rk, rv = cache.read(slots, dtype)
+    assert torch.isfinite(rk).all() and same(rk, want.to(dtype)) and same(rv, -rk)
+
+
+def test_every_16_bit_value(device):
+    # each next to a seven that fixes the scale, at several sizes
+    for dtype in DTYPES:
+        x = torch.arange(65536, device=device, dtype=torch.int32).to(torch.int16).view(dtype)
+        x = x[torch.isfinite(x)]
+        x = torch.cat((x, x.new_zeros(-x.shape[0] % 31))).view(-1, 31)
+        for size in (7.0, 7.0 / 64, 7.0 * 64):
+            r = torch.cat((x.clamp(-size, size), torch.full_like(x[:, :1], size)), -1)[:, None, :].contiguous()
+            cache = PagedKVCache.allocate(r.shape[0], 1, 1, 32, F4, device)
+            slots = torch.arange(r.shape[0], device=device)
+            cache.write(r, r, slots)
+            rk, _ = cache.read(slots, dtype)
+            assert same(rk, P.encode(r)[0].to(dtype))
+
+
+@pytest.mark.parametrize("d", [32, 96, 128, 256])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_row_with_an_infinity_or_nan_reads_back_as_nan(device, bad, d):
+    cache = PagedKVCache.allocate(1, 8, 2, d, F4, device)
+    k, v = normal((8, 2, d), torch.bfloat16, device, 4), normal((8, 2, d), torch.bfloat16, device, 5)
+    k[3, 1, d - 15] = bad
+    cache.write(k, v, torch.arange(8, device=device))
+    rk, rv = cache.read(torch.arange(8, device=device))
+    assert torch.isnan(rk[3, 1]).all() and torch.isfinite(rv).all()
+    rk[3, 1] = 0
+    assert torch.isfinite(rk).all()
+
+
+@pytest.mark.parametrize("slot_type", [torch.int32, torch.int64])
+def test_slots_outside_the_cache(device, slot_type):
+    cache = PagedKVCache.allocate(4, 4, 2, 64, F4, device)
+    slots = torch.tensor([3, -1, 16, 0, -(2**31), 2**31 - 1, 15], dtype=slot_type, device=device)
+    k, v = normal((7, 2, 64), torch.bfloat16, device, 9), normal((7, 2, 64), torch.bfloat16, device, 10)
+    cache.write(k, v, slots)
+    inside = torch.tensor([0, 3, 6], device=device)
+    for t in cache.read(slots):
+        outside = torch.ones(7, dtype=torch.bool, device=device)
+        outside[inside] = False
+        assert (t[outside] == 0).all() and (t[inside] != 0).any(-1).all()
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        assert flat(t).ne(0).flatten(1).any(-1).nonzero().flatten().tolist() == [0, 3, 15]
+
+
+def test_strided_inputs_and_a_cache_for_all_layers(device):
+    layers, d = 3, 96
+    codes = [torch.zeros((6, layers, 8, 2, d // 2), dtype=torch.uint8, device=device).view(F4) for _ in "kv"]
+    scales = [torch.zeros((6, layers, 8, 2, d // 32), dtype=torch.uint8, device=device).view(E8) for _ in "kv"]
+    mixed = normal((20, 8, d), torch.float16, device, 11)  # q, k and v of a projection: 4 + 2 + 2 heads
+    slots = torch.randperm(48, generator=gen(device, 12), device=device)[:20]
+    want = [P.encode(x)[0].half() for x in (mixed[:, 4:6], mixed[:, 6:])]
+    for layer in range(layers):
+        cache = PagedKVCache(*(t[:, layer] for t in (*codes, *scales)))
+        cache.write(mixed[:, 4:6], mixed[:, 6:], slots)
+        for x, got in zip(want, cache.read(slots, torch.float16)):
+            assert same(got, x)
+    # an odd layout is copied first
+    odd = normal((d, 2, 20), torch.float16, device, 13).permute(2, 1, 0)
+    cache.write(odd, odd, slots)
+    assert same(cache.read(slots, torch.float16)[0], P.encode(odd)[0].half())
+
+
+def test_offsets_beyond_32_bits(device):
+    # pages 2^24 bytes apart, 300 of them: slots behind 2^32 bytes, scales too
+    size, step = 300 << 24, (1 << 24, 64, 32, 1)
+    codes = [torch.zeros(size, dtype=torch.uint8, device=device).as_strided((300, 16, 1, 32), step).view(F4) for _ in "kv"]
+    scales = [torch.zeros(size, dtype=torch.uint8, device=device).as_strided((300, 16, 1, 2), (1 << 24, 5, 3, 1)).view(E8) for _ in "kv"]
+    cache = PagedKVCache(*codes, *scales)
+    n = 2000
+    k, v = normal((n, 1, 64), torch.float16, device, 14), normal((n, 1, 64), torch.float16, device, 15)
+    table = torch.randperm(300, generator=gen(device, 16), device=device)[:126].view(1, 126).int()
+    table[0, 125] = 299
+    slots = slots_of(table, torch.zeros(n, device=device), torch.arange(n, device=device), 16)
+    cache.write(k, v, slots)
+    rk, rv = cache.read(slots, torch.float16)
+    assert same(rk, P.encode(k)[0].half()) and same(rv, P.encode(v)[0].half())
+    for new in (1, 40):
+        q = normal((new, 4, 64), torch.float16, device, 17)
+        starts = torch.tensor([0, new], dtype=torch.int32, device=device)
+        lengths = torch.tensor([n], dtype=torch.int32, device=device)
+        got = paged_attention(q, cache, table, starts, lengths, max_query=new)
+        want, bound = A.paged_attention(q, rk.view(125, 16, 1, 64), rv.view(125, 16, 1, 64), None, None,
+                                        torch.arange(125, device=device).view(1, 125), starts, lengths, dtype=torch.float16)
+        assert ((got.double() - want).abs() <= bound).all()
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------
+def sequences(device, dtype, new, context, h, h_kv, d, page, seed=20, size=1.0):
+    """A cache of garbage with the sequences' keys and values in pages of their own, in random order; its tables."""
+    b = len(new)
+    width = max(1, -(-max(context) // page)) + 1
+    pages = b * width + 2
+    order = torch.randperm(pages, generator=gen(device, seed), device=device)
+    table = order[: b * width].view(b, width).int()
+    cache = PagedKVCache.allocate(pages, page, h_kv, d, F4, device)
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):  # what no sequence has written is NaN ...
+        t.view(torch.uint8).fill_(255)
+    for s in range(b):
+        n = context[s]
+        if n:
+            k, v = normal((n, h_kv, d), dtype, device, seed + 2 * s + 1, size), normal((n, h_kv, d), dtype, device, seed + 2 * s + 2, size)
+            at = torch.arange(n, device=device)
+            cache.write(k, v, slots_of(table, torch.full((n,), s, device=device), at, page))
+        used = -(-n // page)  # ... and table entries behind a sequence's end name no page
+        table[s, used:] = torch.tensor([-1, 2**31 - 1], dtype=torch.int32, device=device).repeat(width)[: width - used]
+    starts = torch.tensor([sum(new[:s]) for s in range(b + 1)], dtype=torch.int32, device=device)
+    lengths = torch.tensor(context, dtype=torch.int32, device=device)
+    q = normal((sum(new), h, d), dtype, device, seed + 99, 1.5)
+    return q, cache, table, starts, lengths
+
+
+def oracle(q, cache, table, starts, lengths, **kw):
+    held = [P.decode(c.view(torch.uint8), s.view(torch.uint8)) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale))]
+    return A.paged_attention(q, *held, None, None, table.clamp(0, cache.pages - 1), starts, lengths, dtype=q.dtype, **kw)
+
+
+def check(q, cache, table, starts, lengths, max_query=None, max_context=None, **kw):
+    max_query = max_query or max(1, int((starts[1:] - starts[:-1]).max()))
+    got = paged_attention(q, cache, table, starts, lengths, max_query=max_query, max_context=max_context, **kw)
+    want, bound = oracle(q, cache, table, starts, lengths, **kw)
+    assert torch.isfinite(got).all()
+    err = (got.double() - want).abs()
+    assert (err <= bound).all(), (err.max().item(), (err / bound.clamp(min=1e-30)).max().item())
+    return got
+
+
+DIMS = [32, 64, 96, 128, 160, 192, 256]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", DIMS)
+def test_single_tokens(device, dtype, d):
+    check(*sequences(device, dtype, [1, 1, 1, 1, 1], [1, 2, 33, 400, 64], 4, 2, d, 16))
+    check(*sequences(device, dtype, [1, 1], [700, 129], 8, 1, d, 64))
+    check(*sequences(device, dtype, [1, 1], [700, 129], 8, 1, d, 48), window=100, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", DIMS)
+def test_chunks(device, dtype, d):
+    check(*sequences(device, dtype, [40, 1, 17], [40, 300, 90], 4, 2, d, 16))
+    check(*sequences(device, dtype, [70, 33], [500, 129], 8, 1, d, 48), window=100, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [2.0**-14, 2.0**-9, 2.0**7])
+def test_small_and_large_values(device, dtype, size):
+    # in fp16 the smallest of these values and most of their products with probabilities are subnormal
+    for new in ([1, 1], [33, 10]):
+        q, *rest = sequences(device, dtype, new, [300, 777], 4, 2, 64, 16, size=size)
+        check(q, *rest, scale=0.125 / size)
+
+
+def test_fp16_queries_over_values_beyond_fp16(device):
+    # written in bf16: keys and values from 2^-60 to 2^40, far outside what fp16 holds, the results inside
+    for new in (1, 40):
+        cache = PagedKVCache.allocate(20, 16, 2, 64, F4, device)
+        k, v = normal((300, 2, 64), torch.bfloat16, device, 31, 2.0**40), normal((300, 2, 64), torch.bfloat16, device, 32, 2.0**-10)
+        table = torch.randperm(20, generator=gen(device, 33), device=device)[:19].view(1, 19).int()
+        cache.write(k, v, slots_of(table, torch.zeros(300, device=device), torch.arange(300, device=device), 16))
+        q = normal((new, 8, 64), torch.float16, device, 34)
+        starts, lengths = torch.tensor([0, new], dtype=torch.int32, device=device), torch.tensor([300], dtype=torch.int32, device=device)
+        check(q, cache, table, starts, lengths, scale=2.0**-43)
+
+
+@pytest.mark.parametrize("page", [1, 3, 16, 31, 32, 64, 100, 256])
+def test_page_sizes(device, page):
+    for new in ([1, 1], [50, 20]):
+        for d in (64, 128):
+            check(*sequences(device, torch.bfloat16, new, [321, 64], 4, 2, d, page))
+
+
+@pytest.mark.parametrize("h,h_kv,new", [(1, 1, 1), (16, 1, 1), (17, 1, 1), (5, 1, 3), (6, 2, 5), (3, 1, 6), (64, 2, 1), (12, 12, 16), (12, 12, 17), (40, 1, 9)])
+def test_rows_around_the_change_of_kernels(device, h, h_kv, new):
+    check(*sequences(device, torch.float16, [new, max(1, new - 1)], [new, 777], h, h_kv, 64, 16))
+    check(*sequences(device, torch.bfloat16, [new, max(1, new - 1)], [new, 777], h, h_kv, 128, 32))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,context", [([1], [20001]), ([1, 1], [9000, 100]), ([30], [12345]), ([200, 3], [6000, 5000])])
+def test_long_sequences_are_split(device, dtype, new, context):
+    args = sequences(device, dtype, new, context, 4, 2, 64, 64)
+    got = check(*args)
+    assert torch.equal(got, check(*args))  # the same bits again
+    check(*args, window=3000, sinks=5)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (0, 2), (15, 0), (16, 40), (500, 700), (None, 9), (2**31 - 1, 2**31 - 1)])
+def test_windows_and_sinks(device, window, sinks):
+    for new in ([1, 1, 1], [20, 45, 1]):
+        check(*sequences(device, torch.bfloat16, new, [600, 45, 31], 4, 2, 64, 16), window=window, sinks=sinks)
+
+
+def test_sequences_without_tokens_or_keys(device):
+    got = check(*sequences(device, torch.bfloat16, [1, 0, 1, 0], [5, 7, 0, 0], 4, 2, 64, 16))
+    assert (got[1] == 0).all()
+    got = check(*sequences(device, torch.bfloat16, [30, 0, 20], [10, 7, 0], 4, 2, 64, 16))  # more tokens than keys
+    assert (got[:20] == 0).all() and (got[20:30] != 0).any() and (got[30:] == 0).all()
+
+
+@pytest.mark.parametrize("scale", [-0.4, 0.0, 2.0])
+def test_scales(device, scale):
+    for dtype in DTYPES:
+        for new in ([1, 1], [33, 10]):
+            check(*sequences(device, dtype, new, [100, 333], 4, 2, 64, 16), scale=scale)
+
+
+def test_bounds_larger_than_the_lengths(device):
+    args = sequences(device, torch.bfloat16, [3, 1], [300, 77], 4, 2, 64, 16)
+    for max_query, max_context in ((3, 300), (3, 301), (4, 5000), (60, None)):  # other kernels and numbers of parts
+        check(*args, max_query=max_query, max_context=max_context)
+
+
+def test_layouts(device):
+    q, cache, table, starts, lengths = sequences(device, torch.float16, [3, 40], [50, 222], 4, 2, 64, 16)
+    want = check(q, cache, table, starts, lengths)
+    wide = torch.zeros((43, 9, 64), dtype=torch.float16, device=device)
+    wide[:, 1:5] = q
+    assert torch.equal(check(wide[:, 1:5], cache, table, starts, lengths), want)
+    spread = torch.full((table.shape[0], table.shape[1] * 2), -1, dtype=torch.int32, device=device)
+    spread[:, ::2] = table
+    assert torch.equal(check(q, cache, spread[:, ::2], starts, lengths), want)
+    # rows of codes and of scales apart from one another
+    codes = [torch.full((cache.pages, 16, 3, 64), 255, dtype=torch.uint8, device=device) for _ in "kv"]
+    scales = [torch.full((cache.pages, 16, 3, 5), 255, dtype=torch.uint8, device=device) for _ in "kv"]
+    for to, t in zip((*codes, *scales), (cache.k, cache.v, cache.k_scale, cache.v_scale)):
+        to[:, :, :2, 16 * (to.shape[3] == 64) : 16 * (to.shape[3] == 64) + t.shape[3]] = t.view(torch.uint8)
+    apart = PagedKVCache(*(c[:, :, :2, 16:48].view(F4) for c in codes), *(c[:, :, :2, :2].view(E8) for c in scales))
+    assert torch.equal(check(q, apart, table, starts, lengths), want)
+
+
+def test_tables_that_point_outside_are_kept_inside(device):
+    q, cache, table, starts, lengths = sequences(device, torch.bfloat16, [1, 30], [60, 90], 4, 2, 64, 16)
+    for broken_starts, broken_lengths in ((starts, lengths + 100000), (starts, lengths * -1), (starts * 1000, lengths), (starts.flip(0), lengths)):
+        for max_query in (1, 30):
+            paged_attention(q, cache, table, broken_starts, broken_lengths, max_query=max_query)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_key_that_is_nan_is_not_seen_through_the_mask(device, dtype, d):
+    for new in ([1, 40], [3, 2]):
+        q, cache, table, starts, lengths = sequences(device, dtype, new, [100, 140], 4, 2, d, 16)
+        want = paged_attention(q, cache, table, starts, lengths, max_query=40, window=20)
+        first = [100 - new[0] - 21, 140 - new[1] - 21]  # the last key that no row of the sequence sees
+        for s, j in enumerate(first):
+            for t in (cache.k_scale, cache.v_scale):  # one of the row's scales
+                t.view(torch.uint8)[table[s, j // 16].long(), j % 16, :, d // 32 - 1] = 255
+        assert torch.equal(paged_attention(q, cache, table, starts, lengths, max_query=40, window=20), want)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,d", [(4, 64), (4, 128), (40, 64), (40, 96), (40, 256)])
+def test_a_nan_reaches_the_rows_that_see_it_and_no_others(device, dtype, which, new, d):
+    q, cache, table, starts, lengths = sequences(device, dtype, [new], [200], 4, 2, d, 16)
+    want = paged_attention(q, cache, table, starts, lengths, max_query=new)
+    j = 200 - 3  # the last three tokens see it; the first of two heads' keys
+    t = cache.k_scale if which == "k" else cache.v_scale
+    t.view(torch.uint8)[table[0, j // 16].long(), j % 16, 0, 0] = 255
+    got = paged_attention(q, cache, table, starts, lengths, max_query=new)
+    assert torch.isnan(got[-3:, :2]).all()
+    assert torch.equal(got[:-3], want[:-3]) and torch.equal(got[:, 2:], want[:, 2:])
+
+
+def test_in_a_graph(device):
+    q, cache, table, starts, lengths = sequences(device, torch.bfloat16, [1, 1], [3000, 900], 8, 2, 128, 64)
+    k, v = normal((2, 2, 128), torch.bfloat16, device, 50), normal((2, 2, 128), torch.bfloat16, device, 51)
+    slots = torch.tensor([-1, -1], device=device)
+
+    def step():
+        cache.write(k, v, slots)
+        return paged_attention(q, cache, table, starts, lengths, max_query=1, max_context=4096), *cache.read(slots)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):  # the lengths and the query change between the replays
+        lengths.copy_(torch.tensor([3000 - 500 * i, 900 - 200 * i], dtype=torch.int32))
+        q.copy_(normal(q.shape, q.dtype, device, 60 + i))
+        slots.copy_(slots_of(table, torch.arange(2, device=device), lengths - 1, 64))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, step()):
+            assert torch.equal(x, y)
+
+
+def test_on_another_stream(device):
+    args = sequences(device, torch.bfloat16, [1, 1], [3000, 900], 8, 2, 128, 64)
+    want = paged_attention(*args, max_query=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = paged_attention(*args, max_query=1)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_without_the_native_calls_the_same_bits(device, monkeypatch):
+    def everything():
+        q, cache, table, starts, lengths = sequences(device, torch.float16, [1, 30], [3000, 900], 8, 2, 128, 64)
+        return (paged_attention(q, cache, table, starts, lengths, max_query=30, window=700, sinks=2),
+                paged_attention(q[:1], cache, table[:1], starts[:2], lengths[:1], max_query=1, max_context=3000),
+                *cache.read(torch.arange(60, device=device), torch.float16))
+
+    want = everything()
+    monkeypatch.setattr(_lib, "calls", lambda *tensors: None)
+    for x, y in zip(want, everything()):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+
+
+def test_no_tokens_at_all(device):
+    q, cache, table, starts, lengths = sequences(device, torch.bfloat16, [1], [10], 4, 2, 64, 16)
+    assert paged_attention(q[:0], cache, table, starts * 0, lengths, max_query=1).shape == (0, 4, 64)
+    none = torch.empty((0, 2, 64), dtype=torch.bfloat16, device=device)
+    cache.write(none, none, torch.empty(0, dtype=torch.int64, device=device))
+    assert cache.read(torch.empty(0, dtype=torch.int64, device=device))[0].shape == (0, 2, 64)
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+def test_refusals(device):
+    def codes(*shape):
+        return torch.zeros(shape, dtype=torch.uint8, device=device).view(F4)
+
+    def scales(*shape):
+        return torch.zeros(shape, dtype=torch.uint8, device=device).view(E8)
+
+    k, s = codes(4, 16, 2, 32), scales(4, 16, 2, 2)
+    for args, message in (
+        ((k, k), "needs k_scale"), ((k, k, s, s[:2]), "scales must be"), ((k, k, s, s.view(torch.uint8)), "scales must be float8_e8m0fnu"),
+        ((k, k, torch.zeros((4, 16, 2), device=device), s), "scales must be"), ((k[..., :24], k[..., :24], s, s), "head dim 48 must be a multiple of 32"),
+        ((codes(4, 16, 2, 144), codes(4, 16, 2, 144), scales(4, 16, 2, 9), scales(4, 16, 2, 9)), "head dim 288"), ((k[..., 8:24], k[..., 8:24], s[..., :1], s[..., :1]), "16-byte boundary"),
+        ((k, k, scales(4, 16, 2, 4)[..., ::2], s), "must be dense"), ((k, k, s.cpu(), s), "GPU"),
+    ):
+        with pytest.raises(RuntimeError, match=message):
+            PagedKVCache(*args)
+    cache = PagedKVCache(k, codes(4, 16, 2, 32), s, scales(4, 16, 2, 2))
+    x = torch.zeros((3, 2, 64), dtype=torch.bfloat16, device=device)
+    slots = torch.arange(3, device=device)
+    for call, message in (
+        (lambda: cache.write(x[..., :32], x[..., :32], slots), "shape"), (lambda: cache.write(x.float(), x.float(), slots), "fp16 and bf16"),
+        (lambda: cache.read(slots, torch.float32), "fp16 and bf16"), (lambda: cache.write(x.cpu(), x.cpu(), slots), "GPU"),
+    ):
+        with pytest.raises(RuntimeError, match=message):
+            call()
+    table = torch.zeros((2, 3), dtype=torch.int32, device=device)
+    starts, lengths = torch.tensor([0, 1, 2], dtype=torch.int32, device=device), torch.tensor([5, 6], dtype=torch.int32, device=device)
+    q = torch.zeros((2, 4, 32), dtype=torch.bfloat16, device=device)
+    with pytest.raises(RuntimeError, match="head dim 32, the cache 64"):
+        paged_attention(q, cache, table, starts, lengths, max_query=1)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        paged_attention(q.clone().requires_grad_(), cache, table, starts, lengths, max_query=1)
