@@ -41,13 +41,15 @@ static void cache_source(const CacheArgs& a, int source, hipStream_t stream) {
 }
 template <typename T, bool WRITE>
 static void cache4_rows(const CacheArgs& a, hipStream_t stream) {
-    const int lanes = a.d <= 32 ? 2 : a.d <= 64 ? 4 : a.d <= 128 ? 8 : 16;
+    constexpr int kElems = cache4_elems<WRITE>();
+    const int lanes = a.d <= kElems * 2 ? 2 : a.d <= kElems * 4 ? 4 : a.d <= kElems * 8 ? 8 : a.d <= kElems * 16 ? 16 : 32;
     const uint32_t blocks = (uint32_t)((a.rows * lanes + 255) / 256);
     switch (lanes) {
-        case 2: cache4_kernel<T, 2, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        case 2: if constexpr (WRITE) cache4_kernel<T, 2, WRITE><<<blocks, 256, 0, stream>>>(a); break;  // (32 dims)
         case 4: cache4_kernel<T, 4, WRITE><<<blocks, 256, 0, stream>>>(a); break;
         case 8: cache4_kernel<T, 8, WRITE><<<blocks, 256, 0, stream>>>(a); break;
-        default: cache4_kernel<T, 16, WRITE><<<blocks, 256, 0, stream>>>(a);
+        case 16: cache4_kernel<T, 16, WRITE><<<blocks, 256, 0, stream>>>(a); break;
+        default: if constexpr (!WRITE) cache4_kernel<T, 32, WRITE><<<blocks, 256, 0, stream>>>(a);  // (above 128)
     }
 }
 hipError_t launch_cache(const CacheArgs& a, int source, int dtype, bool write, hipStream_t stream) {
@@ -245,11 +247,18 @@ static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, i
     int64_t splits = (target + units - 1) / units;
     const int64_t most = (keys + 255) / 256;
     if (splits > most) splits = most;
-    if (splits > 128) splits = 128;
+    if (splits > kMostParts) splits = kMostParts;
     if (splits < 1) splits = 1;
     p.splits = (int)splits;
     p.bytes = splits > 1 ? splits * tokens * h * (d + 1) * (int64_t)sizeof(float) : 0;
     return p;
+}
+
+// Key heads to a wave of the single tokens over 4 bits: two, where a row's scales are fetched at once, their rows fit the columns
+// and half the workgroups are two to a CU.
+static int token4_heads(const AttnArgs& a) {
+    const bool two = token4_fetch(a, padded(a.d)) == kFetchRows && a.d <= 128 && a.kv % 2 == 0 && 2 * a.sq * a.group <= 16;
+    return two && (int64_t)a.b * a.kv * a.splits >= 1024 ? 2 : 1;
 }
 
 static int check_paged_sizes(int b, int tokens, int max_query, int max_context, int h, int h_kv, int d, const char* what) {
@@ -542,6 +551,7 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
         page_strides(a.ks_st, k_scale_strides);
         page_strides(a.vs_st, v_scale_strides);
     }
+    if (plan.token && source == kPagedF4) a.heads = token4_heads(a);
     hipStream_t s = (hipStream_t)stream;
     NEOX_TRY(check_launch(plan.token ? run_token(a, source, dtype, s) : run_fwd(a, source, dtype, s), what));
     return a.splits > 1 ? check_launch(launch_attn_join(a, dtype, s), what) : (int)NEOX_OK;

@@ -69,6 +69,7 @@ struct AttnArgs {
     float* part_o;               //   [split][row slot][d] and
     float* part_lse;             //   [split][row slot], row slot = (token * kv + key head) * group + head in the group
     int64_t part_rows;           //   row slots of one split
+    int heads;                   // 4-bit pages, single tokens: key heads of a wave
     FastDiv by_group, by_page, by_row_tiles, by_kv, by_splits;
     // backward
     const char *dout;            // [token, sample, head] like q
@@ -320,8 +321,10 @@ __device__ __forceinline__ u32x4 widen4(uint32_t word, float scale) {
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 3))};
     }
 }
-// what the byte of a 4-bit scale stands for (0 instead of 2^-127), as the kernels multiply by it
-constexpr uint32_t kScaleNan = 255;
+// what the byte of a 4-bit scale stands for (0 instead of 2^-127), as the kernels multiply by it; what is above the largest that
+// is ever written, six times which is a number, counts as NaN: infinities would reach other rows through probabilities of zero
+constexpr uint32_t kScaleNan = 255, kScaleMost = 127 + 125;
+__device__ __forceinline__ uint32_t known_scale(uint32_t byte) { return byte > kScaleMost ? kScaleNan : byte; }
 __device__ __forceinline__ float scale_bits(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 __device__ __forceinline__ float nan_value() { return __builtin_bit_cast(float, 0x7fc00000u); }
 
@@ -485,7 +488,7 @@ struct Stage4 {
         for (int s = 0; s < kSteps; ++s) {
             u32x4 c = codes[s];
             asm("" : "+v"(c.x), "+v"(c.y), "+v"(c.z), "+v"(c.w));
-            uint32_t e = scale[s];
+            uint32_t e = known_scale(scale[s]);
             if constexpr (kKeyScales) {
                 const uint32_t top = group_largest<kLanes>(e);
                 e = (uint32_t)max((int)(e + 127 - top), 0);
@@ -1262,19 +1265,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token_kernel(Attn
     }
 }
 
+constexpr int kMostParts = 128;
+
 // Joins the parts of a split key axis: a workgroup per row, 64 threads for the dims (four each), four groups of them for
 // every fourth part.  O = sum_s 2^(lse_s - m) O_s / sum_s 2^(lse_s - m), m the largest lse.  Latency: 3 to 6 us for 16 to
 // 4096 rows, the launch among them.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 sums[4][64];
-    __shared__ float weights[128];
+    __shared__ float weights[kMostParts];
     const int64_t slot = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, dim = lane * 4;
-    // every wave reduces the parts' logarithms by itself: at most 128 of them
-    float lse[2], high = kNegInf;
+    // every wave reduces the parts' logarithms by itself: at most kMostParts of them
+    float lse[kMostParts / 64], high = kNegInf;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kMostParts / 64; ++i) {
         const int s = i * 64 + lane;
         lse[i] = s < a.splits ? a.part_lse[s * a.part_rows + slot] : kNegInf;
         high = fmaxf(high, lse[i]);
@@ -1283,7 +1288,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const float base = high == kNegInf ? 0.f : high;
     float total = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kMostParts / 64; ++i) {
         const float f = __builtin_amdgcn_exp2f(lse[i] - base);
         total += f;
         if (wave == 0) weights[i * 64 + lane] = f;
@@ -1293,7 +1298,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     if (dim < a.d) {
         const float* from = a.part_o + slot * a.d + dim;
-#pragma unroll 4
+#pragma unroll 8
         for (int s = wave; s < a.splits; s += 4) sum += *reinterpret_cast<const f32x4*>(from + s * a.part_rows * a.d) * weights[s];
     }
     sums[wave][lane] = sum;

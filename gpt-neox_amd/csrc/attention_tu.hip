@@ -26,7 +26,24 @@ static void token(const AttnArgs& a, int source, hipStream_t stream) {
         case kPaged16: attn_token_kernel<T, DP, kPaged16, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedI8: attn_token_kernel<T, DP, kPagedI8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedF8: attn_token_kernel<T, DP, kPagedF8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
-        case kPagedF4: attn_token4_kernel<T, DP, SPLIT><<<grid, 256, 0, stream>>>(a); break;
+        case kPagedF4: break;  // (token4)
+    }
+}
+
+template <typename T, bool SPLIT>
+static void token4(AttnArgs a, hipStream_t stream) {
+    constexpr int DP = NEOX_ATTN_DIM;
+    const int fetch = token4_fetch(a, DP), groups = a.kv / a.heads;
+    a.by_kv = FastDiv::by((uint32_t)groups);
+    const uint32_t grid = ((uint32_t)a.b * a.splits + 7) / 8 * 8 * groups;
+    if (fetch == kFetchOwn) {
+        attn_token4_kernel<T, DP, 1, SPLIT, kFetchOwn><<<grid, 256, 0, stream>>>(a);
+    } else if (fetch == kFetchHalves) {
+        if constexpr (DP != 96) attn_token4_kernel<T, DP, 1, SPLIT, kFetchHalves><<<grid, 256, 0, stream>>>(a);  // (96: always rows)
+    } else if (a.heads == 1) {
+        attn_token4_kernel<T, DP, 1, SPLIT, kFetchRows><<<grid, 256, 0, stream>>>(a);
+    } else {
+        if constexpr (DP <= 128) attn_token4_kernel<T, DP, 2, SPLIT, kFetchRows><<<grid, 256, 0, stream>>>(a);
     }
 }
 
@@ -39,6 +56,11 @@ hipError_t launch_attn_fwd<NEOX_ATTN_DIM>(const AttnArgs& a, int source, int dty
 
 template <>
 hipError_t launch_attn_token<NEOX_ATTN_DIM>(const AttnArgs& a, int source, int dtype, hipStream_t stream) {
+    if (source == kPagedF4) {
+        if (dtype == NEOX_BF16) a.splits > 1 ? token4<BF16, true>(a, stream) : token4<BF16, false>(a, stream);
+        else a.splits > 1 ? token4<F16, true>(a, stream) : token4<F16, false>(a, stream);
+        return hipGetLastError();
+    }
     if (dtype == NEOX_BF16) a.splits > 1 ? token<BF16, true>(a, source, stream) : token<BF16, false>(a, source, stream);
     else a.splits > 1 ? token<F16, true>(a, source, stream) : token<F16, false>(a, source, stream);
     return hipGetLastError();

@@ -31,7 +31,8 @@ class PagedKVCache:
     Values in 4 bits are 0, 0.5, 1, 1.5, 2, 3, 4 or 6 times a power of two, with a sign.  ``write`` takes the least power of
     which seven times is no less than the 32 values' largest magnitude, from 2^-125 up to 2^125 (bf16) or 2^13 (fp16), and rounds to
     the nearest of these, to the even code at ties; what is above six times the power becomes six times.  A token's
-    head that holds an infinity or a NaN gets NaN scales and reads back as NaN, as in 8 bits.
+    head that holds an infinity or a NaN gets NaN scales and reads back as NaN, as in 8 bits.  (In a cache filled otherwise, scales above
+    2^125 count as NaN, and values whose scale is below 2^-125 may count as zero.)
 
     The tensors may be views (of one buffer for all layers, say) as long as every head's values are dense and start on
     16-byte boundaries.  They are looked at once, here, and stay: other tensors are another cache.

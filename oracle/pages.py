@@ -39,7 +39,9 @@ def encode(x):
 
 
 def decode(codes, scales):
-    """Bytes ``[..., d / 2]`` and ``[..., d / 32]`` -> float64 ``[..., d]``; a row with a NaN scale is NaN."""
+    """Bytes ``[..., d / 2]`` and ``[..., d / 32]`` -> float64 ``[..., d]``; a row with a NaN scale is NaN,
+    and so is one with a scale above the largest that is ever written."""
+    scales = torch.where(scales > 127 + MOST[torch.bfloat16], NAN, scales)
     table = torch.tensor(VALUES + tuple(-v for v in VALUES), dtype=torch.float64, device=codes.device)
     x = table[torch.stack((codes & 15, codes >> 4), -1).flatten(-2).long()]
     f = torch.exp2(scales.double() - 127).masked_fill(scales == NAN, float("nan")).repeat_interleave(GROUP, -1)

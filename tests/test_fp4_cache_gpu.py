@@ -348,6 +348,49 @@ def test_a_nan_reaches_the_rows_that_see_it_and_no_others(device, dtype, which, 
     assert torch.equal(got[:-3], want[:-3]) and torch.equal(got[:, 2:], want[:, 2:])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("b,h,h_kv,new,context", [(64, 32, 16, 1, 45), (16, 16, 16, 3, 1000), (8, 64, 8, 1, 4300), (128, 12, 4, 2, 600)])
+def test_many_heads(device, dtype, d, b, h, h_kv, new, context):
+    # from 1024 units of work on, two neighbouring heads go together
+    lengths = [max(new, context - 7 * i * context // (8 * b)) for i in range(b)]
+    args = sequences(device, dtype, [new] * b, lengths, h, h_kv, d, 16 if d == 64 else 48)
+    got = check(*args)
+    assert torch.equal(got, check(*args))
+    check(*args, window=70, sinks=2, max_context=context)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [255, 253])  # (a scale that large counts as NaN)
+def test_a_nan_stays_with_its_head(device, dtype, which, bad):
+    for d, h_kv in ((128, 16), (64, 2)):
+        q, cache, table, starts, lengths = sequences(device, dtype, [1] * 16, [1000] * 16, 2 * h_kv, h_kv, d, 32)
+        want = paged_attention(q, cache, table, starts, lengths, max_query=1)
+        t = (cache.k_scale if which == "k" else cache.v_scale).view(torch.uint8)
+        t[table[3, 17].long(), 5, 1, d // 32 - 1] = bad
+        got = paged_attention(q, cache, table, starts, lengths, max_query=1)
+        hit = torch.zeros(got.shape[:2], dtype=torch.bool, device=device)
+        hit[3, 2:4] = True
+        if which == "k":
+            assert torch.isnan(got[hit]).all()
+        else:
+            assert torch.isnan(got[hit]).any()
+        assert torch.equal(got[~hit], want[~hit])
+
+
+def test_scales_that_are_not_aligned(device):
+    # their rows cannot be fetched as words
+    for d in (64, 128, 256):
+        q, cache, table, starts, lengths = sequences(device, torch.bfloat16, [1] * 4, [300] * 4, 4, 4, d, 32)
+        want = check(q, cache, table, starts, lengths)
+        odd = [torch.empty(t.numel() + 1, dtype=torch.uint8, device=device)[1:].view(t.shape) for t in (cache.k_scale, cache.v_scale)]
+        for to, t in zip(odd, (cache.k_scale, cache.v_scale)):
+            to.copy_(t.view(torch.uint8))
+        apart = PagedKVCache(cache.k, cache.v, *(t.view(E8) for t in odd))
+        assert torch.equal(check(q, apart, table, starts, lengths), want)
+
+
 def test_in_a_graph(device):
     q, cache, table, starts, lengths = sequences(device, torch.bfloat16, [1, 1], [3000, 900], 8, 2, 128, 64)
     k, v = normal((2, 2, 128), torch.bfloat16, device, 50), normal((2, 2, 128), torch.bfloat16, device, 51)
