@@ -1,6 +1,8 @@
 // extern "C" entry points of the attention kernels and of the paged cache: argument validation, the choice of the
 // kernel and of the parts of a split key axis, and the launches.  As in api.hip, validation finishes before the
 // first HIP call.
+#include <algorithm>
+
 #include "internal.hpp"
 
 namespace neox {
@@ -233,7 +235,22 @@ struct PagedPlan {
 // 132; 161, 127; 68, 78; 147, 173; 205, 232; 328, 355.  Single tokens: eight, twice what fits, because sequences differ in length and
 // the host does not know by how much: 64 sequences of 2048 to 8192 tokens, int8, take 191 us with four (170 before four fitted),
 // 158 with eight, 169 with sixteen; one of 131001 tokens in bf16 takes 125 us with 128 parts and 128 with 256.
-static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, int h, int h_kv, int d, int window, int sinks, bool codes) {
+//
+// Single tokens over 4 bits have less to read for each key, and parts cost them more: no more of them than that, one up to 640 keys; else a
+// workgroup to a CU, two where parts are longer than 640 keys then, eight where they are longer than 1024 (and a single one than
+// 2048), of 1024 keys at least.  us by parts, bf16, 128 dims, 8 key heads: 16 sequences of 517 tokens 1: 9.1, 2: 10.3, 4: 10.4; 64 of
+// 1000 1: 15.1, 2: 19.9, 4: 22.7; 64 of 2000 1: 24.4, 2: 27.9; 16 of 2000 2: 16.9, 4: 15.0, 8: 16.5, 16: 19.7; 1 of 4000 16: 10.8, 32: 9.3; 4 of
+// 2000 4: 12.0, 8: 10.4, 16: 11.9; 4 of 32000 16: 28.1, 32: 26.6, 64: 28.8; 64 of 8192 1: 116, 2: 98, 4: 88, 8: 88, 12: 95; 256 dims, fp16, 16 drafts of 5
+// tokens in a window of 1024 1: 27.3, 2: 23.7, 4: 24.9, 6: 32.0.
+static int parts_token4(int64_t units, int64_t keys, int64_t most) {
+    int64_t parts = std::min(most, (256 + units - 1) / units);
+    if (keys <= 640) parts = 1;
+    if (keys > 640 * parts) parts = std::min(most, (512 + units - 1) / units);
+    if (keys > (parts == 1 ? 2048 : 1024 * parts)) parts = std::min({most, (2048 + units - 1) / units, (keys + 1023) / 1024});
+    return (int)parts;
+}
+static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, int h, int h_kv, int d, int window, int sinks, int source) {
+    const bool codes = source != kPaged16;
     PagedPlan p{};
     const int64_t group = h / h_kv, rows = max_query * group;
     p.token = rows <= 16;
@@ -249,8 +266,8 @@ static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, i
     if (splits > most) splits = most;
     if (splits > kMostParts) splits = kMostParts;
     if (splits < 1) splits = 1;
-    p.splits = (int)splits;
-    p.bytes = splits > 1 ? splits * tokens * h * (d + 1) * (int64_t)sizeof(float) : 0;
+    p.splits = p.token && source == kPagedF4 ? parts_token4(units, keys, splits) : (int)splits;
+    p.bytes = p.splits > 1 ? (int64_t)p.splits * tokens * h * (d + 1) * (int64_t)sizeof(float) : 0;
     return p;
 }
 
@@ -477,7 +494,7 @@ int neox_paged_attention_workspace(int64_t* bytes, int32_t b, int32_t tokens, in
     if (!bytes) return fail(NEOX_ERR_NULL_POINTER, "%s: bytes is null", what);
     NEOX_TRY(check_paged_sizes(b, tokens, max_query, max_context, h, h_kv, d, what));
     NEOX_TRY(check_scale_window(1.f, sinks, what));
-    *bytes = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, false).bytes;  // (codes need no more)
+    *bytes = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, kPaged16).bytes;  // (codes need no more)
     return NEOX_OK;
 }
 
@@ -504,7 +521,7 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
         return fail(NEOX_ERR_BAD_SHAPE, "%s: page_table needs a column and no negative stride (%d, %lld)", what, table_columns, (long long)table_stride);
     NEOX_TRY(check_scale_window(scale, sinks, what));
     const int source = cache_source_of(cache_dtype, dtype);
-    const PagedPlan plan = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, source != kPaged16);
+    const PagedPlan plan = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, source);
     if (plan.bytes > 0) {
         NEOX_TRY(check_pointer(workspace, 16, what, "workspace"));
         if (workspace_bytes < plan.bytes)
