@@ -21,7 +21,7 @@ struct PoolArgs {
     FastDiv by_page;
 };
 
-constexpr int kPoolThreads = 1024;
+constexpr int kPoolThreads = 1024, kOwnTokens = 8;
 
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
@@ -74,6 +74,26 @@ __device__ __forceinline__ void place(const PoolArgs& a, uint32_t t, int s, uint
     a.slots[t] = slot;
 }
 
+// The tokens from t on of a sequence that has a few, no more than a page holds: its own thread's, whose two pages are fetched at once and which
+// searches nothing (1000 sequences, 5 tokens each: 6.5 us, by the search 7.5).
+__device__ __forceinline__ void place_own(const PoolArgs& a, uint32_t t, uint32_t count, int s, uint32_t old, uint32_t need, uint32_t first, bool granted,
+                                          int left) {
+    if (count == 0) return;
+    const uint32_t size = a.by_page.d, column = a.by_page.div(old), have = pages_of(a, old);
+    int32_t* const row = a.table + (int64_t)s * a.table_stride;
+    int32_t pages[2] = {-1, -1};  // of `column` and the next
+    if (granted) {
+        const bool begun = column < have;
+        if (begun) pages[0] = row[column];
+        if (need) row[column + begun] = pages[begun] = a.free[left - 1 - (int)first];  // (no more than one)
+    }
+    for (uint32_t i = 0, in = old - column * size; i < count; ++i, ++in) {
+        const bool next = in >= size;
+        a.positions[t + i] = (int32_t)(old + i);
+        a.slots[t + i] = granted ? (int64_t)pages[next] * size + (in - (next ? size : 0)) : -1;
+    }
+}
+
 // TOKENS: the tokens' places too; otherwise they are left to place_kernel.
 template <bool TOKENS>
 __global__ __launch_bounds__(kPoolThreads) void extend_kernel(PoolArgs a) {
@@ -105,7 +125,9 @@ __global__ __launch_bounds__(kPoolThreads) void extend_kernel(PoolArgs a) {
             if (granted && need) atomicMax(&taken, upto);
             if (!TOKENS) a.first[s] = (int32_t)first;
         }
-        if constexpr (TOKENS) {
+        if (TOKENS && !__syncthreads_or(count > kOwnTokens || kOwnTokens > a.by_page.d)) {
+            place_own(a, end - count, min(count, most - min(most, end - count)), s, old, need, first, granted, left);
+        } else if constexpr (TOKENS) {
             ends[threadIdx.x] = min(end, most);
             olds[threadIdx.x] = old;
             firsts[threadIdx.x] = granted ? first : ~0u;

@@ -528,19 +528,30 @@ bool pool_list(const Tensor& t, const Tensor& lengths) { return int_list(t, leng
 int64_t row_stride(const Tensor& table) { return table.size(0) > 1 ? table.stride(0) : 0; }
 int32_t* words(const Tensor& t) { return static_cast<int32_t*>(t.mutable_data_ptr()); }
 
+// `count` elements of `type`, `offset` of them behind the start of t's memory
+Tensor part_of(const Tensor& t, at::ScalarType type, int64_t offset, int64_t count) {
+    Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), c10::scalarTypeToTypeMeta(type));
+    part.unsafeGetTensorImpl()->set_sizes_contiguous({count});
+    part.unsafeGetTensorImpl()->set_storage_offset(offset);
+    return part;
+}
+
 // starts, positions, slots and whether granted, or None
 std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> pages_extend(const Tensor& table, const Tensor& lengths, const Tensor& free, const Tensor& left,
                                                                        const Tensor& tokens, int64_t page_size, int64_t max_tokens) {
     if (!pool_list(tokens, lengths) || max_tokens < 0 || max_tokens >= 1 << 30) return std::nullopt;
     const c10::DeviceGuard guard(table.device());
     const int64_t n = lengths.size(0);
-    // (one allocation for what has 32 bits, the workspace behind it)
-    const Tensor all = at::empty({2 * (n + 1) + max_tokens}, lengths.options());
-    Tensor starts = all.narrow(0, 0, n + 1), positions = all.narrow(0, n + 1, max_tokens);
-    Tensor slots = at::empty({max_tokens}, lengths.options().dtype(at::kLong)), granted = at::empty({n}, lengths.options().dtype(at::kBool));
-    check(neox_pages_extend(words(starts), words(positions), static_cast<int64_t*>(slots.mutable_data_ptr()), static_cast<uint8_t*>(granted.mutable_data_ptr()),
-                            words(all) + n + 1 + max_tokens, words(table), words(lengths), words(free), words(left), words(tokens), (int32_t)n,
-                            (int32_t)table.size(1), row_stride(table), (int32_t)free.size(0), (int32_t)page_size, (int32_t)max_tokens, stream_of(table)));
+    // one allocation: 64-bit words, 32-bit ones, the workspace, bytes (a launch of its own size costs less than three more of these calls)
+    const int64_t words64 = max_tokens, words32 = 2 * (n + 1) + max_tokens;
+    const Tensor all = at::empty({words64 + (words32 + 1) / 2 + (n + 7) / 8}, lengths.options().dtype(at::kLong));
+    auto* const base = static_cast<int64_t*>(all.mutable_data_ptr());
+    auto* const base32 = reinterpret_cast<int32_t*>(base + words64);
+    Tensor starts = part_of(all, at::kInt, 2 * words64, n + 1), positions = part_of(all, at::kInt, 2 * words64 + n + 1, max_tokens);
+    Tensor slots = part_of(all, at::kLong, 0, max_tokens), granted = part_of(all, at::kBool, 8 * (words64 + (words32 + 1) / 2), n);
+    check(neox_pages_extend(base32, base32 + n + 1, base, static_cast<uint8_t*>(granted.mutable_data_ptr()), base32 + n + 1 + max_tokens, words(table),
+                            words(lengths), words(free), words(left), words(tokens), (int32_t)n, (int32_t)table.size(1), row_stride(table),
+                            (int32_t)free.size(0), (int32_t)page_size, (int32_t)max_tokens, stream_of(table)));
     return std::make_tuple(starts, positions, slots, granted);
 }
 

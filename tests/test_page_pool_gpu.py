@@ -110,6 +110,32 @@ def test_more_than_a_workgroup_gives_back_at_once(device):
     assert pool.left.item() == 9000 and (pool.page_table == -1).all()
 
 
+@pytest.mark.parametrize("empty", [0, 1, 1023, 1024, 2500])
+def test_many_sequences_without_tokens(device, empty):
+    # between the sequences of a workgroup's tokens, and behind the last one
+    new = []
+    for n in (3, 1021, 1, 1024, 7000, 2, 900, 130):
+        new += [n] + [0] * empty
+    pool = PagePool.allocate(2600, 4, len(new), 1750, device)
+    want = twin(pool)
+    extend(pool, want, new)
+    extend(pool, want, [1] * len(new), max(8200, len(new) + 5))
+    truncate(pool, want, [3 * (i % 2) for i in range(len(new))])
+
+
+def test_outputs_do_not_share(device):
+    # writing into one output leaves the others and the pool
+    pool = PagePool.allocate(50, 16, 7, 10, device)
+    step = pool.extend(int32([5, 0, 17, 3, 1, 0, 9], device), max_tokens=41)
+    kept = [t.clone() for t in step]
+    for i, t in enumerate(step):
+        assert t.is_contiguous() and t.shape == kept[i].shape
+        t.fill_(1)
+        for j in range(i + 1, 4):
+            assert torch.equal(step[j], kept[j])
+    assert [t.dtype for t in step] == [torch.int32, torch.int32, torch.int64, torch.bool]
+
+
 def test_refusals(device):
     pool = PagePool.allocate(9, 16, 4, 3, device)
     new = int32([1] * 4, device)
