@@ -1,11 +1,11 @@
 """One attention layer with a sliding window and sinks: a training step, a prompt in chunks, and generation.
 
-    python examples/windowed_layer.py [--codes int8|fp8|16bit] [--window 256] [--sinks 4]
+    python examples/windowed_layer.py [--codes int8|fp8|fp4|16bit] [--window 256] [--sinks 4]
 
 The layer rotates q and k (``apply_rotary_pos_emb``), and attends with ``window_attention`` in training.  For serving
-it writes k and v into a ``PagedKVCache`` and attends with ``paged_attention``: the prompts of two sequences of
-different lengths in chunks, then one token of both at a time.  What generation gives is compared with the training
-path over the whole sequences; the difference is what the cache's 8-bit codes cost.
+a ``PagePool`` says where the new tokens go, k and v are written there into a ``PagedKVCache``, and ``paged_attention`` attends: the
+prompts of two sequences of different lengths in chunks, then one token of both at a time.  What generation gives is compared with the training
+path over the whole sequences; the difference is what the cache's codes cost.
 """
 import argparse
 import os
@@ -15,9 +15,9 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from gpt_neox_amd import PagedKVCache, RotaryEmbedding, apply_rotary_pos_emb, paged_attention, slots_of, window_attention  # noqa: E402
+from gpt_neox_amd import PagedKVCache, PagePool, RotaryEmbedding, apply_rotary_pos_emb, paged_attention, window_attention  # noqa: E402
 
-CODES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn, "16bit": torch.bfloat16}
+CODES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn, "fp4": torch.float4_e2m1fn_x2, "16bit": torch.bfloat16}
 
 
 class Layer(torch.nn.Module):
@@ -43,18 +43,16 @@ class Layer(torch.nn.Module):
         return self.dense(out.reshape(*x.shape))
 
     @torch.no_grad()
-    def step(self, x, positions, cache, table, lengths):
-        """New tokens of every sequence: ``x`` a list of ``[n, hidden]``, which stand at ``positions`` onwards; ``lengths``
-        (int32 ``[b]``) counts them too.  Returns a list like ``x``."""
+    def step(self, x, positions, cache, pool):
+        """New tokens of every sequence: ``x`` a list of ``[n, hidden]``, which stand at ``positions`` onwards.  Returns a list
+        like ``x``."""
         parts = [self.project(t[:, None], p) for t, p in zip(x, positions)]
         q, k, v = (torch.cat([part[i][:, 0] for part in parts]) for i in range(3))
         count = [t.shape[0] for t in x]
-        sample = torch.cat([torch.full((n,), s, device="cuda") for s, n in enumerate(count)])
-        position = torch.cat([torch.arange(p, p + n, device="cuda") for p, n in zip(positions, count)])
-        cache.write(k, v, slots_of(table, sample, position, cache.page_size))
-        starts = torch.tensor([sum(count[:s]) for s in range(len(count) + 1)], dtype=torch.int32, device="cuda")
-        out = paged_attention(q, cache, table, starts, lengths, max_query=max(count), max_context=max(p + n for p, n in zip(positions, count)),
-                              window=self.window, sinks=self.sinks)
+        places = pool.extend(torch.tensor(count, dtype=torch.int32, device="cuda"), max_tokens=sum(count))
+        cache.write(k, v, places.slots)
+        out = paged_attention(q, cache, pool.page_table, places.query_starts, pool.lengths, max_query=max(count),
+                              max_context=max(p + n for p, n in zip(positions, count)), window=self.window, sinks=self.sinks)
         return list(self.dense(out.view(out.shape[0], -1)).split(count))
 
 
@@ -83,19 +81,13 @@ def main(argv=None):
     # serving: the prompts in chunks of 200 tokens, then a token at a time
     pages = sum(-(-n // page) for n in lengths) + 1
     cache = PagedKVCache.allocate(pages, page, kv, hidden // heads, CODES[args.codes])
-    order = torch.randperm(pages - 1, device="cuda").int() + 1
-    table = torch.zeros((2, -(-max(lengths) // page)), dtype=torch.int32, device="cuda")
-    used = 0
-    for s, n in enumerate(lengths):
-        table[s, : -(-n // page)] = order[used : used + -(-n // page)]
-        used += -(-n // page)
+    pool = PagePool.allocate(pages, page, 2, -(-max(lengths) // page))
     got = [[], []]
     at = [0, 0]
     while at != lengths:
         count = [min(200, prompts[s] - at[s]) if at[s] < prompts[s] else min(1, lengths[s] - at[s]) for s in range(2)]
         new = [x[at[s] : at[s] + count[s], s] for s in range(2)]
-        total = torch.tensor([a + n for a, n in zip(at, count)], dtype=torch.int32, device="cuda")
-        for s, out in enumerate(layer.step(new, at, cache, table, total)):
+        for s, out in enumerate(layer.step(new, at, cache, pool)):
             got[s].append(out)
         at = [a + n for a, n in zip(at, count)]
     worst = 0.0

@@ -395,7 +395,8 @@ int neox_window_attention_bwd(void* dq, void* dk, void* dv, void* workspace, int
  * count bytes too, and need no alignment: byte s stands for 2^(s - 127), 255 for NaN.  A code's low three bits stand for 0, 0.5,
  * 1, 1.5, 2, 3, 4, 6, the fourth for the sign.  write takes the least power of two of which seven times is no less than the largest of
  * the 32 magnitudes, from 2^-125 to 2^125 (bf16; fp16: 2^13), and rounds to the nearest value, to the even code at ties, at
- * most to six times the power.  Where a scale of a row is NaN, attention takes the whole row for NaN.
+ * most to six times the power.  Where a scale of a row is NaN, attention takes the whole row for NaN; so it does where one is above
+ * 2^125, which write never makes, and those values read as NaN.  What is below 2^-125 may count as zero.
  * slots: int32 or int64 [tokens] in device memory, slot = page * page_size + token in the page.
  * write: k, v [tokens, h_kv, d] by strides {token, head} into their slots; a slot outside the cache is
  * skipped, and no slot may be named twice.  read: the reverse; a slot outside the cache reads as zeros.

@@ -111,6 +111,21 @@ def test_a_row_with_an_infinity_or_nan_reads_back_as_nan(device, bad, d):
     assert torch.isfinite(rk).all()
 
 
+def test_scales_that_are_never_written(device):
+    # above 2^125: NaN; the largest that is written: numbers
+    cache = PagedKVCache.allocate(1, 4, 1, 64, F4, device)
+    for t, codes in ((cache.k, 0x76), (cache.v, 0xF1)):  # 4 and 6, 0.5 and -6
+        t.view(torch.uint8).fill_(codes)
+    for t in (cache.k_scale, cache.v_scale):
+        t.view(torch.uint8)[0, :, 0] = torch.tensor([[252, 252], [253, 127], [254, 255], [127, 2]], dtype=torch.uint8, device=device)
+    k, v = (x[:, 0].double() for x in cache.read(torch.arange(4, device=device)))
+    for x, (low, high) in ((k, (4.0, 6.0)), (v, (0.5, -6.0))):
+        want = torch.tensor([low, high] * 16, dtype=torch.float64, device=device)
+        assert torch.equal(x[0], torch.cat((want, want)) * 2.0**125)
+        assert torch.isnan(x[1, :32]).all() and torch.equal(x[1, 32:], want) and torch.isnan(x[2]).all()
+        assert torch.equal(x[3, :32], want) and torch.equal(x[3, 32:], want * 2.0**-125)
+
+
 @pytest.mark.parametrize("slot_type", [torch.int32, torch.int64])
 def test_slots_outside_the_cache(device, slot_type):
     cache = PagedKVCache.allocate(4, 4, 2, 64, F4, device)

@@ -136,6 +136,17 @@ def test_outputs_do_not_share(device):
     assert [t.dtype for t in step] == [torch.int32, torch.int32, torch.int64, torch.bool]
 
 
+@pytest.mark.parametrize("codes", ["fp4", "int8"])
+def test_the_example_serves_with_a_pool(device, codes):
+    import os
+    import sys
+
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import windowed_layer
+
+    assert 0 < windowed_layer.main(["--codes", codes]) < 1
+
+
 def test_refusals(device):
     pool = PagePool.allocate(9, 16, 4, 3, device)
     new = int32([1] * 4, device)
