@@ -220,6 +220,7 @@ static GradPlan plan_grad(int b, int sq, int sk, int h, int h_kv, int d, int win
 struct PagedPlan {
     bool token;
     int row_tiles, splits;
+    int waves;  // of a workgroup: single tokens over 4 bits
     int64_t bytes;
 };
 
@@ -236,15 +237,17 @@ struct PagedPlan {
 // the host does not know by how much: 64 sequences of 2048 to 8192 tokens, int8, take 191 us with four (170 before four fitted),
 // 158 with eight, 169 with sixteen; one of 131001 tokens in bf16 takes 125 us with 128 parts and 128 with 256.
 //
-// Single tokens over 4 bits have less to read for each key, and parts cost them more: no more of them than that, one up to 640 keys; else a
-// workgroup to a CU, two where parts are longer than 640 keys then, eight where they are longer than 1024 (and a single one than
-// 2048), of 1024 keys at least.  us by parts, bf16, 128 dims, 8 key heads: 16 sequences of 517 tokens 1: 9.1, 2: 10.3, 4: 10.4; 64 of
+// Single tokens over 4 bits have less to read for each key, and parts cost them more: no more of them than that, one up to 640 keys and up
+// to eight for each workgroup of a single round; else a workgroup to a CU, two where parts are longer than 640 keys then, eight where they are longer than
+// 1024 (and a single one than 2048), of 1024 keys at least.  One part of more than 256 keys, and no more workgroups than CUs: eight waves,
+// which are slower wherever workgroups share a CU (us with four and eight: four sequences of 517 tokens, 12 heads of 64 dims, 8.5, 7.5; 16 of 517
+// 7.7, 7.0; 16 of 1000 of 8 heads of 128 12.3, 11.3; 64 of 1000 15.3, 16.4; one of 120 5.5, 6.0).  us by parts, bf16, 128 dims, 8 key heads: 16 sequences of 517 tokens 1: 9.1, 2: 10.3, 4: 10.4; 64 of
 // 1000 1: 15.1, 2: 19.9, 4: 22.7; 64 of 2000 1: 24.4, 2: 27.9; 16 of 2000 2: 16.9, 4: 15.0, 8: 16.5, 16: 19.7; 1 of 4000 16: 10.8, 32: 9.3; 4 of
 // 2000 4: 12.0, 8: 10.4, 16: 11.9; 4 of 32000 16: 28.1, 32: 26.6, 64: 28.8; 64 of 8192 1: 116, 2: 98, 4: 88, 8: 88, 12: 95; 256 dims, fp16, 16 drafts of 5
 // tokens in a window of 1024 1: 27.3, 2: 23.7, 4: 24.9, 6: 32.0.
 static int parts_token4(int64_t units, int64_t keys, int64_t most) {
     int64_t parts = std::min(most, (256 + units - 1) / units);
-    if (keys <= 640) parts = 1;
+    if (keys <= std::max((int64_t)640, 8 * std::min(units, (int64_t)256))) return 1;
     if (keys > 640 * parts) parts = std::min(most, (512 + units - 1) / units);
     if (keys > (parts == 1 ? 2048 : 1024 * parts)) parts = std::min({most, (2048 + units - 1) / units, (keys + 1023) / 1024});
     return (int)parts;
@@ -267,6 +270,7 @@ static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, i
     if (splits > kMostParts) splits = kMostParts;
     if (splits < 1) splits = 1;
     p.splits = p.token && source == kPagedF4 ? parts_token4(units, keys, splits) : (int)splits;
+    p.waves = p.splits == 1 && units <= 256 && keys > 256 ? 8 : 4;
     p.bytes = p.splits > 1 ? (int64_t)p.splits * tokens * h * (d + 1) * (int64_t)sizeof(float) : 0;
     return p;
 }
@@ -536,6 +540,7 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
     a.tokens = tokens;
     a.row_tiles = plan.row_tiles;
     a.splits = plan.splits;
+    a.waves = plan.waves;
     a.part_rows = (int64_t)tokens * h;
     a.part_o = static_cast<float*>(workspace);
     a.part_lse = a.part_o + a.splits * a.part_rows * d;

@@ -69,7 +69,7 @@ struct AttnArgs {
     float* part_o;               //   [split][row slot][d] and
     float* part_lse;             //   [split][row slot], row slot = (token * kv + key head) * group + head in the group
     int64_t part_rows;           //   row slots of one split
-    int heads;                   // 4-bit pages, single tokens: key heads of a wave
+    int heads, waves;            // 4-bit pages, single tokens: key heads of a wave, waves of a workgroup
     FastDiv by_group, by_page, by_row_tiles, by_kv, by_splits;
     // backward
     const char *dout;            // [token, sample, head] like q

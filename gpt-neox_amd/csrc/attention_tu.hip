@@ -30,21 +30,28 @@ static void token(const AttnArgs& a, int source, hipStream_t stream) {
     }
 }
 
-template <typename T, bool SPLIT>
+template <typename T, bool SPLIT, int WAVES>
 static void token4(AttnArgs a, hipStream_t stream) {
     constexpr int DP = NEOX_ATTN_DIM;
     const int fetch = token4_fetch(a, DP), groups = a.kv / a.heads;
     a.by_kv = FastDiv::by((uint32_t)groups);
-    const uint32_t grid = ((uint32_t)a.b * a.splits + 7) / 8 * 8 * groups;
+    const dim3 grid(((uint32_t)a.b * a.splits + 7) / 8 * 8 * groups), threads(64 * WAVES);
     if (fetch == kFetchOwn) {
-        attn_token4_kernel<T, DP, 1, SPLIT, kFetchOwn><<<grid, 256, 0, stream>>>(a);
+        attn_token4_kernel<T, DP, 1, SPLIT, kFetchOwn, WAVES><<<grid, threads, 0, stream>>>(a);
     } else if (fetch == kFetchHalves) {
-        if constexpr (DP != 96) attn_token4_kernel<T, DP, 1, SPLIT, kFetchHalves><<<grid, 256, 0, stream>>>(a);  // (96: always rows)
+        if constexpr (DP != 96) attn_token4_kernel<T, DP, 1, SPLIT, kFetchHalves, WAVES><<<grid, threads, 0, stream>>>(a);  // (96: always rows)
     } else if (a.heads == 1) {
-        attn_token4_kernel<T, DP, 1, SPLIT, kFetchRows><<<grid, 256, 0, stream>>>(a);
+        attn_token4_kernel<T, DP, 1, SPLIT, kFetchRows, WAVES><<<grid, threads, 0, stream>>>(a);
     } else {
-        if constexpr (DP <= 128) attn_token4_kernel<T, DP, 2, SPLIT, kFetchRows><<<grid, 256, 0, stream>>>(a);
+        if constexpr (DP <= 128 && WAVES == 4) attn_token4_kernel<T, DP, 2, SPLIT, kFetchRows, WAVES><<<grid, threads, 0, stream>>>(a);
     }
+}
+template <typename T, bool SPLIT>
+static void token4(const AttnArgs& a, hipStream_t stream) {
+    if constexpr (!SPLIT) {
+        if (a.waves == 8) return token4<T, SPLIT, 8>(a, stream);
+    }
+    token4<T, SPLIT, 4>(a, stream);
 }
 
 template <>

@@ -173,15 +173,15 @@ inline Fetch4 token4_fetch(const AttnArgs& a, int dp) {
     return a.d == dp && (dp == 96 || bits % (dp / 32) == 0) ? kFetchRows : kFetchHalves;
 }
 
-template <typename T, int DP, int HEADS, bool SPLIT, int FETCH>
-__global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(AttnArgs a) {
+template <typename T, int DP, int HEADS, bool SPLIT, int FETCH, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) void attn_token4_kernel(AttnArgs a) {
     typedef Piece4<DP> P;
     typedef typename P::Codes Codes;
     constexpr bool kTwo = __is_same(T, F16), EVEN = FETCH != kFetchOwn, kScaleRows = FETCH == kFetchRows;
     constexpr int kKeys = 32, kLoads = P::kLoads, kWords = P::kWords, kColumns = 16 / HEADS;  // columns of a head
     constexpr int kWaveBytes = kKeys * Tile<DP>::kRow;
-    __shared__ __attribute__((aligned(512))) char lds[4 * kWaveBytes];
-    __shared__ float wave_m[4][16], wave_l[4][16];
+    __shared__ __attribute__((aligned(512))) char lds[WAVES * kWaveBytes];
+    __shared__ float wave_m[WAVES][16], wave_l[WAVES][16];
 
     // The heads of one part of a sequence run on one XCD at about the same time: their rows are neighbours in memory.  (by_kv: by the
     // groups of HEADS heads)
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(Att
     const KeyTiles tiles = key_tiles<kKeys>(position0, position0 + tokens - 1, keys, a.window, a.sinks);
     int first = 0, end = tiles.count;
     if constexpr (SPLIT) {
-        const int each = ((tiles.count + a.splits - 1) / a.splits + 3) / 4 * 4;
+        const int each = ((tiles.count + a.splits - 1) / a.splits + WAVES - 1) / WAVES * WAVES;
         first = min(split * each, tiles.count);
         end = min(first + each, tiles.count);
     }
@@ -228,11 +228,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(Att
     // otherwise those of a lane's own two keys, one block ahead.
     uint32_t page_set[2];
     auto look_up = [&](int n) {  // n: blocks from the wave's first one
-        const int i = first + 4 * (n + (lane >> 1)), key = tiles.tile(i) * kKeys + 16 * (lane & 1);
+        const int i = first + WAVES * (n + (lane >> 1)), key = tiles.tile(i) * kKeys + 16 * (lane & 1);
         return i < end && key < keys ? (uint32_t)table[a.by_page.div(key)] : ~0u;
     };
     auto look_up_own = [&](int n) {
-        const int i = first + 4 * n;
+        const int i = first + WAVES * n;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const int key = tiles.tile(i) * kKeys + 16 * kb + col;
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(Att
     for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = kNegInf, l = 0.f;
 
-    for (int i = first; i < end; i += 4) {
+    for (int i = first; i < end; i += WAVES) {
         const int key0 = tiles.tile(i) * kKeys;
         asm("" : "+v"(put_at), "+v"(get_at));
         typedef __attribute__((address_space(3))) u32x4 lds16;
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(Att
             __builtin_amdgcn_wave_barrier();
         };
         put(0);
-        if (HEADS == 1 && i + 4 < end) fetch(i + 4);
+        if (HEADS == 1 && i + WAVES < end) fetch(i + WAVES);
         // (the last token sees furthest ahead, the first least; a window's near end moves with both)
         const bool all = key0 + kKeys - 1 <= position0 && key0 + kKeys <= keys &&
                          (a.window < 0 || key0 >= position0 + tokens - 1 - a.window || key0 + kKeys <= a.sinks);
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(Att
 #pragma unroll
         for (int h = 0; h < HEADS; ++h) {
             if (h > 0) put(h);
-            if (HEADS > 1 && h == HEADS - 1 && i + 4 < end) fetch(i + 4);
+            if (HEADS > 1 && h == HEADS - 1 && i + WAVES < end) fetch(i + WAVES);
             u32x4 mine_p, mine_low;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -568,7 +568,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(Att
         }
     }
 
-    // the four waves' results: rows of DP values in each wave's own LDS, joined by the whole workgroup
+    // the waves' results: rows of DP values in each wave's own LDS, joined by the whole workgroup
     l = both_halves_sum(l + __shfl_xor(l, 16));
     float* const own = reinterpret_cast<float*>(vt);
 #pragma unroll
@@ -578,16 +578,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 3 : 2) void attn_token4_kernel(Att
         wave_l[wave][col] = l;
     }
     __syncthreads();
-    for (int at = threadIdx.x * 8; at < 16 * DP; at += 256 * 8) {
+    for (int at = threadIdx.x * 8; at < 16 * DP; at += 64 * WAVES * 8) {
         const int c = at / DP, r = c % kColumns, dim = at % DP;
         if (r >= rows || dim >= a.d) continue;
         float high = wave_m[0][c];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) high = fmaxf(high, wave_m[w][c]);
+        for (int w = 1; w < WAVES; ++w) high = fmaxf(high, wave_m[w][c]);
         const float base = high == kNegInf ? 0.f : high;
         float total = 0.f, x[8] = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float f = __builtin_amdgcn_exp2f(wave_m[w][c] - base);
             total += wave_l[w][c] * f;
             const float* from = reinterpret_cast<const float*>(lds + w * kWaveBytes) + c * DP + dim;
