@@ -278,7 +278,7 @@ static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, i
 // Key heads to a wave of the single tokens over 4 bits: two, where a row's scales are fetched at once, their rows fit the columns
 // and half the workgroups are two to a CU.
 static int token4_heads(const AttnArgs& a) {
-    const bool two = token4_fetch(a, padded(a.d)) == kFetchRows && a.d <= 128 && a.kv % 2 == 0 && 2 * a.sq * a.group <= 16;
+    const bool two = token4_fetch(a, padded4(a.d)) == kFetchRows && a.d <= 128 && a.kv % 2 == 0 && 2 * a.sq * a.group <= 16;
     return two && (int64_t)a.b * a.kv * a.splits >= 1024 ? 2 : 1;
 }
 

@@ -556,9 +556,9 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 // dims, window 512 (fp16) 99, 457 TFLOP/s, of which a quarter of the columns are padding and the edges of the window are
 // computed and masked.  Chunks of 512 tokens of four sequences over 16384 keys, window 4096, 32 heads on 8, fp8: 200, 513
 // TFLOP/s, the widening of codes being work of its own.
-// Over codes at 256 dims the fp16 kernels spill 6 to 11 registers.
+// Over 8-bit codes at 256 dims the fp16 kernels spill 6 to 11 registers, over 4 bits, two workgroups to a CU, 40 to 70.
 template <typename T, int DP, int SRC, bool SPLIT>
-__global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged16 ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged16 ? 3 : 2) : SRC == kPagedF4 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
     constexpr bool kPages = SRC != kStrided;
     constexpr bool kF4 = SRC == kPagedF4;
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8 || kF4;
@@ -566,8 +566,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     constexpr int kBytes = kCodes ? 1 : 2;
     // Keys of one step.  32 leave registers and LDS for a third workgroup on a CU (measured with 64 and 32, us: 2 x 64
     // heads of 96 dims, 2048 keys, window 512: 126, 105; 32 heads of 128 dims, 8192 keys, window 4096: 562, 539); with
-    // codes, whose widening takes the registers anyway, 64 save barriers (chunks of 512 over 16384 in fp8: 251, 275).
-    constexpr int kFwdKeys = kCodes ? 64 : 32;
+    // codes, whose widening takes the registers anyway, 64 save barriers (chunks of 512 over 16384 in fp8: 251, 275).  Over 4 bits above
+    // 128 dims 32 leave LDS for a second one: 4 x 512 tokens over 8192 keys of 256 dims, window 4096, fp16 345, 262, bf16 the same; of 160 dims, which
+    // have kernels of their own there, 4 x 98 over 7053 158, 81 (with 256 dims' padding 117), 1 x 1024 over 16000 in bf16 511, 279.
+    constexpr int kFwdKeys = kCodes && !(kF4 && DP > 128) ? 64 : 32;
     constexpr int kTile = kFwdKeys * Tile<DP>::kRow;
     __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile + (kCodes ? 2 * 2 * kFwdKeys * 4 : 0)];
     __shared__ __attribute__((aligned(16))) uint32_t nan_keys[kF4 && !kKeyScales ? 2 : 1][4];  // [buffer][wave that staged it]

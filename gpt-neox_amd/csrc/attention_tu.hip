@@ -14,7 +14,15 @@ static void forward(const AttnArgs& a, int source, hipStream_t stream) {
         case kPaged16: attn_fwd_kernel<T, DP, kPaged16, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedI8: attn_fwd_kernel<T, DP, kPagedI8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
         case kPagedF8: attn_fwd_kernel<T, DP, kPagedF8, SPLIT><<<grid, 256, 0, stream>>>(a); break;
-        case kPagedF4: attn_fwd_kernel<T, DP, kPagedF4, SPLIT><<<grid, 256, 0, stream>>>(a); break;
+        case kPagedF4:
+            if constexpr (DP == 256) {
+                if (padded4(a.d) == 160) {
+                    attn_fwd_kernel<T, 160, kPagedF4, SPLIT><<<grid, 256, 0, stream>>>(a);
+                    break;
+                }
+            }
+            attn_fwd_kernel<T, DP, kPagedF4, SPLIT><<<grid, 256, 0, stream>>>(a);
+            break;
     }
 }
 
@@ -30,28 +38,35 @@ static void token(const AttnArgs& a, int source, hipStream_t stream) {
     }
 }
 
-template <typename T, bool SPLIT, int WAVES>
+template <typename T, int DP, bool SPLIT, int WAVES>
 static void token4(AttnArgs a, hipStream_t stream) {
-    constexpr int DP = NEOX_ATTN_DIM;
     const int fetch = token4_fetch(a, DP), groups = a.kv / a.heads;
     a.by_kv = FastDiv::by((uint32_t)groups);
     const dim3 grid(((uint32_t)a.b * a.splits + 7) / 8 * 8 * groups), threads(64 * WAVES);
     if (fetch == kFetchOwn) {
         attn_token4_kernel<T, DP, 1, SPLIT, kFetchOwn, WAVES><<<grid, threads, 0, stream>>>(a);
     } else if (fetch == kFetchHalves) {
-        if constexpr (DP != 96) attn_token4_kernel<T, DP, 1, SPLIT, kFetchHalves, WAVES><<<grid, threads, 0, stream>>>(a);  // (96: always rows)
+        // (of 96 and 160 dims: always rows)
+        if constexpr (DP != 96 && DP != 160) attn_token4_kernel<T, DP, 1, SPLIT, kFetchHalves, WAVES><<<grid, threads, 0, stream>>>(a);
     } else if (a.heads == 1) {
         attn_token4_kernel<T, DP, 1, SPLIT, kFetchRows, WAVES><<<grid, threads, 0, stream>>>(a);
     } else {
         if constexpr (DP <= 128 && WAVES == 4) attn_token4_kernel<T, DP, 2, SPLIT, kFetchRows, WAVES><<<grid, threads, 0, stream>>>(a);
     }
 }
-template <typename T, bool SPLIT>
+template <typename T, int DP>
+static void token4_of(const AttnArgs& a, hipStream_t stream) {
+    if (a.splits > 1) token4<T, DP, true, 4>(a, stream);
+    else if (a.waves == 8) token4<T, DP, false, 8>(a, stream);
+    else token4<T, DP, false, 4>(a, stream);
+}
+template <typename T>
 static void token4(const AttnArgs& a, hipStream_t stream) {
-    if constexpr (!SPLIT) {
-        if (a.waves == 8) return token4<T, SPLIT, 8>(a, stream);
+    constexpr int DP = NEOX_ATTN_DIM;
+    if constexpr (DP == 256) {
+        if (padded4(a.d) == 160) return token4_of<T, 160>(a, stream);
     }
-    token4<T, SPLIT, 4>(a, stream);
+    token4_of<T, DP>(a, stream);
 }
 
 template <>
@@ -64,8 +79,7 @@ hipError_t launch_attn_fwd<NEOX_ATTN_DIM>(const AttnArgs& a, int source, int dty
 template <>
 hipError_t launch_attn_token<NEOX_ATTN_DIM>(const AttnArgs& a, int source, int dtype, hipStream_t stream) {
     if (source == kPagedF4) {
-        if (dtype == NEOX_BF16) a.splits > 1 ? token4<BF16, true>(a, stream) : token4<BF16, false>(a, stream);
-        else a.splits > 1 ? token4<F16, true>(a, stream) : token4<F16, false>(a, stream);
+        dtype == NEOX_BF16 ? token4<BF16>(a, stream) : token4<F16>(a, stream);
         return hipGetLastError();
     }
     if (dtype == NEOX_BF16) a.splits > 1 ? token<BF16, true>(a, source, stream) : token<BF16, false>(a, source, stream);

@@ -137,11 +137,11 @@ struct Piece4 {
     typedef std::conditional_t<kWords == 4, u32x4, u32x2> Codes;
 };
 
-// the scales of a row of DP dims: as many bytes as a load takes, three by themselves at 96
+// the scales of a row of DP dims: as many bytes as a load takes, one by one at 96 and 160
 template <int DP>
 struct Scales4 {
-    typedef std::conditional_t<DP == 64, uint16_t, std::conditional_t<DP == 96, uint8_t, uint32_t>> Unit;
-    static constexpr int kUnits = DP == 96 ? 3 : DP == 256 ? 2 : 1;
+    typedef std::conditional_t<DP == 64, uint16_t, std::conditional_t<DP == 96 || DP == 160, uint8_t, uint32_t>> Unit;
+    static constexpr int kUnits = DP == 96 ? 3 : DP == 160 ? 5 : DP == 256 ? 2 : 1;
 };
 
 // the larger of the values of lane l and of lane l ^ 16
@@ -158,6 +158,9 @@ __device__ __forceinline__ C buf_codes(rsrc_t r, uint32_t at) {
     else return buf_ld64(r, (int)at, 0);
 }
 
+// The head dims that the kernels over 4 bits are built for.
+inline int padded4(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 160 ? 160 : 256; }
+
 // How the kernel may fetch: half a block, 16 keys, through one buffer if pages hold whole halves, keys and values are laid out alike,
 // and a row's bytes lie before the next row's (kFetchHalves); and the scales of a row at once if there are DP dims and these are
 // aligned (kFetchRows).  Otherwise every lane goes by itself (kFetchOwn).
@@ -170,7 +173,7 @@ inline Fetch4 token4_fetch(const AttnArgs& a, int dp) {
         bits |= a.ks_st[i];
     }
     if (a.by_page.d % 16 != 0 || a.k_st[0] < row || a.ks_st[0] < scales || a.k_st[0] >= kSmallStride || a.ks_st[0] >= kSmallStride) return kFetchOwn;
-    return a.d == dp && (dp == 96 || bits % (dp / 32) == 0) ? kFetchRows : kFetchHalves;
+    return a.d == dp && (dp == 96 || dp == 160 || bits % (dp / 32) == 0) ? kFetchRows : kFetchHalves;
 }
 
 template <typename T, int DP, int HEADS, bool SPLIT, int FETCH, int WAVES>
@@ -414,12 +417,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) voi
 #pragma unroll
                 for (int u = 0; u < Scales4<DP>::kUnits; ++u) w[u] = rows_of[h][u];
                 if constexpr (DP == 96) w[0] |= w[1] << 8 | w[2] << 16;
+                if constexpr (DP == 160) {
+                    w[0] |= w[1] << 8 | w[2] << 16 | w[3] << 24;
+                    w[1] = w[4];
+                }
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int st = 0; st < kLoads; ++st) {
                         // (of a lane's 8, 16 or 32 dims: byte dim / 32)
-                        const uint32_t word = w[DP == 256 ? st : 0], byte = DP >= 128 ? quad : DP == 96 && st == 1 ? 2 : quad >> 1;
+                        const uint32_t word = w[DP > 128 ? st : 0], byte = DP >= 128 ? quad : DP == 96 && st == 1 ? 2 : quad >> 1;
                         kf[h][kb][st] = (uint32_t)__shfl((int)word, col + 16 * kb) >> 8 * byte & 0xff;
                         vf[h][kb][st] = (uint32_t)__shfl((int)word, col + 16 * kb + 32) >> 8 * byte & 0xff;
                     }
