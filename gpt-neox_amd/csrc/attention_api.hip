@@ -237,7 +237,12 @@ struct PagedPlan {
 // the host does not know by how much: 64 sequences of 2048 to 8192 tokens, int8, take 191 us with four (170 before four fitted),
 // 158 with eight, 169 with sixteen; one of 131001 tokens in bf16 takes 125 us with 128 parts and 128 with 256.
 //
-// Single tokens over 4 bits have less to read for each key, and parts cost them more: no more of them than that, one up to 640 keys and up
+// Single tokens over 4 bits take up to 48 rows in blocks of 16 (64 above 160 dims), whose workgroups read the same keys: a few tokens of
+// a draft would leave row tiles of 128 mostly empty.  us in row tiles and in blocks: bf16, 128 dims, 16 sequences of 8000 tokens, 4 key heads, 20
+// rows 39, 28, 40 rows 47, 35, 48 rows 47, 39, 64 rows 49, 44; 64 of 4000, 8 key heads, 64 rows 115, 125; one of 30000, 64 rows 33, 37; 256 dims, fp16, 64 of
+// 2000, 20 rows 231, 78; 64 of 4000, 64 rows 492, 241.
+//
+// They have less to read for each key, and parts cost them more: no more of them than that, one up to 640 keys and up
 // to eight for each workgroup of a single round; else a workgroup to a CU, two where parts are longer than 640 keys then, eight where they are longer than
 // 1024 (and a single one than 2048), of 1024 keys at least.  One part of more than 256 keys, and no more workgroups than CUs: eight waves,
 // which are slower wherever workgroups share a CU (us with four and eight: four sequences of 517 tokens, 12 heads of 64 dims, 8.5, 7.5; 16 of 517
@@ -263,14 +268,21 @@ static PagedPlan plan_paged(int b, int tokens, int max_query, int max_context, i
         const int64_t seen = (int64_t)window + max_query + sinks;
         if (seen < keys) keys = seen;
     }
-    const int64_t units = (int64_t)b * h_kv * p.row_tiles, target = 256 * (p.token ? 8 : codes ? 2 : 3);
+    const bool blocks = source == kPagedF4 && rows <= (d <= 160 ? 48 : 64);
+    const int64_t units = (int64_t)b * h_kv * p.row_tiles, target = 256 * (p.token ? 8 : codes && !blocks ? 2 : 3);
     int64_t splits = (target + units - 1) / units;
     const int64_t most = (keys + 255) / 256;
     if (splits > most) splits = most;
     if (splits > kMostParts) splits = kMostParts;
     if (splits < 1) splits = 1;
-    p.splits = p.token && source == kPagedF4 ? parts_token4(units, keys, splits) : (int)splits;
-    p.waves = p.splits == 1 && units <= 256 && keys > 256 ? 8 : 4;
+    p.splits = (int)splits;
+    if (blocks) {
+        p.token = true;
+        p.row_tiles = (int)((rows + 15) / 16);
+        const int64_t groups = (int64_t)b * h_kv * p.row_tiles;
+        p.splits = parts_token4(groups, keys, splits);
+        p.waves = p.splits == 1 && groups <= 256 && keys > 256 ? 8 : 4;
+    }
     p.bytes = p.splits > 1 ? (int64_t)p.splits * tokens * h * (d + 1) * (int64_t)sizeof(float) : 0;
     return p;
 }

@@ -40,7 +40,7 @@ static void token(const AttnArgs& a, int source, hipStream_t stream) {
 
 template <typename T, int DP, bool SPLIT, int WAVES>
 static void token4(AttnArgs a, hipStream_t stream) {
-    const int fetch = token4_fetch(a, DP), groups = a.kv / a.heads;
+    const int fetch = token4_fetch(a, DP), groups = a.kv / a.heads * a.row_tiles;
     a.by_kv = FastDiv::by((uint32_t)groups);
     const dim3 grid(((uint32_t)a.b * a.splits + 7) / 8 * 8 * groups), threads(64 * WAVES);
     if (fetch == kFetchOwn) {

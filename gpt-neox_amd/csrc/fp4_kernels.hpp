@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void cache4_kernel(CacheArgs a) {
 }
 
 // ---- single tokens ----------------------------------------------------------------------------------------
-// As attn_token_kernel in attention_kernels.hpp: few rows per key head, every wave streams blocks of 32 keys of its own,
+// As attn_token_kernel in attention_kernels.hpp: 16 rows of a key head to a workgroup, every wave streams blocks of 32 keys of its own,
 // 16x16x32 tiles, the values through LDS of the wave's own for the transposing reads.  A lane fetches pieces of keys l % 16 and
 // 16 + l % 16 of which one scale holds all: 32 dims from 128 s + 32 (l / 16), at 64 and 96 dims 16 from 64 s + 16 (l / 16).
 // Codes take their scale along as bf16, exactly.  fp16 queries and the probabilities that go with them have 11 bits where
@@ -186,26 +186,28 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) voi
     __shared__ __attribute__((aligned(512))) char lds[WAVES * kWaveBytes];
     __shared__ float wave_m[WAVES][16], wave_l[WAVES][16];
 
-    // The heads of one part of a sequence run on one XCD at about the same time: their rows are neighbours in memory.  (by_kv: by the
-    // groups of HEADS heads)
+    // The heads of one part of a sequence, and the blocks of 16 rows of a head, run on one XCD at about the same time: what they read is
+    // in the same lines.  (by_kv: by the groups of HEADS heads, times the blocks)
     const uint32_t turn = blockIdx.x >> 3, at = a.by_kv.div(turn), item = at * 8 + (blockIdx.x & 7);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4, col = lane & 15;
-    const int g0 = (turn - at * a.by_kv.d) * HEADS;
+    const uint32_t sub = turn - at * a.by_kv.d, group_of = a.by_row_tiles.div(sub);
+    const int g0 = group_of * HEADS, row0 = (sub - group_of * a.row_tiles) * 16;
     if (item >= (uint32_t)a.b * a.splits) return;
     const int b = SPLIT ? a.by_splits.div(item) : item, split = SPLIT ? item - b * a.splits : 0;
     int token0, tokens, keys;
     paged_sample(a, b, token0, tokens, keys);
-    const int rows = min(tokens * a.group, kColumns);
-    if (rows == 0) return;
+    const int rows = min(tokens * a.group - row0, kColumns);
+    if (rows <= 0) return;
     const int position0 = keys - tokens;
+    const int first_position = position0 + (int)a.by_group.div(row0), last_position = position0 + (int)a.by_group.div(row0 + rows - 1);
 
     const int mine = col / kColumns;  // of the heads
     const bool there = col % kColumns < rows;
-    const int row = min(col % kColumns, rows - 1);
+    const int row = row0 + min(col % kColumns, rows - 1);
     const int token = a.by_group.div(row), head = (g0 + mine) * a.group + row - token * a.group;
     const int position = position0 + token;
 
-    const KeyTiles tiles = key_tiles<kKeys>(position0, position0 + tokens - 1, keys, a.window, a.sinks);
+    const KeyTiles tiles = key_tiles<kKeys>(first_position, last_position, keys, a.window, a.sinks);
     int first = 0, end = tiles.count;
     if constexpr (SPLIT) {
         const int each = ((tiles.count + a.splits - 1) / a.splits + WAVES - 1) / WAVES * WAVES;
@@ -503,8 +505,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) voi
         put(0);
         if (HEADS == 1 && i + WAVES < end) fetch(i + WAVES);
         // (the last token sees furthest ahead, the first least; a window's near end moves with both)
-        const bool all = key0 + kKeys - 1 <= position0 && key0 + kKeys <= keys &&
-                         (a.window < 0 || key0 >= position0 + tokens - 1 - a.window || key0 + kKeys <= a.sinks);
+        const bool all = key0 + kKeys - 1 <= first_position && key0 + kKeys <= keys &&
+                         (a.window < 0 || key0 >= last_position - a.window || key0 + kKeys <= a.sinks);
         if (!all) {
             const int lo = a.window < 0 ? 0 : position - a.window, hi = min(position, keys - 1);
 #pragma unroll
@@ -604,7 +606,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) voi
         const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= inverse;
-        const int t = a.by_group.div(r), h = (g0 + c / kColumns) * a.group + r - t * a.group;
+        const int t = a.by_group.div(row0 + r), h = (g0 + c / kColumns) * a.group + row0 + r - t * a.group;
         if constexpr (SPLIT) {
             const int64_t slot = (int64_t)split * a.part_rows + (int64_t)(token0 + t) * a.kv * a.group + h;
             float* p = a.part_o + slot * a.d + dim;

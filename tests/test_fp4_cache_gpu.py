@@ -376,6 +376,18 @@ def test_many_heads(device, dtype, d, b, h, h_kv, new, context):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 160, 224, 256])
+@pytest.mark.parametrize("h,h_kv,new", [(4, 2, 8), (8, 2, 5), (3, 1, 15), (12, 1, 4), (7, 1, 7), (40, 1, 1), (64, 1, 1), (13, 1, 5)])
+def test_rows_in_blocks(device, dtype, d, h, h_kv, new):
+    # 16 rows of a key head to a block, the last one not full, tokens whose heads two blocks share
+    args = sequences(device, dtype, [new, max(1, new - 3), new], [3 * new, 1300, 200], h, h_kv, d, 32)
+    got = check(*args)
+    assert torch.equal(got, check(*args))
+    check(*args, window=90, sinks=3)
+    check(*args, max_query=new + 30)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("bad", [255, 253])  # (a scale that large counts as NaN)
 def test_a_nan_stays_with_its_head(device, dtype, which, bad):
