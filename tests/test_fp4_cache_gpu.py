@@ -406,6 +406,30 @@ def test_a_nan_stays_with_its_head(device, dtype, which, bad):
         assert torch.equal(got[~hit], want[~hit])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", DIMS)
+@pytest.mark.parametrize("page,aligned", [(31, True), (48, True), (48, False)])
+def test_every_way_of_fetching(device, dtype, d, page, aligned):
+    # pages that no 16 keys fit, those that they do, scales that are no words; one part in four and in eight waves, and several
+    for context in ([200, 90], [600, 257], [1500, 40, 1]):
+        q, cache, table, starts, lengths = sequences(device, dtype, [1] * len(context), context, 4, 2, d, page)
+        if not aligned:
+            odd = [torch.empty(t.numel() + 1, dtype=torch.uint8, device=device)[1:].view(t.shape) for t in (cache.k_scale, cache.v_scale)]
+            for to, t in zip(odd, (cache.k_scale, cache.v_scale)):
+                to.copy_(t.view(torch.uint8))
+            cache = PagedKVCache(cache.k, cache.v, *(t.view(E8) for t in odd))
+        check(q, cache, table, starts, lengths, max_context=max(context))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_many_long_sequences(device, dtype, d):
+    # two heads to a wave, and parts
+    args = sequences(device, dtype, [1] * 64, [2300 - 31 * i for i in range(64)], 16, 8, d, 64)
+    got = check(*args, max_context=2300)
+    assert torch.equal(got, check(*args, max_context=2300))
+
+
 def test_scales_that_are_not_aligned(device):
     # their rows cannot be fetched as words
     for d in (64, 128, 256):
