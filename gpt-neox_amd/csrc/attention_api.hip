@@ -538,6 +538,8 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
     NEOX_TRY(check_scale_window(scale, sinks, what));
     const int source = cache_source_of(cache_dtype, dtype);
     const PagedPlan plan = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, source);
+    if ((int64_t)b * h_kv * plan.row_tiles * plan.splits >= kMost)
+        return fail(NEOX_ERR_BAD_SHAPE, "%s: b=%d h_kv=%d of %d rows is too large for one call", what, b, h_kv, max_query * (h / h_kv));
     if (plan.bytes > 0) {
         NEOX_TRY(check_pointer(workspace, 16, what, "workspace"));
         if (workspace_bytes < plan.bytes)

@@ -103,6 +103,11 @@ def test_attention_over_4_bits(p):
         refused(paged(p, **change), code, message)
 
 
+def test_more_blocks_than_a_launch_has(p):
+    strides = dict(h=48, h_kv=1, os=st(64 * 64, 64), qs=st(64 * 64, 64), kcs=st(512, 32, 32), vcs=st(512, 32, 32), kss=st(32, 2, 2), vss=st(32, 2, 2))
+    refused(paged(p, b=1 << 29, max_query=1, max_context=16, **strides), -3, "too large for one call")
+
+
 def test_writing_4_bits(p):
     def write(**change):
         a = dict(kc=p, vc=p, ks=p, vs=p + 1, k=p, v=p, slots=p, wide=1, tokens=3, h=2, d=64, pages=4, page=16, kcs=st(1024, 64, 32), vcs=st(1024, 64, 32),
