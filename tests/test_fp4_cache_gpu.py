@@ -297,6 +297,13 @@ def test_sequences_without_tokens_or_keys(device):
     assert (got[:20] == 0).all() and (got[20:30] != 0).any() and (got[30:] == 0).all()
 
 
+@pytest.mark.parametrize("d", [64, 128, 160, 256])
+def test_blocks_of_rows_without_keys(device, d):
+    # more tokens than keys: whole blocks of rows see nothing, others some
+    got = check(*sequences(device, torch.float16, [12, 0, 10, 12], [3, 7, 0, 12], 4, 2, d, 16))
+    assert (got[:9] == 0).all() and (got[9:12] != 0).any() and (got[12:22] == 0).all()
+
+
 @pytest.mark.parametrize("scale", [-0.4, 0.0, 2.0])
 def test_scales(device, scale):
     for dtype in DTYPES:

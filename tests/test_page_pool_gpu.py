@@ -136,6 +136,36 @@ def test_outputs_do_not_share(device):
     assert [t.dtype for t in step] == [torch.int32, torch.int32, torch.int64, torch.bool]
 
 
+def test_in_inference_mode(device):
+    pool, cache = PagePool.allocate(20, 16, 3, 8, device), PagedKVCache.allocate(20, 16, 2, 64, torch.float4_e2m1fn_x2, device)
+    new = int32([20, 0, 5], device)
+    with torch.inference_mode():
+        step = pool.extend(new, max_tokens=25)
+        kv = torch.randn((25, 2, 64), device=device).bfloat16()
+        cache.write(kv, kv, step.slots)
+        out = paged_attention(kv, cache, pool.page_table, step.query_starts, pool.lengths, max_query=20)
+        step.positions.add_(1)
+        assert (step.slots + 0).tolist() == [*range(20), *range(32, 37)] and step.positions.tolist() == [*range(1, 21), *range(1, 6)]
+    assert torch.isfinite(out).all() and step.granted.all()
+    pool.truncate(int32([0, 0, 0], device))
+    assert pool.left.item() == 20
+
+
+def test_on_another_stream(device):
+    pool = PagePool.allocate(100, 16, 5, 20, device)
+    want = twin(pool)
+    new = int32([100, 0, 33, 16, 1], device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step = pool.extend(new, max_tokens=150)
+        pool.truncate(int32([90, 0, 0, 16, 1], device))
+    torch.cuda.current_stream().wait_stream(side)
+    assert step.slots.tolist() == want.extend(new.tolist(), 150)[2]
+    want.truncate([90, 0, 0, 16, 1])
+    assert pool.lengths.tolist() == want.lengths and pool.free.tolist()[: want.left] == want.free[: want.left]
+
+
 @pytest.mark.parametrize("codes", ["fp4", "int8"])
 def test_the_example_serves_with_a_pool(device, codes):
     import os
