@@ -325,8 +325,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) voi
                     }
                 }
         } else {
-            // Lanes with nothing to fetch read the head's first piece instead: what comes for a key that is not there is masked, its
-            // value and what lies behind d count for nothing with a scale of next to zero.
+            // Lanes with nothing to fetch read the head's first piece instead, and throw it away when its turn comes.
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 const int key = key0 + 16 * kb + col;
@@ -405,14 +404,21 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) voi
         typedef __attribute__((address_space(3))) u32x4 lds16;
         typedef __attribute__((address_space(3))) s16x4 lds4;
         if constexpr (!EVEN) {
+            // zeros where a key is behind the last one or its page outside the cache, and behind d
 #pragma unroll
             for (int h = 0; h < HEADS; ++h)
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int st = 0; st < kLoads; ++st) {
-                        ke[h][kb][st] = dim_of(st) < a.d ? ke[h][kb][st] : (uint8_t)0;
-                        ve[h][kb][st] = key_there[kb] && dim_of(st) < a.d ? ve[h][kb][st] : (uint8_t)0;
+                        const bool ok = key_there[kb] && dim_of(st) < a.d;
+                        ke[h][kb][st] = ok ? ke[h][kb][st] : (uint8_t)0;
+                        ve[h][kb][st] = ok ? ve[h][kb][st] : (uint8_t)0;
+#pragma unroll
+                        for (int t = 0; t < kWords; ++t) {
+                            kw[h][kb][st][t] = ok ? kw[h][kb][st][t] : 0;
+                            vw[h][kb][st][t] = ok ? vw[h][kb][st][t] : 0;
+                        }
                     }
         }
         uint32_t kf[HEADS][2][kLoads], vf[HEADS][2][kLoads];  // scales

@@ -343,6 +343,41 @@ def test_tables_that_point_outside_are_kept_inside(device):
     torch.cuda.synchronize()
 
 
+def spare_page_0(cache, table):
+    """Moves what a sequence has in page 0 to a page that nobody has, so that page 0 belongs to nobody."""
+    free = [p for p in range(1, cache.pages) if not (table == p).any()]
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        t.view(torch.uint8)[free[0]] = t.view(torch.uint8)[0].clone()
+    table[table == 0] = free[0]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", DIMS)
+@pytest.mark.parametrize("page,aligned", [(16, True), (31, True), (48, True), (48, False)])
+@pytest.mark.parametrize("first_scale", [131, 255])
+def test_pages_outside_the_cache_count_as_zeros(device, dtype, d, page, aligned, first_scale):
+    # entries of the table that name no page, in the middle of what a sequence sees: in every way of fetching, and in chunks.  In the first
+    # place of the cache stands a row that nobody has: large numbers, or NaN
+    for new, context in (([1, 1], [200, 90]), ([1, 1, 1], [1500, 40, 333]), ([5, 2], [257, 90]), ([70, 30], [300, 140])):
+        q, cache, table, starts, lengths = sequences(device, dtype, new, context, 4, 2, d, page)
+        spare_page_0(cache, table)
+        for t, fill in ((cache.k, 0x77), (cache.v, 0x77), (cache.k_scale, first_scale), (cache.v_scale, first_scale)):
+            t.view(torch.uint8)[0] = fill
+        if not aligned:
+            odd = [torch.empty(t.numel() + 1, dtype=torch.uint8, device=device)[1:].view(t.shape) for t in (cache.k_scale, cache.v_scale)]
+            for to, t in zip(odd, (cache.k_scale, cache.v_scale)):
+                to.copy_(t.view(torch.uint8))
+            cache = PagedKVCache(cache.k, cache.v, *(t.view(E8) for t in odd))
+        table[0, 1], table[0, 3], table[1, 0] = -1, cache.pages, 2**31 - 1
+        held = [P.decode(c.view(torch.uint8), s.view(torch.uint8)) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale))]
+        held = [torch.cat((t, torch.zeros_like(t[:1]))) for t in held]  # (the last page: what the others count as)
+        inside = torch.where((table >= 0) & (table < cache.pages), table, cache.pages)
+        got = paged_attention(q, cache, table, starts, lengths, max_query=max(new), max_context=max(context))
+        want, bound = A.paged_attention(q, *held, None, None, inside, starts, lengths, dtype=dtype)
+        assert torch.isfinite(got).all()
+        assert ((got.double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_a_key_that_is_nan_is_not_seen_through_the_mask(device, dtype, d):
