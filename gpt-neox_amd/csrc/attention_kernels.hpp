@@ -230,6 +230,21 @@ __device__ __forceinline__ uint32_t pack_with_rest(float x, float y, uint32_t& r
     rest = Elem<T>::pack(x - a, y - b);
     return w;
 }
+// Eight fp16 numbers as the sums of two bf16 numbers each (nothing is left of an infinity).
+__device__ __forceinline__ u32x4 two_bf16(const u32x4& x, u32x4& low) {
+    u32x4 high;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        uint32_t rest;
+        Elem<F16>::unpack(x[i], a, b);
+        high[i] = pack_with_rest<BF16>(a, b, rest);
+        if (__builtin_fabsf(a) == __builtin_inff()) rest &= 0xffff0000u;
+        if (__builtin_fabsf(b) == __builtin_inff()) rest &= 0x0000ffffu;
+        low[i] = rest;
+    }
+    return high;
+}
 // Writes the 32 columns' results of one wave (lane: column, registers: 32 dims per block) times f as rows of 16-bit
 // elements, and with LOW at `low` what the rounding took from them.  The halves exchange registers, so that every lane
 // stores 16 bytes.
@@ -324,6 +339,7 @@ __device__ __forceinline__ u32x4 widen4(uint32_t word, float scale) {
 // what the byte of a 4-bit scale stands for (0 instead of 2^-127), as the kernels multiply by it; what is above the largest that
 // is ever written, six times which is a number, counts as NaN: infinities would reach other rows through probabilities of zero
 constexpr uint32_t kScaleNan = 255, kScaleMost = 127 + 125;
+constexpr uint32_t kScaleHalfLeast = 127 - 23, kScaleHalfMost = 127 + 13;  // with these every code is a number of fp16
 __device__ __forceinline__ uint32_t known_scale(uint32_t byte) { return byte > kScaleMost ? kScaleNan : byte; }
 __device__ __forceinline__ float scale_bits(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 __device__ __forceinline__ float nan_value() { return __builtin_bit_cast(float, 0x7fc00000u); }
@@ -451,14 +467,13 @@ struct Stage {
     }
 };
 
-// The same for 4-bit codes: 32 to a thread, which are one scale's.  In bf16 they take their scale along; a NaN scale of the
-// values (which would reach every row through zero probabilities) is told to the rows instead, as a number of the key's own, 0 or
-// NaN.  In fp16 a key's largest scale stays a factor of its own, as in 8 bits, and the codes are multiplied by what
-// theirs is below it: 23 powers of two below the largest they begin to lose bits.  Neighbouring quads of threads have rows 4, 8
+// The same for 4-bit codes: 32 to a thread, which are one scale's and take it along.  As bf16 numbers they do so exactly whatever it is, as
+// fp16 numbers from 2^-23, whose half is the least there is, to 2^13, six times which is near the most: a tile that has
+// another is `wide`, and goes into LDS as bf16.  A NaN scale of the values (which would reach every row through zero probabilities) is told to
+// the rows instead, as a number of the key's own, 0 or NaN.  Neighbouring quads of threads have rows 4, 8
 // and 12 apart, whose turns send their four pieces to sixteen different places.
-template <typename T, int DP, int ROWS>
+template <int DP, int ROWS>
 struct Stage4 {
-    static constexpr bool kKeyScales = __is_same(T, F16);
     static constexpr int kLanes = DP <= 64 ? 2 : DP <= 128 ? 4 : 8;  // of a row
     static constexpr int kRowsAtOnce = 256 / kLanes;
     static constexpr int kSteps = (ROWS + kRowsAtOnce - 1) / kRowsAtOnce;
@@ -480,8 +495,18 @@ struct Stage4 {
             scale[step] = *scale_at;
         }
     }
-    // keys: [ROWS]; whether one of this thread's keys has a NaN that `keys` holds
-    template <bool VALUES>
+    // whether one of this thread's scales is beyond those that fp16 numbers take along (below them, zeros do)
+    __device__ __forceinline__ bool wide() const {
+        bool is = false;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const uint32_t digits = (codes[s].x | codes[s].y | codes[s].z | codes[s].w) & 0x77777777u;
+            is |= (scale[s] > kScaleHalfMost && scale[s] <= kScaleMost) || (scale[s] < kScaleHalfLeast && digits);
+        }
+        return is;
+    }
+    // keys: [ROWS], for values; whether one of this thread's keys has a NaN that `keys` holds
+    template <typename T, bool VALUES>
     __device__ __forceinline__ bool put(char* tile, float* keys) const {
         bool bad = false;
 #pragma unroll
@@ -489,11 +514,7 @@ struct Stage4 {
             u32x4 c = codes[s];
             asm("" : "+v"(c.x), "+v"(c.y), "+v"(c.z), "+v"(c.w));
             uint32_t e = known_scale(scale[s]);
-            if constexpr (kKeyScales) {
-                const uint32_t top = group_largest<kLanes>(e);
-                e = (uint32_t)max((int)(e + 127 - top), 0);
-                if (works(s) && piece() == 0) keys[row(s)] = top == kScaleNan ? nan_value() : scale_bits(top);
-            } else if constexpr (VALUES) {
+            if constexpr (VALUES) {
                 const bool nan = group_largest<kLanes>(e) == kScaleNan;
                 bad |= nan;
                 e = e == kScaleNan ? 0 : e;
@@ -556,13 +577,15 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 // dims, window 512 (fp16) 99, 457 TFLOP/s, of which a quarter of the columns are padding and the edges of the window are
 // computed and masked.  Chunks of 512 tokens of four sequences over 16384 keys, window 4096, 32 heads on 8, fp8: 200, 513
 // TFLOP/s, the widening of codes being work of its own.
-// Over 8-bit codes at 256 dims the fp16 kernels spill 6 to 11 registers, over 4 bits, two workgroups to a CU, 40 to 70.
+// Over 8-bit codes at 256 dims the fp16 kernels spill 5 to 11 registers; over 4 bits, two workgroups to a CU, those of 256 dims 77 to 146 (the
+// most in fp16, whose second loop is for wide tiles) and of 128 dims up to 4.
 template <typename T, int DP, int SRC, bool SPLIT>
 __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged16 ? 3 : 2) : SRC == kPagedF4 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
     constexpr bool kPages = SRC != kStrided;
     constexpr bool kF4 = SRC == kPagedF4;
     constexpr bool kCodes = SRC == kPagedI8 || SRC == kPagedF8 || kF4;
-    constexpr bool kKeyScales = kCodes && !(kF4 && __is_same(T, BF16));  // a factor for each key, apart from its codes
+    constexpr bool kHalf4 = kF4 && __is_same(T, F16);
+    constexpr bool kKeyScales = kCodes && !kF4;  // a factor for each key, apart from its codes
     constexpr int kBytes = kCodes ? 1 : 2;
     // Keys of one step.  32 leave registers and LDS for a third workgroup on a CU (measured with 64 and 32, us: 2 x 64
     // heads of 96 dims, 2048 keys, window 512: 126, 105; 32 heads of 128 dims, 8192 keys, window 4096: 562, 539); with
@@ -572,7 +595,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     constexpr int kFwdKeys = kCodes && !(kF4 && DP > 128) ? 64 : 32;
     constexpr int kTile = kFwdKeys * Tile<DP>::kRow;
     __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile + (kCodes ? 2 * 2 * kFwdKeys * 4 : 0)];
-    __shared__ __attribute__((aligned(16))) uint32_t nan_keys[kF4 && !kKeyScales ? 2 : 1][4];  // [buffer][wave that staged it]
+    __shared__ __attribute__((aligned(16))) uint32_t nan_keys[kF4 ? 2 : 1][4], wide_tiles[kHalf4 ? 2 : 1][4];  // [buffer][wave that staged it]
 
     // block -> (sample, key head), row tile, part: neighbours in time on one XCD (blocks go to the 8 XCDs in
     // turn) are the row tiles of one key head, whose keys they share
@@ -624,7 +647,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
 
     // One tile of keys and values into one of the buffers: 16-bit rows are copied there as they are; codes come through
     // registers and are widened on the way, which put() does when the tile's turn is near.
-    typedef std::conditional_t<kF4, Stage4<T, DP, kFwdKeys>, Stage<T, DP, kCodes ? SRC : kPagedI8, kFwdKeys>> St;
+    typedef std::conditional_t<kF4, Stage4<DP, kFwdKeys>, Stage<T, DP, kCodes ? SRC : kPagedI8, kFwdKeys>> St;
     typedef Flight<DP, kFwdKeys> Fl;
     Fl fl;
     constexpr int kSteps = kCodes ? St::kSteps : Fl::kSteps;
@@ -732,13 +755,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
         }
     };
     float* const scales = reinterpret_cast<float*>(lds + 2 * 2 * kTile);  // [buffer][keys, values][64]
-    auto put = [&](int buffer) {
+    auto put4 = [&](auto type, int buffer) {  // 4-bit codes as 16-bit values of this type
         if constexpr (kF4) {
-            ks.template put<false>(lds + buffer * 2 * kTile, scales + buffer * 2 * kFwdKeys);
-            const bool bad = vs.template put<true>(lds + buffer * 2 * kTile + kTile, scales + (buffer * 2 + 1) * kFwdKeys);
-            if constexpr (!kKeyScales) {
-                const uint32_t any = __any(bad);
-                if (lane == 0) nan_keys[buffer][wave] = any;
+            typedef decltype(type) V;
+            char* const kt = lds + buffer * 2 * kTile;
+            ks.template put<V, false>(kt, nullptr);
+            const uint32_t any = __any(vs.template put<V, true>(kt + kTile, scales + (buffer * 2 + 1) * kFwdKeys));
+            if (lane == 0) nan_keys[buffer][wave] = any;
+        }
+    };
+    auto put = [&](auto is_wide, int buffer) {
+        if constexpr (kF4) {
+            constexpr bool kWide = decltype(is_wide)::value;
+            put4(std::conditional_t<kWide, BF16, T>{}, buffer);
+            if constexpr (kHalf4 && !kWide) {
+                const uint32_t any = __any(ks.wide() | vs.wide());
+                if (lane == 0) wide_tiles[buffer][wave] = any;
             }
         } else if constexpr (kCodes) {
             ks.put(lds + buffer * 2 * kTile);
@@ -756,7 +788,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     float m = kNegInf, l = 0.f;
     constexpr bool kLifted = kKeyScales && __is_same(T, F16);
-    constexpr float kBits = probability_bits<T, kCodes>();
+    constexpr float kBits = probability_bits<T, kKeyScales>();
     Lift lift;
 
     // the first tile is on its way before the queries are waited for
@@ -778,150 +810,201 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
         }
     }
 
-    if (first_tile < end_tile) put(0);
+    if (first_tile < end_tile) put(std::false_type{}, 0);
     __syncthreads();
 
-    for (int it = first_tile; it < end_tile; ++it) {
-        const int buffer = (it - first_tile) & 1, next = buffer ^ 1;
-        const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
-        const int key0 = tiles.tile(it) * kFwdKeys;
-        if (it + 1 < end_tile) {
-            fetch(tiles.tile(it + 1), next);
-            if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
-        }
-        // what of the tile this wave's rows see: nothing, all, or some of it
-        const int key_end = key0 + kFwdKeys;
-        const bool none = !wave_works || key0 > wv_last || key0 >= keys ||
-                          (a.window >= 0 && key_end - 1 < wv_first - a.window && key0 >= a.sinks);
-        const bool all = key_end - 1 <= wv_first && key_end <= keys &&
-                         (a.window < 0 || key0 >= wv_last - a.window || key_end <= a.sinks);
-        if (!none) {
-            f32x16 s[kFwdKeys / 32];
-#pragma unroll
-            for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
-                matrix_first(!kCodes);
-#pragma unroll
-                for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<T>::op(kt_ops.rows(32 * kb, st), q[st], s[kb]);
-                matrix_done(!kCodes);
+    // The tiles from this one on, or up to one that is wide; from that on they are bf16 numbers, and queries and probabilities the sums of two such
+    // numbers, as in attn_token4_kernel.  (One loop with both in it spills 35 registers at 128 dims and 310 at 256.)
+    auto steps = [&](auto is_wide, const int from) __attribute__((always_inline)) {
+        constexpr bool kWide = decltype(is_wide)::value;
+        typedef std::conditional_t<kWide, BF16, T> V;
+        for (int it = from; it < end_tile; ++it) {
+            const int buffer = (it - first_tile) & 1, next = buffer ^ 1;
+            const Operands<DP> kt_ops(lds_byte(lds) + buffer * 2 * kTile), vt_ops(lds_byte(lds) + buffer * 2 * kTile + kTile);
+            const int key0 = tiles.tile(it) * kFwdKeys;
+            if constexpr (kHalf4 && !kWide) {
+                const u32x4 any = *reinterpret_cast<const u32x4*>(wide_tiles[buffer]);
+                if (__builtin_amdgcn_readfirstlane(any.x | any.y | any.z | any.w)) return it;
             }
-            if constexpr (kKeyScales) {
-                const float* f = scales + buffer * 2 * kFwdKeys;
+            if (it + 1 < end_tile) {
+                fetch(tiles.tile(it + 1), next);
+                if (it + 2 < end_tile) look_up(tiles.tile(it + 2));
+            }
+            // what of the tile this wave's rows see: nothing, all, or some of it
+            const int key_end = key0 + kFwdKeys;
+            const bool none = !wave_works || key0 > wv_last || key0 >= keys ||
+                              (a.window >= 0 && key_end - 1 < wv_first - a.window && key0 >= a.sinks);
+            const bool all = key_end - 1 <= wv_first && key_end <= keys &&
+                             (a.window < 0 || key0 >= wv_last - a.window || key_end <= a.sinks);
+            if (!none) {
+                f32x16 s[kFwdKeys / 32];
+                if constexpr (kWide) {
+#pragma unroll
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st) {
+                        u32x4 x = q[st], low;
+                        asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w));  // (or all of them are taken apart before the loop)
+                        const u32x4 high = two_bf16(x, low);
+#pragma unroll
+                        for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
+                            const u32x4 k = kt_ops.rows(32 * kb, st);
+                            s[kb] = Mma<V>::op(k, high, s[kb]);
+                            s[kb] = Mma<V>::op(k, low, s[kb]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+                        matrix_first(!kCodes);
+#pragma unroll
+                        for (int st = 0; st < DP / 16; ++st) s[kb] = Mma<V>::op(kt_ops.rows(32 * kb, st), q[st], s[kb]);
+                        matrix_done(!kCodes);
+                    }
+                }
+                if constexpr (kKeyScales) {
+                    const float* f = scales + buffer * 2 * kFwdKeys;
+#pragma unroll
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 16; r += 4) {
+                            const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[kb][r + i] *= c[i];
+                        }
+                }
+                if (!all) {
+#pragma unroll
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
+                        const Sight sight(position, keys, a.window, a.sinks, key0 + 32 * kb, half);
+                        if (key0 < a.sinks) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[kb][r] = sight.any(r) ? s[kb][r] : kNegInf;
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[kb][r] = sight.window(r) ? s[kb][r] : kNegInf;
+                        }
+                    }
+                }
+                float top = kNegInf;
 #pragma unroll
                 for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
+                    for (int r = 0; r < 16; r += 2) top = max3(top, s[kb][r], s[kb][r + 1]);
+                top = both_halves_max(top) * a.scale_log2;
+                // The running maximum follows only where a row has outgrown it by 2^8: until then its exponentials stay
+                // below 256 and the accumulators need no rescaling.
+                if (__any(top > m + 8.f)) {
+                    const float higher = fmaxf(m, top);
+                    float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
+                    m = higher;
+                    l *= f;
+                    if constexpr (kLifted) f = lift.follow(f);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[kb][r + i] *= c[i];
+                    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+                }
+                const float base = (m == kNegInf ? 0.f : m) - kBits;
+                float sum = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], a.scale_log2, -base));
+                        sum += s[kb][r];
                     }
-            }
-            if (!all) {
+                l += sum;
+                if constexpr (kF4) {
+                    const u32x4 any = *reinterpret_cast<const u32x4*>(nan_keys[buffer]);
+                    if (__builtin_amdgcn_readfirstlane(any.x | any.y | any.z | any.w)) {
 #pragma unroll
-                for (int kb = 0; kb < kFwdKeys / 32; ++kb) {
-                    const Sight sight(position, keys, a.window, a.sinks, key0 + 32 * kb, half);
-                    if (key0 < a.sinks) {
+                        for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[kb][r] = sight.any(r) ? s[kb][r] : kNegInf;
-                    } else {
+                            for (int r = 0; r < 16; r += 4) {
+                                const f32x4 c = *reinterpret_cast<const f32x4*>(scales + (buffer * 2 + 1) * kFwdKeys + 32 * kb + 2 * r + 4 * half);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[kb][r] = sight.window(r) ? s[kb][r] : kNegInf;
+                                for (int i = 0; i < 4; ++i) s[kb][r + i] = s[kb][r + i] != 0.f ? s[kb][r + i] + c[i] : 0.f;
+                            }
                     }
                 }
-            }
-            float top = kNegInf;
-#pragma unroll
-            for (int kb = 0; kb < kFwdKeys / 32; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) top = max3(top, s[kb][r], s[kb][r + 1]);
-            top = both_halves_max(top) * a.scale_log2;
-            // The running maximum follows only where a row has outgrown it by 2^8: until then its exponentials stay
-            // below 256 and the accumulators need no rescaling.
-            if (__any(top > m + 8.f)) {
-                const float higher = fmaxf(m, top);
-                float f = __builtin_amdgcn_exp2f(m - (higher == kNegInf ? 0.f : higher));
-                m = higher;
-                l *= f;
-                if constexpr (kLifted) f = lift.follow(f);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[i][r] *= f;
-            }
-            const float base = (m == kNegInf ? 0.f : m) - kBits;
-            float sum = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < kFwdKeys / 32; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], a.scale_log2, -base));
-                    sum += s[kb][r];
-                }
-            l += sum;
-            if constexpr (kF4 && !kKeyScales) {
-                const u32x4 any = *reinterpret_cast<const u32x4*>(nan_keys[buffer]);
-                if (__builtin_amdgcn_readfirstlane(any.x | any.y | any.z | any.w)) {
+                if (kKeyScales && !all) {  // a hidden value's scale may be anything
 #pragma unroll
                     for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
                         for (int r = 0; r < 16; r += 4) {
                             const f32x4 c = *reinterpret_cast<const f32x4*>(scales + (buffer * 2 + 1) * kFwdKeys + 32 * kb + 2 * r + 4 * half);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[kb][r + i] = s[kb][r + i] != 0.f ? s[kb][r + i] + c[i] : 0.f;
+                            for (int i = 0; i < 4; ++i) s[kb][r + i] = s[kb][r + i] != 0.f ? s[kb][r + i] * c[i] : 0.f;
+                        }
+                } else if constexpr (kKeyScales) {
+                    const float* f = scales + (buffer * 2 + 1) * kFwdKeys;
+#pragma unroll
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 16; r += 4) {
+                            const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[kb][r + i] *= c[i];
                         }
                 }
-            }
-            if (kKeyScales && !all) {  // a hidden value's scale may be anything
+                if constexpr (kLifted) {
+                    float most = 0.f;
 #pragma unroll
-                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb) most = fmaxf(most, largest(s[kb]));
+                    most = both_halves_max(most);
+                    if (__any(lift.short_of(most))) {
+                        const float f = lift.lower(most);
 #pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const f32x4 c = *reinterpret_cast<const f32x4*>(scales + (buffer * 2 + 1) * kFwdKeys + 32 * kb + 2 * r + 4 * half);
+                        for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[kb][r + i] = s[kb][r + i] != 0.f ? s[kb][r + i] * c[i] : 0.f;
+                            for (int r = 0; r < 16; ++r) acc[i][r] *= f;
                     }
-            } else if constexpr (kKeyScales) {
-                const float* f = scales + (buffer * 2 + 1) * kFwdKeys;
 #pragma unroll
-                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+                    for (int kb = 0; kb < kFwdKeys / 32; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const f32x4 c = *reinterpret_cast<const f32x4*>(f + 32 * kb + 8 * (r >> 2) + 4 * half);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[kb][r + i] *= c[i];
-                    }
-            }
-            if constexpr (kLifted) {
-                float most = 0.f;
-#pragma unroll
-                for (int kb = 0; kb < kFwdKeys / 32; ++kb) most = fmaxf(most, largest(s[kb]));
-                most = both_halves_max(most);
-                if (__any(lift.short_of(most))) {
-                    const float f = lift.lower(most);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+                        for (int r = 0; r < 16; ++r) s[kb][r] *= lift.times;
                 }
 #pragma unroll
-                for (int kb = 0; kb < kFwdKeys / 32; ++kb)
+                for (int t = 0; t < kFwdKeys / 16; ++t) {
+                    u32x4 p, p_low;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] *= lift.times;
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = s[t >> 1][8 * (t & 1) + 2 * e], y = s[t >> 1][8 * (t & 1) + 2 * e + 1];
+                        if constexpr (kWide) {
+                            uint32_t rest;
+                            p[e] = pack_with_rest<V>(x, y, rest);
+                            p_low[e] = rest;
+                        } else {
+                            p[e] = Elem<V>::pack(x, y);
+                        }
+                    }
+                    matrix_first(!kCodes);
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) {
+                        const u32x4 v = vt_ops.columns(16 * t, i);
+                        acc[i] = Mma<V>::op(v, p, acc[i]);
+                        if constexpr (kWide) acc[i] = Mma<V>::op(v, p_low, acc[i]);
+                    }
+                    matrix_done(!kCodes);
+                }
             }
-#pragma unroll
-            for (int t = 0; t < kFwdKeys / 16; ++t) {
-                u32x4 p;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) p[e] = Elem<T>::pack(s[t >> 1][8 * (t & 1) + 2 * e], s[t >> 1][8 * (t & 1) + 2 * e + 1]);
-                matrix_first(!kCodes);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) acc[i] = Mma<T>::op(vt_ops.columns(16 * t, i), p, acc[i]);
-                matrix_done(!kCodes);
-            }
+            if (it + 1 < end_tile) put(is_wide, next);
+            __syncthreads();
         }
-        if (it + 1 < end_tile) put(next);
-        __syncthreads();
+        return end_tile;
+    };
+    const int at = steps(std::false_type{}, first_tile);
+    if constexpr (kHalf4) {
+        if (at < end_tile) {  // (for all waves; the codes of this tile are still in the registers)
+            put4(BF16{}, (at - first_tile) & 1);
+            __syncthreads();
+            steps(std::true_type{}, at);
+        }
     }
 
     const float total = both_halves_sum(l);

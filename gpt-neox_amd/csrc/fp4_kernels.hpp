@@ -375,21 +375,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : DP <= 128 ? 3 : 2) voi
                 const int dim = dim_of(s) + 8 * t;
                 u32x4 x = load8(p + dim * 2, there && dim < a.d);
                 x ^= a.flip;
-                if constexpr (kTwo) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float lo, hi;
-                        uint32_t rest;
-                        Elem<F16>::unpack(x[i], lo, hi);
-                        q[s * kWords + t][i] = pack_with_rest<BF16>(lo, hi, rest);
-                        // (nothing is left of an infinity)
-                        if (__builtin_fabsf(lo) == __builtin_inff()) rest &= 0xffff0000u;
-                        if (__builtin_fabsf(hi) == __builtin_inff()) rest &= 0x0000ffffu;
-                        q_low[s * kWords + t][i] = rest;
-                    }
-                } else {
-                    q[s * kWords + t] = x;
-                }
+                if constexpr (kTwo) q[s * kWords + t] = two_bf16(x, q_low[s * kWords + t]);
+                else q[s * kWords + t] = x;
             }
     }
 

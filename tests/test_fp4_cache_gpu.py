@@ -262,6 +262,46 @@ def test_fp16_queries_over_values_beyond_fp16(device):
         check(q, cache, table, starts, lengths, scale=2.0**-43)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 96, 128, 160, 256])
+@pytest.mark.parametrize("written,loud,quiet", [(torch.float16, 4e4, 1e-3), (torch.float16, 4e4, 1e-5), (torch.float16, 4e4, 2.0**-22), (torch.float16, 2.0, 2.0**-22),
+                                                (torch.bfloat16, 2.0**40, 1e-3), (torch.bfloat16, 4e4, 2.0**-30), (torch.bfloat16, 1.5 * 2.0**16, 2.0**-23)])
+def test_small_values_next_to_large_ones(device, dtype, d, written, loud, quiet):
+    # The 32 values of every scale have a size of their own, which changes along the sequence.  Every channel of the output is held to the size of its
+    # own values, in single tokens, in a few and in chunks; the queries look at quiet dims of the keys only, so that nothing hides what these lose.
+    page, context = 16, 333
+    run = torch.arange(context, device=device) // 70  # (tokens that are alike: tiles of one kind and mixed ones)
+    group = torch.arange(d // 32, device=device)
+    at = run[:, None] + group
+    v_size = torch.tensor([loud, quiet, 1.0, quiet * 4], device=device)[at % 4]
+    k_size = torch.tensor([loud, 1.0, quiet], device=device)[at % 3]
+    k_size[:, 0] = v_size[:, -1] = quiet
+    k, v = ((normal((context, 2, d), torch.float32, device, seed).clamp(-2, 2) / 2 * size.repeat_interleave(32, -1)[:, None]).to(written)
+            for seed, size in ((72, k_size), (71, v_size)))
+    cache = PagedKVCache.allocate(24, page, 2, d, F4, device)
+    table = torch.randperm(24, generator=gen(device, 73), device=device)[:22].view(1, 22).int()
+    slots = slots_of(table, torch.zeros(context, device=device), torch.arange(context, device=device), page)
+    cache.write(k, v, slots)
+    k, v = (P.decode(flat(x)[slots], flat(s)[slots]) for x, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    for new, window, sinks in ((1, None, 0), (7, None, 0), (100, None, 0), (1, 150, 5), (100, 150, 5)):
+        starts, lengths = torch.tensor([0, new], dtype=torch.int32, device=device), torch.tensor([context], dtype=torch.int32, device=device)
+        q = normal((new, 4, d), dtype, device, 74)
+        q[..., 32:] = 0
+        got = paged_attention(q, cache, table, starts, lengths, max_query=new, scale=1.0 / quiet, window=window, sinks=sinks).double()
+        sees = A.visible(new, context, window, sinks, device=device)
+        for h in range(4):
+            qh, kh, vh = q[:, h].double(), k[:, h // 2], v[:, h // 2]
+            want, p = A.one_head(qh, kh, vh, sees, 1.0 / quiet)
+            scores = torch.where(sees, (qh.abs() @ kh.abs().T) / quiet, 0.0).amax(1, keepdim=True)
+            u = A.ROUND[dtype]
+            # Probabilities are rounded once.  In fp16 the largest is held between 2^7 and 2^15, and what is below the type's normal numbers is off by
+            # 2^-25: by 2^-32 of it.  The output is rounded once; scores, exponentials and sums are in 32 bits.
+            bound = (1.05 * u + 2.0**-20 * (4 + scores)) * (p @ vh.abs()) + 1.05 * u * want.abs() + 2.0**-32 * (sees.double() @ vh.abs()) + 2 * A.TINY[dtype]
+            holds = want.abs() + bound < torch.finfo(dtype).max  # (what is beyond the type is an infinity there)
+            err = (got[:, h] - want).abs()
+            assert (err <= bound)[holds].all(), (new, h, (err / bound)[holds].max().item())
+
+
 @pytest.mark.parametrize("page", [1, 3, 16, 31, 32, 64, 100, 256])
 def test_page_sizes(device, page):
     for new in ([1, 1], [50, 20]):
