@@ -10,11 +10,13 @@ namespace neox {
 // ---- launches whose kernels do not depend on the head dim ------------------------------------------------
 // A wave for each row where there are many rows in few parts, else a workgroup (bf16, 128 dims, us: 32768 rows in 2 parts
 // 24 with a workgroup, 11 with a wave; 16384 in 4 14, 9; 4096 in 16 8.6, 7.2; 2048 in 4 4.4, 4.5; 512 in 16 4.8, 6.4).
+static bool join_by_waves(const AttnArgs& a) { return a.splits <= 16 && a.part_rows >= 4096; }
+static int64_t join_blocks(const AttnArgs& a) { return join_by_waves(a) ? (a.part_rows + 3) / 4 : a.part_rows; }
 hipError_t launch_attn_join(const AttnArgs& a, int dtype, hipStream_t stream) {
-    const uint32_t blocks = (uint32_t)a.part_rows;
-    if (a.splits <= 16 && a.part_rows >= 4096) {
-        if (dtype == NEOX_BF16) attn_join_rows_kernel<BF16><<<(blocks + 3) / 4, 256, 0, stream>>>(a);
-        else attn_join_rows_kernel<F16><<<(blocks + 3) / 4, 256, 0, stream>>>(a);
+    const uint32_t blocks = (uint32_t)join_blocks(a);
+    if (join_by_waves(a)) {
+        if (dtype == NEOX_BF16) attn_join_rows_kernel<BF16><<<blocks, 256, 0, stream>>>(a);
+        else attn_join_rows_kernel<F16><<<blocks, 256, 0, stream>>>(a);
         return hipGetLastError();
     }
     if (dtype == NEOX_BF16) attn_join_kernel<BF16><<<blocks, 256, 0, stream>>>(a);
@@ -22,10 +24,17 @@ hipError_t launch_attn_join(const AttnArgs& a, int dtype, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// Threads of a row: a power of two, for as many elements each as the kernels take.
+static int cache_lanes(int d, int source, bool write) {
+    const int elems = write && source != kPaged16 ? 16 : 8;
+    int lanes = write && source == kPagedF4 ? 2 : 4;
+    while (lanes * elems < d) lanes *= 2;
+    return lanes;
+}
 template <typename T, int SRC, bool WRITE>
 static void cache_rows(const CacheArgs& a, hipStream_t stream) {
     constexpr int kElems = cache_elems<SRC, WRITE>();
-    const int lanes = a.d <= kElems * 4 ? 4 : a.d <= kElems * 8 ? 8 : a.d <= kElems * 16 ? 16 : 32;
+    const int lanes = cache_lanes(a.d, SRC, WRITE);
     const uint32_t blocks = (uint32_t)((a.rows * lanes + 255) / 256);
     switch (lanes) {
         case 4: cache_kernel<T, SRC, 4, WRITE><<<blocks, 256, 0, stream>>>(a); break;
@@ -43,8 +52,7 @@ static void cache_source(const CacheArgs& a, int source, hipStream_t stream) {
 }
 template <typename T, bool WRITE>
 static void cache4_rows(const CacheArgs& a, hipStream_t stream) {
-    constexpr int kElems = cache4_elems<WRITE>();
-    const int lanes = a.d <= kElems * 2 ? 2 : a.d <= kElems * 4 ? 4 : a.d <= kElems * 8 ? 8 : a.d <= kElems * 16 ? 16 : 32;
+    const int lanes = cache_lanes(a.d, kPagedF4, WRITE);
     const uint32_t blocks = (uint32_t)((a.rows * lanes + 255) / 256);
     switch (lanes) {
         case 2: if constexpr (WRITE) cache4_kernel<T, 2, WRITE><<<blocks, 256, 0, stream>>>(a); break;  // (32 dims)
@@ -67,6 +75,9 @@ hipError_t launch_cache(const CacheArgs& a, int source, int dtype, bool write, h
 
 // ---- validation ------------------------------------------------------------------------------------------------
 constexpr int kMost = 1 << 30;  // sizes and positions stay below, so that sums of two stay in 32 bits
+
+// A launch has less than 2^32 threads in one direction.  (Workgroups of 512 there are 256 at most.)
+static bool launches(int64_t blocks) { return blocks * 256 < (int64_t)1 << 32; }
 
 static int check_heads(int h, int h_kv, int d, const char* what) {
     if (h < 1 || h_kv < 1 || h % h_kv != 0)
@@ -362,6 +373,8 @@ static int cache_call(const char* what, void* k, void* v, const void* kc, const 
     NEOX_TRY(check_strides(v_st, 2, h_kv, d, 8, what, "v"));
     NEOX_TRY(check_cache(kc, vc, ks, vs, kc_st, vc_st, ks_st, vs_st, pages, page_size, h_kv, d, dtype, cache_dtype, what));
     const int source = cache_source_of(cache_dtype, dtype);
+    if (!launches((tokens * h_kv * cache_lanes(d, source, write) + 255) / 256))
+        return fail(NEOX_ERR_BAD_SHAPE, "%s: %lld tokens of %d heads of %d dims are too large for one call", what, (long long)tokens, h_kv, d);
     CacheArgs a{};
     a.k = static_cast<char*>(k);
     a.v = static_cast<char*>(v);
@@ -538,8 +551,6 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
     NEOX_TRY(check_scale_window(scale, sinks, what));
     const int source = cache_source_of(cache_dtype, dtype);
     const PagedPlan plan = plan_paged(b, tokens, max_query, max_context, h, h_kv, d, window, sinks, source);
-    if ((int64_t)b * h_kv * plan.row_tiles * plan.splits >= kMost)
-        return fail(NEOX_ERR_BAD_SHAPE, "%s: b=%d h_kv=%d of %d rows is too large for one call", what, b, h_kv, max_query * (h / h_kv));
     if (plan.bytes > 0) {
         NEOX_TRY(check_pointer(workspace, 16, what, "workspace"));
         if (workspace_bytes < plan.bytes)
@@ -587,7 +598,10 @@ int neox_paged_attention(void* out, void* workspace, int64_t workspace_bytes, co
         page_strides(a.ks_st, k_scale_strides);
         page_strides(a.vs_st, v_scale_strides);
     }
-    if (plan.token && source == kPagedF4) a.heads = token4_heads(a);
+    a.heads = plan.token && source == kPagedF4 ? token4_heads(a) : 1;
+    const int64_t blocks = (int64_t)(h_kv / a.heads) * a.row_tiles * (plan.token ? ((int64_t)b * a.splits + 7) / 8 * 8 : b);
+    if (!launches(blocks) || (a.splits > 1 && !launches(join_blocks(a))))
+        return fail(NEOX_ERR_BAD_SHAPE, "%s: b=%d h_kv=%d of %d rows is too large for one call", what, b, h_kv, max_query * (h / h_kv));
     hipStream_t s = (hipStream_t)stream;
     NEOX_TRY(check_launch(plan.token ? run_token(a, source, dtype, s) : run_fwd(a, source, dtype, s), what));
     return a.splits > 1 ? check_launch(launch_attn_join(a, dtype, s), what) : (int)NEOX_OK;

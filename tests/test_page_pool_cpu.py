@@ -133,3 +133,36 @@ def test_a_cache_in_4_bits_looks_at_its_tensors():
         PagedKVCache(k.view(torch.uint8), k.view(torch.uint8), s, s)
     with pytest.raises(RuntimeError, match="multiple of 32"):
         PagedKVCache.allocate(4, 16, 2, 48, F4, "cpu")
+
+
+HUGE = 1 << 24  # blocks of 256 threads: a launch has less than 2^32 in one direction
+
+
+@pytest.mark.parametrize("cache", [_lib.NEOX_F4, _lib.NEOX_I8, _lib.NEOX_BF16])
+@pytest.mark.parametrize("change", [
+    dict(b=HUGE, max_context=16, h=1, h_kv=1), dict(b=HUGE - 3, max_context=16, h=1, h_kv=1), dict(b=HUGE // 3 + 1, max_context=16, h=6, h_kv=3),
+    dict(b=HUGE // 2, max_query=100, max_context=100, h=4, h_kv=2),
+    dict(b=1, tokens=HUGE // 32, max_query=1, max_context=100000, h=32, h_kv=2, ws=True, size=1 << 62),  # (the parts' join: a block for each row)
+])
+def test_launches_that_do_not_fit(p, cache, change):
+    codes = 2 if cache == _lib.NEOX_F4 else 1
+    wide = {n: st(4096, 256, 64 // codes) for n in ("kcs", "vcs")}
+    change = {**change, **({"ws": p} if "ws" in change else {})}
+    refused(paged(p, cache=cache, os=st(2048, 64), qs=st(2048, 64), **wide, **change), -3, "too large for one call")
+
+
+def test_blocks_of_rows_that_do_not_fit(p):
+    strides = dict(h=48, h_kv=1, os=st(64 * 64, 64), qs=st(64 * 64, 64))  # three blocks of 16 rows
+    refused(paged(p, b=HUGE // 3 + 1, max_query=1, max_context=16, **strides), -3, "too large for one call")
+
+
+@pytest.mark.parametrize("cache,d,into,back", [(_lib.NEOX_F4, 32, None, 2**30 - 1), (_lib.NEOX_F4, 256, 2**28, 2**27), (_lib.NEOX_F4, 160, 2**28 - 1, 2**27),
+                                               (_lib.NEOX_I8, 128, 2**29, 2**28), (_lib.NEOX_F16, 256, 2**27, 2**27)])
+def test_caches_whose_launches_do_not_fit(p, cache, d, into, back):
+    # tokens of one head, from 2 to 32 threads each
+    row = d // 2 if cache == _lib.NEOX_F4 else d
+    outside, held, scales = st(d, d), st(64 * row, row, row), st(64, 8, 8)
+    lib, types = _lib.lib(), (_lib.NEOX_F16, cache, None)
+    refused(lib.neox_cache_read(p, p, p, p, p, p, p, 1, back, 1, d, 4, 16, outside, outside, held, held, scales, scales, *types), -3, "too large for one call")
+    if into:
+        refused(lib.neox_cache_write(p, p, p, p, p, p, p, 1, into, 1, d, 4, 16, held, held, scales, scales, outside, outside, *types), -3, "too large for one call")
