@@ -489,6 +489,32 @@ def test_a_nan_stays_with_its_head(device, dtype, which, bad):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("d,h_kv,page,aligned", [(128, 16, 32, True), (64, 16, 32, True), (96, 16, 32, True), (64, 2, 32, True), (64, 2, 31, True), (64, 2, 32, False), (128, 2, 31, True),
+                                                 (160, 2, 32, True), (192, 2, 48, True), (256, 2, 31, True), (256, 2, 32, True), (256, 2, 48, False)])
+def test_one_nan_scale_is_the_whole_row_of_single_tokens(device, dtype, which, d, h_kv, page, aligned):
+    # whichever of the row's scales it is: every dim of the heads that see it, in each way of fetching, one and two heads to a wave
+    b = 16
+    q, cache, table, starts, lengths = sequences(device, dtype, [1] * b, [1000] * b, 2 * h_kv, h_kv, d, page)
+    if not aligned:
+        odd = [torch.empty(t.numel() + 1, dtype=torch.uint8, device=device)[1:].view(t.shape) for t in (cache.k_scale, cache.v_scale)]
+        for to, t in zip(odd, (cache.k_scale, cache.v_scale)):
+            to.copy_(t.view(torch.uint8))
+        cache = PagedKVCache(cache.k, cache.v, *(t.view(E8) for t in odd))
+    want = paged_attention(q, cache, table, starts, lengths, max_query=1, max_context=1000)
+    t = (cache.k_scale if which == "k" else cache.v_scale).view(torch.uint8)
+    for group in range(d // 32):
+        at = (table[3, 990 // page].long(), 990 % page, 1, group)
+        before = t[at].clone()
+        t[at] = 255
+        got = paged_attention(q, cache, table, starts, lengths, max_query=1, max_context=1000)
+        t[at] = before
+        hit = torch.zeros(got.shape[:2], dtype=torch.bool, device=device)
+        hit[3, 2:4] = True
+        assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", DIMS)
 @pytest.mark.parametrize("page,aligned", [(31, True), (48, True), (48, False)])
 def test_every_way_of_fetching(device, dtype, d, page, aligned):
