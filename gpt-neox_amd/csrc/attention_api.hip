@@ -260,7 +260,11 @@ struct PagedPlan {
 // 7.7, 7.0; 16 of 1000 of 8 heads of 128 12.3, 11.3; 64 of 1000 15.3, 16.4; one of 120 5.5, 6.0).  us by parts, bf16, 128 dims, 8 key heads: 16 sequences of 517 tokens 1: 9.1, 2: 10.3, 4: 10.4; 64 of
 // 1000 1: 15.1, 2: 19.9, 4: 22.7; 64 of 2000 1: 24.4, 2: 27.9; 16 of 2000 2: 16.9, 4: 15.0, 8: 16.5, 16: 19.7; 1 of 4000 16: 10.8, 32: 9.3; 4 of
 // 2000 4: 12.0, 8: 10.4, 16: 11.9; 4 of 32000 16: 28.1, 32: 26.6, 64: 28.8; 64 of 8192 1: 116, 2: 98, 4: 88, 8: 88, 12: 95; 256 dims, fp16, 16 drafts of 5
-// tokens in a window of 1024 1: 27.3, 2: 23.7, 4: 24.9, 6: 32.0.
+// tokens in a window of 1024 1: 24.0, 2: 23.2, 3: 24.5.
+// Next to the rule's borders: those drafts, 128 units, with windows of 880 1: 23.3, 2: 21.4, of 1014 1: 23.8, 2: 23.2; 16 sequences of 1024 tokens of 8 heads of 128
+// 1: 12.6, 2: 12.9, of 1060 1: 12.7, 2: 13.8, of 1280 2: 14.1, 4: 14.4, of 1300 2: 14.9, 4: 14.5; 4 of 640 1: 9.4, 3: 9.6, of 660 1: 10.2, 3: 9.6; 64 of 2048
+// 1: 36.7, 2: 33.5, 3: 35.1, of 2060 1: 36.8, 2: 35.0, 3: 36.0; 32 of 2048 1: 18.8, 2: 21.5, of 2100 1: 18.5, 3: 22.5, of 3000 1: 23.9, 3: 27.6.  The
+// rule is within 10 % of the better side but for those 256 units of equal length above 2048 keys, 15 to 22 %; unequal ones need the parts.
 static int parts_token4(int64_t units, int64_t keys, int64_t most) {
     int64_t parts = std::min(most, (256 + units - 1) / units);
     if (keys <= std::max((int64_t)640, 8 * std::min(units, (int64_t)256))) return 1;

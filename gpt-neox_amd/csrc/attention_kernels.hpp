@@ -590,8 +590,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     // Keys of one step.  32 leave registers and LDS for a third workgroup on a CU (measured with 64 and 32, us: 2 x 64
     // heads of 96 dims, 2048 keys, window 512: 126, 105; 32 heads of 128 dims, 8192 keys, window 4096: 562, 539); with
     // codes, whose widening takes the registers anyway, 64 save barriers (chunks of 512 over 16384 in fp8: 251, 275).  Over 4 bits above
-    // 128 dims 32 leave LDS for a second one: 4 x 512 tokens over 8192 keys of 256 dims, window 4096, fp16 345, 262, bf16 the same; of 160 dims, which
-    // have kernels of their own there, 4 x 98 over 7053 158, 81 (with 256 dims' padding 117), 1 x 1024 over 16000 in bf16 511, 279.
+    // 128 dims 32 leave LDS for a second one: 4 x 512 tokens over 8192 keys of 256 dims, 16 heads on 8, window 4096, fp16 301, 285, bf16 290, 267; of 160
+    // dims, which have kernels of their own, 4 x 98 over 7053 in fp16 106, 78 (padded to 256 128), 1 x 1024 over 16000 in bf16 368, 271 (473).
     constexpr int kFwdKeys = kCodes && !(kF4 && DP > 128) ? 64 : 32;
     constexpr int kTile = kFwdKeys * Tile<DP>::kRow;
     __shared__ __attribute__((aligned(512))) char lds[2 * 2 * kTile + (kCodes ? 2 * 2 * kFwdKeys * 4 : 0)];
@@ -814,7 +814,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? (SRC == kStrided || SRC == kPaged1
     __syncthreads();
 
     // The tiles from this one on, or up to one that is wide; from that on they are bf16 numbers, and queries and probabilities the sums of two such
-    // numbers, as in attn_token4_kernel.  (One loop with both in it spills 35 registers at 128 dims and 310 at 256.)
+    // numbers, as in attn_token4_kernel.  (One loop with both in it spills 35 registers at 128 dims and 310 at 256.)  4 x 512 tokens over 16384
+    // keys, 32 heads on 8, window 4096, us, fp16 without and with a scale of 2^14 everywhere: 64 dims 136, 204, 128 dims 178, 313.
     auto steps = [&](auto is_wide, const int from) __attribute__((always_inline)) {
         constexpr bool kWide = decltype(is_wide)::value;
         typedef std::conditional_t<kWide, BF16, T> V;

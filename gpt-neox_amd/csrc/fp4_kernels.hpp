@@ -129,7 +129,10 @@ __global__ __launch_bounds__(256) void cache4_kernel(CacheArgs a) {
 // no less than two; but four sequences of 4099 with 8 heads 17.4, 18.6: two take CUs that have work enough.
 //
 // Measured: 64 sequences of 2048 to 8192 tokens, a token each, 32 heads on 8 of 128 dims, bf16, 84 us, 4.2 TB/s; one of 131001 28.9, 4.9; the launch
-// that joins the parts 4.7 to 4.9.  At 4 sequences of 517 tokens 7.5 us are the latency of one block of keys after the other.
+// that joins the parts 4.7 to 4.9.  At 4 sequences of 517 tokens 7.5 us are the latency of one block of keys after the other.  In fp16, whose two-head
+// kernels of 96 and 128 dims spill 3 registers, the 64 sequences take 93.6 with the join, in bf16 89.0.
+// With bf16 queries the probabilities are rounded to bf16 for the second product, half an ulp of each as in the other kernels: outputs are off by 1.2
+// times their own rounding.  Two instructions each, as in fp16, would take that away; the sums stay in 32 bits either way.
 //
 // Scales come by rows, lanes 0-31 the keys' and 32-63 the values', and go to the lanes that need them from there: loads of a byte for
 // each lane cost as much as those of its 16 bytes of codes (64 sequences of 2048 to 8192 tokens: 98 us, so 85).
@@ -162,7 +165,8 @@ __device__ __forceinline__ C buf_codes(rsrc_t r, uint32_t at) {
     else return buf_ld64(r, (int)at, 0);
 }
 
-// The head dims that the kernels over 4 bits are built for.
+// The head dims that the kernels over 4 bits are built for.  (160: for chunks, whose figures are at the forward kernel; 64 sequences of 2048 to 8192
+// tokens of 16 heads on 8, a token each, take 138 us there and padded to 256.)
 inline int padded4(int d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 160 ? 160 : 256; }
 
 // How the kernel may fetch: half a block, 16 keys, through one buffer if pages hold whole halves, keys and values are laid out alike,
